@@ -509,6 +509,71 @@ int lq_weight_grad_acc8(const void *dy, const void *x, int8_t *q_inout, const vo
 int lq_weight_grad_plan(int form, int64_t M, int64_t N, int64_t K, int compute_units, int *rows, int *columns, int *waves);
 
 /* ---------------------------------------------------------------------------
+ * Paged 8-bit cache of keys and values, and attention over it (the cache that the reference's chat demo and
+ * PTQ/quant/fused_attn.py:96-199 keep as past_key_value tensors; no counterpart function).
+ *
+ * The cache is a pool of num_blocks blocks of LQ_KV_BLOCK tokens, for kv_heads heads of dim dimensions (64, 96, 128 or 256):
+ *   k_codes  uint8 [num_blocks][kv_heads][64][dim]
+ *   v_codes  uint8 [num_blocks][kv_heads][16][dim][4]    token t of a block at [t / 4][d][t % 4]
+ *   k_scale, v_scale  float [num_blocks][kv_heads]       value = (code - 128) * scale, codes 1 .. 255
+ * block_table int32 [batch][table_width] lists the blocks of each sequence in order, seq_lens int32 [batch] the tokens
+ * of each sequence in the cache INCLUDING the new ones. Operands hold the new tokens of all sequences one after the
+ * other, `tokens` rows in all: cu_tokens int32 [batch + 1] has each sequence's first row and, last, the number of
+ * rows (null: every sequence has tokens / batch). The new tokens of sequence i are its last n_i =
+ * cu_tokens[i + 1] - cu_tokens[i]; token t of them is at position seq_lens[i] - n_i + t. max_tokens >= every n_i and max_len >= every
+ * seq_lens[i] are host values that size the launch (rows beyond max_tokens of a sequence are not computed; a max_len
+ * that is too small costs time, not correctness).
+ * dtype: 0 = bf16, 1 = f16. Strides are in elements, multiples of 8; the last dimension is contiguous; q, k, v, outputs,
+ * rotation tables and codes are 16-byte aligned. What the kernels read on the device is kept inside the operands: a
+ * block_table entry outside the pool is read as the last block and never written to, tokens beyond table_width blocks or before
+ * position 0 are not stored, positions beyond the rotation tables use their last row.
+ * Offsets into the cache are 64 bits wide. No atomics: results do not depend on an order.
+ * ------------------------------------------------------------------------- */
+#define LQ_KV_BLOCK 64
+
+/* Appends the new tokens' keys and values (rows of kv_heads x dim) to the cache; cos / sin given: keys are
+ * rotated by their position on the way, and q (rows of heads x dim, may be null; q_out may be q) into q_out.
+ * Rotation of the first rot_dim dimensions (a multiple of 16): halves (a, b) -> (a cos - b sin, b cos + a sin), float32
+ * tables [positions][rot_dim / 2], in fp32; q_out is rounded once, keys go to 8 bits unrounded.
+ * A (block, head)'s scale is max(A, 2^-90) / 127, A the largest finite |x| of its new tokens, or what it was where
+ * that is larger and the block held tokens of the sequence (then also: where it grows, the codes c that are there become
+ * rint(c * (old / new))). New codes: 128 + clamp(rint(x * (1 / scale)), -127, 127), NaN -> 128 (zero). Slots of a block
+ * beyond the sequence's tokens stay as they are. A block that takes tokens belongs to one sequence of the call. */
+int lq_kv8_append(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                  int64_t v_head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride, void *q_out,
+                  int64_t q_out_token_stride, int64_t q_out_head_stride, const float *cos_table, const float *sin_table,
+                  int64_t positions, int rot_dim, void *k_codes, void *v_codes, float *k_scale, float *v_scale,
+                  int64_t num_blocks, const int32_t *block_table, int64_t table_width, const int32_t *seq_lens,
+                  const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens, int heads, int kv_heads, int dim,
+                  int dtype, void *stream);
+
+/* The values of n blocks: k_out, v_out [n][64][kv_heads][dim], contiguous; dtype as above or 2 = f32: the fp32 product (code - 128) * scale,
+ * rounded to the type. A block outside the pool gives zeros. */
+int lq_kv8_read(const void *k_codes, const void *v_codes, const float *k_scale, const float *v_scale, int64_t num_blocks,
+                const int32_t *blocks, int64_t n, int kv_heads, int dim, int dtype, void *k_out, void *v_out, void *stream);
+
+/* out = softmax(scale * q K^T) V of the new tokens (rows of heads x dim; query head j reads kv head j / (heads / kv_heads)) over
+ * the sequence's tokens in the cache: those at positions <= the row's own (causal = 0: all), and with window > 0
+ * only the last `window` of positions up to the row's own. A row that sees nothing gives zeros. lse (null, or float
+ * [tokens][heads]): the natural logarithm of the softmax's denominator, -inf for such a row. scale > 0.
+ * q becomes f16 by a power of two for each row (exact but for elements under 2^-37 of the row's largest), codes are exact, scores,
+ * softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits) relative to the largest contribution so far.
+ * workspace (16-byte aligned, or null): with it, calls of few rows cut the keys into slices that a second launch
+ * joins in order; lq_kv8_attention_plan says how many and the bytes they take. Calls sharing a workspace are
+ * ordered on one stream. */
+int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes,
+                     const float *k_scale, const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width,
+                     const int32_t *seq_lens, const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens,
+                     int64_t max_len, int heads, int kv_heads, int dim, int dtype, float scale, int causal, int64_t window, void *out,
+                     int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace, int64_t workspace_bytes,
+                     void *stream);
+
+/* What lq_kv8_attention does with a call of these sizes (launches nothing; compute_units <= 0: the current device's): *kernel 0 = few
+ * rows, 1 = prompt; *slices of the keys; *needed = the bytes of workspace that these slices take (as many as workspace_bytes holds). */
+int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
+                          int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *slices, int64_t *needed);
+
+/* ---------------------------------------------------------------------------
  * Layout converters (device side).
  * GPTQ layout (reference PTQ/quant/quant_linear.py:343-389): qweight is
  * int32[K/8, N] with code(k, n) at bits 4*(k%8) of word [k/8, n].

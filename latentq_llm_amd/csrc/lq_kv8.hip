@@ -1,0 +1,502 @@
+// Appending keys and values to the paged 8-bit cache, with the position rotation on the way, and reading blocks back.
+//
+//   k'  = rotate(k, p):  of the first rot dimensions, halves (a, b) -> (a cos_p - b sin_p, b cos_p + a sin_p), in fp32
+//   s'  = max(s, max(A, 2^-90) / 127),  A = the largest finite |x| of the block's new tokens, s = 0 in a block that opens
+//   old codes c -> rint(c * (s / s')) where the scale grows,  new ones clamp(rint(x * (1 / s')), -127, 127), NaN -> 0
+//
+// One workgroup owns a (block, head) of the keys or of the values, so nothing is shared and nothing depends on an order: the new
+// tokens' values stay in registers between the maximum and the rounding, and a block's old codes are touched only when its scale
+// grows. The rotation of the queries needs no maximum and is spread over workgroups of the same launch.
+#include "lq_kv8.h"
+
+namespace {
+
+constexpr float kLeast = 0x1p-90f;  // so that scales, their reciprocals and their logarithms are all normal numbers
+
+struct Append {
+    const void *k, *v, *q;
+    void *q_out;
+    const float *cos, *sin;
+    uint8_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;
+    const int *table, *lens, *cu;
+    int64_t k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;  // strides in elements
+    int positions, rot, blocks, width, batch, tokens, heads, kv_heads, per_seq;
+};
+
+// Largest finite magnitude, NaN and infinities left out
+__device__ __forceinline__ float most_of(float most, float x) {
+    const float m = fabsf(x);
+    return m <= 3.402823466e38f ? fmaxf(most, m) : most;
+}
+
+__device__ __forceinline__ unsigned code(float x, float r) {
+    const float y = x * r;
+    return (unsigned)(int)((y == y ? __builtin_amdgcn_fmed3f(rintf(y), -127.0f, 127.0f) : 0.0f) + 128.0f);
+}
+
+__device__ __forceinline__ unsigned code_again(unsigned u, float ratio) {
+    return (unsigned)(int)(rintf((float)((int)u - 128) * ratio) + 128.0f);
+}
+
+__device__ __forceinline__ unsigned word_again(unsigned w, float ratio) {
+    unsigned o = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o |= code_again((w >> (8 * j)) & 0xFFu, ratio) << (8 * j);
+    return o;
+}
+
+template <int kThreads>
+__device__ __forceinline__ float block_max(float m) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if constexpr (kThreads > 64) {
+        __shared__ float part[kThreads / 64];
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = part[0];
+#pragma unroll
+        for (int i = 1; i < kThreads / 64; ++i) m = fmaxf(m, part[i]);
+    }
+    return m;
+}
+
+// A pair of 8-element pieces of one token's head, `pair` of dim / 16: the two pieces that the rotation combines, or, beyond the
+// rotated dimensions, two that follow each other.
+__device__ __forceinline__ void pieces(int pair, int rot, int &c0, int &c1) {
+    const int r = rot >> 4;
+    c0 = pair < r ? pair : 2 * pair;
+    c1 = pair < r ? pair + r : 2 * pair + 1;
+}
+
+template <bool kF16>
+__device__ __forceinline__ void load_rotated(const Append &a, const uint16_t *row, int pair, int pos, float x[16], int &c0, int &c1) {
+    pieces(pair, a.rot, c0, c1);
+    kv8_load8<kF16>(*(const u32x4_t *)(row + 8 * c0), x);
+    kv8_load8<kF16>(*(const u32x4_t *)(row + 8 * c1), x + 8);
+    if (pair < (a.rot >> 4)) {
+        const int64_t at = (int64_t)min(max(pos, 0), a.positions - 1) * (a.rot >> 1) + 8 * pair;
+        float c[8], s[8];
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            *(f32x4_t *)(c + i) = *(const f32x4_t *)(a.cos + at + i);
+            *(f32x4_t *)(s + i) = *(const f32x4_t *)(a.sin + at + i);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float lo = x[i], hi = x[8 + i];
+            x[i] = lo * c[i] - hi * s[i];
+            x[8 + i] = hi * c[i] + lo * s[i];
+        }
+    }
+}
+
+template <bool kF16>
+__device__ __forceinline__ u32x4_t pack8(const float x[8]) {
+    return u32x4_t{kv8_pack<kF16>(x[0], x[1]), kv8_pack<kF16>(x[2], x[3]), kv8_pack<kF16>(x[4], x[5]), kv8_pack<kF16>(x[6], x[7])};
+}
+
+// kThreads 256: a whole block of new tokens at once; 64: at most kFew of them (decoding)
+constexpr int kFew = 8;
+
+template <int D, int kThreads, bool kF16>
+__global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
+    const int seq = blockIdx.x / a.per_seq, jb = blockIdx.x % a.per_seq, role = blockIdx.y, tid = threadIdx.x;
+    int start, n;
+    kv8_span(a.cu, a.batch, a.tokens, seq, start, n);
+    if (n == 0) return;
+    const int len = max(a.lens[seq], 0), first = len - n;
+    const int place = max(first, 0) / KV8_BLOCK + jb;  // which block of the sequence
+    const int begin = place * KV8_BLOCK, hi = min(len, begin + KV8_BLOCK);
+    const int64_t row0 = (int64_t)start - first;  // row of the operands that position 0 would have
+
+    if (role >= 2 * a.kv_heads) {  // queries of one head: positions of this block, and with its first block any before position 0
+        const int h = role - 2 * a.kv_heads, from = jb ? begin : first, count = hi - from;
+        const uint16_t *src = (const uint16_t *)a.q + h * a.q_head;
+        uint16_t *dst = (uint16_t *)a.q_out + h * a.qo_head;
+        for (int item = tid; item < count * (D / 16); item += kThreads) {
+            const int pos = from + item / (D / 16);
+            float x[16];
+            int c0, c1;
+            load_rotated<kF16>(a, src + (row0 + pos) * a.q_token, item % (D / 16), pos, x, c0, c1);
+            uint16_t *o = dst + (row0 + pos) * a.qo_token;
+            *(u32x4_t *)(o + 8 * c0) = pack8<kF16>(x);
+            *(u32x4_t *)(o + 8 * c1) = pack8<kF16>(x + 8);
+        }
+        return;
+    }
+
+    const int lo = max(first, begin), count = hi - lo;
+    if (count <= 0 || place >= a.width) return;
+    const int block = a.table[(int64_t)seq * a.width + place];
+    if (block < 0 || block >= a.blocks) return;
+    const bool keys = role < a.kv_heads;
+    const int h = keys ? role : role - a.kv_heads;
+    const int64_t bh = (int64_t)block * a.kv_heads + h;
+    float *scale_at = (keys ? a.k_scale : a.v_scale) + bh;
+    const int kept = lo - begin;  // tokens that the block holds already
+    const float held = kept ? *scale_at : 0.0f;
+
+    if (keys) {
+        constexpr int kPairs = D / 16, kItems = ((kThreads == 64 ? kFew : KV8_BLOCK) * kPairs + kThreads - 1) / kThreads;
+        const uint16_t *src = (const uint16_t *)a.k + h * a.k_head;
+        float x[kItems][16], most = 0.0f;
+        int c0[kItems], c1[kItems];
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+            const int item = tid + it * kThreads, t = item / kPairs;
+            if (t < count) {
+                load_rotated<kF16>(a, src + (row0 + lo + t) * a.k_token, item % kPairs, lo + t, x[it], c0[it], c1[it]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = most_of(most, x[it][i]);
+            }
+        }
+        most = block_max<kThreads>(most);
+        const float scale = fmaxf(held, fmaxf(most, kLeast) * (1.0f / 127.0f)), r = 1.0f / scale;
+        if (tid == 0) *scale_at = scale;
+        uint8_t *codes = a.k_codes + bh * (KV8_BLOCK * D);
+        if (kept && scale > held) {
+            const float ratio = held / scale;
+            for (int i = tid; i < kept * (D / 4); i += kThreads) ((unsigned *)codes)[i] = word_again(((unsigned *)codes)[i], ratio);
+        }
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+            const int t = (tid + it * kThreads) / kPairs;
+            if (t < count) {
+                unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i >> 2] |= code(x[it][i], r) << (8 * (i & 3));
+                uint8_t *o = codes + (kept + t) * D;
+                *(u32x2_t *)(o + 8 * c0[it]) = u32x2_t{w[0], w[1]};
+                *(u32x2_t *)(o + 8 * c1[it]) = u32x2_t{w[2], w[3]};
+            }
+        }
+    } else {
+        // an item: 4 tokens of a group, 8 dimensions, so that its words are whole
+        constexpr int kPieces = D / 8, kGroups = kThreads == 64 ? (kFew + 6) / 4 : KV8_BLOCK / 4;
+        constexpr int kItems = (kGroups * kPieces + kThreads - 1) / kThreads;
+        const uint16_t *src = (const uint16_t *)a.v + h * a.v_head;
+        const int group0 = kept >> 2, end = kept + count;  // slots kept .. end - 1 are new
+        float x[kItems][4][8], most = 0.0f;
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+            const int item = tid + it * kThreads, g = group0 + item / kPieces, piece = item % kPieces;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int slot = 4 * g + j;
+                if (slot >= kept && slot < end) {
+                    kv8_load8<kF16>(*(const u32x4_t *)(src + (row0 + begin + slot) * a.v_token + 8 * piece), x[it][j]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) most = most_of(most, x[it][j][i]);
+                }
+            }
+        }
+        most = block_max<kThreads>(most);
+        const float scale = fmaxf(held, fmaxf(most, kLeast) * (1.0f / 127.0f)), r = 1.0f / scale;
+        if (tid == 0) *scale_at = scale;
+        const bool grows = kept && scale > held;
+        const float ratio = held / scale;
+        uint8_t *codes = a.v_codes + bh * (KV8_BLOCK * D);
+        if (grows)
+            for (int i = tid; i < group0 * D; i += kThreads) ((unsigned *)codes)[i] = word_again(((unsigned *)codes)[i], ratio);
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+            const int item = tid + it * kThreads, g = group0 + item / kPieces, piece = item % kPieces;
+            if (4 * g < end) {
+                unsigned *o = (unsigned *)codes + g * D + 8 * piece;
+                const bool part = 4 * g < kept || 4 * g + 4 > end;  // slots of the group that are not new
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    u32x4_t w = {0, 0, 0, 0};
+                    if (part) w = *(const u32x4_t *)(o + i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int slot = 4 * g + j, at = 8 * j;
+                        const bool fresh = slot >= kept && slot < end;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            const unsigned was = (w[d] >> at) & 0xFFu;
+                            const unsigned now = fresh ? code(x[it][j][i + d], r) : grows && slot < kept ? code_again(was, ratio) : was;
+                            w[d] = (w[d] & ~(0xFFu << at)) | (now << at);
+                        }
+                    }
+                    *(u32x4_t *)(o + i) = w;
+                }
+            }
+        }
+    }
+}
+
+// ---- reading back ----------------------------------------------------------
+// kOut 0: bf16, 1: f16, 2: f32
+template <int kOut>
+__device__ __forceinline__ void store4(void *out, int64_t at, const float f[4]) {
+    if constexpr (kOut == 2)
+        *(f32x4_t *)((float *)out + at) = f32x4_t{f[0], f[1], f[2], f[3]};
+    else
+        *(u32x2_t *)((uint16_t *)out + at) = u32x2_t{kv8_pack<kOut == 1>(f[0], f[1]), kv8_pack<kOut == 1>(f[2], f[3])};
+}
+
+template <int D, int kOut>
+__global__ __launch_bounds__(256) void read_kernel(const uint8_t *k_codes, const uint8_t *v_codes, const float *k_scale, const float *v_scale,
+                                                   const int *blocks, void *k_out, void *v_out, int kv_heads, int pool) {
+    const int h = blockIdx.x % kv_heads, at = blockIdx.x / kv_heads, block = blocks[at];
+    const bool there = block >= 0 && block < pool;
+    const int64_t bh = (int64_t)(there ? block : 0) * kv_heads + h;
+    const float ks = there ? k_scale[bh] : 0.0f, vs = there ? v_scale[bh] : 0.0f;
+    const u32x4_t *k = (const u32x4_t *)(k_codes + bh * (KV8_BLOCK * D)), *v = (const u32x4_t *)(v_codes + bh * (KV8_BLOCK * D));
+    const int64_t out0 = ((int64_t)at * KV8_BLOCK * kv_heads + h) * D, step = (int64_t)kv_heads * D;
+    for (int i = threadIdx.x; i < KV8_BLOCK * D / 16; i += 256) {
+        const u32x4_t kw = k[i], vw = v[i];
+        const int t = i / (D / 16), d = i % (D / 16) * 16;   // keys: 16 dimensions of a token
+        const int g = i / (D / 4), e = i % (D / 4) * 4;      // values: 4 tokens of 4 dimensions
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[4], w[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                f[b] = there ? (float)((int)((kw[j] >> (8 * b)) & 0xFFu) - 128) * ks : 0.0f;
+                w[b] = there ? (float)((int)((vw[b] >> (8 * j)) & 0xFFu) - 128) * vs : 0.0f;
+                // a product is an fp32 number before it is rounded to its type (left alone, some would go to f16 in one instruction)
+                asm("" : "+v"(f[b]), "+v"(w[b]));
+            }
+            store4<kOut>(k_out, out0 + t * step + d + 4 * j, f);
+            store4<kOut>(v_out, out0 + (4 * g + j) * step + e, w);
+        }
+    }
+}
+
+template <int D>
+void launch_append(const Append &a, bool few, bool f16, dim3 grid, hipStream_t s) {
+    if (few) {
+        if (f16) append_kernel<D, 64, true><<<grid, 64, 0, s>>>(a);
+        else append_kernel<D, 64, false><<<grid, 64, 0, s>>>(a);
+    } else {
+        if (f16) append_kernel<D, 256, true><<<grid, 256, 0, s>>>(a);
+        else append_kernel<D, 256, false><<<grid, 256, 0, s>>>(a);
+    }
+}
+
+template <int D>
+void launch_read(const void *k_codes, const void *v_codes, const float *k_scale, const float *v_scale, const int *blocks, void *k_out,
+                 void *v_out, int64_t n, int kv_heads, int pool, int type, hipStream_t s) {
+    const dim3 grid((unsigned)(n * kv_heads));
+    const uint8_t *k = (const uint8_t *)k_codes, *v = (const uint8_t *)v_codes;
+    if (type == 0) read_kernel<D, 0><<<grid, 256, 0, s>>>(k, v, k_scale, v_scale, blocks, k_out, v_out, kv_heads, pool);
+    else if (type == 1) read_kernel<D, 1><<<grid, 256, 0, s>>>(k, v, k_scale, v_scale, blocks, k_out, v_out, kv_heads, pool);
+    else read_kernel<D, 2><<<grid, 256, 0, s>>>(k, v, k_scale, v_scale, blocks, k_out, v_out, kv_heads, pool);
+}
+
+// ---- attention: slices joined ----------------------------------------------
+// out = sum_i 2^(lse_i - m) o_i / sum_i 2^(lse_i - m): a slice without a visible key has lse -inf and is not read.
+template <int D, bool kF16>
+__global__ __launch_bounds__(256) void join_kernel(const Kv8Attn a) {
+    constexpr int kUnits = D / 4, kRows = 256 / kUnits;
+    const int64_t rows = (int64_t)a.tokens * a.heads, row = (int64_t)blockIdx.x * kRows + threadIdx.x / kUnits;
+    const int d = threadIdx.x % kUnits * 4;
+    if (threadIdx.x >= kRows * kUnits || row >= rows) return;
+    float m = -__builtin_inff();
+    bool nan = false;
+    for (int i = 0; i < a.slices; ++i) {
+        const float l = a.part_lse[i * rows + row];
+        nan |= l != l;
+        m = fmaxf(m, l);
+    }
+    f32x4_t o = {0, 0, 0, 0};
+    float total = 0.0f;
+    if (m > -__builtin_inff() || nan) {
+        for (int i = 0; i < a.slices; ++i) {
+            const float l = a.part_lse[i * rows + row];
+            if (l == -__builtin_inff()) continue;
+            const float w = __builtin_amdgcn_exp2f(l - m);
+            total += w;
+            const f32x4_t p = *(const f32x4_t *)(a.part + (i * rows + row) * D + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(w, p[j], o[j]);
+        }
+        const float r = 1.0f / total;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] *= r;
+    }
+    const int64_t token = row / a.heads, head = row % a.heads;
+    *(u32x2_t *)((uint16_t *)a.out + token * a.o_token + head * a.o_head + d) = u32x2_t{kv8_pack<kF16>(o[0], o[1]), kv8_pack<kF16>(o[2], o[3])};
+    if (a.lse && d == 0) a.lse[row] = nan ? __builtin_nanf("") : (m + __builtin_amdgcn_logf(total)) * 0.693147180559945f;
+}
+
+template <int D>
+void launch_join(const Kv8Attn &a, bool f16, hipStream_t s) {
+    constexpr int kRows = 256 / (D / 4);
+    const dim3 grid((unsigned)(((int64_t)a.tokens * a.heads + kRows - 1) / kRows));
+    if (f16) join_kernel<D, true><<<grid, 256, 0, s>>>(a);
+    else join_kernel<D, false><<<grid, 256, 0, s>>>(a);
+}
+
+bool good_dim(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 256; }
+
+// How a call is cut: rows of a (sequence, kv head) that go to the kernel of few rows, and slices of the keys.
+struct Plan {
+    bool few;
+    int slices, tiles, row_tiles;
+};
+
+// Most rows of the kernel for few: beyond it the prompt kernel (its tiles of 128 rows)
+int most_rows(int dim) { return dim <= 128 ? 64 : 32; }
+
+Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t workspace, int cus) {
+    Plan p;
+    const int64_t rows = max_tokens * (heads / kv_heads);
+    p.few = rows <= most_rows(dim);
+    p.row_tiles = p.few ? 1 : (int)((rows + 127) / 128);
+    int64_t keys = max_len;
+    if (window && window + max_tokens + KV8_BLOCK < keys) keys = window + max_tokens + KV8_BLOCK;
+    const int64_t tiles = keys > 0 ? (keys + KV8_BLOCK - 1) / KV8_BLOCK : 1;
+    const int64_t units = batch * kv_heads * p.row_tiles;
+    const int64_t want = p.few ? 4 * (int64_t)cus : 2 * (int64_t)cus, least = p.few ? 4 : 8;  // workgroups, tiles of a slice
+    int64_t slices = units >= want ? 1 : (want + units - 1) / units;
+    const int64_t slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;
+    if (slices > 64) slices = 64;
+    if (slices > 1 && slice_bytes > 0 && slices > workspace / slice_bytes) slices = workspace / slice_bytes;
+    if (slices < 1) slices = 1;
+    int64_t per = (tiles + slices - 1) / slices;
+    if (per < least) per = least;
+    p.slices = (int)((tiles + per - 1) / per);
+    p.tiles = (int)per;
+    return p;
+}
+
+}  // namespace
+
+extern "C" int lq_kv8_append(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                             int64_t v_head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride, void *q_out,
+                             int64_t q_out_token_stride, int64_t q_out_head_stride, const float *cos_table, const float *sin_table,
+                             int64_t positions, int rot_dim, void *k_codes, void *v_codes, float *k_scale, float *v_scale,
+                             int64_t num_blocks, const int32_t *block_table, int64_t table_width, const int32_t *seq_lens,
+                             const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens, int heads, int kv_heads, int dim,
+                             int dtype, void *stream) {
+    LQ_REQUIRE(batch >= 0 && tokens >= 0 && max_tokens >= 0, "kv8_append: sizes must not be negative");
+    LQ_REQUIRE(good_dim(dim), "kv8_append: head dimension must be 64, 96, 128 or 256, got %d", dim);
+    LQ_REQUIRE(dtype == 0 || dtype == 1, "kv8_append: dtype must be 0 (bf16) or 1 (f16), got %d", dtype);
+    LQ_REQUIRE(kv_heads > 0 && heads >= 0, "kv8_append: needs at least one kv head");
+    if (batch == 0 || tokens == 0 || max_tokens == 0) return LQ_OK;
+    LQ_REQUIRE(k && v && k_codes && v_codes && k_scale && v_scale && block_table && seq_lens, "kv8_append: null pointer");
+    LQ_REQUIRE(!q == !q_out, "kv8_append: q and q_out go together");
+    LQ_REQUIRE(!cos_table == !sin_table, "kv8_append: cos and sin go together");
+    LQ_REQUIRE(!q || cos_table, "kv8_append: q is taken to be rotated: it needs cos and sin");
+    LQ_REQUIRE(!cos_table || (rot_dim > 0 && rot_dim <= dim && rot_dim % 16 == 0), "kv8_append: rotated dimensions must be a multiple of 16 up to %d, got %d", dim, rot_dim);
+    LQ_REQUIRE(!cos_table || (positions > 0 && positions <= INT32_MAX), "kv8_append: the rotation tables need at least one position");
+    LQ_REQUIRE(num_blocks > 0 && num_blocks <= INT32_MAX && table_width > 0 && table_width <= INT32_MAX / KV8_BLOCK,
+               "kv8_append: a pool of blocks and a block table of 1 to %d columns are needed", INT32_MAX / KV8_BLOCK);
+    LQ_REQUIRE(tokens <= INT32_MAX && batch <= INT32_MAX, "kv8_append: too many tokens or sequences");
+    LQ_REQUIRE(cu_tokens || tokens % batch == 0, "kv8_append: without cu_tokens every sequence has the same number of tokens: %lld do not divide by %lld",
+               (long long)tokens, (long long)batch);
+    LQ_REQUIRE((!q || heads > 0) && 2 * (int64_t)kv_heads + (q ? heads : 0) <= 65535, "kv8_append: too many heads");
+    for (int64_t s : {k_token_stride, k_head_stride, v_token_stride, v_head_stride, q ? q_token_stride : 0, q ? q_head_stride : 0, q ? q_out_token_stride : 0,
+                      q ? q_out_head_stride : 0})
+        LQ_REQUIRE(s >= 0 && s % 8 == 0, "kv8_append: strides must be multiples of 8 elements, got %lld", (long long)s);
+    for (const void *p : {k, v, q, (const void *)q_out, (const void *)cos_table, (const void *)sin_table, (const void *)k_codes, (const void *)v_codes})
+        LQ_REQUIRE(lq_aligned(p, 16), "kv8_append: k, v, q, the tables and the codes must be 16-byte aligned");
+    Append a{k, v, q, q_out, cos_table, sin_table, (uint8_t *)k_codes, (uint8_t *)v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens,
+             k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride,
+             (int)positions, cos_table ? rot_dim : 0, (int)num_blocks, (int)table_width, (int)batch, (int)tokens, heads, kv_heads, 0};
+    if (max_tokens > tokens) max_tokens = tokens;
+    const int64_t per = (max_tokens + KV8_BLOCK - 2) / KV8_BLOCK + 1;
+    LQ_REQUIRE(per * batch <= INT32_MAX, "kv8_append: too many tokens or sequences");
+    a.per_seq = (int)per;
+    const dim3 grid((unsigned)(per * batch), (unsigned)(2 * kv_heads + (q ? heads : 0)));
+    const bool few = max_tokens <= kFew;
+    hipStream_t s = (hipStream_t)stream;
+    if (dim == 64) launch_append<64>(a, few, dtype == 1, grid, s);
+    else if (dim == 96) launch_append<96>(a, few, dtype == 1, grid, s);
+    else if (dim == 128) launch_append<128>(a, few, dtype == 1, grid, s);
+    else launch_append<256>(a, few, dtype == 1, grid, s);
+    return lq_check_launch("kv8_append");
+}
+
+extern "C" int lq_kv8_read(const void *k_codes, const void *v_codes, const float *k_scale, const float *v_scale, int64_t num_blocks,
+                           const int32_t *blocks, int64_t n, int kv_heads, int dim, int dtype, void *k_out, void *v_out, void *stream) {
+    LQ_REQUIRE(n >= 0, "kv8_read: the number of blocks must not be negative");
+    LQ_REQUIRE(good_dim(dim), "kv8_read: head dimension must be 64, 96, 128 or 256, got %d", dim);
+    LQ_REQUIRE(dtype >= 0 && dtype <= 2, "kv8_read: dtype must be 0 (bf16), 1 (f16) or 2 (f32), got %d", dtype);
+    LQ_REQUIRE(kv_heads > 0, "kv8_read: needs at least one kv head");
+    if (n == 0) return LQ_OK;
+    LQ_REQUIRE(k_codes && v_codes && k_scale && v_scale && blocks && k_out && v_out, "kv8_read: null pointer");
+    LQ_REQUIRE(num_blocks > 0 && num_blocks <= INT32_MAX, "kv8_read: a pool of blocks is needed");
+    LQ_REQUIRE(n * kv_heads <= INT32_MAX, "kv8_read: too many blocks");
+    for (const void *p : {k_codes, v_codes, (const void *)k_out, (const void *)v_out})
+        LQ_REQUIRE(lq_aligned(p, 16), "kv8_read: codes and outputs must be 16-byte aligned");
+    hipStream_t s = (hipStream_t)stream;
+    if (dim == 64) launch_read<64>(k_codes, v_codes, k_scale, v_scale, blocks, k_out, v_out, n, kv_heads, (int)num_blocks, dtype, s);
+    else if (dim == 96) launch_read<96>(k_codes, v_codes, k_scale, v_scale, blocks, k_out, v_out, n, kv_heads, (int)num_blocks, dtype, s);
+    else if (dim == 128) launch_read<128>(k_codes, v_codes, k_scale, v_scale, blocks, k_out, v_out, n, kv_heads, (int)num_blocks, dtype, s);
+    else launch_read<256>(k_codes, v_codes, k_scale, v_scale, blocks, k_out, v_out, n, kv_heads, (int)num_blocks, dtype, s);
+    return lq_check_launch("kv8_read");
+}
+
+namespace {
+int attention_sizes(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window) {
+    LQ_REQUIRE(batch >= 0 && tokens >= 0 && max_tokens >= 0 && max_len >= 0, "kv8_attention: sizes must not be negative");
+    LQ_REQUIRE(good_dim(dim), "kv8_attention: head dimension must be 64, 96, 128 or 256, got %d", dim);
+    LQ_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "kv8_attention: heads must be a multiple of kv heads, got %d and %d", heads, kv_heads);
+    LQ_REQUIRE(window >= 0, "kv8_attention: the window must not be negative");
+    LQ_REQUIRE(tokens * heads <= INT32_MAX && batch * kv_heads <= INT32_MAX, "kv8_attention: too many tokens or sequences");
+    return LQ_OK;
+}
+}  // namespace
+
+extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
+                                     int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *slices, int64_t *needed) {
+    if (const int rc = attention_sizes(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window)) return rc;
+    LQ_REQUIRE(kernel && slices && needed, "kv8_attention_plan: null pointer");
+    if (max_tokens > tokens) max_tokens = tokens;
+    const Plan p = batch && tokens && max_tokens
+                       ? plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, workspace_bytes, compute_units > 0 ? compute_units : lq_device_cu_count())
+                       : Plan{true, 1, 0, 0};
+    *kernel = p.few ? 0 : 1;
+    *slices = p.slices;
+    *needed = p.slices > 1 ? (int64_t)p.slices * tokens * heads * (dim + 1) * 4 : 0;
+    return LQ_OK;
+}
+
+extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes,
+                                const float *k_scale, const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width,
+                                const int32_t *seq_lens, const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens,
+                                int64_t max_len, int heads, int kv_heads, int dim, int dtype, float scale, int causal, int64_t window, void *out,
+                                int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
+    if (const int rc = attention_sizes(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window)) return rc;
+    LQ_REQUIRE(dtype == 0 || dtype == 1, "kv8_attention: dtype must be 0 (bf16) or 1 (f16), got %d", dtype);
+    LQ_REQUIRE(scale > 0.0f && scale <= 3.402823466e38f, "kv8_attention: the scale of the scores must be positive and finite");
+    if (batch == 0 || tokens == 0) return LQ_OK;
+    LQ_REQUIRE(max_tokens > 0, "kv8_attention: max_tokens must be the largest number of tokens of a sequence, got 0");
+    LQ_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && block_table && seq_lens && out, "kv8_attention: null pointer");
+    LQ_REQUIRE(num_blocks > 0 && num_blocks <= INT32_MAX && table_width > 0 && table_width <= INT32_MAX / KV8_BLOCK,
+               "kv8_attention: a pool of blocks and a block table of 1 to %d columns are needed", INT32_MAX / KV8_BLOCK);
+    LQ_REQUIRE(cu_tokens || tokens % batch == 0, "kv8_attention: without cu_tokens every sequence has the same number of tokens: %lld do not divide by %lld",
+               (long long)tokens, (long long)batch);
+    for (int64_t s : {q_token_stride, q_head_stride, out_token_stride, out_head_stride})
+        LQ_REQUIRE(s >= 0 && s % 8 == 0, "kv8_attention: strides must be multiples of 8 elements, got %lld", (long long)s);
+    for (const void *p : {q, k_codes, v_codes, (const void *)out, (const void *)workspace})
+        LQ_REQUIRE(lq_aligned(p, 16), "kv8_attention: q, codes, output and workspace must be 16-byte aligned");
+    LQ_REQUIRE(workspace_bytes >= 0, "kv8_attention: the workspace's size must not be negative");
+    if (max_tokens > tokens) max_tokens = tokens;
+    if (max_len > table_width * KV8_BLOCK) max_len = table_width * KV8_BLOCK;
+    const Plan p = plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, workspace ? workspace_bytes : 0, lq_device_cu_count());
+    Kv8Attn a{};
+    a.q = q; a.k = (const uint8_t *)k_codes; a.v = (const uint8_t *)v_codes; a.ks = k_scale; a.vs = v_scale;
+    a.table = block_table; a.lens = seq_lens; a.cu = cu_tokens; a.out = out; a.lse = lse;
+    a.part = (float *)workspace;
+    a.part_lse = a.part + (int64_t)p.slices * tokens * heads * dim;
+    a.q_token = q_token_stride; a.q_head = q_head_stride; a.o_token = out_token_stride; a.o_head = out_head_stride;
+    a.window = window; a.scale = scale * 1.442695040888963f;
+    a.blocks = (int)num_blocks; a.width = (int)table_width; a.batch = (int)batch; a.tokens = (int)tokens; a.heads = heads; a.kv_heads = kv_heads;
+    a.causal = causal != 0; a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles;
+    LQ_REQUIRE((int64_t)p.slices * batch * kv_heads * p.row_tiles <= INT32_MAX, "kv8_attention: too many tokens or sequences");
+    const int64_t rows = max_tokens * (heads / kv_heads);
+    const int rc = p.few ? kv8_launch_few(a, (int)rows, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
+    if (rc != LQ_OK || p.slices == 1) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (dim == 64) launch_join<64>(a, dtype == 1, s);
+    else if (dim == 96) launch_join<96>(a, dtype == 1, s);
+    else if (dim == 128) launch_join<128>(a, dtype == 1, s);
+    else launch_join<256>(a, dtype == 1, s);
+    return lq_check_launch("kv8_attention (join)");
+}

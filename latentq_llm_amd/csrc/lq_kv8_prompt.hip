@@ -1,0 +1,248 @@
+// Attention of many rows over the paged 8-bit cache (lq_kv8.h): prompts, and pieces of prompts. A workgroup takes 128 rows
+// (tokens times the query heads of a kv head), 32 to a wave, and goes over tiles of 64 keys; the arithmetic is that of
+// lq_kv8_few.hip on 32x32x16 f16 matrix instructions.
+//
+// The codes of a tile become halves once for all waves: requested a tile ahead into registers, converted on their way into
+// shared memory, two buffers, one barrier a tile. Keys lie there by rows with their 16-byte pieces exchanged by the row
+// number (a wave reads 32 rows at one piece), values as finished operands.
+#include "lq_kv8.h"
+
+namespace {
+
+constexpr float kNone = -3e38f;
+
+template <int D, bool kF16>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
+    constexpr int kSteps = D / 16, kTiles = D / 32, kPieces = D / 8;
+    constexpr int kRows = 128;
+    // per buffer: keys [64][D] halves, values [8 halves of steps][D][8]
+    __shared__ u32x4_t lds_k[2][KV8_BLOCK * kPieces], lds_v[2][8 * D];
+
+    const int units = a.batch * a.kv_heads;
+    const int unit = blockIdx.x % units, rest = blockIdx.x / units;
+    const int slice = rest % a.slices, tile = a.row_tiles - 1 - rest / a.slices;  // the last rows see most keys: first
+    const int seq = unit / a.kv_heads, h = unit % a.kv_heads;
+    const Kv8Rows s = kv8_rows(a, seq);
+    const int group = a.heads / a.kv_heads;
+    const int64_t all_rows = (int64_t)s.n * group;
+    const int row0 = tile * kRows;
+    if (row0 >= all_rows) return;
+    const int rows = (int)min((int64_t)kRows, all_rows - row0);
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int pos_first = s.first + row0 / group, pos_last = s.first + (row0 + rows - 1) / group;
+    const int seen = a.causal ? min(pos_last + 1, s.len) : s.len;  // keys before this are seen by some row
+    int64_t lo64 = a.window ? (int64_t)pos_first - a.window + 1 : 0;
+    const int t_first = (int)(lo64 > 0 ? min(lo64, (int64_t)max(seen, 0)) : 0) / KV8_BLOCK, t_last = (max(seen, 0) + KV8_BLOCK - 1) / KV8_BLOCK;
+    const int t_lo = t_first + slice * a.tiles, t_hi = slice == a.slices - 1 ? t_last : min(t_last, t_lo + a.tiles);
+
+    // this lane's row
+    const int r = wave * 32 + col, row = row0 + r, token = row / group, head = h * group + row % group;
+    const bool there = r < rows;
+    const int pos = s.first + token;
+    const int last = !there ? -1 : a.causal ? min(pos, s.len - 1) : s.len - 1;
+    const int before = a.window ? (int)max((int64_t)pos - a.window, (int64_t)-1) : -1;
+    // tiles that some row of this wave sees
+    const int wave_last = wave * 32 >= rows ? -1 : a.causal ? min(s.first + (row0 + min(wave * 32 + 31, rows - 1)) / group, s.len - 1) : s.len - 1;
+    const int64_t wave_before = a.window ? (int64_t)s.first + (row0 + wave * 32) / group - a.window : -1;
+
+    f16x8_t q[kSteps];
+    float factor;
+    {
+        const uint16_t *src = (const uint16_t *)a.q + (int64_t)(s.start + (there ? token : 0)) * a.q_token + (int64_t)(there ? head : 0) * a.q_head;
+        u32x4_t w[kSteps];
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float f[8];
+            w[i] = *(const u32x4_t *)(src + 16 * i + 8 * half);
+            kv8_load8<kF16>(w[i], f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(f[j]));
+        }
+        most = fmaxf(most, __shfl_xor(most, 32));
+        float to, back;
+        kv8_row_power(most, to, back);
+        factor = back * a.scale;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            float f[8];
+            kv8_load8<kF16>(w[i], f);
+            u32x4_t x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = kv8_pack_f16(f[2 * j] * to, f[2 * j + 1] * to);
+            q[i] = __builtin_bit_cast(f16x8_t, x);
+        }
+    }
+
+    f32x16_t o[kTiles];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
+    float M = kNone, L = 0.0f;
+
+    const int *table = a.table + (int64_t)seq * a.width;
+    const auto block_of = [&](int t) { return (int64_t)min((unsigned)table[t], (unsigned)(a.blocks - 1)) * a.kv_heads + h; };
+    // place of a key row's 16-byte piece: exchanged within 8 pieces by the row, within 4 where the last ones are only 4 (96 dimensions)
+    const auto placed = [](int piece, int row) { return piece ^ (row & (piece < (kPieces & ~7) ? 7 : 3)); };
+    // A thread's part of a tile: 16 bytes of keys (16 dimensions of a token) and of values (4 tokens of 4 dimensions) at a time
+    constexpr int kAll = KV8_BLOCK * D / 16, kN = (kAll + 255) / 256;
+    u32x4_t kr[kN], vr[kN];
+    const auto request = [&](int64_t bh) {
+        const u32x4_t *k = (const u32x4_t *)(a.k + bh * (KV8_BLOCK * D)), *v = (const u32x4_t *)(a.v + bh * (KV8_BLOCK * D));
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * 256;
+            if (kAll % 256 == 0 || u < kAll) {
+                kr[i] = k[u];
+                vr[i] = v[u];
+            }
+        }
+    };
+    const auto store = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int u = threadIdx.x + i * 256;
+            if (kAll % 256 == 0 || u < kAll) {
+                const int t = u / (D / 16), piece = u % (D / 16) * 2;
+                u32x4_t *row_at = lds_k[buffer] + t * kPieces;
+                row_at[placed(piece, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[i][0], kr[i][1]));
+                row_at[placed(piece + 1, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[i][2], kr[i][3]));
+                // 4-token group c belongs to step c / 4, half c & 1, first or second 4 tokens of the operand by bit 1
+                const int c = u / (D / 4), d = u % (D / 4) * 4;
+                u32x2_t *v_at = (u32x2_t *)(lds_v[buffer] + ((c >> 2) * 2 + (c & 1)) * D + d) + ((c >> 1) & 1);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v_at[2 * j] = kv8_halves(vr[i][j]);
+            }
+        }
+    };
+
+    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    int64_t bh_next = 0;
+    if (t_lo < t_hi) {
+        bh_next = block_of(t_lo);
+        request(bh_next);
+        ks_next = a.ks[bh_next];
+        vs_next = a.vs[bh_next];
+        store(0);
+        ks = ks_next;
+        vs = vs_next;
+    }
+    __syncthreads();
+    for (int t = t_lo; t < t_hi; ++t) {
+        const int buffer = (t - t_lo) & 1;
+        if (t + 1 < t_hi) {
+            bh_next = block_of(t + 1);
+            request(bh_next);
+            ks_next = a.ks[bh_next];
+            vs_next = a.vs[bh_next];
+        }
+        const int key0 = t * KV8_BLOCK;
+        if (key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before) {
+            f32x16_t c[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) c[x][j] = 0.0f;
+                const int at = x * 32 + col;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const f16x8_t k = __builtin_bit_cast(f16x8_t, lds_k[buffer][at * kPieces + placed(2 * i + half, at)]);
+                    c[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], c[x], 0, 0, 0);
+                }
+            }
+            // accumulator element j is key 32 x + (j & 3) + 8 (j >> 2) + 4 half
+            if (__any(key0 + KV8_BLOCK - 1 > last || key0 <= before)) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int key = key0 + 32 * x + (j & 3) + 8 * (j >> 2) + 4 * half;
+                        if (key > last || key <= before) c[x][j] = -__builtin_inff();
+                    }
+            }
+            const float f = fmaxf(ks * factor, 0x1p-100f), lv = __builtin_amdgcn_logf(vs), rv = 1.0f / vs;
+            float most = c[0][0];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) most = fmaxf(most, c[x][j]);
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float m = fmaxf(M, fmaf(most, f, lv)), shift = lv - m, fade = __builtin_amdgcn_exp2f(M - m);
+            if (__any(m > M)) {
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) o[i] *= fade;
+            }
+            M = m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    c[x][j] = __builtin_amdgcn_exp2f(fmaf(c[x][j], f, shift));
+                    sum += c[x][j];
+                }
+            L = fmaf(sum, rv, L * fade);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // 16 keys
+                u32x4_t w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = kv8_pack_f16(c[e >> 1][8 * (e & 1) + 2 * j], c[e >> 1][8 * (e & 1) + 2 * j + 1]);
+                const f16x8_t p = __builtin_bit_cast(f16x8_t, w);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    const f16x8_t v = __builtin_bit_cast(f16x8_t, lds_v[buffer][(2 * e + half) * D + 32 * i + col]);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[i], 0, 0, 0);
+                }
+            }
+        }
+        if (t + 1 < t_hi) {
+            store(buffer ^ 1);
+            ks = ks_next;
+            vs = vs_next;
+        }
+        __syncthreads();
+    }
+
+    if (!there) return;
+    L += __shfl_xor(L, 32);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const float lse = L == 0.0f ? -__builtin_inff() : M + __builtin_amdgcn_logf(L);
+    const int64_t all = (int64_t)a.tokens * a.heads, at = (int64_t)(s.start + token) * a.heads + head;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = 32 * i + 8 * b + 4 * half;
+            f32x4_t x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = o[i][4 * b + j] * inv;
+            if (a.slices == 1)
+                *(u32x2_t *)((uint16_t *)a.out + (int64_t)(s.start + token) * a.o_token + head * a.o_head + d) = u32x2_t{kv8_pack<kF16>(x[0], x[1]), kv8_pack<kF16>(x[2], x[3])};
+            else
+                *(f32x4_t *)(a.part + (slice * all + at) * D + d) = x;
+        }
+    if (half == 0) {
+        if (a.slices > 1) a.part_lse[slice * all + at] = lse;
+        else if (a.lse) a.lse[at] = lse * 0.693147180559945f;
+    }
+}
+
+template <int D>
+int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.slices * a.row_tiles));
+    if (f16) prompt_kernel<D, true><<<grid, 256, 0, s>>>(a);
+    else prompt_kernel<D, false><<<grid, 256, 0, s>>>(a);
+    return lq_check_launch("kv8_attention (prompt)");
+}
+
+}  // namespace
+
+int kv8_launch_prompt(const Kv8Attn &a, int dim, bool f16, void *stream) {
+    hipStream_t s = (hipStream_t)stream;
+    if (dim == 64) return launch<64>(a, f16, s);
+    if (dim == 96) return launch<96>(a, f16, s);
+    if (dim == 128) return launch<128>(a, f16, s);
+    return launch<256>(a, f16, s);
+}

@@ -951,3 +951,211 @@ def latent_w8_requant(latent, qscales, residual_int, k1, b1, k2, b2, k3):
         _C.call("lq_latent_w8_requant", latent.data_ptr(), qscales.data_ptr(), codes.data_ptr(), residual_int.data_ptr(), N, K,
                 int(k1), float(b1), int(k2), float(b2), int(k3), _stream(latent))
     return codes
+
+
+# ---- paged 8-bit cache of keys and values (include/latentq.h, lq_kv8_*) ----------------------------------------------
+KV_BLOCK = 64
+KV_DIMS = (64, 96, 128, 256)
+_KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _kv8_cache(k_codes, v_codes, k_scale, v_scale):
+    """(blocks, kv heads, dim) of a cache, checked."""
+    for t, dtype, name in ((k_codes, torch.uint8, "k_codes"), (v_codes, torch.uint8, "v_codes"), (k_scale, torch.float32, "k_scale"),
+                           (v_scale, torch.float32, "v_scale")):
+        _chk(t, dtype, name)
+        if t.device != k_codes.device:
+            raise ValueError(f"{name} must be on the device of k_codes")
+    if k_codes.dim() != 4 or k_codes.shape[2] != KV_BLOCK or k_codes.shape[3] not in KV_DIMS:
+        raise ValueError(f"k_codes must be [blocks, kv_heads, {KV_BLOCK}, dim] with dim one of {KV_DIMS}, got {tuple(k_codes.shape)}")
+    n, heads, _, dim = k_codes.shape
+    if tuple(v_codes.shape) != (n, heads, KV_BLOCK // 4, dim, 4):
+        raise ValueError(f"v_codes must be {(n, heads, KV_BLOCK // 4, dim, 4)}, got {tuple(v_codes.shape)}")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if tuple(t.shape) != (n, heads):
+            raise ValueError(f"{name} must be {(n, heads)}, got {tuple(t.shape)}")
+    if n == 0 or heads == 0:
+        raise ValueError("the cache needs at least one block and one kv head")
+    return n, heads, dim
+
+
+def _kv8_rows(t, name, heads, dim, like, dtype=None):
+    """Rows [tokens, heads, dim] of a 16-bit type with a contiguous last dimension and 16-byte aligned pieces."""
+    if not t.is_cuda:
+        raise _C.LatentQError(f"{name} must be a GPU tensor: the HIP kernels have no CPU fallback")
+    if t.dtype not in (torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name}: expected {dtype or 'bfloat16 or float16'}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on the device of the cache")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError(f"the operators of the 8-bit cache have no backward, and {name} requires a gradient")
+    return t
+
+
+def _kv8_in_form(t):
+    return t.stride(2) == 1 and all(t.stride(i) % 8 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0
+
+
+def _kv8_layout(t):
+    """t itself where the kernels take its strides, else a contiguous copy."""
+    return t if not t.numel() or _kv8_in_form(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _kv8_result(t, name, like):
+    """An output given by the caller: rows like `like`, none of them in another's place."""
+    _kv8_rows(t, name, like.shape[1], like.shape[2], like, like.dtype)
+    if t.shape != like.shape:
+        raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
+    if t.numel() and (not _kv8_in_form(t) or any(t.shape[i] > 1 and t.stride(i) < t.shape[2] for i in (0, 1))):
+        raise ValueError(f"{name} must have a contiguous last dimension and 16-byte aligned heads of their own")
+    return t
+
+
+def _kv8_sequences(block_table, seq_lens, cu_tokens, max_tokens, tokens, like):
+    """(batch, table width, max_tokens) of a call, checked."""
+    for t, name in ((block_table, "block_table"), (seq_lens, "seq_lens"), (cu_tokens, "cu_tokens")):
+        if t is not None:
+            _chk(t, torch.int32, name)
+            if t.device != like.device:
+                raise ValueError(f"{name} must be on the device of the cache")
+    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0]:
+        raise ValueError(f"block_table must be [batch, blocks of a sequence] and seq_lens [batch], got {tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
+    batch, width = block_table.shape
+    if cu_tokens is not None:
+        if tuple(cu_tokens.shape) != (batch + 1,):
+            raise ValueError(f"cu_tokens must be [{batch + 1}], got {tuple(cu_tokens.shape)}")
+        most = tokens
+    else:
+        if (tokens % batch if batch else tokens):
+            raise ValueError(f"without cu_tokens every sequence has the same number of tokens: {tokens} rows for {batch} sequences")
+        most = tokens // batch if batch else 0
+    if tokens and not width:
+        raise ValueError("block_table has no columns")
+    if max_tokens is not None and (max_tokens < 0 or (cu_tokens is None and max_tokens < most) or (max_tokens == 0 and tokens)):
+        raise ValueError(f"max_tokens is the largest number of new tokens of a sequence, got {max_tokens} for {tokens} rows of {batch} sequences")
+    return batch, width, most if max_tokens is None else min(int(max_tokens), most)
+
+
+def kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, *, q=None, cos=None, sin=None, cu_tokens=None,
+               max_tokens=None, q_out=None):
+    """Append the new tokens' keys and values [tokens, kv_heads, dim] to a paged 8-bit cache (lq_kv8_append; the cache's
+    layout and rounding: include/latentq.h). seq_lens counts the new tokens. cos, sin (float32 [positions, rotated dims / 2]):
+    keys are rotated by their position, and so is q [tokens, heads, dim], which is returned (q_out may be q itself). With
+    several tokens a sequence, cu_tokens (int32 [batch + 1]) has each sequence's first row; max_tokens, the largest number of new tokens
+    of a sequence, sizes the launch (default: what the number of rows allows). Returns the rotated q, or None."""
+    n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    k = _kv8_layout(_kv8_rows(k, "k", kv_heads, dim, k_codes))
+    v = _kv8_layout(_kv8_rows(v, "v", kv_heads, dim, k_codes, k.dtype))
+    tokens = k.shape[0]
+    if v.shape[0] != tokens:
+        raise ValueError(f"k has {tokens} rows and v {v.shape[0]}")
+    batch, width, most = _kv8_sequences(block_table, seq_lens, cu_tokens, max_tokens, tokens, k_codes)
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    rot = 0
+    if cos is not None:
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            _chk(t, torch.float32, name)
+            if t.device != k_codes.device:
+                raise ValueError(f"{name} must be on the device of the cache")
+            if t.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned")
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] == 0 or cos.shape[1] % 8 or not 0 < 2 * cos.shape[1] <= dim:
+            raise ValueError(f"cos and sin must be [positions, rotated dims / 2] with a multiple of 16 rotated dims up to {dim}, got {tuple(cos.shape)} and {tuple(sin.shape)}")
+        rot = 2 * cos.shape[1]
+    out = None
+    if q is not None:
+        if cos is None:
+            raise ValueError("q is taken to be rotated: it needs cos and sin")
+        _kv8_rows(q, "q", None, dim, k_codes, k.dtype)
+        if q.shape[0] != tokens:
+            raise ValueError(f"q must have {tokens} rows, got {q.shape[0]}")
+        if q_out is not None:
+            _kv8_result(q_out, "q_out", q)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        q = _kv8_layout(q)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if tokens and batch:
+        qs = (q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1)) if q is not None and q.numel() else (None, 0, 0, None, 0, 0)
+        with torch.cuda.device(k_codes.device):
+            _C.call("lq_kv8_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *qs,
+                    cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, cos.shape[0] if rot else 0, rot, k_codes.data_ptr(),
+                    v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(),
+                    None if cu_tokens is None else cu_tokens.data_ptr(), batch, tokens, most, 0 if q is None else q.shape[1], kv_heads, dim,
+                    _KV_TYPES[k.dtype], _stream(k_codes))
+    return out
+
+
+def kv8_read(k_codes, v_codes, k_scale, v_scale, blocks, dtype=torch.bfloat16):
+    """(keys, values) [n, 64, kv_heads, dim] that the n blocks (int32) of a paged 8-bit cache stand for (lq_kv8_read), as bfloat16,
+    float16 or float32."""
+    n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    _chk(blocks, torch.int32, "blocks")
+    if blocks.dim() != 1 or blocks.device != k_codes.device:
+        raise ValueError("blocks must be one-dimensional, on the device of the cache")
+    if dtype not in _KV_TYPES:
+        raise TypeError(f"dtype: expected bfloat16, float16 or float32, got {dtype}")
+    k = torch.empty((blocks.numel(), KV_BLOCK, kv_heads, dim), dtype=dtype, device=k_codes.device)
+    v = torch.empty_like(k)
+    if blocks.numel():
+        with torch.cuda.device(k_codes.device):
+            _C.call("lq_kv8_read", k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, blocks.data_ptr(),
+                    blocks.numel(), kv_heads, dim, _KV_TYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(k_codes))
+    return k, v
+
+
+KV8_KERNELS = ("few", "prompt")
+
+
+def kv8_attention_plan(batch: int, tokens: int, max_tokens: int, max_len: int, heads: int, kv_heads: int, dim: int, window: int = 0,
+                       workspace_bytes: int = WORKSPACE_MAX_BYTES, compute_units: int = 0):
+    """(kernel name, slices of the keys, bytes of workspace these take) kv8_attention would use for a call of these sizes
+    (lq_kv8_attention_plan). Launches nothing, as a16w4_plan."""
+    import ctypes
+    kernel, slices, needed = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
+    _C.call("lq_kv8_attention_plan", batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, workspace_bytes, compute_units,
+            ctypes.addressof(kernel), ctypes.addressof(slices), ctypes.addressof(needed))
+    return KV8_KERNELS[kernel.value], slices.value, needed.value
+
+
+def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,
+                  causal=True, window=0, out=None, return_lse=False):
+    """Attention of the last tokens of each sequence, q [tokens, heads, dim], over its blocks of a paged 8-bit cache (lq_kv8_attention):
+    softmax(scale * q K^T) V, scale 1 / sqrt(dim) by default, query head j on kv head j // (heads // kv_heads). A row sees
+    the positions up to its own (causal=False: the whole sequence), with window > 0 only the last `window` of them; one that sees
+    nothing gives zeros. max_tokens and max_len, the largest numbers of new tokens and of tokens of a sequence, size the launch
+    (defaults: what the rows and the block table allow). return_lse: also the logarithm of the softmax's denominator, float32 [tokens, heads]."""
+    n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    _kv8_rows(q, "q", None, dim, k_codes)
+    tokens, heads = q.shape[0], q.shape[1]
+    if heads == 0 or heads % kv_heads:
+        raise ValueError(f"the number of query heads must be a multiple of {kv_heads}, got {heads}")
+    batch, width, most = _kv8_sequences(block_table, seq_lens, cu_tokens, max_tokens, tokens, k_codes)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 3.4e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    window = int(window or 0)
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    max_len = width * KV_BLOCK if max_len is None else min(int(max_len), width * KV_BLOCK)
+    if max_len < 0:
+        raise ValueError(f"max_len must not be negative, got {max_len}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _kv8_result(out, "out", q)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if tokens and batch:
+        q = _kv8_layout(q)
+        with torch.cuda.device(k_codes.device):
+            needed = kv8_attention_plan(batch, tokens, most, max_len, heads, kv_heads, dim, window)[2]
+            keep, ws, ws_bytes = _workspace(q, 1, -(-needed // 32)) if needed else (None, None, 0)
+            _C.call("lq_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
+                    v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(), None if cu_tokens is None else cu_tokens.data_ptr(),
+                    batch, tokens, most, max_len, heads, kv_heads, dim, _KV_TYPES[q.dtype], scale, int(bool(causal)), window, out.data_ptr(),
+                    out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws, ws_bytes, _stream(q))
+            del keep
+    return (out, lse) if return_lse else out
