@@ -558,8 +558,8 @@ int lq_kv8_read(const void *k_codes, const void *v_codes, const float *k_scale, 
  * [tokens][heads]): the natural logarithm of the softmax's denominator, -inf for such a row. scale > 0.
  * q becomes f16 by a power of two for each row (exact but for elements under 2^-37 of the row's largest), codes are exact, scores,
  * softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits) relative to the largest contribution so far.
- * workspace (16-byte aligned, or null): with it, calls of few rows cut the keys into slices that a second launch
- * joins in order; lq_kv8_attention_plan says how many and the bytes they take. Calls sharing a workspace are
+ * workspace (16-byte aligned, or null): with it, calls of few rows share the keys among more workgroups, whose partial results a
+ * second launch joins in order; lq_kv8_attention_plan says how many and the bytes they take. Calls sharing a workspace are
  * ordered on one stream. */
 int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes,
                      const float *k_scale, const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width,
@@ -569,9 +569,10 @@ int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_strid
                      void *stream);
 
 /* What lq_kv8_attention does with a call of these sizes (launches nothing; compute_units <= 0: the current device's): *kernel 0 = few
- * rows, 1 = prompt; *slices of the keys; *needed = the bytes of workspace that these slices take (as many as workspace_bytes holds). */
+ * rows, 1 = prompt; *parts = few rows: workgroups that share the keys (0: one for each sequence and kv head, nothing to join), prompt: slices of
+ * the keys (1: nothing to join); *needed = the bytes of workspace that they take, no more than workspace_bytes. */
 int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
-                          int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *slices, int64_t *needed);
+                          int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *parts, int64_t *needed);
 
 /* ---------------------------------------------------------------------------
  * Layout converters (device side).

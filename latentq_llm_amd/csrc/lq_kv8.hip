@@ -287,80 +287,55 @@ void launch_read(const void *k_codes, const void *v_codes, const float *k_scale,
     else read_kernel<D, 2><<<grid, 256, 0, s>>>(k, v, k_scale, v_scale, blocks, k_out, v_out, kv_heads, pool);
 }
 
-// ---- attention: slices joined ----------------------------------------------
-// out = sum_i 2^(lse_i - m) o_i / sum_i 2^(lse_i - m): a slice without a visible key has lse -inf and is not read.
-template <int D, bool kF16>
-__global__ __launch_bounds__(256) void join_kernel(const Kv8Attn a) {
-    constexpr int kUnits = D / 4, kRows = 256 / kUnits;
-    const int64_t rows = (int64_t)a.tokens * a.heads, row = (int64_t)blockIdx.x * kRows + threadIdx.x / kUnits;
-    const int d = threadIdx.x % kUnits * 4;
-    if (threadIdx.x >= kRows * kUnits || row >= rows) return;
-    float m = -__builtin_inff();
-    bool nan = false;
-    for (int i = 0; i < a.slices; ++i) {
-        const float l = a.part_lse[i * rows + row];
-        nan |= l != l;
-        m = fmaxf(m, l);
-    }
-    f32x4_t o = {0, 0, 0, 0};
-    float total = 0.0f;
-    if (m > -__builtin_inff() || nan) {
-        for (int i = 0; i < a.slices; ++i) {
-            const float l = a.part_lse[i * rows + row];
-            if (l == -__builtin_inff()) continue;
-            const float w = __builtin_amdgcn_exp2f(l - m);
-            total += w;
-            const f32x4_t p = *(const f32x4_t *)(a.part + (i * rows + row) * D + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = fmaf(w, p[j], o[j]);
-        }
-        const float r = 1.0f / total;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] *= r;
-    }
-    const int64_t token = row / a.heads, head = row % a.heads;
-    *(u32x2_t *)((uint16_t *)a.out + token * a.o_token + head * a.o_head + d) = u32x2_t{kv8_pack<kF16>(o[0], o[1]), kv8_pack<kF16>(o[2], o[3])};
-    if (a.lse && d == 0) a.lse[row] = nan ? __builtin_nanf("") : (m + __builtin_amdgcn_logf(total)) * 0.693147180559945f;
-}
-
-template <int D>
-void launch_join(const Kv8Attn &a, bool f16, hipStream_t s) {
-    constexpr int kRows = 256 / (D / 4);
-    const dim3 grid((unsigned)(((int64_t)a.tokens * a.heads + kRows - 1) / kRows));
-    if (f16) join_kernel<D, true><<<grid, 256, 0, s>>>(a);
-    else join_kernel<D, false><<<grid, 256, 0, s>>>(a);
-}
-
 bool good_dim(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 256; }
 
-// How a call is cut: rows of a (sequence, kv head) that go to the kernel of few rows, and slices of the keys.
+// How a call is cut.
 struct Plan {
     bool few;
-    int slices, tiles, row_tiles;
+    int workgroups;                // few rows: that share all tiles, 0: one for each (sequence, kv head)
+    int slices, tiles, row_tiles;  // prompt
+    int64_t slots, slot_rows;      // of the workspace
 };
 
 // Most rows of the kernel for few: beyond it the prompt kernel (its tiles of 128 rows)
 int most_rows(int dim) { return dim <= 128 ? 64 : 32; }
 
-Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t workspace, int cus) {
-    Plan p;
-    const int64_t rows = max_tokens * (heads / kv_heads);
+Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t width, int64_t workspace, int cus) {
+    Plan p{};
+    const int64_t rows = max_tokens * (heads / kv_heads), units = batch * kv_heads;
     p.few = rows <= most_rows(dim);
-    p.row_tiles = p.few ? 1 : (int)((rows + 127) / 128);
     int64_t keys = max_len;
     if (window && window + max_tokens + KV8_BLOCK < keys) keys = window + max_tokens + KV8_BLOCK;
     const int64_t tiles = keys > 0 ? (keys + KV8_BLOCK - 1) / KV8_BLOCK : 1;
-    const int64_t units = batch * kv_heads * p.row_tiles;
-    const int64_t want = p.few ? 4 * (int64_t)cus : 2 * (int64_t)cus, least = p.few ? 4 : 8;  // workgroups, tiles of a slice
-    int64_t slices = units >= want ? 1 : (want + units - 1) / units;
-    const int64_t slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;
-    if (slices > 64) slices = 64;
-    if (slices > 1 && slice_bytes > 0 && slices > workspace / slice_bytes) slices = workspace / slice_bytes;
-    if (slices < 1) slices = 1;
-    int64_t per = (tiles + slices - 1) / slices;
-    if (per < least) per = least;
-    p.slices = (int)((tiles + per - 1) / per);
-    p.tiles = (int)per;
+    if (p.few) {
+        // One workgroup for a (sequence, kv head) and one launch, or the tiles of all of them in equal shares and a launch that
+        // joins (2 to 3 us): a unit up to 16 KiB of keys and values for each of its tiles goes through a compute unit at some 40 GB/s, so
+        // long keys are shared where units leave compute units idle, and, lengths in a batch being what they are, where
+        // that costs little for equal ones. us by units / by shares, 128 dimensions: 32 units of 16 tiles 10.3 / 9.4, 32 tiles 16.9 / 10.6; 128 of 32
+        // 18.7 / 18.1, of 64 33.7 / 27.6; 256 of 64 42.0 / 46.8 (lengths down to a quarter 35.9 / 35.2), of 128 79.9 / 85.5 (67.6 / 59.9); 384 of 64
+        // 72.0 / 68.5 (60.2 / 49.4); 512 of 64 80.6 / 83.7 (64.4 / 61.7). 64 dimensions are level at twice the tiles.
+        const int64_t rounds = (units + cus - 1) / cus, equal = tiles * dim / 128;  // tiles of 16 KiB
+        const bool split = equal >= 24 && equal * rounds * cus >= 80 * units && batch <= 512 && units * width <= INT32_MAX;
+        int64_t share = (int64_t)cus * kv8_few_workgroups(dim, (int)rows);
+        if (share > workspace / (2 * rows * ((int64_t)dim + 1) * 4)) share = workspace / (2 * rows * ((int64_t)dim + 1) * 4);
+        p.workgroups = split && share > 1 ? (int)share : 0;
+        p.slots = 2 * p.workgroups;
+        p.slot_rows = rows;
+        p.slices = 1;
+    } else {
+        p.row_tiles = (int)((rows + 127) / 128);
+        const int64_t want = 2 * (int64_t)cus, least = 8, slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;  // workgroups, tiles of a slice
+        int64_t slices = units * p.row_tiles >= want ? 1 : (want + units * p.row_tiles - 1) / (units * p.row_tiles);
+        if (slices > 64) slices = 64;
+        if (slices > 1 && slices > workspace / slice_bytes) slices = workspace / slice_bytes;
+        if (slices < 1) slices = 1;
+        int64_t per = (tiles + slices - 1) / slices;
+        if (per < least) per = least;
+        p.slices = (int)((tiles + per - 1) / per);
+        p.tiles = (int)per;
+        p.slots = p.slices > 1 ? p.slices : 0;
+        p.slot_rows = tokens * heads;
+    }
     return p;
 }
 
@@ -444,16 +419,16 @@ int attention_sizes(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t m
 }  // namespace
 
 extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
-                                     int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *slices, int64_t *needed) {
+                                     int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *parts, int64_t *needed) {
     if (const int rc = attention_sizes(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window)) return rc;
-    LQ_REQUIRE(kernel && slices && needed, "kv8_attention_plan: null pointer");
+    LQ_REQUIRE(kernel && parts && needed, "kv8_attention_plan: null pointer");
     if (max_tokens > tokens) max_tokens = tokens;
     const Plan p = batch && tokens && max_tokens
-                       ? plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, workspace_bytes, compute_units > 0 ? compute_units : lq_device_cu_count())
-                       : Plan{true, 1, 0, 0};
+                       ? plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, (max_len + KV8_BLOCK - 1) / KV8_BLOCK, workspace_bytes, compute_units > 0 ? compute_units : lq_device_cu_count())
+                       : Plan{true, 0, 1, 0, 0, 0, 0};
     *kernel = p.few ? 0 : 1;
-    *slices = p.slices;
-    *needed = p.slices > 1 ? (int64_t)p.slices * tokens * heads * (dim + 1) * 4 : 0;
+    *parts = p.few ? p.workgroups : p.slices;
+    *needed = p.slots * p.slot_rows * (dim + 1) * 4;
     return LQ_OK;
 }
 
@@ -479,24 +454,17 @@ extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q
     LQ_REQUIRE(workspace_bytes >= 0, "kv8_attention: the workspace's size must not be negative");
     if (max_tokens > tokens) max_tokens = tokens;
     if (max_len > table_width * KV8_BLOCK) max_len = table_width * KV8_BLOCK;
-    const Plan p = plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, workspace ? workspace_bytes : 0, lq_device_cu_count());
+    const Plan p = plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, table_width, workspace ? workspace_bytes : 0, lq_device_cu_count());
     Kv8Attn a{};
     a.q = q; a.k = (const uint8_t *)k_codes; a.v = (const uint8_t *)v_codes; a.ks = k_scale; a.vs = v_scale;
     a.table = block_table; a.lens = seq_lens; a.cu = cu_tokens; a.out = out; a.lse = lse;
     a.part = (float *)workspace;
-    a.part_lse = a.part + (int64_t)p.slices * tokens * heads * dim;
+    a.part_lse = a.part + p.slots * p.slot_rows * dim;
     a.q_token = q_token_stride; a.q_head = q_head_stride; a.o_token = out_token_stride; a.o_head = out_head_stride;
     a.window = window; a.scale = scale * 1.442695040888963f;
     a.blocks = (int)num_blocks; a.width = (int)table_width; a.batch = (int)batch; a.tokens = (int)tokens; a.heads = heads; a.kv_heads = kv_heads;
-    a.causal = causal != 0; a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles;
-    LQ_REQUIRE((int64_t)p.slices * batch * kv_heads * p.row_tiles <= INT32_MAX, "kv8_attention: too many tokens or sequences");
-    const int64_t rows = max_tokens * (heads / kv_heads);
-    const int rc = p.few ? kv8_launch_few(a, (int)rows, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
-    if (rc != LQ_OK || p.slices == 1) return rc;
-    hipStream_t s = (hipStream_t)stream;
-    if (dim == 64) launch_join<64>(a, dtype == 1, s);
-    else if (dim == 96) launch_join<96>(a, dtype == 1, s);
-    else if (dim == 128) launch_join<128>(a, dtype == 1, s);
-    else launch_join<256>(a, dtype == 1, s);
-    return lq_check_launch("kv8_attention (join)");
+    a.causal = causal != 0; a.workgroups = p.workgroups; a.rows = (int)(max_tokens * (heads / kv_heads));
+    a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles;
+    LQ_REQUIRE(p.few || (int64_t)p.slices * batch * kv_heads * p.row_tiles <= INT32_MAX, "kv8_attention: too many tokens or sequences");
+    return p.few ? kv8_launch_few(a, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
 }

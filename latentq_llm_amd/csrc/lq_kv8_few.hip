@@ -12,28 +12,124 @@
 // their (M, L, O) through shared memory at the end; slices of the keys in several workgroups go through the workspace.
 #include "lq_kv8.h"
 
+#include <type_traits>
+
 namespace {
 
-constexpr float kNone = -3e38f;  // running maximum before the first key
+// Loads from a tile of the cache through a buffer descriptor (in scalar registers, bounded by the tile): one vector register holds a
+// lane's offset for all of a tile's loads, where a 64-bit address for every few of them took 40. A byte of the cache is read once:
+// non-temporal (64 x 8192 keys of 8 heads 180 -> 160 us, 6.0 -> 6.7 TB/s; a plain read of 1 GiB 7.1).
+struct TileLoads {
+    __amdgpu_buffer_rsrc_t at;
+    __device__ __forceinline__ TileLoads(const uint8_t *tile, int bytes) : at(__builtin_amdgcn_make_buffer_rsrc((void *)tile, 0, bytes, 0x00027000)) {}
+    static constexpr int kNonTemporal = 2;
+    __device__ __forceinline__ u32x4_t load16(int lane_offset, int offset) const {
+        return __builtin_amdgcn_raw_buffer_load_b128(at, lane_offset + (offset & 4095), offset & ~4095, kNonTemporal);
+    }
+    __device__ __forceinline__ u32x2_t load8(int lane_offset, int offset) const {
+        return __builtin_amdgcn_raw_buffer_load_b64(at, lane_offset + (offset & 4095), offset & ~4095, kNonTemporal);
+    }
+};
+
+// The tiles of all (sequence, kv head)s one after the other, shared evenly among the workgroups: the first `more` of them have per + 1
+// tiles, the others per. A share begins and ends in the middle of a unit: the sequences of a batch differ in length, and whole
+// units, or slices of one length, leave part of the device idle at the end (64 sequences of 2048 to 8192 keys, 8 heads: 125 us by
+// whole units, 127 to 152 by slices of 64 to 16 tiles, 112 by shares). The host keeps the number of all tiles within 31 bits.
+constexpr int kLeast = 4;  // tiles of a share, one for each wave
+
+struct Shares {
+    int total, workgroups, per, more;  // workgroups: those that have any
+    __device__ __forceinline__ Shares(const Kv8Attn &a, int tiles) {
+        total = tiles * a.kv_heads;
+        workgroups = max(1, min(a.workgroups, (int)(((unsigned)total + kLeast - 1) / kLeast)));
+        per = (unsigned)total / (unsigned)workgroups;
+        more = total - per * workgroups;
+    }
+    __device__ __forceinline__ int begin(int w) const { return per * w + min(w, more); }
+    __device__ __forceinline__ int holder(int tile) const {  // the workgroup that has it
+        const int large = (per + 1) * more;
+        return tile < large ? (unsigned)tile / (unsigned)(per + 1) : more + (unsigned)(tile - large) / (unsigned)per;
+    }
+};
+
+// Sequences base .. base + 63, one to a lane, by one wave and the same in every one: the tiles of those up to the lane's own.
+__device__ __forceinline__ Kv8Rows scanned(const Kv8Attn &a, int base, int lane, int &upto) {
+    if (a.batch == 1) {
+        const Kv8Rows r = kv8_rows<true>(a, 0);
+        upto = r.tiles;
+        return r;
+    }
+    const Kv8Rows r = kv8_rows<false>(a, min(base + lane, a.batch - 1));
+    const int n = min(a.batch - base, 64);
+    upto = r.tiles;
+    for (int o = 1; o < n; o <<= 1) {
+        const int x = __shfl_up(upto, o);
+        if (lane >= o) upto += x;
+    }
+    return r;
+}
+__device__ __forceinline__ int at_lane(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
 
 template <int D, int RT, bool kF16>
-__global__ __launch_bounds__(256, RT == 1 && D <= 128 ? 2 : 1) void few_kernel(const Kv8Attn a) {
+__global__ __launch_bounds__(256, kv8_few_waves(D, RT)) void few_kernel(const Kv8Attn a) {
     constexpr int S = D / 64, kTail = D % 64 / 32, kSteps = 2 * S + kTail, kTiles = D / 16;  // k steps of 32 dimensions; dim tiles
     constexpr int kWaves = 4, kPad = D + 4;
     __shared__ float lds_o[kWaves][16][kPad];
     __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
 
-    const int unit = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-    const int seq = unit / a.kv_heads, h = unit % a.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const Kv8Rows s = kv8_rows(a, seq);
-    if (s.n == 0) return;
-    const int group = a.heads / a.kv_heads, rows = min(s.n * group, 16 * RT);
+    const int group = a.heads / a.kv_heads;
 
-    // tiles that the rows see, and those of this slice
-    int64_t lo64 = a.window ? (int64_t)s.first - a.window + 1 : 0;
-    const int t_first = (int)(lo64 > 0 ? min(lo64, (int64_t)s.len) : 0) / KV8_BLOCK, t_last = (s.len + KV8_BLOCK - 1) / KV8_BLOCK;
-    const int t_lo = t_first + slice * a.tiles, t_hi = slice == a.slices - 1 ? t_last : min(t_last, t_lo + a.tiles);
+    // this workgroup's tiles: `left` of them, from tile `from` of (seq, h) on
+    int seq, h, from, left;
+    Kv8Rows lanes;  // of this share's first sequence
+    if (a.workgroups) {
+        int sum = 0, upto, base = 0;
+        for (; base < a.batch; base += 64) {
+            lanes = scanned(a, base, lane, upto);
+            sum += at_lane(upto, min(a.batch - base, 64) - 1);
+        }
+        const Shares shares(a, sum);
+        if ((int)blockIdx.x >= shares.workgroups || sum == 0) return;
+        const int begin = shares.begin(blockIdx.x);
+        left = shares.begin(blockIdx.x + 1) - begin;
+        int before = 0;
+        for (base = 0;; base += 64) {
+            if (a.batch > 64) lanes = scanned(a, base, lane, upto);
+            const int n = min(a.batch - base, 64);
+            const uint64_t past = __ballot(lane < n && (before + upto) * a.kv_heads > begin);
+            if (past) {
+                const int i = __builtin_ctzll(past);
+                seq = base + i;
+                if (i) before += at_lane(upto, i - 1);
+                lanes = Kv8Rows{at_lane(lanes.start, i), at_lane(lanes.n, i), at_lane(lanes.len, i), at_lane(lanes.first, i), at_lane(lanes.t_first, i), at_lane(lanes.tiles, i)};
+                break;
+            }
+            before += at_lane(upto, n - 1);
+        }
+        const unsigned at = (unsigned)(begin - before * a.kv_heads);
+        h = at / (unsigned)lanes.tiles;
+        from = at % (unsigned)lanes.tiles;
+    } else {
+        seq = blockIdx.x / a.kv_heads;
+        h = blockIdx.x % a.kv_heads;
+        from = 0;
+        lanes = kv8_rows<true>(a, seq);
+        left = lanes.tiles;
+        if (lanes.n == 0) return;
+    }
+    // uniform, all of it: said so, or descriptors and addresses would be made lane by lane
+    const auto scalar = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    Kv8Rows s{scalar(lanes.start), scalar(lanes.n), scalar(lanes.len), scalar(lanes.first), scalar(lanes.t_first), scalar(lanes.tiles)};
+    seq = scalar(seq);
+    h = scalar(h);
+    from = scalar(from);
+    left = scalar(left);
+
+    for (bool again = false;; again = true) {
+    const int rows = min(s.n * group, a.rows);  // at most 16 RT
+    const int t_lo = s.t_first + from, t_hi = s.t_first + min(s.tiles, from + left);
+    const bool whole = t_hi - t_lo == s.tiles;
 
     // queries as operands: lane (row col, g) has dimensions 64 s + 16 g + 8 e .. + 7 of steps (s, e), then 64 S + 8 g ..
     f16x8_t q[RT][kSteps];
@@ -80,40 +176,42 @@ __global__ __launch_bounds__(256, RT == 1 && D <= 128 ? 2 : 1) void few_kernel(c
     }
 
     const int *table = a.table + (int64_t)seq * a.width;
-    const auto block_of = [&](int t) { return (int64_t)min((unsigned)table[t], (unsigned)(a.blocks - 1)) * a.kv_heads + h; };
+    const auto block_of = [&](int id) { return (int64_t)min((unsigned)id, (unsigned)(a.blocks - 1)) * a.kv_heads + h; };
     // keys of the tile: 4 groups of 16 tokens; values: the same 4 groups, 4 tokens of 4 dimensions a word group
     u32x4_t kr[4][S], vr[4][S];
     u32x2_t kt[4], vt[4];  // dimensions beyond a multiple of 64
+    const int k_at = col * D + 16 * g, k_tail = col * D + 8 * g, v_at = (g * D + 4 * col) * 4, v_tail = (g * D + 2 * col) * 4;
     const auto load_k = [&](int64_t bh) {
-        const uint8_t *p = a.k + bh * (KV8_BLOCK * D);
+        const TileLoads p(a.k + bh * (KV8_BLOCK * D), KV8_BLOCK * D);
+        int k_lane = k_at;
+        asm volatile("" : "+v"(k_lane));  // (so that the loads' constants are theirs, not sums kept in registers)
 #pragma unroll
         for (int tg = 0; tg < 4; ++tg) {
 #pragma unroll
-            for (int i = 0; i < S; ++i) kr[tg][i] = *(const u32x4_t *)(p + (tg * 16 + col) * D + 64 * i + 16 * g);
-            if constexpr (kTail) kt[tg] = *(const u32x2_t *)(p + (tg * 16 + col) * D + 64 * S + 8 * g);
+            for (int i = 0; i < S; ++i) kr[tg][i] = p.load16(k_lane, tg * 16 * D + 64 * i);
+            if constexpr (kTail) kt[tg] = p.load8(k_tail, tg * 16 * D + 64 * S);
         }
     };
     const auto load_v = [&](int64_t bh) {
-        const uint8_t *p = a.v + bh * (KV8_BLOCK * D);
+        const TileLoads p(a.v + bh * (KV8_BLOCK * D), KV8_BLOCK * D);
+        int v_lane = v_at;
+        asm volatile("" : "+v"(v_lane));
 #pragma unroll
         for (int tg = 0; tg < 4; ++tg) {
 #pragma unroll
-            for (int i = 0; i < S; ++i) vr[tg][i] = *(const u32x4_t *)(p + ((tg * 4 + g) * D + 64 * i + 4 * col) * 4);
-            if constexpr (kTail) vt[tg] = *(const u32x2_t *)(p + ((tg * 4 + g) * D + 64 * S + 2 * col) * 4);
+            for (int i = 0; i < S; ++i) vr[tg][i] = p.load16(v_lane, tg * 16 * D + 256 * i);
+            if constexpr (kTail) vt[tg] = p.load8(v_tail, tg * 16 * D + 256 * S);
         }
     };
 
-    int t = t_lo + wave;
+    // one tile; more: the wave has another one, whose keys are requested as soon as this one's are used (a branch around the requests
+    // would make every wait for this tile's values a wait for them too)
+    int t = t_lo + wave, id_next = 0;
     int64_t bh = 0;
     float k_scale = 0.0f, v_scale = 0.0f;
-    if (t < t_hi) {
-        bh = block_of(t);
-        load_k(bh);
-        k_scale = a.ks[bh];
-        v_scale = a.vs[bh];
-    }
-    for (; t < t_hi; t += kWaves) {
+    const auto tile = [&](auto more) {
         load_v(bh);
+        __builtin_amdgcn_sched_barrier(0);  // (not below the wait for the keys)
         const float ks = k_scale, vs = v_scale;
         f32x4_t c[RT][4];
 #pragma unroll
@@ -129,11 +227,13 @@ __global__ __launch_bounds__(256, RT == 1 && D <= 128 ? 2 : 1) void few_kernel(c
                 for (int rt = 0; rt < RT; ++rt) c[rt][tg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][i], c[rt][tg], 0, 0, 0);
             }
         }
-        if (t + kWaves < t_hi) {
-            bh = block_of(t + kWaves);
+        if constexpr (decltype(more)::value) {
+            bh = block_of(id_next);
             load_k(bh);
-            k_scale = a.ks[bh];
-            v_scale = a.vs[bh];
+            k_scale = kv8_uniform(a.ks + bh);
+            v_scale = kv8_uniform(a.vs + bh);
+            id_next = kv8_uniform(table + min(t + 2 * kWaves, t_hi - 1));
+            __builtin_amdgcn_sched_barrier(0);
         }
         const int key0 = t * KV8_BLOCK;
         const float lv = __builtin_amdgcn_logf(vs), rv = 1.0f / vs;
@@ -156,8 +256,7 @@ __global__ __launch_bounds__(256, RT == 1 && D <= 128 ? 2 : 1) void few_kernel(c
             for (int tg = 0; tg < 4; ++tg)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) most = fmaxf(most, c[rt][tg][i]);
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
+            most = kv8_max32(kv8_max16(most));
             const float m = fmaxf(M[rt], fmaf(most, f, lv)), shift = lv - m;
             const float fade = __builtin_amdgcn_exp2f(M[rt] - m);
             if (__any(m > M[rt])) {
@@ -189,17 +288,28 @@ __global__ __launch_bounds__(256, RT == 1 && D <= 128 ? 2 : 1) void few_kernel(c
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[rt][e], o[rt][i], 0, 0, 0);
             }
+    };
+    if (t < t_hi) {
+        bh = block_of(kv8_uniform(table + t));
+        load_k(bh);
+        k_scale = kv8_uniform(a.ks + bh);
+        v_scale = kv8_uniform(a.vs + bh);
+        id_next = kv8_uniform(table + min(t + kWaves, t_hi - 1));
+        for (; t + kWaves < t_hi; t += kWaves) tile(std::true_type{});
+        tile(std::false_type{});
     }
 
     // join the waves, 16 rows at a time
-    const int64_t all = (int64_t)a.tokens * a.heads;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (what follows from it is computed here, not kept in registers over the tiles)
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (from == 0);  // a share has at most one end of a unit and one beginning
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (rt * 16 >= rows) break;
         float l = L[rt];
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        if (rt) __syncthreads();
+        if (rt || again) __syncthreads();
         if (g == 0) {
             lds_m[wave][col] = M[rt];
             lds_l[wave][col] = l;
@@ -217,61 +327,118 @@ __global__ __launch_bounds__(256, RT == 1 && D <= 128 ? 2 : 1) void few_kernel(c
         }
         __syncthreads();
         constexpr int kUnits = D / 4;
-        for (int u = threadIdx.x; u < 16 * kUnits; u += 256) {
+        for (int u = tid; u < 16 * kUnits; u += 256) {
             const int c = u / kUnits, d = u % kUnits * 4, r = rt * 16 + c;
             if (r >= rows) break;
-            float m = lds_m[0][c];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds_m[w][c]);
-            float total = 0.0f;
-            f32x4_t x = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f(lds_m[w][c] - m);
-                total = fmaf(f, lds_l[w][c], total);
-                const f32x4_t y = *(const f32x4_t *)&lds_o[w][c][d];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = fmaf(f, y[j], x[j]);
-            }
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] *= inv;
-            const float lse = total == 0.0f ? -__builtin_inff() : m + __builtin_amdgcn_logf(total);
-            const int token = s.start + r / group, head = h * group + r % group;
-            const int64_t row = (int64_t)token * a.heads + head;
-            if (a.slices == 1) {
-                *(u32x2_t *)((uint16_t *)a.out + token * a.o_token + head * a.o_head + d) = u32x2_t{kv8_pack<kF16>(x[0], x[1]), kv8_pack<kF16>(x[2], x[3])};
-                if (a.lse && d == 0) a.lse[row] = lse * 0.693147180559945f;
+            float m, total;
+            f32x4_t x;
+            kv8_join_parts<kWaves>((const f32x4_t *)&lds_o[0][c][d], &lds_m[0][c], &lds_l[0][c], 16 * kPad / 4, 16, m, total, x);
+            if (whole) {
+                kv8_finish<kF16>(a, s.start + r / group, h * group + r % group, d, m, total, x);
             } else {
-                *(f32x4_t *)(a.part + (slice * all + row) * D + d) = x;
-                if (d == 0) a.part_lse[slice * all + row] = lse;
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] *= inv;
+                *(f32x4_t *)(a.part + (slot * a.rows + r) * D + d) = x;
+                if (d == 0) a.part_lse[slot * a.rows + r] = total == 0.0f ? -__builtin_inff() : m + __builtin_amdgcn_logf(total);
             }
         }
     }
+    // the next unit of the share
+    left -= t_hi - t_lo;
+    if (left <= 0) return;
+    from = 0;
+    if (++h == a.kv_heads) {
+        h = 0;
+        do s = kv8_rows<true>(a, ++seq);
+        while (s.tiles == 0);
+    }
+    }
+}
+
+// The pieces of the units that no workgroup had as a whole, joined: workgroups blockIdx.x for (sequence, kv head), blockIdx.y for
+// kRows of its rows; dim / 4 threads side by side, kParts of them at pieces p, p + kParts, ... Units without a tile get their zeros here.
+// (Joined by the last holder of each unit inside the one launch, waiting for the others' pieces behind tags: 0.5 to 1 us faster up to
+// 12 us, as fast beyond, 5 us slower where a unit has 96 pieces.)
+template <int D, int kParts, bool kF16>
+__global__ __launch_bounds__(256) void join_few_kernel(const Kv8Attn a) {
+    constexpr int kUnits = D / 4, kRows = 256 / (kUnits * kParts);
+    __shared__ f32x4_t lds_o[kParts][kRows * kUnits];
+    __shared__ float lds_m[kParts][kRows], lds_l[kParts][kRows];
+    const int lane = threadIdx.x & 63, seq = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+    const int unit = threadIdx.x % kUnits, at = threadIdx.x / kUnits, part = at % kParts, mine = at / kParts, r = blockIdx.y * kRows + mine;
+    const Kv8Rows s = kv8_rows<true>(a, seq);
+    const bool there = mine < kRows && r < min(s.n * group, a.rows);
+    int first = 0, pieces = 0;
+    if (s.tiles) {
+        int sum = 0, before = 0;
+        for (int base = 0; base < a.batch; base += 64) {
+            int upto;
+            scanned(a, base, lane, upto);
+            if (seq >= base && seq < base + 64) before = seq > base ? sum + at_lane(upto, seq - base - 1) : sum;
+            sum += at_lane(upto, min(a.batch - base, 64) - 1);
+        }
+        const Shares shares(a, sum);
+        const int begin = before * a.kv_heads + h * s.tiles;
+        first = shares.holder(begin);
+        pieces = shares.holder(begin + s.tiles - 1) - first + 1;
+        if (pieces == 1) return;  // one workgroup had it all
+        // the first workgroup has the unit's beginning; the others begin inside it
+    }
+    float m = kNone, total = 0.0f;
+    f32x4_t o = {0, 0, 0, 0};
+    if (there)
+        kv8_join<D>(a.part, a.part_lse, a.rows, r, 4 * unit, part, kParts, pieces, [&](int i) { return 2 * (int64_t)(first + i) + (i == 0); }, m, total, o);
+    if constexpr (kParts > 1) {
+        if (there) {
+            lds_o[part][mine * kUnits + unit] = o;
+            if (unit == 0) {
+                lds_m[part][mine] = m;
+                lds_l[part][mine] = total;
+            }
+        }
+        __syncthreads();
+        if (!there || part) return;
+        kv8_join_parts<kParts>(&lds_o[0][mine * kUnits + unit], &lds_m[0][mine], &lds_l[0][mine], kRows * kUnits, kRows, m, total, o);
+    }
+    if (there) kv8_finish<kF16>(a, s.start + r / group, h * group + r % group, 4 * unit, m, total, o);
+}
+
+template <int D, int kParts>
+void launch_join(const Kv8Attn &a, bool f16, hipStream_t s) {
+    constexpr int kRows = 256 / (D / 4 * kParts);
+    const dim3 grid((unsigned)(a.batch * a.kv_heads), (unsigned)((a.rows + kRows - 1) / kRows));
+    if (f16) join_few_kernel<D, kParts, true><<<grid, 256, 0, s>>>(a);
+    else join_few_kernel<D, kParts, false><<<grid, 256, 0, s>>>(a);
 }
 
 template <int D, int RT>
 int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.slices));
+    const dim3 grid((unsigned)(a.workgroups ? a.workgroups : a.batch * a.kv_heads));
     if (f16) few_kernel<D, RT, true><<<grid, 256, 0, s>>>(a);
     else few_kernel<D, RT, false><<<grid, 256, 0, s>>>(a);
-    return lq_check_launch("kv8_attention (few rows)");
+    const int rc = lq_check_launch("kv8_attention (few rows)");
+    if (rc != LQ_OK || !a.workgroups) return rc;
+    constexpr int kMost = D <= 128 ? 8 : 4;
+    if (a.workgroups > 8 * (int64_t)a.batch * a.kv_heads) launch_join<D, kMost>(a, f16, s);
+    else launch_join<D, 1>(a, f16, s);
+    return lq_check_launch("kv8_attention (join)");
 }
 
 template <int D>
-int launch_rows(const Kv8Attn &a, int rows, bool f16, hipStream_t s) {
-    if (rows <= 16) return launch<D, 1>(a, f16, s);
-    if (rows <= 32) return launch<D, 2>(a, f16, s);
+int launch_rows(const Kv8Attn &a, bool f16, hipStream_t s) {
+    if (a.rows <= 16) return launch<D, 1>(a, f16, s);
+    if (a.rows <= 32) return launch<D, 2>(a, f16, s);
     if constexpr (D <= 128) return launch<D, 4>(a, f16, s);
-    return lq_fail(LQ_ERR_UNSUPPORTED, "kv8_attention: %d rows at %d dimensions are not for the kernel of few rows", rows, D);
+    return lq_fail(LQ_ERR_UNSUPPORTED, "kv8_attention: %d rows at %d dimensions are not for the kernel of few rows", a.rows, D);
 }
 
 }  // namespace
 
-int kv8_launch_few(const Kv8Attn &a, int rows, int dim, bool f16, void *stream) {
+int kv8_launch_few(const Kv8Attn &a, int dim, bool f16, void *stream) {
     hipStream_t s = (hipStream_t)stream;
-    if (dim == 64) return launch_rows<64>(a, rows, f16, s);
-    if (dim == 96) return launch_rows<96>(a, rows, f16, s);
-    if (dim == 128) return launch_rows<128>(a, rows, f16, s);
-    return launch_rows<256>(a, rows, f16, s);
+    if (dim == 64) return launch_rows<64>(a, f16, s);
+    if (dim == 96) return launch_rows<96>(a, f16, s);
+    if (dim == 128) return launch_rows<128>(a, f16, s);
+    return launch_rows<256>(a, f16, s);
 }

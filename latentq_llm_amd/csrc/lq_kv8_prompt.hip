@@ -9,8 +9,6 @@
 
 namespace {
 
-constexpr float kNone = -3e38f;
-
 template <int D, bool kF16>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
     constexpr int kSteps = D / 16, kTiles = D / 32, kPieces = D / 8;
@@ -22,7 +20,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
     const int unit = blockIdx.x % units, rest = blockIdx.x / units;
     const int slice = rest % a.slices, tile = a.row_tiles - 1 - rest / a.slices;  // the last rows see most keys: first
     const int seq = unit / a.kv_heads, h = unit % a.kv_heads;
-    const Kv8Rows s = kv8_rows(a, seq);
+    const Kv8Rows s = kv8_rows<true>(a, seq);
     const int group = a.heads / a.kv_heads;
     const int64_t all_rows = (int64_t)s.n * group;
     const int row0 = tile * kRows;
@@ -229,12 +227,58 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
     }
 }
 
+// ---- slices of the keys joined: one workgroup for kRows rows, dim / 4 threads side by side, kParts of them at slices p, p + kParts,
+// ... of the same row.
+template <int D, int kParts, bool kF16>
+__global__ __launch_bounds__(256) void join_kernel(const Kv8Attn a) {
+    constexpr int kUnits = D / 4, kRows = 256 / (kUnits * kParts);
+    static_assert(kRows >= 1, "");
+    __shared__ f32x4_t lds_o[kParts][kRows * kUnits];
+    __shared__ float lds_m[kParts][kRows], lds_l[kParts][kRows];
+    const int64_t rows = (int64_t)a.tokens * a.heads;
+    const int unit = threadIdx.x % kUnits, at = threadIdx.x / kUnits, part = at % kParts, mine = at / kParts;
+    const int64_t row = (int64_t)blockIdx.x * kRows + mine;
+    const bool there = mine < kRows && row < rows;
+    float m = kNone, total = 0.0f;
+    f32x4_t o = {0, 0, 0, 0};
+    if (there) kv8_join<D>(a.part, a.part_lse, rows, row, 4 * unit, part, kParts, a.slices, [](int i) { return (int64_t)i; }, m, total, o);
+    if constexpr (kParts > 1) {
+        if (there) {
+            lds_o[part][mine * kUnits + unit] = o;
+            if (unit == 0) {
+                lds_m[part][mine] = m;
+                lds_l[part][mine] = total;
+            }
+        }
+        __syncthreads();
+        if (!there || part) return;
+        kv8_join_parts<kParts>(&lds_o[0][mine * kUnits + unit], &lds_m[0][mine], &lds_l[0][mine], kRows * kUnits, kRows, m, total, o);
+    }
+    if (there) kv8_finish<kF16>(a, row / a.heads, (int)(row % a.heads), 4 * unit, m, total, o);
+}
+
+template <int D, int kParts>
+void launch_join_parts(const Kv8Attn &a, bool f16, hipStream_t s) {
+    constexpr int kRows = 256 / (D / 4 * kParts);
+    const dim3 grid((unsigned)(((int64_t)a.tokens * a.heads + kRows - 1) / kRows));
+    if (f16) join_kernel<D, kParts, true><<<grid, 256, 0, s>>>(a);
+    else join_kernel<D, kParts, false><<<grid, 256, 0, s>>>(a);
+}
+
+template <int D>
+int launch_join(const Kv8Attn &a, bool f16, hipStream_t s) {
+    if (a.slices > 4) launch_join_parts<D, 4>(a, f16, s);
+    else launch_join_parts<D, 1>(a, f16, s);
+    return lq_check_launch("kv8_attention (join)");
+}
+
 template <int D>
 int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.slices * a.row_tiles));
     if (f16) prompt_kernel<D, true><<<grid, 256, 0, s>>>(a);
     else prompt_kernel<D, false><<<grid, 256, 0, s>>>(a);
-    return lq_check_launch("kv8_attention (prompt)");
+    if (const int rc = lq_check_launch("kv8_attention (prompt)")) return rc;
+    return a.slices > 1 ? launch_join<D>(a, f16, s) : LQ_OK;
 }
 
 }  // namespace

@@ -1112,13 +1112,14 @@ KV8_KERNELS = ("few", "prompt")
 
 def kv8_attention_plan(batch: int, tokens: int, max_tokens: int, max_len: int, heads: int, kv_heads: int, dim: int, window: int = 0,
                        workspace_bytes: int = WORKSPACE_MAX_BYTES, compute_units: int = 0):
-    """(kernel name, slices of the keys, bytes of workspace these take) kv8_attention would use for a call of these sizes
-    (lq_kv8_attention_plan). Launches nothing, as a16w4_plan."""
+    """(kernel name, parts, bytes of workspace these take) kv8_attention would use for a call of these sizes (lq_kv8_attention_plan):
+    parts are workgroups that share the keys ("few"; 0: one for each sequence and kv head) or slices of the keys ("prompt"; 1: whole).
+    Launches nothing, as a16w4_plan."""
     import ctypes
-    kernel, slices, needed = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
+    kernel, parts, needed = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
     _C.call("lq_kv8_attention_plan", batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, workspace_bytes, compute_units,
-            ctypes.addressof(kernel), ctypes.addressof(slices), ctypes.addressof(needed))
-    return KV8_KERNELS[kernel.value], slices.value, needed.value
+            ctypes.addressof(kernel), ctypes.addressof(parts), ctypes.addressof(needed))
+    return KV8_KERNELS[kernel.value], parts.value, needed.value
 
 
 def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,

@@ -102,12 +102,12 @@ def test_rows_that_see_nothing(hip_lib, tokens):
 
 @pytest.mark.parametrize("tokens", [1, 20, 90])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_slices_of_the_keys(hip_lib, tokens, dim):
+def test_parts_of_the_keys(hip_lib, tokens, dim):
     """Long keys for few rows: several workgroups to a row and a second launch; the same rows without a workspace agree."""
     from latentq_llm_amd import _C, ops
     lens, news, heads = [5000, 3000], [tokens, tokens], 2
-    kernel, slices, _ = ops.kv8_attention_plan(2, 2 * tokens, tokens, 5000, heads, heads, dim)
-    assert slices > 1
+    kernel, parts, _ = ops.kv8_attention_plan(2, 2 * tokens, tokens, 5000, heads, heads, dim)
+    assert parts > 1
     run(lens, news, heads, heads, dim, F16, seed=3)
     run(lens, news, heads, heads, dim, F16, seed=3, window=900)
     cache = ref.Cache(130, heads, dim, seed=4)
@@ -120,6 +120,28 @@ def test_slices_of_the_keys(hip_lib, tokens, dim):
     want, _, bound = ref.attention(cache, q.cpu(), table, lens, news)
     holds(one, want, bound)
     holds(ops.kv8_attention(q, *tensors, t, n), want, bound)
+
+
+@pytest.mark.parametrize("batch", [3, 70, 200])
+def test_shares_over_a_batch(hip_lib, batch):
+    """Equal shares of all tiles: units of one tile to many, sequences without new tokens and without keys between them, more than
+    one pass of 64 sequences; and repeated calls give the same bits."""
+    from latentq_llm_amd import ops
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in np.exp2(rng.uniform(0, 8.5, batch))]
+    lens[1], lens[0] = 3300, 0
+    if batch > 3:
+        lens[-1], lens[64], lens[65] = 1700, 0, 2
+    for most in (1, 3):
+        news = [most if i % 4 else min(most, i % 3) for i in range(batch)]
+        assert ops.kv8_attention_plan(batch, sum(news), most, 20000, 4, 2, 64)[1] > 1
+        run(lens, news, 4, 2, 64, BF16, seed=batch, max_len=20000, max_tokens=most, width=313)
+        run(lens, news, 4, 2, 64, BF16, seed=batch, max_len=20000, max_tokens=most, width=313, window=200)
+    cache = ref.Cache(sum(-(-n // 64) for n in lens) + 1, 2, 64)
+    table, t = ref.blocks_of(lens, len(cache.scale[0])), cache.tensors()
+    q = rows((batch, 4, 64), BF16, 1)
+    first = call(t, q, table, lens, [1] * batch)
+    assert all(torch.equal(call(t, q, table, lens, [1] * batch), first) for _ in range(3))
 
 
 def test_a_max_len_that_is_too_small_costs_nothing_but_time(hip_lib):

@@ -79,16 +79,20 @@ def test_plan_of_attention(hip_lib):
     # rows of a kv head: tokens times the query heads that share it
     assert plan(1, 1, 1019, 32, 32)[0] == plan(1, 64, 1019, 32, 32)[0] == plan(1, 16, 1019, 32, 8)[0] == "few"
     assert plan(1, 65, 1019, 32, 32)[0] == plan(1, 17, 1019, 32, 8)[0] == plan(1, 33, 1019, 32, 32, 256)[0] == "prompt"
-    # enough workgroups, or few keys: one slice, no workspace
-    assert plan(64, 1, 8192, 32, 32)[1:] == plan(1, 8192, 8192, 32, 32)[1:] == plan(1, 1, 64, 32, 32)[1:] == (1, 0)
-    # few rows on many keys: slices, whose partial results fit the workspace
-    for case in ((1, 1, 131072, 32, 8), (1, 512, 16384, 32, 8), (2, 5, 4096, 8, 8)):
-        kernel, slices, needed = plan(*case)
-        assert slices > 1 and needed == slices * case[0] * case[1] * case[3] * 129 * 4 <= ops.WORKSPACE_MAX_BYTES
-        assert plan(*case, workspace_bytes=0)[1:] == (1, 0)
-        assert plan(*case, workspace_bytes=needed // slices * 2)[1] == 2
-    # a window bounds the keys that are cut
-    assert plan(1, 1, 131072, 32, 8, window=128)[1] < plan(1, 1, 131072, 32, 8)[1]
-    assert plan(0, 0, 0, 8, 8) == ("few", 1, 0)
+    # enough workgroups, or few keys: nothing to join, no workspace
+    assert plan(64, 1, 2048, 32, 32)[1:] == plan(1, 1, 64, 32, 32)[1:] == (0, 0) and plan(1, 8192, 8192, 32, 32)[1:] == (1, 0)
+    # few rows on many keys: shares, whose partial results fit the workspace
+    for case in ((1, 1, 131072, 32, 8), (2, 5, 4096, 8, 8), (64, 1, 8192, 32, 8)):
+        kernel, parts, needed = plan(*case)
+        assert parts > 1 and needed == 2 * parts * case[1] * case[3] // case[4] * 129 * 4 <= ops.WORKSPACE_MAX_BYTES
+        assert plan(*case, workspace_bytes=0)[1:] == (0, 0)
+        assert plan(*case, workspace_bytes=needed // parts * 2)[1] == 2
+    # a piece of a prompt: slices
+    kernel, parts, needed = plan(1, 512, 16384, 32, 8)
+    assert parts > 1 and needed == parts * 512 * 32 * 129 * 4 <= ops.WORKSPACE_MAX_BYTES
+    assert plan(1, 512, 16384, 32, 8, workspace_bytes=0)[1:] == (1, 0)
+    # a window bounds the keys
+    assert plan(1, 1, 131072, 32, 8, window=128)[1] == 0
+    assert plan(0, 0, 0, 8, 8) == ("few", 0, 0)
     with pytest.raises(LatentQError, match="multiple of kv heads"):
         plan(1, 1, 100, 8, 3)
