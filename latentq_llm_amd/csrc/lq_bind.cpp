@@ -20,21 +20,27 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "../../include/latentq.h"
 
 namespace {
 
 PyObject *g_error = nullptr;  // LatentQError
 
+constexpr c10::DispatchKeySet kWrappedKeys({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Batched,
+                                            c10::DispatchKey::Functionalize, c10::DispatchKey::Python, c10::DispatchKey::ZeroTensor,
+                                            c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
+
+constexpr int64_t kWorkspaceBytes = 64 << 20;  // what ops.py keeps for each device, stream and host thread
+
 // A plain tensor (Tensor or Parameter, no other subclass) on a GPU, contiguous, of the given type. The wrappers of function
 // transforms (vmap, functional gradients, functionalisation) have the Python type of a plain tensor and no memory of their own.
 const at::Tensor *plain(PyObject *o, at::ScalarType type) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor &t = THPVariable_Unpack(o);
-    constexpr c10::DispatchKeySet kWrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                            c10::DispatchKey::Batched, c10::DispatchKey::Functionalize, c10::DispatchKey::Python,
-                                            c10::DispatchKey::ZeroTensor, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
-    if (t.key_set().has_any(kWrapped) || !t.has_storage()) return nullptr;
+    if (t.key_set().has_any(kWrappedKeys) || !t.has_storage()) return nullptr;
     return t.is_cuda() && t.scalar_type() == type && t.is_contiguous() ? &t : nullptr;
 }
 
@@ -603,6 +609,168 @@ PyObject *adam8_w8(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     return a[11];
 }
 
+// ---- paged 8-bit cache of keys and values
+// Rows [tokens, heads, dim] of a 16-bit type in the strides the kernels take, without a gradient to keep
+struct Rows16 {
+    const at::Tensor *t = nullptr;
+    int dtype = 0;  // as the C entry points number them
+    bool load(PyObject *o) {
+        if (!THPVariable_CheckExact(o)) return false;
+        const at::Tensor &x = THPVariable_Unpack(o);
+        const bool f16 = x.scalar_type() == at::kHalf;
+        if (!x.is_cuda() || (!f16 && x.scalar_type() != at::kBFloat16) || x.dim() != 3 || x.numel() == 0 || !x.has_storage()) return false;
+        if (x.key_set().has_any(kWrappedKeys) || x.stride(2) != 1 || x.stride(0) % 8 || x.stride(1) % 8 || !aligned16(&x)) return false;
+        if (x.requires_grad() && c10::GradMode::is_enabled()) return false;
+        t = &x;
+        dtype = f16;
+        return true;
+    }
+    // rows of their own, to be written
+    bool separate() const {
+        return (t->size(0) == 1 || t->stride(0) >= t->size(2)) && (t->size(1) == 1 || t->stride(1) >= t->size(2));
+    }
+};
+
+struct Cache8 {
+    const at::Tensor *kc, *vc, *ks, *vs;
+    int64_t blocks, heads, dim;
+    bool load(PyObject *const *a) {
+        kc = plain(a[0], at::kByte);
+        vc = plain(a[1], at::kByte);
+        ks = plain(a[2], at::kFloat);
+        vs = plain(a[3], at::kFloat);
+        if (!kc || !vc || !ks || !vs || kc->dim() != 4 || vc->dim() != 5 || ks->dim() != 2 || vs->dim() != 2) return false;
+        blocks = kc->size(0);
+        heads = kc->size(1);
+        dim = kc->size(3);
+        return blocks > 0 && heads > 0 && kc->size(2) == LQ_KV_BLOCK && (dim == 64 || dim == 96 || dim == 128 || dim == 256) &&
+               vc->sizes() == at::IntArrayRef({blocks, heads, LQ_KV_BLOCK / 4, dim, 4}) && ks->sizes() == at::IntArrayRef({blocks, heads}) &&
+               vs->sizes() == ks->sizes() && same_device(kc, vc) && same_device(kc, ks) && same_device(kc, vs) && aligned16(kc) && aligned16(vc);
+    }
+};
+
+// block_table, seq_lens; cu_tokens and max_tokens (None: what the rows allow)
+struct Sequences {
+    const at::Tensor *table, *lens;
+    const int32_t *cu = nullptr;
+    int64_t batch, width, most;
+    bool load(PyObject *o_table, PyObject *o_lens, PyObject *o_cu, PyObject *o_most, int64_t tokens, const at::Tensor *like) {
+        table = plain(o_table, at::kInt);
+        lens = plain(o_lens, at::kInt);
+        if (!table || !lens || table->dim() != 2 || lens->dim() != 1 || !same_device(table, like) || !same_device(lens, like)) return false;
+        batch = table->size(0);
+        width = table->size(1);
+        if (batch == 0 || width == 0 || lens->size(0) != batch) return false;
+        most = tokens;
+        if (o_cu != Py_None) {
+            const at::Tensor *c = plain(o_cu, at::kInt);
+            if (!c || c->dim() != 1 || c->size(0) != batch + 1 || !same_device(c, like)) return false;
+            cu = (const int32_t *)c->data_ptr();
+        } else {
+            if (tokens % batch) return false;
+            most = tokens / batch;
+        }
+        if (o_most == Py_None) return true;
+        const int64_t given = integer(o_most);
+        if (given <= 0 || (!cu && given < most)) return false;
+        most = std::min(most, given);
+        return true;
+    }
+};
+
+// k, v, cache (4), block_table, seq_lens, q, cos, sin, cu_tokens, max_tokens, q_out -> the rotated q, or True without one
+PyObject *kv8_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    LQ_ARGS(14)
+    Rows16 k, v, q, o;
+    Cache8 c;
+    Sequences s;
+    const bool with_q = a[8] != Py_None, rotates = a[9] != Py_None;
+    if (!k.load(a[0]) || !v.load(a[1]) || !c.load(a + 2) || !same_device(k.t, c.kc) || !same_device(v.t, c.kc) || k.dtype != v.dtype ||
+        k.t->size(1) != c.heads || k.t->size(2) != c.dim || v.t->sizes() != k.t->sizes() || rotates != (a[10] != Py_None) || (with_q && !rotates) ||
+        (!with_q && a[13] != Py_None))
+        return none();
+    const int64_t tokens = k.t->size(0);
+    if (!s.load(a[6], a[7], a[11], a[12], tokens, c.kc)) return none();
+    const at::Tensor *cos = rotates ? plain(a[9], at::kFloat) : nullptr, *sin = rotates ? plain(a[10], at::kFloat) : nullptr;
+    if (rotates && (!cos || !sin || cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->numel() == 0 || cos->size(1) % 8 || 2 * cos->size(1) > c.dim ||
+                    !same_device(cos, c.kc) || !same_device(sin, c.kc) || !aligned16(cos) || !aligned16(sin)))
+        return none();
+    if (with_q && (!q.load(a[8]) || !same_device(q.t, c.kc) || q.dtype != k.dtype || q.t->size(0) != tokens || q.t->size(2) != c.dim)) return none();
+    if (a[13] != Py_None && (!o.load(a[13]) || !same_device(o.t, c.kc) || o.dtype != k.dtype || o.t->sizes() != q.t->sizes() || !o.separate())) return none();
+    On on(*c.kc);
+    at::Tensor made;
+    if (with_q && !o.t) {
+        made = make(q.t->sizes(), q.t->scalar_type(), *q.t);
+        o.t = &made;
+    }
+    LQ_CALL(lq_kv8_append, k.t->data_ptr(), k.t->stride(0), k.t->stride(1), v.t->data_ptr(), v.t->stride(0), v.t->stride(1),
+            with_q ? q.t->data_ptr() : nullptr, with_q ? q.t->stride(0) : 0, with_q ? q.t->stride(1) : 0, with_q ? o.t->data_ptr() : nullptr,
+            with_q ? o.t->stride(0) : 0, with_q ? o.t->stride(1) : 0, rotates ? (const float *)cos->data_ptr() : nullptr,
+            rotates ? (const float *)sin->data_ptr() : nullptr, rotates ? cos->size(0) : 0, rotates ? (int)(2 * cos->size(1)) : 0, c.kc->data_ptr(),
+            c.vc->data_ptr(), (float *)c.ks->data_ptr(), (float *)c.vs->data_ptr(), c.blocks, (const int32_t *)s.table->data_ptr(), s.width,
+            (const int32_t *)s.lens->data_ptr(), s.cu, s.batch, tokens, s.most, with_q ? (int)q.t->size(1) : 0, (int)c.heads, (int)c.dim, k.dtype, on.stream);
+    if (!with_q) Py_RETURN_TRUE;
+    if (made.defined()) return wrap(std::move(made));
+    Py_INCREF(a[13]);
+    return a[13];
+}
+
+// q, cache (4), block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, causal, window, return_lse, workspace -> out, or (out, lse);
+// without a workspace where one is wanted: its bytes, and nothing is done
+PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    LQ_ARGS(15)
+    Rows16 q;
+    Cache8 c;
+    Sequences s;
+    if (!q.load(a[0]) || !c.load(a + 1) || !same_device(q.t, c.kc) || q.t->size(2) != c.dim || q.t->size(1) % c.heads) return none();
+    const int64_t tokens = q.t->size(0), heads = q.t->size(1);
+    if (!s.load(a[5], a[6], a[7], a[8], tokens, c.kc)) return none();
+    int64_t max_len = s.width * LQ_KV_BLOCK;
+    if (a[9] != Py_None) {
+        const int64_t given = integer(a[9]);
+        if (given < 0) return none();
+        max_len = std::min(max_len, given);
+    }
+    const double scale = a[10] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(a[10]);
+    const int64_t window = a[12] == Py_None ? 0 : integer(a[12]);
+    const int causal = PyObject_IsTrue(a[11]), with_lse = PyObject_IsTrue(a[13]);
+    if (PyErr_Occurred() || !(scale > 0.0 && scale <= 3.4e38) || window < 0) return none();
+    void *ws;
+    int64_t ws_bytes;
+    if (!workspace(a[14], q.t, &ws, &ws_bytes)) return none();
+    On on(*c.kc);
+    if (!ws) {
+        int kernel, parts;
+        int64_t needed;
+        if (const int rc = lq_kv8_attention_plan(s.batch, tokens, s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, window, kWorkspaceBytes, 0, &kernel, &parts, &needed))
+            return fail("lq_kv8_attention_plan", rc);
+        if (needed) return PyLong_FromLongLong(needed);
+    }
+    at::Tensor out = make(q.t->sizes(), q.t->scalar_type(), *q.t), lse;
+    if (with_lse) lse = make({tokens, heads}, at::kFloat, *q.t);
+    LQ_CALL(lq_kv8_attention, q.t->data_ptr(), q.t->stride(0), q.t->stride(1), c.kc->data_ptr(), c.vc->data_ptr(), (const float *)c.ks->data_ptr(),
+            (const float *)c.vs->data_ptr(), c.blocks, (const int32_t *)s.table->data_ptr(), s.width, (const int32_t *)s.lens->data_ptr(), s.cu, s.batch, tokens,
+            s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, window, out.data_ptr(), out.stride(0), out.stride(1),
+            with_lse ? (float *)lse.data_ptr() : nullptr, ws, ws_bytes, on.stream);
+    if (!with_lse) return wrap(std::move(out));
+    return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
+}
+
+// cache (4), blocks, dtype as the C entry points number them -> (k, v)
+PyObject *kv8_read(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    LQ_ARGS(6)
+    Cache8 c;
+    const at::Tensor *b = plain(a[4], at::kInt);
+    const int64_t dtype = integer(a[5]);
+    if (!c.load(a) || !b || b->dim() != 1 || b->numel() == 0 || !same_device(b, c.kc) || dtype < 0 || dtype > 2) return none();
+    On on(*c.kc);
+    const at::ScalarType type = dtype == 0 ? at::kBFloat16 : dtype == 1 ? at::kHalf : at::kFloat;
+    at::Tensor k = make({b->numel(), LQ_KV_BLOCK, c.heads, c.dim}, type, *c.kc), v = make(k.sizes(), type, *c.kc);
+    LQ_CALL(lq_kv8_read, c.kc->data_ptr(), c.vc->data_ptr(), (const float *)c.ks->data_ptr(), (const float *)c.vs->data_ptr(), c.blocks,
+            (const int32_t *)b->data_ptr(), b->numel(), (int)c.heads, (int)c.dim, (int)dtype, k.data_ptr(), v.data_ptr(), on.stream);
+    return Py_BuildValue("NN", wrap(std::move(k)), wrap(std::move(v)));
+}
+
 // device index -> the current stream's handle
 PyObject *current_stream(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     LQ_ARGS(1)
@@ -651,7 +819,7 @@ PyMethodDef methods[] = {
     LQ_METHOD(linear4), LQ_METHOD(linear4_eval), LQ_METHOD(dx4), LQ_METHOD(gate_up), LQ_METHOD(dx_silu), LQ_METHOD(dx_pair), LQ_METHOD(linear8), LQ_METHOD(infer8),
     LQ_METHOD(infer8_eval), LQ_METHOD(dx8), LQ_METHOD(quant8), LQ_METHOD(quant8_token), LQ_METHOD(dequant8), LQ_METHOD(weight_grad),
     LQ_METHOD(weight_grad_acc), LQ_METHOD(weight_grad_acc8), LQ_METHOD(gradq8), LQ_METHOD(adam8_param), LQ_METHOD(adam8_sr),
-    LQ_METHOD(adam8_queue), LQ_METHOD(adam8_run), LQ_METHOD(adam8_w4), LQ_METHOD(adam8_w8), LQ_METHOD(current_stream),
+    LQ_METHOD(adam8_queue), LQ_METHOD(adam8_run), LQ_METHOD(adam8_w4), LQ_METHOD(adam8_w8), LQ_METHOD(kv8_append), LQ_METHOD(kv8_attention), LQ_METHOD(kv8_read), LQ_METHOD(current_stream),
     LQ_METHOD(records_plainly), LQ_METHOD(set_error), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lqbind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1045,6 +1045,9 @@ def kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
     keys are rotated by their position, and so is q [tokens, heads, dim], which is returned (q_out may be q itself). With
     several tokens a sequence, cu_tokens (int32 [batch + 1]) has each sequence's first row; max_tokens, the largest number of new tokens
     of a sequence, sizes the launch (default: what the number of rows allows). Returns the rotated q, or None."""
+    done = (_native or _fast()).kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, q, cos, sin, cu_tokens, max_tokens, q_out)
+    if done is not None:
+        return None if q is None else done
     n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     k = _kv8_layout(_kv8_rows(k, "k", kv_heads, dim, k_codes))
     v = _kv8_layout(_kv8_rows(v, "v", kv_heads, dim, k_codes, k.dtype))
@@ -1092,6 +1095,9 @@ def kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
 def kv8_read(k_codes, v_codes, k_scale, v_scale, blocks, dtype=torch.bfloat16):
     """(keys, values) [n, 64, kv_heads, dim] that the n blocks (int32) of a paged 8-bit cache stand for (lq_kv8_read), as bfloat16,
     float16 or float32."""
+    r = (_native or _fast()).kv8_read(k_codes, v_codes, k_scale, v_scale, blocks, _KV_TYPES.get(dtype, -1))
+    if r is not None:
+        return r
     n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     _chk(blocks, torch.int32, "blocks")
     if blocks.dim() != 1 or blocks.device != k_codes.device:
@@ -1129,6 +1135,13 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
     the positions up to its own (causal=False: the whole sequence), with window > 0 only the last `window` of them; one that sees
     nothing gives zeros. max_tokens and max_len, the largest numbers of new tokens and of tokens of a sequence, size the launch
     (defaults: what the rows and the block table allow). return_lse: also the logarithm of the softmax's denominator, float32 [tokens, heads]."""
+    if out is None:
+        args = (q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, causal, window, return_lse)
+        r = (_native or _fast()).kv8_attention(*args, None)
+        if type(r) is int:  # the bytes that its parts want
+            r = _native.kv8_attention(*args, _workspace(q, 1, -(-r // 32))[0])
+        if r is not None:
+            return r
     n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     _kv8_rows(q, "q", None, dim, k_codes)
     tokens, heads = q.shape[0], q.shape[1]
