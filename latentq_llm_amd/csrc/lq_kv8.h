@@ -63,6 +63,12 @@ __device__ __forceinline__ unsigned kv8_pack_f16(float a, float b) {  // v_cvt_p
     return __builtin_bit_cast(unsigned, h);
 }
 
+// sum + both halves of a word, in fp32 (v_dot2_f32_f16)
+__device__ __forceinline__ float kv8_add_halves(unsigned w, float sum) {
+    const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), one, sum, false);
+}
+
 template <bool kF16>
 __device__ __forceinline__ unsigned kv8_pack(float a, float b) {
     if constexpr (kF16) return kv8_pack_f16(a, b);

@@ -9,6 +9,8 @@
 
 namespace {
 
+constexpr float kLazy = 8.0f;
+
 template <int D, bool kF16>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
     constexpr int kSteps = D / 16, kTiles = D / 32, kPieces = D / 8;
@@ -81,37 +83,51 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
     float M = kNone, L = 0.0f;
 
     const int *table = a.table + (int64_t)seq * a.width;
-    const auto block_of = [&](int t) { return (int64_t)min((unsigned)table[t], (unsigned)(a.blocks - 1)) * a.kv_heads + h; };
-    // place of a key row's 16-byte piece: exchanged within 8 pieces by the row, within 4 where the last ones are only 4 (96 dimensions)
-    const auto placed = [](int piece, int row) { return piece ^ (row & (piece < (kPieces & ~7) ? 7 : 3)); };
-    // A thread's part of a tile: 16 bytes of keys (16 dimensions of a token) and of values (4 tokens of 4 dimensions) at a time
-    constexpr int kAll = KV8_BLOCK * D / 16, kN = (kAll + 255) / 256;
-    u32x4_t kr[kN], vr[kN];
+    const auto block_of = [&](int t) { return (int64_t)min((unsigned)kv8_uniform(table + t), (unsigned)(a.blocks - 1)) * a.kv_heads + h; };
+    // Shared memory gives 16 lanes their 16 bytes at a time from 64 banks, so the lanes of such a group go to 16 different places of
+    // 256 bytes. Keys: 16 rows at one piece; pieces are exchanged by bits of the row. Values: 16 dimensions that follow each other
+    // (read) or are 4 apart (written); a dimension moves on within its 16 by the number of the 16. (Without: 63 % of the cycles
+    // that shared memory was busy were conflicts, 650 us for 8192 tokens of 32 heads.)
+    const auto placed = [](int piece, int row) { return piece ^ (D == 64 ? row >> 1 & 7 : D == 96 ? row >> 2 & 3 : row & 15); };
+    const auto dim_at = [](int d) { return d ^ (d >> 4 & 3); };
+    // A thread's part of a tile: 16 bytes of keys (16 dimensions of a token) at a time; of values 4 dimensions of the 8 tokens that
+    // make an operand, two groups of 4
+    constexpr int kKeys = KV8_BLOCK * D / 16, kNk = (kKeys + 255) / 256, kValues = kKeys / 2, kNv = (kValues + 255) / 256;
+    u32x4_t kr[kNk], vr[kNv][2];
     const auto request = [&](int64_t bh) {
         const u32x4_t *k = (const u32x4_t *)(a.k + bh * (KV8_BLOCK * D)), *v = (const u32x4_t *)(a.v + bh * (KV8_BLOCK * D));
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
+        for (int i = 0; i < kNk; ++i) {
             const int u = threadIdx.x + i * 256;
-            if (kAll % 256 == 0 || u < kAll) {
-                kr[i] = k[u];
-                vr[i] = v[u];
+            if (kKeys % 256 == 0 || u < kKeys) kr[i] = k[u];
+        }
+#pragma unroll
+        for (int i = 0; i < kNv; ++i) {
+            // operand (step e, half h) has groups 4 e + h and 4 e + h + 2
+            const int u = threadIdx.x + i * 256, pair = u / (D / 4), group = (pair >> 1) * 4 + (pair & 1), d = u % (D / 4);
+            if (kValues % 256 == 0 || u < kValues) {
+                vr[i][0] = v[group * (D / 4) + d];
+                vr[i][1] = v[(group + 2) * (D / 4) + d];
             }
         }
     };
     const auto store = [&](int buffer) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            const int u = threadIdx.x + i * 256;
-            if (kAll % 256 == 0 || u < kAll) {
-                const int t = u / (D / 16), piece = u % (D / 16) * 2;
+        for (int i = 0; i < kNk; ++i) {
+            const int u = threadIdx.x + i * 256, t = u / (D / 16), piece = u % (D / 16) * 2;
+            if (kKeys % 256 == 0 || u < kKeys) {
                 u32x4_t *row_at = lds_k[buffer] + t * kPieces;
                 row_at[placed(piece, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[i][0], kr[i][1]));
                 row_at[placed(piece + 1, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[i][2], kr[i][3]));
-                // 4-token group c belongs to step c / 4, half c & 1, first or second 4 tokens of the operand by bit 1
-                const int c = u / (D / 4), d = u % (D / 4) * 4;
-                u32x2_t *v_at = (u32x2_t *)(lds_v[buffer] + ((c >> 2) * 2 + (c & 1)) * D + d) + ((c >> 1) & 1);
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v_at[2 * j] = kv8_halves(vr[i][j]);
+        for (int i = 0; i < kNv; ++i) {
+            const int u = threadIdx.x + i * 256, pair = u / (D / 4), d = u % (D / 4) * 4;
+            if (kValues % 256 == 0 || u < kValues) {
+                u32x4_t *v_at = lds_v[buffer] + pair * D;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v_at[dim_at(d + j)] = __builtin_bit_cast(u32x4_t, kv8_operand(vr[i][0][j], vr[i][1][j]));
             }
         }
     };
@@ -121,8 +137,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
     if (t_lo < t_hi) {
         bh_next = block_of(t_lo);
         request(bh_next);
-        ks_next = a.ks[bh_next];
-        vs_next = a.vs[bh_next];
+        ks_next = kv8_uniform(a.ks + bh_next);
+        vs_next = kv8_uniform(a.vs + bh_next);
         store(0);
         ks = ks_next;
         vs = vs_next;
@@ -133,23 +149,41 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
         if (t + 1 < t_hi) {
             bh_next = block_of(t + 1);
             request(bh_next);
-            ks_next = a.ks[bh_next];
-            vs_next = a.vs[bh_next];
+            ks_next = kv8_uniform(a.ks + bh_next);
+            vs_next = kv8_uniform(a.vs + bh_next);
         }
         const int key0 = t * KV8_BLOCK;
         if (key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before) {
+            // Two chains of products at a time (keys 0 .. 31 and 32 .. 63), operands read two steps ahead of them.
             f32x16_t c[2];
+            f16x8_t k[2][4];
+            const auto read_k = [&](int set, int i) {  // steps i and i + 1
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+                for (int y = 0; y < 4; ++y) {
+                    const int at = (y & 1) * 32 + col;
+                    k[set][y] = __builtin_bit_cast(f16x8_t, lds_k[buffer][at * kPieces + placed(2 * (i + (y >> 1)) + half, at)]);
+                }
+            };
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) c[x][j] = 0.0f;
-                const int at = x * 32 + col;
+            read_k(0, 0);
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const f16x8_t k = __builtin_bit_cast(f16x8_t, lds_k[buffer][at * kPieces + placed(2 * i + half, at)]);
-                    c[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[i], c[x], 0, 0, 0);
-                }
+            for (int i = 0; i < kSteps; i += 2) {
+                if (i + 2 < kSteps) read_k((i >> 1 & 1) ^ 1, i + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) c[y & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i >> 1 & 1][y], q[i + (y >> 1)], c[y & 1], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            // values of the first 16 keys: under the softmax
+            f16x8_t v[2][kTiles];
+            const auto read_v = [&](int set, int e) {
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) v[set][i] = __builtin_bit_cast(f16x8_t, lds_v[buffer][(2 * e + half) * D + dim_at(32 * i + col)]);
+            };
+            read_v(0, 0);
             // accumulator element j is key 32 x + (j & 3) + 8 (j >> 2) + 4 half
             if (__any(key0 + KV8_BLOCK - 1 > last || key0 <= before)) {
 #pragma unroll
@@ -160,40 +194,40 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
                         if (key > last || key <= before) c[x][j] = -__builtin_inff();
                     }
             }
-            const float f = fmaxf(ks * factor, 0x1p-100f), lv = __builtin_amdgcn_logf(vs), rv = 1.0f / vs;
+            const float f = fmaxf(ks * factor, 0x1p-100f), lv = __builtin_amdgcn_logf(vs), rv = __builtin_amdgcn_rcpf(vs);
             float most = c[0][0];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) most = fmaxf(most, c[x][j]);
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float m = fmaxf(M, fmaf(most, f, lv)), shift = lv - m, fade = __builtin_amdgcn_exp2f(M - m);
-            if (__any(m > M)) {
+            most = fmaf(kv8_max32(most), f, lv);
+            // The maximum moves only when it grows by kLazy or more: until then weights are up to 2^kLazy, which f16 holds as well
+            if (__any(most > M + kLazy)) {
+                const float m = fmaxf(M, most), fade = __builtin_amdgcn_exp2f(M - m);
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) o[i] *= fade;
+                L *= fade;
+                M = m;
             }
-            M = m;
+            const float shift = lv - M;
             float sum = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    c[x][j] = __builtin_amdgcn_exp2f(fmaf(c[x][j], f, shift));
-                    sum += c[x][j];
-                }
-            L = fmaf(sum, rv, L * fade);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {  // 16 keys
+            for (int e = 0; e < 4; ++e) {  // 16 keys: their weights, then their products, which run under the next ones' weights
+                if (e < 3) read_v(~e & 1, e + 1);
                 u32x4_t w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = kv8_pack_f16(c[e >> 1][8 * (e & 1) + 2 * j], c[e >> 1][8 * (e & 1) + 2 * j + 1]);
-                const f16x8_t p = __builtin_bit_cast(f16x8_t, w);
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) {
-                    const f16x8_t v = __builtin_bit_cast(f16x8_t, lds_v[buffer][(2 * e + half) * D + 32 * i + col]);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[i], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) {
+                    const float x0 = __builtin_amdgcn_exp2f(fmaf(c[e >> 1][8 * (e & 1) + 2 * j], f, shift));
+                    const float x1 = __builtin_amdgcn_exp2f(fmaf(c[e >> 1][8 * (e & 1) + 2 * j + 1], f, shift));
+                    w[j] = kv8_pack_f16(x0, x1);
+                    sum = kv8_add_halves(w[j], sum);
                 }
+                const f16x8_t p = __builtin_bit_cast(f16x8_t, w);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e & 1][i], p, o[i], 0, 0, 0);
             }
+            L = fmaf(sum, rv, L);
         }
         if (t + 1 < t_hi) {
             store(buffer ^ 1);
