@@ -63,12 +63,6 @@ __device__ __forceinline__ unsigned kv8_pack_f16(float a, float b) {  // v_cvt_p
     return __builtin_bit_cast(unsigned, h);
 }
 
-// sum + both halves of a word, in fp32 (v_dot2_f32_f16)
-__device__ __forceinline__ float kv8_add_halves(unsigned w, float sum) {
-    const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), one, sum, false);
-}
-
 template <bool kF16>
 __device__ __forceinline__ unsigned kv8_pack(float a, float b) {
     if constexpr (kF16) return kv8_pack_f16(a, b);
@@ -124,7 +118,7 @@ struct Kv8Attn {
     int workgroups;               // few rows: that share all tiles; 0: one for each (sequence, kv head)
     int rows;                     // few rows: of a slot, max_tokens * heads / kv_heads
     int slices, tiles;            // prompt: slices of the keys, tiles of 64 keys in each; slots are slices, rows those of the operands
-    int row_tiles;                // prompt: workgroups along a sequence's rows
+    int row_tiles, waves;         // prompt: workgroups along a sequence's rows, of so many waves with 32 rows each
 };
 
 // The new tokens of one sequence: rows start .. start + n - 1 of the operands, its length in the cache, the position of the first,

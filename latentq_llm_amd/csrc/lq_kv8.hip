@@ -293,20 +293,24 @@ bool good_dim(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 2
 struct Plan {
     bool few;
     int workgroups;                // few rows: that share all tiles, 0: one for each (sequence, kv head)
-    int slices, tiles, row_tiles;  // prompt
+    int slices, tiles, row_tiles, waves;  // prompt
     int64_t slots, slot_rows;      // of the workspace
 };
 
-// Most rows of the kernel for few: beyond it the prompt kernel (its tiles of 128 rows)
-int most_rows(int dim) { return dim <= 128 ? 64 : 32; }
+// Whether the kernel of few rows takes a call: rows of a (sequence, kv head), tiles of 64 keys of the longest sequence. It reads keys into
+// operands by itself, which the prompt kernel's workgroups of 128 rows share, and its accumulators cost waves from 17 rows on: us few / prompt,
+// 32 heads on 32: 20 rows 128 dimensions on 64 keys 7.8 / 6.1, 1024 keys 14.9 / 11.8, 16384 keys 30.4 / 61.1, 8 times 2048 keys 26.4 / 58.1;
+// 45 rows 64 dimensions 8.9 / 5.4, 16.7 / 11.3, 31.2 / 56.4, 27.0 / 53.0. 33 rows of 128 dimensions and 17 of 256 do not fit its
+// registers (45 rows of 128 dimensions 14.4 / 6.3, 33.2 / 14.4, 68.1 / 64.1, 62.5 / 60.2).
+bool takes_few(int64_t rows, int64_t tiles, int dim) { return rows <= 16 || (tiles >= 24 && rows <= (dim <= 96 ? 64 : dim == 128 ? 32 : 16)); }
 
 Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t width, int64_t workspace, int cus) {
     Plan p{};
     const int64_t rows = max_tokens * (heads / kv_heads), units = batch * kv_heads;
-    p.few = rows <= most_rows(dim);
     int64_t keys = max_len;
     if (window && window + max_tokens + KV8_BLOCK < keys) keys = window + max_tokens + KV8_BLOCK;
     const int64_t tiles = keys > 0 ? (keys + KV8_BLOCK - 1) / KV8_BLOCK : 1;
+    p.few = takes_few(rows, tiles, dim);
     if (p.few) {
         // One workgroup for a (sequence, kv head) and one launch, or the tiles of all of them in equal shares and a launch that
         // joins (2 to 3 us): a unit up to 16 KiB of keys and values for each of its tiles goes through a compute unit at some 40 GB/s, so
@@ -323,16 +327,33 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
         p.slot_rows = rows;
         p.slices = 1;
     } else {
-        p.row_tiles = (int)((rows + 127) / 128);
-        const int64_t want = 2 * (int64_t)cus, least = 8, slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;  // workgroups, tiles of a slice
-        int64_t slices = units * p.row_tiles >= want ? 1 : (want + units * p.row_tiles - 1) / (units * p.row_tiles);
-        if (slices > 64) slices = 64;
-        if (slices > 1 && slices > workspace / slice_bytes) slices = workspace / slice_bytes;
-        if (slices < 1) slices = 1;
-        int64_t per = (tiles + slices - 1) / slices;
-        if (per < least) per = least;
-        p.slices = (int)((tiles + per - 1) / per);
-        p.tiles = (int)per;
+        // Slices of the keys, and waves of a workgroup, by an estimate in us. A tile takes `busy` of a compute unit that has workgroups
+        // enough, and `alone` at least in each workgroup; the ways in and out cost 3 tiles; slices take their partial results there and
+        // back (4.5 TB/s) and a launch. With 8 waves a row has half the conversions, but there are half the workgroups: single sequences of
+        // 4096 tokens (32 heads of 128) 160 -> 147 us, 1024 on 16384 keys 289 -> 270, but 2048 tokens 54 -> 64, 4 x 1019 39 -> 43. By slices,
+        // measured / estimated: 64 dimensions, 256 tokens on 16384 keys in 4 75 / 80, in 8 59 / 65; 96 dimensions, 12 heads, 2048 tokens in 1
+        // 58 / 56, in 3 39 / 41.
+        const double busy4 = dim == 64 ? 0.73 : dim == 96 ? 0.9 : dim == 128 ? 1.15 : 2.2, alone4 = dim == 64 ? 1.05 : dim == 96 ? 1.6 : dim == 128 ? 1.45 : 2.2;
+        const int64_t slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;
+        const double mean = (double)tiles - (double)max_tokens / (2 * KV8_BLOCK);  // of the rows' tiles, where all of them are causal
+        double best = 0;
+        for (const int waves : {4, 8}) {
+            if (waves == 8 && (dim != 128 || tiles < 64)) break;
+            const int64_t row_tiles = (rows + 32 * waves - 1) / (32 * waves);
+            const double busy = waves == 4 ? busy4 : 2.1, alone = waves == 4 ? alone4 : 2.1;
+            for (int64_t s = 1; s <= 64 && s <= tiles && (s == 1 || s <= workspace / slice_bytes); ++s) {
+                const int64_t per = (tiles + s - 1) / s, load = (units * row_tiles * s + cus - 1) / cus;
+                const double all = busy * (double)load * (mean / (double)s + 3), longest = alone * ((double)per + 3);
+                const double t = (all > longest ? all : longest) + (s > 1 ? 6 + (double)s * (double)slice_bytes * 2 / 4.5e6 : 0);
+                if ((waves == 4 && s == 1) || t < (p.waves == waves ? best : 0.97 * best)) {
+                    best = t;
+                    p.waves = waves;
+                    p.row_tiles = (int)row_tiles;
+                    p.slices = (int)((tiles + per - 1) / per);
+                    p.tiles = (int)per;
+                }
+            }
+        }
         p.slots = p.slices > 1 ? p.slices : 0;
         p.slot_rows = tokens * heads;
     }
@@ -425,7 +446,7 @@ extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_
     if (max_tokens > tokens) max_tokens = tokens;
     const Plan p = batch && tokens && max_tokens
                        ? plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, (max_len + KV8_BLOCK - 1) / KV8_BLOCK, workspace_bytes, compute_units > 0 ? compute_units : lq_device_cu_count())
-                       : Plan{true, 0, 1, 0, 0, 0, 0};
+                       : Plan{true, 0, 1, 0, 0, 0, 0, 0};
     *kernel = p.few ? 0 : 1;
     *parts = p.few ? p.workgroups : p.slices;
     *needed = p.slots * p.slot_rows * (dim + 1) * 4;
@@ -464,7 +485,7 @@ extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q
     a.window = window; a.scale = scale * 1.442695040888963f;
     a.blocks = (int)num_blocks; a.width = (int)table_width; a.batch = (int)batch; a.tokens = (int)tokens; a.heads = heads; a.kv_heads = kv_heads;
     a.causal = causal != 0; a.workgroups = p.workgroups; a.rows = (int)(max_tokens * (heads / kv_heads));
-    a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles;
+    a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles; a.waves = p.waves;
     LQ_REQUIRE(p.few || (int64_t)p.slices * batch * kv_heads * p.row_tiles <= INT32_MAX, "kv8_attention: too many tokens or sequences");
     return p.few ? kv8_launch_few(a, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
 }

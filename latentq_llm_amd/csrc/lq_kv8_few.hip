@@ -1,5 +1,5 @@
 // Attention of a few rows over the paged 8-bit cache (lq_kv8.h): the new tokens of a sequence times the query heads of a kv
-// head, up to 64 rows (32 at 256 dimensions). Every key and value byte is read once from memory for all rows.
+// head, up to 64 rows (32 at 128 dimensions, 16 at 256). Every key and value byte is read once from memory for all rows.
 //
 //   S^T = K Q^T  (16x16x32 f16)   a lane holds 4 keys of one row: c = S^T codes; t = c * (k_scale * scale * log2 e)
 //   p   = 2^(t + log2 v_scale - M),  M the running maximum of t + log2 v_scale over all keys
@@ -428,8 +428,10 @@ int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
 template <int D>
 int launch_rows(const Kv8Attn &a, bool f16, hipStream_t s) {
     if (a.rows <= 16) return launch<D, 1>(a, f16, s);
-    if (a.rows <= 32) return launch<D, 2>(a, f16, s);
-    if constexpr (D <= 128) return launch<D, 4>(a, f16, s);
+    if constexpr (D <= 128)
+        if (a.rows <= 32) return launch<D, 2>(a, f16, s);
+    if constexpr (D <= 96)
+        if (a.rows <= 64) return launch<D, 4>(a, f16, s);
     return lq_fail(LQ_ERR_UNSUPPORTED, "kv8_attention: %d rows at %d dimensions are not for the kernel of few rows", a.rows, D);
 }
 

@@ -11,10 +11,10 @@ namespace {
 
 constexpr float kLazy = 8.0f;
 
-template <int D, bool kF16>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
+template <int D, int kWaves, bool kF16>
+__global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
     constexpr int kSteps = D / 16, kTiles = D / 32, kPieces = D / 8;
-    constexpr int kRows = 128;
+    constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
     // per buffer: keys [64][D] halves, values [8 halves of steps][D][8]
     __shared__ u32x4_t lds_k[2][KV8_BLOCK * kPieces], lds_v[2][8 * D];
 
@@ -92,70 +92,74 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
     const auto dim_at = [](int d) { return d ^ (d >> 4 & 3); };
     // A thread's part of a tile: 16 bytes of keys (16 dimensions of a token) at a time; of values 4 dimensions of the 8 tokens that
     // make an operand, two groups of 4
-    constexpr int kKeys = KV8_BLOCK * D / 16, kNk = (kKeys + 255) / 256, kValues = kKeys / 2, kNv = (kValues + 255) / 256;
+    constexpr int kKeys = KV8_BLOCK * D / 16, kNk = (kKeys + kThreads - 1) / kThreads, kValues = kKeys / 2, kNv = (kValues + kThreads - 1) / kThreads;
     u32x4_t kr[kNk], vr[kNv][2];
     const auto request = [&](int64_t bh) {
         const u32x4_t *k = (const u32x4_t *)(a.k + bh * (KV8_BLOCK * D)), *v = (const u32x4_t *)(a.v + bh * (KV8_BLOCK * D));
 #pragma unroll
         for (int i = 0; i < kNk; ++i) {
-            const int u = threadIdx.x + i * 256;
-            if (kKeys % 256 == 0 || u < kKeys) kr[i] = k[u];
+            const int u = threadIdx.x + i * kThreads;
+            if (kKeys % kThreads == 0 || u < kKeys) kr[i] = k[u];
         }
 #pragma unroll
         for (int i = 0; i < kNv; ++i) {
             // operand (step e, half h) has groups 4 e + h and 4 e + h + 2
-            const int u = threadIdx.x + i * 256, pair = u / (D / 4), group = (pair >> 1) * 4 + (pair & 1), d = u % (D / 4);
-            if (kValues % 256 == 0 || u < kValues) {
+            const int u = threadIdx.x + i * kThreads, pair = u / (D / 4), group = (pair >> 1) * 4 + (pair & 1), d = u % (D / 4);
+            if (kValues % kThreads == 0 || u < kValues) {
                 vr[i][0] = v[group * (D / 4) + d];
                 vr[i][1] = v[(group + 2) * (D / 4) + d];
             }
         }
     };
-    const auto store = [&](int buffer) {
-#pragma unroll
-        for (int i = 0; i < kNk; ++i) {
-            const int u = threadIdx.x + i * 256, t = u / (D / 16), piece = u % (D / 16) * 2;
-            if (kKeys % 256 == 0 || u < kKeys) {
+    // The way into shared memory, in pieces that go between the products of the scores
+    constexpr int kParts = kNk + 2 * kNv;
+    const auto store = [&](int buffer, int part) {
+        if (part < kNk) {
+            const int u = threadIdx.x + part * kThreads, t = u / (D / 16), piece = u % (D / 16) * 2;
+            if (kKeys % kThreads == 0 || u < kKeys) {
                 u32x4_t *row_at = lds_k[buffer] + t * kPieces;
-                row_at[placed(piece, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[i][0], kr[i][1]));
-                row_at[placed(piece + 1, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[i][2], kr[i][3]));
+                row_at[placed(piece, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[part][0], kr[part][1]));
+                row_at[placed(piece + 1, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[part][2], kr[part][3]));
             }
-        }
-#pragma unroll
-        for (int i = 0; i < kNv; ++i) {
-            const int u = threadIdx.x + i * 256, pair = u / (D / 4), d = u % (D / 4) * 4;
-            if (kValues % 256 == 0 || u < kValues) {
+        } else {
+            const int i = (part - kNk) >> 1, u = threadIdx.x + i * kThreads, pair = u / (D / 4), d = u % (D / 4) * 4;
+            if (kValues % kThreads == 0 || u < kValues) {
                 u32x4_t *v_at = lds_v[buffer] + pair * D;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v_at[dim_at(d + j)] = __builtin_bit_cast(u32x4_t, kv8_operand(vr[i][0][j], vr[i][1][j]));
+                for (int j = 2 * ((part - kNk) & 1); j < 2 * ((part - kNk) & 1) + 2; ++j)
+                    v_at[dim_at(d + j)] = __builtin_bit_cast(u32x4_t, kv8_operand(vr[i][0][j], vr[i][1][j]));
             }
         }
     };
+    const auto store_all = [&](int buffer) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) store(buffer, part);
+    };
 
     float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
-    int64_t bh_next = 0;
+    const auto request_tile = [&](int t) {
+        const int64_t bh = block_of(t);
+        request(bh);
+        ks_next = kv8_uniform(a.ks + bh);
+        vs_next = kv8_uniform(a.vs + bh);
+    };
     if (t_lo < t_hi) {
-        bh_next = block_of(t_lo);
-        request(bh_next);
-        ks_next = kv8_uniform(a.ks + bh_next);
-        vs_next = kv8_uniform(a.vs + bh_next);
-        store(0);
+        request_tile(t_lo);
+        store_all(0);
         ks = ks_next;
         vs = vs_next;
+        request_tile(min(t_lo + 1, t_hi - 1));
     }
     __syncthreads();
     for (int t = t_lo; t < t_hi; ++t) {
         const int buffer = (t - t_lo) & 1;
-        if (t + 1 < t_hi) {
-            bh_next = block_of(t + 1);
-            request(bh_next);
-            ks_next = kv8_uniform(a.ks + bh_next);
-            vs_next = kv8_uniform(a.vs + bh_next);
-        }
         const int key0 = t * KV8_BLOCK;
-        if (key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before) {
+        const bool mine = key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before;
+        // (the tile after the last one is the last one again, stored and not used)
+        if (!mine) store_all(buffer ^ 1);
+        f32x16_t c[2];
+        if (mine) {
             // Two chains of products at a time (keys 0 .. 31 and 32 .. 63), operands read two steps ahead of them.
-            f32x16_t c[2];
             f16x8_t k[2][4];
             const auto read_k = [&](int set, int i) {  // steps i and i + 1
 #pragma unroll
@@ -169,14 +173,28 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
 #pragma unroll
                 for (int j = 0; j < 16; ++j) c[x][j] = 0.0f;
             read_k(0, 0);
+            constexpr int kPairs = kSteps / 2;
 #pragma unroll
             for (int i = 0; i < kSteps; i += 2) {
                 if (i + 2 < kSteps) read_k((i >> 1 & 1) ^ 1, i + 2);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int y = 0; y < 4; ++y) c[y & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i >> 1 & 1][y], q[i + (y >> 1)], c[y & 1], 0, 0, 0);
+#pragma unroll
+                for (int part = (i >> 1) * kParts / kPairs; part < ((i >> 1) + 1) * kParts / kPairs; ++part) store(buffer ^ 1, part);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
+        }
+        const float ks_now = ks, vs_now = vs;
+        ks = ks_next;
+        vs = vs_next;
+        if (t + 1 < t_hi) request_tile(min(t + 2, t_hi - 1));
+        if (mine) {
             // values of the first 16 keys: under the softmax
             f16x8_t v[2][kTiles];
             const auto read_v = [&](int set, int e) {
@@ -194,7 +212,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
                         if (key > last || key <= before) c[x][j] = -__builtin_inff();
                     }
             }
-            const float f = fmaxf(ks * factor, 0x1p-100f), lv = __builtin_amdgcn_logf(vs), rv = __builtin_amdgcn_rcpf(vs);
+            const float f = fmaxf(ks_now * factor, 0x1p-100f), lv = __builtin_amdgcn_logf(vs_now), rv = __builtin_amdgcn_rcpf(vs_now);
             float most = c[0][0];
 #pragma unroll
             for (int x = 0; x < 2; ++x)
@@ -220,7 +238,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
                     const float x0 = __builtin_amdgcn_exp2f(fmaf(c[e >> 1][8 * (e & 1) + 2 * j], f, shift));
                     const float x1 = __builtin_amdgcn_exp2f(fmaf(c[e >> 1][8 * (e & 1) + 2 * j + 1], f, shift));
                     w[j] = kv8_pack_f16(x0, x1);
-                    sum = kv8_add_halves(w[j], sum);
+                    sum += x0 + x1;
                 }
                 const f16x8_t p = __builtin_bit_cast(f16x8_t, w);
                 __builtin_amdgcn_sched_barrier(0);
@@ -228,11 +246,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8
                 for (int i = 0; i < kTiles; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[e & 1][i], p, o[i], 0, 0, 0);
             }
             L = fmaf(sum, rv, L);
-        }
-        if (t + 1 < t_hi) {
-            store(buffer ^ 1);
-            ks = ks_next;
-            vs = vs_next;
         }
         __syncthreads();
     }
@@ -309,8 +322,13 @@ int launch_join(const Kv8Attn &a, bool f16, hipStream_t s) {
 template <int D>
 int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.slices * a.row_tiles));
-    if (f16) prompt_kernel<D, true><<<grid, 256, 0, s>>>(a);
-    else prompt_kernel<D, false><<<grid, 256, 0, s>>>(a);
+    if (a.waves == 8) {  // (128 dimensions only)
+        if (f16) prompt_kernel<128, 8, true><<<grid, 512, 0, s>>>(a);
+        else prompt_kernel<128, 8, false><<<grid, 512, 0, s>>>(a);
+    } else {
+        if (f16) prompt_kernel<D, 4, true><<<grid, 256, 0, s>>>(a);
+        else prompt_kernel<D, 4, false><<<grid, 256, 0, s>>>(a);
+    }
     if (const int rc = lq_check_launch("kv8_attention (prompt)")) return rc;
     return a.slices > 1 ? launch_join<D>(a, f16, s) : LQ_OK;
 }

@@ -77,8 +77,9 @@ def test_plan_of_attention(hip_lib):
         return ops.kv8_attention_plan(batch, batch * most, most, length, heads, kv_heads, dim, compute_units=256, **more)
 
     # rows of a kv head: tokens times the query heads that share it
-    assert plan(1, 1, 1019, 32, 32)[0] == plan(1, 64, 1019, 32, 32)[0] == plan(1, 16, 1019, 32, 8)[0] == "few"
-    assert plan(1, 65, 1019, 32, 32)[0] == plan(1, 17, 1019, 32, 8)[0] == plan(1, 33, 1019, 32, 32, 256)[0] == "prompt"
+    assert plan(1, 1, 1019, 32, 32)[0] == plan(1, 16, 1019, 32, 32)[0] == plan(1, 4, 1019, 32, 8)[0] == plan(1, 16, 64, 8, 8, 256)[0] == "few"
+    assert plan(1, 32, 8192, 32, 32)[0] == plan(1, 64, 8192, 32, 32, 64)[0] == "few"
+    assert plan(1, 17, 64, 32, 32)[0] == plan(1, 33, 8192, 32, 32)[0] == plan(1, 17, 8192, 8, 8, 256)[0] == plan(1, 65, 8192, 32, 32, 64)[0] == "prompt"
     # enough workgroups, or few keys: nothing to join, no workspace
     assert plan(64, 1, 2048, 32, 32)[1:] == plan(1, 1, 64, 32, 32)[1:] == (0, 0) and plan(1, 8192, 8192, 32, 32)[1:] == (1, 0)
     # few rows on many keys: shares, whose partial results fit the workspace
