@@ -31,8 +31,9 @@ __device__ __forceinline__ T kv8_uniform(const T *p) {
 // operands, never rows outside.
 __device__ __forceinline__ void kv8_span(const int *cu, int batch, int tokens, int seq, int &start, int &n) {
     if (cu) {
-        start = min(max(cu[seq], 0), tokens);
-        n = min(max(cu[seq + 1], start), tokens) - start;
+        const int begin = kv8_uniform(cu + seq), end = kv8_uniform(cu + seq + 1);
+        start = min(max(begin, 0), tokens);
+        n = min(max(end, start), tokens) - start;
     } else {
         n = tokens / batch;
         start = seq * n;

@@ -21,18 +21,41 @@ struct Append {
     float *k_scale, *v_scale;
     const int *table, *lens, *cu;
     int64_t k_token, k_head, v_token, v_head, q_token, q_head, qo_token, qo_head;  // strides in elements
-    int positions, rot, blocks, width, batch, tokens, heads, kv_heads, per_seq;
+    int positions, rot, blocks, width, batch, tokens, heads, kv_heads, per_seq, q_groups;
 };
 
-// Largest finite magnitude, NaN and infinities left out
-__device__ __forceinline__ float most_of(float most, float x) {
-    const float m = fabsf(x);
-    return m <= 3.402823466e38f ? fmaxf(most, m) : most;
+// Largest finite magnitude of N values, NaN and infinities left out; `finite`: there were none. As bit patterns: those of
+// magnitudes are ordered, and the ones that are not finite come last.
+template <int N>
+__device__ __forceinline__ void most_of(const float *x, unsigned &most, bool &finite) {
+    unsigned all = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) all = max(all, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    if (all < 0x7F800000u) {
+        most = max(most, all);
+    } else {
+        finite = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const unsigned m = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+            most = max(most, m < 0x7F800000u ? m : 0u);
+        }
+    }
 }
 
 __device__ __forceinline__ unsigned code(float x, float r) {
     const float y = x * r;
     return (unsigned)(int)((y == y ? __builtin_amdgcn_fmed3f(rintf(y), -127.0f, 127.0f) : 0.0f) + 128.0f);
+}
+// Byte SEL of `old` replaced by the code of a finite x: |x * r| is at most 127 and a few rounding errors, so nothing is left to clamp
+template <int SEL>
+__device__ __forceinline__ unsigned code_finite(float x, float r, unsigned old) {
+    return act_cvt_pk_u8<SEL>(rintf(x * r) + 128.0f, old);
+}
+// Four codes of a word
+__device__ __forceinline__ unsigned codes_of(float x0, float x1, float x2, float x3, float r, bool finite) {
+    if (finite) return code_finite<3>(x3, r, code_finite<2>(x2, r, code_finite<1>(x1, r, code_finite<0>(x0, r, 0))));
+    return code(x0, r) | code(x1, r) << 8 | code(x2, r) << 16 | code(x3, r) << 24;
 }
 
 __device__ __forceinline__ unsigned code_again(unsigned u, float ratio) {
@@ -69,19 +92,21 @@ __device__ __forceinline__ void pieces(int pair, int rot, int &c0, int &c1) {
     c1 = pair < r ? pair + r : 2 * pair + 1;
 }
 
-template <bool kF16>
-__device__ __forceinline__ void load_rotated(const Append &a, const uint16_t *row, int pair, int pos, float x[16], int &c0, int &c1) {
-    pieces(pair, a.rot, c0, c1);
-    kv8_load8<kF16>(*(const u32x4_t *)(row + 8 * c0), x);
-    kv8_load8<kF16>(*(const u32x4_t *)(row + 8 * c1), x + 8);
-    if (pair < (a.rot >> 4)) {
+// 8 elements that this launch reads once
+__device__ __forceinline__ u32x4_t once(const uint16_t *p) { return __builtin_nontemporal_load((const u32x4_t *)p); }
+
+// cos and sin of one position for the 8 elements of a rotated pair of pieces
+struct Turn {
+    float c[8], s[8];
+    __device__ __forceinline__ void load(const Append &a, int pair, int pos) {
         const int64_t at = (int64_t)min(max(pos, 0), a.positions - 1) * (a.rot >> 1) + 8 * pair;
-        float c[8], s[8];
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
             *(f32x4_t *)(c + i) = *(const f32x4_t *)(a.cos + at + i);
             *(f32x4_t *)(s + i) = *(const f32x4_t *)(a.sin + at + i);
         }
+    }
+    __device__ __forceinline__ void apply(float x[16]) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float lo = x[i], hi = x[8 + i];
@@ -89,46 +114,87 @@ __device__ __forceinline__ void load_rotated(const Append &a, const uint16_t *ro
             x[8 + i] = hi * c[i] + lo * s[i];
         }
     }
-}
+};
 
 template <bool kF16>
 __device__ __forceinline__ u32x4_t pack8(const float x[8]) {
     return u32x4_t{kv8_pack<kF16>(x[0], x[1]), kv8_pack<kF16>(x[2], x[3]), kv8_pack<kF16>(x[4], x[5]), kv8_pack<kF16>(x[6], x[7])};
 }
 
+// One token's pair of pieces from a row to a row
+template <bool kF16>
+__device__ __forceinline__ void turn_row(const Append &a, const uint16_t *in, uint16_t *out, int pair, int pos) {
+    int c0, c1;
+    pieces(pair, a.rot, c0, c1);
+    float x[16];
+    kv8_load8<kF16>(*(const u32x4_t *)(in + 8 * c0), x);
+    kv8_load8<kF16>(*(const u32x4_t *)(in + 8 * c1), x + 8);
+    if (pair < (a.rot >> 4)) {
+        Turn turn;
+        turn.load(a, pair, pos);
+        turn.apply(x);
+    }
+    *(u32x4_t *)(out + 8 * c0) = pack8<kF16>(x);
+    *(u32x4_t *)(out + 8 * c1) = pack8<kF16>(x + 8);
+}
+
+// Heads of queries that a workgroup turns: the tables' 4 bytes an element are read once for so many 2-byte elements. These workgroups
+// are the longest and come first: 8192 tokens of 32 + 8 heads in 41 us behind the others 49, with non-temporal loads 39; by 4 heads 42,
+// by 2 44 (185 MB: 37 at the rate of a copy).
+constexpr int kQHeads = 8;
+
 // kThreads 256: a whole block of new tokens at once; 64: at most kFew of them (decoding)
 constexpr int kFew = 8;
 
 template <int D, int kThreads, bool kF16>
 __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
-    const int seq = blockIdx.x / a.per_seq, jb = blockIdx.x % a.per_seq, role = blockIdx.y, tid = threadIdx.x;
+    const int seq = blockIdx.x / a.per_seq, jb = blockIdx.x % a.per_seq, tid = threadIdx.x;
+    const int role = (int)blockIdx.y - a.q_groups;  // queries (negative: the longest, first), keys, values
     int start, n;
     kv8_span(a.cu, a.batch, a.tokens, seq, start, n);
     if (n == 0) return;
-    const int len = max(a.lens[seq], 0), first = len - n;
+    const int len = max(kv8_uniform(a.lens + seq), 0), first = len - n;
     const int place = max(first, 0) / KV8_BLOCK + jb;  // which block of the sequence
     const int begin = place * KV8_BLOCK, hi = min(len, begin + KV8_BLOCK);
     const int64_t row0 = (int64_t)start - first;  // row of the operands that position 0 would have
 
-    if (role >= 2 * a.kv_heads) {  // queries of one head: positions of this block, and with its first block any before position 0
-        const int h = role - 2 * a.kv_heads, from = jb ? begin : first, count = hi - from;
-        const uint16_t *src = (const uint16_t *)a.q + h * a.q_head;
-        uint16_t *dst = (uint16_t *)a.q_out + h * a.qo_head;
-        for (int item = tid; item < count * (D / 16); item += kThreads) {
-            const int pos = from + item / (D / 16);
-            float x[16];
-            int c0, c1;
-            load_rotated<kF16>(a, src + (row0 + pos) * a.q_token, item % (D / 16), pos, x, c0, c1);
-            uint16_t *o = dst + (row0 + pos) * a.qo_token;
-            *(u32x4_t *)(o + 8 * c0) = pack8<kF16>(x);
-            *(u32x4_t *)(o + 8 * c1) = pack8<kF16>(x + 8);
+    if (role < 0) {  // queries of kQHeads heads: positions of this block, and with its first block any before position 0
+        constexpr int kPairs = D / 16;
+        const int h0 = (role + a.q_groups) * kQHeads, heads = min(kQHeads, a.heads - h0), from = jb ? begin : first, count = hi - from;
+        const uint16_t *src = (const uint16_t *)a.q + h0 * a.q_head;
+        uint16_t *dst = (uint16_t *)a.q_out + h0 * a.qo_head;
+        if constexpr (kThreads == 64) {  // few tokens: heads side by side
+            for (int item = tid; item < count * heads * kPairs; item += kThreads) {
+                const int pair = item % kPairs, h = item / kPairs % heads, pos = from + item / (kPairs * heads);
+                turn_row<kF16>(a, src + (row0 + pos) * a.q_token + h * a.q_head, dst + (row0 + pos) * a.qo_token + h * a.qo_head, pair, pos);
+            }
+        } else {  // heads one after the other, two on the way at a time, with the cos and sin of their token in registers
+            for (int item = tid; item < count * kPairs; item += kThreads) {
+                const int pair = item % kPairs, pos = from + item / kPairs;
+                int c0, c1;
+                pieces(pair, a.rot, c0, c1);
+                Turn turn;
+                const bool turned = pair < (a.rot >> 4);
+                if (turned) turn.load(a, pair, pos);
+                const uint16_t *in = src + (row0 + pos) * a.q_token;
+                uint16_t *out = dst + (row0 + pos) * a.qo_token;
+#pragma unroll 4
+                for (int h = 0; h < heads; ++h) {
+                    float x[16];
+                    kv8_load8<kF16>(once(in + h * a.q_head + 8 * c0), x);
+                    kv8_load8<kF16>(once(in + h * a.q_head + 8 * c1), x + 8);
+                    if (turned) turn.apply(x);
+                    *(u32x4_t *)(out + h * a.qo_head + 8 * c0) = pack8<kF16>(x);
+                    *(u32x4_t *)(out + h * a.qo_head + 8 * c1) = pack8<kF16>(x + 8);
+                }
+            }
         }
         return;
     }
 
     const int lo = max(first, begin), count = hi - lo;
     if (count <= 0 || place >= a.width) return;
-    const int block = a.table[(int64_t)seq * a.width + place];
+    const int block = kv8_uniform(a.table + (int64_t)seq * a.width + place);
     if (block < 0 || block >= a.blocks) return;
     const bool keys = role < a.kv_heads;
     const int h = keys ? role : role - a.kv_heads;
@@ -140,18 +206,28 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
     if (keys) {
         constexpr int kPairs = D / 16, kItems = ((kThreads == 64 ? kFew : KV8_BLOCK) * kPairs + kThreads - 1) / kThreads;
         const uint16_t *src = (const uint16_t *)a.k + h * a.k_head;
-        float x[kItems][16], most = 0.0f;
+        float x[kItems][16], most;
+        unsigned bits = 0;
+        bool finite = true;
         int c0[kItems], c1[kItems];
 #pragma unroll
         for (int it = 0; it < kItems; ++it) {
             const int item = tid + it * kThreads, t = item / kPairs;
             if (t < count) {
-                load_rotated<kF16>(a, src + (row0 + lo + t) * a.k_token, item % kPairs, lo + t, x[it], c0[it], c1[it]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = most_of(most, x[it][i]);
+                const uint16_t *row = src + (row0 + lo + t) * a.k_token;
+                const int pair = item % kPairs;
+                pieces(pair, a.rot, c0[it], c1[it]);
+                kv8_load8<kF16>(once(row + 8 * c0[it]), x[it]);
+                kv8_load8<kF16>(once(row + 8 * c1[it]), x[it] + 8);
+                if (pair < (a.rot >> 4)) {
+                    Turn turn;
+                    turn.load(a, pair, lo + t);
+                    turn.apply(x[it]);
+                }
+                most_of<16>(x[it], bits, finite);
             }
         }
-        most = block_max<kThreads>(most);
+        most = block_max<kThreads>(__uint_as_float(bits));
         const float scale = fmaxf(held, fmaxf(most, kLeast) * (1.0f / 127.0f)), r = 1.0f / scale;
         if (tid == 0) *scale_at = scale;
         uint8_t *codes = a.k_codes + bh * (KV8_BLOCK * D);
@@ -163,9 +239,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
         for (int it = 0; it < kItems; ++it) {
             const int t = (tid + it * kThreads) / kPairs;
             if (t < count) {
-                unsigned w[4] = {0, 0, 0, 0};
+                unsigned w[4];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) w[i >> 2] |= code(x[it][i], r) << (8 * (i & 3));
+                for (int i = 0; i < 4; ++i) w[i] = codes_of(x[it][4 * i], x[it][4 * i + 1], x[it][4 * i + 2], x[it][4 * i + 3], r, finite);
                 uint8_t *o = codes + (kept + t) * D;
                 *(u32x2_t *)(o + 8 * c0[it]) = u32x2_t{w[0], w[1]};
                 *(u32x2_t *)(o + 8 * c1[it]) = u32x2_t{w[2], w[3]};
@@ -177,7 +253,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
         constexpr int kItems = (kGroups * kPieces + kThreads - 1) / kThreads;
         const uint16_t *src = (const uint16_t *)a.v + h * a.v_head;
         const int group0 = kept >> 2, end = kept + count;  // slots kept .. end - 1 are new
-        float x[kItems][4][8], most = 0.0f;
+        float x[kItems][4][8] = {}, most;
+        unsigned bits = 0;
+        bool finite = true;
 #pragma unroll
         for (int it = 0; it < kItems; ++it) {
             const int item = tid + it * kThreads, g = group0 + item / kPieces, piece = item % kPieces;
@@ -186,12 +264,11 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
                 const int slot = 4 * g + j;
                 if (slot >= kept && slot < end) {
                     kv8_load8<kF16>(*(const u32x4_t *)(src + (row0 + begin + slot) * a.v_token + 8 * piece), x[it][j]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) most = most_of(most, x[it][j][i]);
+                    most_of<8>(x[it][j], bits, finite);
                 }
             }
         }
-        most = block_max<kThreads>(most);
+        most = block_max<kThreads>(__uint_as_float(bits));
         const float scale = fmaxf(held, fmaxf(most, kLeast) * (1.0f / 127.0f)), r = 1.0f / scale;
         if (tid == 0) *scale_at = scale;
         const bool grows = kept && scale > held;
@@ -207,17 +284,20 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
                 const bool part = 4 * g < kept || 4 * g + 4 > end;  // slots of the group that are not new
 #pragma unroll
                 for (int i = 0; i < 8; i += 4) {
-                    u32x4_t w = {0, 0, 0, 0};
-                    if (part) w = *(const u32x4_t *)(o + i);
+                    u32x4_t w;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int slot = 4 * g + j, at = 8 * j;
-                        const bool fresh = slot >= kept && slot < end;
+                    for (int d = 0; d < 4; ++d) w[d] = codes_of(x[it][0][i + d], x[it][1][i + d], x[it][2][i + d], x[it][3][i + d], r, finite);
+                    if (part) {
+                        const u32x4_t was = *(const u32x4_t *)(o + i);
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) {
-                            const unsigned was = (w[d] >> at) & 0xFFu;
-                            const unsigned now = fresh ? code(x[it][j][i + d], r) : grows && slot < kept ? code_again(was, ratio) : was;
-                            w[d] = (w[d] & ~(0xFFu << at)) | (now << at);
+                        for (int j = 0; j < 4; ++j) {
+                            const int slot = 4 * g + j, at = 8 * j;
+                            if (slot >= kept && slot < end) continue;
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                const unsigned old = (was[d] >> at) & 0xFFu;
+                                w[d] = (w[d] & ~(0xFFu << at)) | ((grows && slot < kept ? code_again(old, ratio) : old) << at);
+                            }
                         }
                     }
                     *(u32x4_t *)(o + i) = w;
@@ -250,17 +330,27 @@ __global__ __launch_bounds__(256) void read_kernel(const uint8_t *k_codes, const
         const u32x4_t kw = k[i], vw = v[i];
         const int t = i / (D / 16), d = i % (D / 16) * 16;   // keys: 16 dimensions of a token
         const int g = i / (D / 4), e = i % (D / 4) * 4;      // values: 4 tokens of 4 dimensions
+        // (a product is an fp32 number before it is rounded to its type: left alone, some would go to f16 in one instruction)
+        const auto value = [&](unsigned u, float scale) {
+            float f = there ? (float)((int)u - 128) * scale : 0.0f;
+            asm("" : "+v"(f));
+            return f;
+        };
+        float f[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) f[j] = value((kw[j >> 2] >> (8 * (j & 3))) & 0xFFu, ks);
+        if constexpr (kOut == 2) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) store4<kOut>(k_out, out0 + t * step + d + j, f + j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j += 8) *(u32x4_t *)((uint16_t *)k_out + out0 + t * step + d + j) = pack8<kOut == 1>(f + j);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float f[4], w[4];
+            float w[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                f[b] = there ? (float)((int)((kw[j] >> (8 * b)) & 0xFFu) - 128) * ks : 0.0f;
-                w[b] = there ? (float)((int)((vw[b] >> (8 * j)) & 0xFFu) - 128) * vs : 0.0f;
-                // a product is an fp32 number before it is rounded to its type (left alone, some would go to f16 in one instruction)
-                asm("" : "+v"(f[b]), "+v"(w[b]));
-            }
-            store4<kOut>(k_out, out0 + t * step + d + 4 * j, f);
+            for (int b = 0; b < 4; ++b) w[b] = value((vw[b] >> (8 * j)) & 0xFFu, vs);
             store4<kOut>(v_out, out0 + (4 * g + j) * step + e, w);
         }
     }
@@ -393,12 +483,12 @@ extern "C" int lq_kv8_append(const void *k, int64_t k_token_stride, int64_t k_he
         LQ_REQUIRE(lq_aligned(p, 16), "kv8_append: k, v, q, the tables and the codes must be 16-byte aligned");
     Append a{k, v, q, q_out, cos_table, sin_table, (uint8_t *)k_codes, (uint8_t *)v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens,
              k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride,
-             (int)positions, cos_table ? rot_dim : 0, (int)num_blocks, (int)table_width, (int)batch, (int)tokens, heads, kv_heads, 0};
+             (int)positions, cos_table ? rot_dim : 0, (int)num_blocks, (int)table_width, (int)batch, (int)tokens, heads, kv_heads, 0, q ? (heads + kQHeads - 1) / kQHeads : 0};
     if (max_tokens > tokens) max_tokens = tokens;
     const int64_t per = (max_tokens + KV8_BLOCK - 2) / KV8_BLOCK + 1;
     LQ_REQUIRE(per * batch <= INT32_MAX, "kv8_append: too many tokens or sequences");
     a.per_seq = (int)per;
-    const dim3 grid((unsigned)(per * batch), (unsigned)(2 * kv_heads + (q ? heads : 0)));
+    const dim3 grid((unsigned)(per * batch), (unsigned)(2 * kv_heads + a.q_groups));
     const bool few = max_tokens <= kFew;
     hipStream_t s = (hipStream_t)stream;
     if (dim == 64) launch_append<64>(a, few, dtype == 1, grid, s);
