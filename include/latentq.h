@@ -509,8 +509,8 @@ int lq_weight_grad_acc8(const void *dy, const void *x, int8_t *q_inout, const vo
 int lq_weight_grad_plan(int form, int64_t M, int64_t N, int64_t K, int compute_units, int *rows, int *columns, int *waves);
 
 /* ---------------------------------------------------------------------------
- * Paged 8-bit cache of keys and values, and attention over it (the cache that the reference's chat demo and
- * PTQ/quant/fused_attn.py:96-199 keep as past_key_value tensors; no counterpart function).
+ * Paged 8-bit cache of keys and values, and attention over it. An addition: the reference leaves both to its tensor library, in 16
+ * bits; rotation by halves as in PTQ/quant/fused_attn.py:8-93.
  *
  * The cache is a pool of num_blocks blocks of LQ_KV_BLOCK tokens, for kv_heads heads of dim dimensions (64, 96, 128 or 256):
  *   k_codes  uint8 [num_blocks][kv_heads][64][dim]
