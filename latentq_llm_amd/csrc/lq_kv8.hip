@@ -7,6 +7,9 @@
 // One workgroup owns a (block, head) of the keys or of the values, so nothing is shared and nothing depends on an order: the new
 // tokens' values stay in registers between the maximum and the rounding, and a block's old codes are touched only when its scale
 // grows. The rotation of the queries needs no maximum and is spread over workgroups of the same launch.
+//
+// Bound: memory. Appending 8192 tokens of 32 + 8 heads of 128 and turning their queries moves 185 MB in 39 us, 4.7 TB/s, where a copy
+// of 1 GiB reaches 5.0. One token of 32 heads, 4.8 us, is the launch and loads that wait for each other: length, table, scale.
 #include "lq_kv8.h"
 
 namespace {
@@ -383,7 +386,7 @@ bool good_dim(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 2
 struct Plan {
     bool few;
     int workgroups;                // few rows: that share all tiles, 0: one for each (sequence, kv head)
-    int slices, tiles, row_tiles, waves;  // prompt
+    int slices, tiles, row_tiles, waves, sides;  // prompt
     int64_t slots, slot_rows;      // of the workspace
 };
 
@@ -417,27 +420,34 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
         p.slot_rows = rows;
         p.slices = 1;
     } else {
-        // Slices of the keys, and waves of a workgroup, by an estimate in us. A tile takes `busy` of a compute unit that has workgroups
+        // Slices of the keys, and a workgroup's shape, by an estimate in us. A tile takes `busy` of a compute unit that has workgroups
         // enough, and `alone` at least in each workgroup; the ways in and out cost 3 tiles; slices take their partial results there and
         // back (4.5 TB/s) and a launch. With 8 waves a row has half the conversions, but there are half the workgroups: single sequences of
-        // 4096 tokens (32 heads of 128) 160 -> 147 us, 1024 on 16384 keys 289 -> 270, but 2048 tokens 54 -> 64, 4 x 1019 39 -> 43. By slices,
-        // measured / estimated: 64 dimensions, 256 tokens on 16384 keys in 4 75 / 80, in 8 59 / 65; 96 dimensions, 12 heads, 2048 tokens in 1
-        // 58 / 56, in 3 39 / 41.
+        // 4096 tokens (32 heads of 128) 160 -> 147 us, 1024 on 16384 keys 289 -> 270, but 2048 tokens 54 -> 64, 4 x 1019 39 -> 43. Where
+        // every workgroup has a compute unit to itself, two sides of 4 waves take the tiles by turns, `paired` for each (5 more for the ways): 1024
+        // tokens, 32 heads of 128, 28.0 -> 24.4, 8 x 128 on 2048 keys 52.1 -> 40.7, but 70 tokens 8.4 -> 9.1; with more workgroups than that,
+        // 4 x 512, 23.5 -> 28.9. By slices, measured / estimated: 64 dimensions, 256 tokens on 16384 keys in 4 75 / 80, in 8 59 / 65; 96
+        // dimensions, 12 heads, 2048 tokens in 1 58 / 56, in 3 39 / 41.
         const double busy4 = dim == 64 ? 0.73 : dim == 96 ? 0.9 : dim == 128 ? 1.15 : 2.2, alone4 = dim == 64 ? 1.05 : dim == 96 ? 1.6 : dim == 128 ? 1.45 : 2.2;
+        const double paired = dim == 64 ? 0.8 : dim == 96 ? 1.1 : 1.15;
         const int64_t slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;
         const double mean = (double)tiles - (double)max_tokens / (2 * KV8_BLOCK);  // of the rows' tiles, where all of them are causal
         double best = 0;
-        for (const int waves : {4, 8}) {
-            if (waves == 8 && (dim != 128 || tiles < 64)) break;
+        const struct { int waves, sides; } shapes[] = {{4, 1}, {8, 1}, {4, 2}};
+        for (const auto &shape : shapes) {
+            const int waves = shape.waves, sides = shape.sides;
+            if ((waves == 8 && (dim != 128 || tiles < 64)) || (sides == 2 && dim > 128)) continue;
             const int64_t row_tiles = (rows + 32 * waves - 1) / (32 * waves);
-            const double busy = waves == 4 ? busy4 : 2.1, alone = waves == 4 ? alone4 : 2.1;
+            const double busy = waves == 4 ? busy4 : 2.1, alone = sides == 2 ? paired : waves == 4 ? alone4 : 2.1;
             for (int64_t s = 1; s <= 64 && s <= tiles && (s == 1 || s <= workspace / slice_bytes); ++s) {
                 const int64_t per = (tiles + s - 1) / s, load = (units * row_tiles * s + cus - 1) / cus;
-                const double all = busy * (double)load * (mean / (double)s + 3), longest = alone * ((double)per + 3);
+                if (sides == 2 && load > 1) break;
+                const double all = busy * (double)load * (mean / (double)s + 3), longest = alone * (double)(per + (sides == 2 ? 5 : 3));
                 const double t = (all > longest ? all : longest) + (s > 1 ? 6 + (double)s * (double)slice_bytes * 2 / 4.5e6 : 0);
-                if ((waves == 4 && s == 1) || t < (p.waves == waves ? best : 0.97 * best)) {
+                if (p.waves == 0 || t < (p.waves == waves && p.sides == sides ? best : 0.97 * best)) {
                     best = t;
                     p.waves = waves;
+                    p.sides = sides;
                     p.row_tiles = (int)row_tiles;
                     p.slices = (int)((tiles + per - 1) / per);
                     p.tiles = (int)per;
@@ -536,7 +546,7 @@ extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_
     if (max_tokens > tokens) max_tokens = tokens;
     const Plan p = batch && tokens && max_tokens
                        ? plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, (max_len + KV8_BLOCK - 1) / KV8_BLOCK, workspace_bytes, compute_units > 0 ? compute_units : lq_device_cu_count())
-                       : Plan{true, 0, 1, 0, 0, 0, 0, 0};
+                       : Plan{true, 0, 1, 0, 0, 0, 0, 0, 0};
     *kernel = p.few ? 0 : 1;
     *parts = p.few ? p.workgroups : p.slices;
     *needed = p.slots * p.slot_rows * (dim + 1) * 4;
@@ -575,7 +585,7 @@ extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q
     a.window = window; a.scale = scale * 1.442695040888963f;
     a.blocks = (int)num_blocks; a.width = (int)table_width; a.batch = (int)batch; a.tokens = (int)tokens; a.heads = heads; a.kv_heads = kv_heads;
     a.causal = causal != 0; a.workgroups = p.workgroups; a.rows = (int)(max_tokens * (heads / kv_heads));
-    a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles; a.waves = p.waves;
+    a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles; a.waves = p.waves; a.sides = p.sides;
     LQ_REQUIRE(p.few || (int64_t)p.slices * batch * kv_heads * p.row_tiles <= INT32_MAX, "kv8_attention: too many tokens or sequences");
     return p.few ? kv8_launch_few(a, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
 }

@@ -1,22 +1,31 @@
-// Attention of many rows over the paged 8-bit cache (lq_kv8.h): prompts, and pieces of prompts. A workgroup takes 128 rows
+// Attention of many rows over the paged 8-bit cache (lq_kv8.h): prompts, and pieces of prompts. A workgroup takes 128 or 256 rows
 // (tokens times the query heads of a kv head), 32 to a wave, and goes over tiles of 64 keys; the arithmetic is that of
-// lq_kv8_few.hip on 32x32x16 f16 matrix instructions.
+// lq_kv8_few.hip on 32x32x16 f16 matrix instructions, but that the running maximum moves only when it has to.
 //
 // The codes of a tile become halves once for all waves: requested a tile ahead into registers, converted on their way into
-// shared memory, two buffers, one barrier a tile. Keys lie there by rows with their 16-byte pieces exchanged by the row
-// number (a wave reads 32 rows at one piece), values as finished operands.
+// shared memory between the products of the scores, two buffers, one barrier a tile. Keys lie there by rows with their 16-byte pieces
+// exchanged by the row number (a wave reads 32 rows at one piece), values as finished operands. The products of O for 16
+// keys run under the weights of the next 16.
+//
+// Bound: the matrix units, at the clock that they leave (2.17 GHz under this kernel). 8192 causal tokens of 32 heads of 128
+// in 554 us, 993 TFLOP/s of the visible half, where a large f16 product of the tensor library reaches 1162; 512 tokens on 16384 keys, 32 heads on
+// 8, 148 us, 915. A wave alone on its tile waits for its own products and weights in turn, so short prompts are bound by the
+// way of one workgroup through its tiles, 1.45 us each (1024 tokens of 32 heads 24 us).
 #include "lq_kv8.h"
 
 namespace {
 
 constexpr float kLazy = 8.0f;
 
-template <int D, int kWaves, bool kF16>
-__global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
+// kWaves: waves side by side on 32 rows each; kSides: groups of them that take every kSides-th tile of the keys of the same rows,
+// each with shared memory of its own, joined at the end
+template <int D, int kWaves, int kSides, bool kF16>
+__global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt_kernel(const Kv8Attn a) {
     constexpr int kSteps = D / 16, kTiles = D / 32, kPieces = D / 8;
     constexpr int kRows = 32 * kWaves, kThreads = 64 * kWaves;
     // per buffer: keys [64][D] halves, values [8 halves of steps][D][8]
-    __shared__ u32x4_t lds_k[2][KV8_BLOCK * kPieces], lds_v[2][8 * D];
+    constexpr int kHalf = KV8_BLOCK * kPieces;  // = 8 D
+    __shared__ u32x4_t lds[kSides][2][2 * kHalf];
 
     const int units = a.batch * a.kv_heads;
     const int unit = blockIdx.x % units, rest = blockIdx.x / units;
@@ -29,7 +38,8 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
     if (row0 >= all_rows) return;
     const int rows = (int)min((int64_t)kRows, all_rows - row0);
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % kWaves), col = lane & 31, half = lane >> 5;
+    const int side = kSides == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads), tid = threadIdx.x % kThreads;
     const int pos_first = s.first + row0 / group, pos_last = s.first + (row0 + rows - 1) / group;
     const int seen = a.causal ? min(pos_last + 1, s.len) : s.len;  // keys before this are seen by some row
     int64_t lo64 = a.window ? (int64_t)pos_first - a.window + 1 : 0;
@@ -98,13 +108,13 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
         const u32x4_t *k = (const u32x4_t *)(a.k + bh * (KV8_BLOCK * D)), *v = (const u32x4_t *)(a.v + bh * (KV8_BLOCK * D));
 #pragma unroll
         for (int i = 0; i < kNk; ++i) {
-            const int u = threadIdx.x + i * kThreads;
+            const int u = tid + i * kThreads;
             if (kKeys % kThreads == 0 || u < kKeys) kr[i] = k[u];
         }
 #pragma unroll
         for (int i = 0; i < kNv; ++i) {
             // operand (step e, half h) has groups 4 e + h and 4 e + h + 2
-            const int u = threadIdx.x + i * kThreads, pair = u / (D / 4), group = (pair >> 1) * 4 + (pair & 1), d = u % (D / 4);
+            const int u = tid + i * kThreads, pair = u / (D / 4), group = (pair >> 1) * 4 + (pair & 1), d = u % (D / 4);
             if (kValues % kThreads == 0 || u < kValues) {
                 vr[i][0] = v[group * (D / 4) + d];
                 vr[i][1] = v[(group + 2) * (D / 4) + d];
@@ -115,16 +125,16 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
     constexpr int kParts = kNk + 2 * kNv;
     const auto store = [&](int buffer, int part) {
         if (part < kNk) {
-            const int u = threadIdx.x + part * kThreads, t = u / (D / 16), piece = u % (D / 16) * 2;
+            const int u = tid + part * kThreads, t = u / (D / 16), piece = u % (D / 16) * 2;
             if (kKeys % kThreads == 0 || u < kKeys) {
-                u32x4_t *row_at = lds_k[buffer] + t * kPieces;
+                u32x4_t *row_at = lds[side][buffer] + t * kPieces;
                 row_at[placed(piece, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[part][0], kr[part][1]));
                 row_at[placed(piece + 1, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[part][2], kr[part][3]));
             }
         } else {
-            const int i = (part - kNk) >> 1, u = threadIdx.x + i * kThreads, pair = u / (D / 4), d = u % (D / 4) * 4;
+            const int i = (part - kNk) >> 1, u = tid + i * kThreads, pair = u / (D / 4), d = u % (D / 4) * 4;
             if (kValues % kThreads == 0 || u < kValues) {
-                u32x4_t *v_at = lds_v[buffer] + pair * D;
+                u32x4_t *v_at = lds[side][buffer] + kHalf + pair * D;
 #pragma unroll
                 for (int j = 2 * ((part - kNk) & 1); j < 2 * ((part - kNk) & 1) + 2; ++j)
                     v_at[dim_at(d + j)] = __builtin_bit_cast(u32x4_t, kv8_operand(vr[i][0][j], vr[i][1][j]));
@@ -143,18 +153,19 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
         ks_next = kv8_uniform(a.ks + bh);
         vs_next = kv8_uniform(a.vs + bh);
     };
-    if (t_lo < t_hi) {
-        request_tile(t_lo);
+    const int steps = (t_hi - t_lo + kSides - 1) / kSides;  // of every side; in the last one a side may be without a tile
+    if (steps > 0) {
+        request_tile(min(t_lo + side, t_hi - 1));
         store_all(0);
         ks = ks_next;
         vs = vs_next;
-        request_tile(min(t_lo + 1, t_hi - 1));
+        request_tile(min(t_lo + side + kSides, t_hi - 1));
     }
     __syncthreads();
-    for (int t = t_lo; t < t_hi; ++t) {
-        const int buffer = (t - t_lo) & 1;
+    for (int n = 0; n < steps; ++n) {
+        const int buffer = n & 1, t = t_lo + side + n * kSides;
         const int key0 = t * KV8_BLOCK;
-        const bool mine = key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before;
+        const bool mine = (kSides == 1 || t < t_hi) && key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before;
         // (the tile after the last one is the last one again, stored and not used)
         if (!mine) store_all(buffer ^ 1);
         f32x16_t c[2];
@@ -165,7 +176,7 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     const int at = (y & 1) * 32 + col;
-                    k[set][y] = __builtin_bit_cast(f16x8_t, lds_k[buffer][at * kPieces + placed(2 * (i + (y >> 1)) + half, at)]);
+                    k[set][y] = __builtin_bit_cast(f16x8_t, lds[side][buffer][at * kPieces + placed(2 * (i + (y >> 1)) + half, at)]);
                 }
             };
 #pragma unroll
@@ -193,13 +204,13 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
         const float ks_now = ks, vs_now = vs;
         ks = ks_next;
         vs = vs_next;
-        if (t + 1 < t_hi) request_tile(min(t + 2, t_hi - 1));
+        if (n + 1 < steps) request_tile(min(t + 2 * kSides, t_hi - 1));
         if (mine) {
             // values of the first 16 keys: under the softmax
             f16x8_t v[2][kTiles];
             const auto read_v = [&](int set, int e) {
 #pragma unroll
-                for (int i = 0; i < kTiles; ++i) v[set][i] = __builtin_bit_cast(f16x8_t, lds_v[buffer][(2 * e + half) * D + dim_at(32 * i + col)]);
+                for (int i = 0; i < kTiles; ++i) v[set][i] = __builtin_bit_cast(f16x8_t, lds[side][buffer][kHalf + (2 * e + half) * D + dim_at(32 * i + col)]);
             };
             read_v(0, 0);
             // accumulator element j is key 32 x + (j & 3) + 8 (j >> 2) + 4 half
@@ -250,6 +261,27 @@ __global__ __launch_bounds__(64 * kWaves, D <= 128 ? 2 : 1) void prompt_kernel(c
         __syncthreads();
     }
 
+    if constexpr (kSides == 2) {  // the second side's sums come through shared memory
+        float *mail = (float *)lds + wave * (64 * (16 * kTiles + 2)) + lane;
+        static_assert(kSides == 1 || kWaves * 64 * (16 * kTiles + 2) * 4 <= (int)sizeof(lds), "");
+        if (side) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) mail[(16 * i + j) * 64] = o[i][j];
+            mail[16 * kTiles * 64] = M;
+            mail[(16 * kTiles + 1) * 64] = L;
+        }
+        __syncthreads();
+        if (side) return;
+        const float M1 = mail[16 * kTiles * 64], m = fmaxf(M, M1), f0 = __builtin_amdgcn_exp2f(M - m), f1 = __builtin_amdgcn_exp2f(M1 - m);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = fmaf(mail[(16 * i + j) * 64], f1, o[i][j] * f0);
+        L = fmaf(mail[(16 * kTiles + 1) * 64], f1, L * f0);
+        M = m;
+    }
     if (!there) return;
     L += __shfl_xor(L, 32);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -323,11 +355,14 @@ template <int D>
 int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.slices * a.row_tiles));
     if (a.waves == 8) {  // (128 dimensions only)
-        if (f16) prompt_kernel<128, 8, true><<<grid, 512, 0, s>>>(a);
-        else prompt_kernel<128, 8, false><<<grid, 512, 0, s>>>(a);
+        if (f16) prompt_kernel<128, 8, 1, true><<<grid, 512, 0, s>>>(a);
+        else prompt_kernel<128, 8, 1, false><<<grid, 512, 0, s>>>(a);
+    } else if (a.sides == 2) {  // (up to 128 dimensions)
+        if (f16) prompt_kernel<D <= 128 ? D : 128, 4, 2, true><<<grid, 512, 0, s>>>(a);
+        else prompt_kernel<D <= 128 ? D : 128, 4, 2, false><<<grid, 512, 0, s>>>(a);
     } else {
-        if (f16) prompt_kernel<D, 4, true><<<grid, 256, 0, s>>>(a);
-        else prompt_kernel<D, 4, false><<<grid, 256, 0, s>>>(a);
+        if (f16) prompt_kernel<D, 4, 1, true><<<grid, 256, 0, s>>>(a);
+        else prompt_kernel<D, 4, 1, false><<<grid, 256, 0, s>>>(a);
     }
     if (const int rc = lq_check_launch("kv8_attention (prompt)")) return rc;
     return a.slices > 1 ? launch_join<D>(a, f16, s) : LQ_OK;

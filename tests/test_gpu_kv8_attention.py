@@ -69,6 +69,49 @@ def test_prompts(hip_lib, lens, news, heads, kv_heads, dim, dtype):
     run(lens, news, heads, kv_heads, dim, dtype, seed=lens[0])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("lens, news, how", [
+    ([449], [449], {}), ([512, 70, 0], [130, 70, 3], {}), ([640], [60], {"causal": False}), ([577, 420], [90, 420], {"window": 400}), ([700], [100], {"window": 30})])
+def test_prompts_of_a_few_sequences(hip_lib, lens, news, how, dim, dtype):
+    """Few workgroups with many keys each: even and odd numbers of tiles, also for some rows only, rows without any."""
+    run(lens, news, 4, 2, dim, dtype, seed=lens[0], **how)
+    cache = ref.Cache(30, 1, dim, seed=5)  # the tiles' weights far apart, in either order
+    cache.scale[1] = np.exp2(np.random.default_rng(2).integers(-60, 1, cache.scale[1].shape)).astype(np.float32)
+    cache.scale[0] *= np.float32(8)
+    table, q = ref.blocks_of(lens, 30, seed=1), rows((sum(news), 2, dim), BF16, 8)
+    want, _, bound = ref.attention(cache, q, table, lens, news, **how)
+    holds(call(cache.tensors(), q, table, lens, news, **how), want, bound)
+
+
+@pytest.mark.parametrize("how", [{}, {"causal": False}, {"window": 500}])
+@pytest.mark.parametrize("dim, heads, kv_heads", [(128, 32, 8), (64, 32, 32), (256, 16, 4), (96, 12, 12)])
+def test_long_prompts(hip_lib, dim, heads, kv_heads, how):
+    """Some thousands of tokens of all heads, against 64 bits on the card; the bound is tests/kv8_ref.py's."""
+    n, new = 4221, 4090
+    cache = ref.Cache(68, kv_heads, dim, seed=dim)
+    table, q = ref.blocks_of([n], 68), rows((new, heads, dim), BF16, 9)
+    out, lse = call(cache.tensors(), q, table, [n], [new], return_lse=True, **how)
+    pos = torch.arange(n - new, n).cuda()[:, None]
+    key = torch.arange(n).cuda()[None]
+    seen = (key <= pos if how.get("causal", True) else key >= 0) & (key > pos - how.get("window", n))
+    for h in range(heads):
+        kv, blocks = h // (heads // kv_heads), table[0].astype(np.int64)
+        k, v = (torch.from_numpy(cache.values(w)[blocks, kv]).reshape(-1, dim)[:n].cuda() for w in (0, 1))
+        x = q[:, h].cuda().double()
+        s = ((x @ k.T.contiguous()) * dim ** -0.5).masked_fill(~seen, -torch.inf)
+        want_lse = torch.logsumexp(s, 1)
+        w = torch.exp(s - want_lse[:, None])
+        want, size = w @ v, w @ v.abs()
+        near = (x.abs() @ k.abs().T.contiguous()).masked_fill(~seen, 0).amax(1)
+        score = (dim + 8) * 2.0 ** -24 * near * dim ** -0.5 + 2.0 ** -22 * s.masked_fill(~seen, 0).abs().amax(1)
+        scale = torch.from_numpy(cache.scale[1][blocks, kv].astype(np.float64)).repeat_interleave(64)[:n].cuda()
+        under = seen.sum(1) * 2.0 ** -25 * 127 * (seen * scale).amax(1)
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2 * score + 2.0 ** -18)[:, None] * size + under[:, None]
+        assert ((out[:, h].double() - want).abs() <= bound).all()
+        assert ((lse[:, h].double() - want_lse).abs() <= score + 2.0 ** -20 * (1 + want_lse.abs())).all()
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 100, 1000])
 @pytest.mark.parametrize("tokens", [1, 4, 90])
