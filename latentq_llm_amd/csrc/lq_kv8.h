@@ -120,6 +120,7 @@ struct Kv8Attn {
     int rows;                     // few rows: of a slot, max_tokens * heads / kv_heads
     int slices, tiles;            // prompt: slices of the keys, tiles of 64 keys in each; slots are slices, rows those of the operands
     int row_tiles, waves, sides;  // prompt: workgroups along a sequence's rows, of so many waves with 32 rows each, and so many groups of those
+    int ranked;                   // prompt: workgroups in the order of their rows' positions, of all sequences
 };
 
 // The new tokens of one sequence: rows start .. start + n - 1 of the operands, its length in the cache, the position of the first,

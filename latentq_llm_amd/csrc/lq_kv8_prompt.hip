@@ -17,6 +17,42 @@ namespace {
 
 constexpr float kLazy = 8.0f;
 
+// Sum over the lanes (in rows of 16 by lane shifts, then the four rows)
+__device__ __forceinline__ int lanes_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    return __builtin_amdgcn_readlane(x, 15) + __builtin_amdgcn_readlane(x, 31) + __builtin_amdgcn_readlane(x, 47) + __builtin_amdgcn_readlane(x, 63);
+}
+
+// Workgroups of a batch whose sequences differ in length: the (sequence, tile of kRows rows)s in the order of their last positions, those
+// that see most keys first. Sequence i has one such pair at each level base_i + 1 .. base_i + n_i, one level being kRows rows further;
+// the one of rank p is on the highest level with more than p pairs on it and above. A lane knows a sequence.
+template <int kRows>
+__device__ __forceinline__ bool ranked(const Kv8Attn &a, int rank, int group, Kv8Rows &s, int &seq, int &tile) {
+    const int lane = threadIdx.x & 63;
+    const Kv8Rows r = kv8_rows<false>(a, min(lane, a.batch - 1));
+    const int count = lane < a.batch ? (int)min(((int64_t)r.n * group + kRows - 1) / kRows, (int64_t)a.row_tiles) : 0;
+    const int base = (int)min((int64_t)max(r.first, 0) * group / kRows, (int64_t)1 << 29), top = base + count;
+    if (lanes_sum(count) <= rank) return false;
+    int low = 1, above = 0, span = 1;  // the level is among low .. low + span - 1; pairs on higher ones
+    while (__any(top >= low + span)) span *= 2;
+    while (span > 1) {
+        span /= 2;
+        const int n = lanes_sum(max(min(top - (low + span) + 1, count), 0));
+        if (n > rank) low += span;
+        else above = n;
+    }
+    uint64_t level = __ballot(base < low && low <= top);
+    for (int skip = rank - above; skip > 0; --skip) level &= level - 1;
+    seq = __builtin_ctzll(level);
+    const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, seq); };
+    s = Kv8Rows{of(r.start), of(r.n), of(r.len), of(r.first), of(r.t_first), of(r.tiles)};
+    tile = low - of(base) - 1;
+    return true;
+}
+
 // kWaves: waves side by side on 32 rows each; kSides: groups of them that take every kSides-th tile of the keys of the same rows,
 // each with shared memory of its own, joined at the end
 template <int D, int kWaves, int kSides, bool kF16>
@@ -27,12 +63,21 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
     constexpr int kHalf = KV8_BLOCK * kPieces;  // = 8 D
     __shared__ u32x4_t lds[kSides][2][2 * kHalf];
 
-    const int units = a.batch * a.kv_heads;
-    const int unit = blockIdx.x % units, rest = blockIdx.x / units;
-    const int slice = rest % a.slices, tile = a.row_tiles - 1 - rest / a.slices;  // the last rows see most keys: first
-    const int seq = unit / a.kv_heads, h = unit % a.kv_heads;
-    const Kv8Rows s = kv8_rows<true>(a, seq);
     const int group = a.heads / a.kv_heads;
+    int seq, h, tile, slice;
+    Kv8Rows s;
+    if (a.ranked) {
+        slice = blockIdx.x / a.kv_heads % a.slices;
+        h = blockIdx.x % a.kv_heads;
+        if (!ranked<kRows>(a, blockIdx.x / (a.kv_heads * a.slices), group, s, seq, tile)) return;
+    } else {
+        const int units = a.batch * a.kv_heads, unit = blockIdx.x % units, rest = blockIdx.x / units;
+        slice = rest % a.slices;
+        tile = a.row_tiles - 1 - rest / a.slices;  // the last rows see most keys: first
+        seq = unit / a.kv_heads;
+        h = unit % a.kv_heads;
+        s = kv8_rows<true>(a, seq);
+    }
     const int64_t all_rows = (int64_t)s.n * group;
     const int row0 = tile * kRows;
     if (row0 >= all_rows) return;

@@ -84,6 +84,20 @@ def test_prompts_of_a_few_sequences(hip_lib, lens, news, how, dim, dtype):
     holds(call(cache.tensors(), q, table, lens, news, **how), want, bound)
 
 
+@pytest.mark.parametrize("batch", [2, 17, 64, 65])
+@pytest.mark.parametrize("how", [{}, {"window": 90}, {"causal": False}])
+def test_prompts_of_different_lengths(hip_lib, batch, how):
+    """Many rows of many sequences: none, a few and all of their tokens new, prefixes of no and of many tokens, rows before the first position."""
+    rng = np.random.default_rng(batch)
+    news = [int(n) for n in np.exp2(rng.uniform(0, 6, batch))]
+    lens = [n + int(p) for n, p in zip(news, rng.integers(0, 200, batch) * rng.integers(0, 2, batch))]
+    news[0], lens[0] = 70, 70
+    if batch > 2:
+        news[1], lens[2], lens[3] = 0, 0, max(news[3] - 1, 0)
+    run(lens, news, 16, 1, 64, BF16, seed=batch, **how)
+    run(lens[:9], news[:9], 18, 2, 128, F16, seed=batch, **how)
+
+
 @pytest.mark.parametrize("how", [{}, {"causal": False}, {"window": 500}])
 @pytest.mark.parametrize("dim, heads, kv_heads", [(128, 32, 8), (64, 32, 32), (256, 16, 4), (96, 12, 12)])
 def test_long_prompts(hip_lib, dim, heads, kv_heads, how):
