@@ -554,11 +554,11 @@ int lq_kv8_read(const void *k_codes, const void *v_codes, const float *k_scale, 
 
 /* out = softmax(scale * q K^T) V of the new tokens (rows of heads x dim; query head j reads kv head j / (heads / kv_heads)) over
  * the sequence's tokens in the cache: those at positions <= the row's own (causal = 0: all), and with window > 0
- * only the last `window` of positions up to the row's own. A row that sees nothing gives zeros. lse (null, or float
+ * none at positions <= the row's own less `window`. A row that sees nothing gives zeros. lse (null, or float
  * [tokens][heads]): the natural logarithm of the softmax's denominator, -inf for such a row. scale > 0.
  * q becomes f16 by a power of two for each row (exact but for elements under 2^-37 of the row's largest), codes are exact, scores,
  * softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits) relative to the largest contribution so far.
- * workspace (16-byte aligned, or null): with it, calls of few rows share the keys among more workgroups, whose partial results a
+ * workspace (16-byte aligned, or null): with it, long keys are shared among more workgroups, whose partial results a
  * second launch joins in order; lq_kv8_attention_plan says how many and the bytes they take. Calls sharing a workspace are
  * ordered on one stream. */
 int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes,

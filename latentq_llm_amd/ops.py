@@ -1132,7 +1132,7 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
                   causal=True, window=0, out=None, return_lse=False):
     """Attention of the last tokens of each sequence, q [tokens, heads, dim], over its blocks of a paged 8-bit cache (lq_kv8_attention):
     softmax(scale * q K^T) V, scale 1 / sqrt(dim) by default, query head j on kv head j // (heads // kv_heads). A row sees
-    the positions up to its own (causal=False: the whole sequence), with window > 0 only the last `window` of them; one that sees
+    the positions up to its own (causal=False: the whole sequence), with window > 0 none before the last `window` up to its own; one that sees
     nothing gives zeros. max_tokens and max_len, the largest numbers of new tokens and of tokens of a sequence, size the launch
     (defaults: what the rows and the block table allow). return_lse: also the logarithm of the softmax's denominator, float32 [tokens, heads]."""
     if out is None:
