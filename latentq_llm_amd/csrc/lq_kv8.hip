@@ -423,22 +423,23 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
         // Slices of the keys, and a workgroup's shape, by an estimate in us. A tile takes `busy` of a compute unit that has workgroups
         // enough, and `alone` at least in each workgroup; the ways in and out cost 3 tiles; slices take their partial results there and
         // back (4.5 TB/s) and a launch. With 8 waves a row has half the conversions, but there are half the workgroups: single sequences of
-        // 4096 tokens (32 heads of 128) 160 -> 147 us, 1024 on 16384 keys 289 -> 270, but 2048 tokens 54 -> 64, 4 x 1019 39 -> 43. Where
-        // every workgroup has a compute unit to itself, two sides of 4 waves take the tiles by turns, `paired` for each (5 more for the ways): 1024
-        // tokens, 32 heads of 128, 28.0 -> 24.4, 8 x 128 on 2048 keys 52.1 -> 40.7, but 70 tokens 8.4 -> 9.1; with more workgroups than that,
-        // 4 x 512, 23.5 -> 28.9. By slices, measured / estimated: 64 dimensions, 256 tokens on 16384 keys in 4 75 / 80, in 8 59 / 65; 96
-        // dimensions, 12 heads, 2048 tokens in 1 58 / 56, in 3 39 / 41.
+        // 4096 tokens (32 heads of 128) 160 -> 147 us, 1024 on 16384 keys 289 -> 270, but 2048 tokens 54 -> 64, 4 x 1019 39 -> 43; of 96
+        // dimensions 4096 tokens 142 -> 127, 8192 489 -> 468; of 64 dimensions never (8192 tokens 336 -> 362). Where every workgroup has a compute
+        // unit to itself, two sides of 4 waves take the tiles by turns, `paired` for each (5 more for the ways): 1024 tokens, 32 heads of 128,
+        // 28.0 -> 24.4, 8 x 128 on 2048 keys 52.1 -> 40.7, but 70 tokens 8.4 -> 9.1; with more workgroups than that, 4 x 512, 23.5 -> 28.9.
+        // By slices, measured / estimated: 64 dimensions, 256 tokens on 16384 keys in 4 75 / 80, in 8 59 / 65; 96 dimensions, 12 heads, 2048
+        // tokens in 1 58 / 56, in 3 39 / 41.
         const double busy4 = dim == 64 ? 0.73 : dim == 96 ? 0.9 : dim == 128 ? 1.15 : 2.2, alone4 = dim == 64 ? 1.05 : dim == 96 ? 1.6 : dim == 128 ? 1.45 : 2.2;
-        const double paired = dim == 64 ? 0.8 : dim == 96 ? 1.1 : 1.15;
+        const double busy8 = dim == 96 ? 1.7 : 2.1, paired = dim == 64 ? 0.8 : dim == 96 ? 1.1 : 1.15;
         const int64_t slice_bytes = tokens * heads * ((int64_t)dim + 1) * 4;
         const double mean = (double)tiles - (double)max_tokens / (2 * KV8_BLOCK);  // of the rows' tiles, where all of them are causal
         double best = 0;
         const struct { int waves, sides; } shapes[] = {{4, 1}, {8, 1}, {4, 2}};
         for (const auto &shape : shapes) {
             const int waves = shape.waves, sides = shape.sides;
-            if ((waves == 8 && (dim != 128 || tiles < 64)) || (sides == 2 && dim > 128)) continue;
+            if ((waves == 8 && ((dim != 96 && dim != 128) || tiles < 64)) || (sides == 2 && dim > 128)) continue;
             const int64_t row_tiles = (rows + 32 * waves - 1) / (32 * waves);
-            const double busy = waves == 4 ? busy4 : 2.1, alone = sides == 2 ? paired : waves == 4 ? alone4 : 2.1;
+            const double busy = waves == 4 ? busy4 : busy8, alone = sides == 2 ? paired : waves == 4 ? alone4 : busy8;
             for (int64_t s = 1; s <= 64 && s <= tiles && (s == 1 || s <= workspace / slice_bytes); ++s) {
                 const int64_t per = (tiles + s - 1) / s, load = (units * row_tiles * s + cus - 1) / cus;
                 if (sides == 2 && load > 1) break;

@@ -399,9 +399,10 @@ int launch_join(const Kv8Attn &a, bool f16, hipStream_t s) {
 template <int D>
 int launch(const Kv8Attn &a, bool f16, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.batch * a.kv_heads * a.slices * a.row_tiles));
-    if (a.waves == 8) {  // (128 dimensions only)
-        if (f16) prompt_kernel<128, 8, 1, true><<<grid, 512, 0, s>>>(a);
-        else prompt_kernel<128, 8, 1, false><<<grid, 512, 0, s>>>(a);
+    constexpr int kWide = D == 96 ? 96 : 128;
+    if (a.waves == 8) {  // (96 and 128 dimensions)
+        if (f16) prompt_kernel<kWide, 8, 1, true><<<grid, 512, 0, s>>>(a);
+        else prompt_kernel<kWide, 8, 1, false><<<grid, 512, 0, s>>>(a);
     } else if (a.sides == 2) {  // (up to 128 dimensions)
         if (f16) prompt_kernel<D <= 128 ? D : 128, 4, 2, true><<<grid, 512, 0, s>>>(a);
         else prompt_kernel<D <= 128 ? D : 128, 4, 2, false><<<grid, 512, 0, s>>>(a);

@@ -99,7 +99,7 @@ def test_prompts_of_different_lengths(hip_lib, batch, how):
 
 
 @pytest.mark.parametrize("how", [{}, {"causal": False}, {"window": 500}])
-@pytest.mark.parametrize("dim, heads, kv_heads", [(128, 32, 8), (64, 32, 32), (256, 16, 4), (96, 12, 12)])
+@pytest.mark.parametrize("dim, heads, kv_heads", [(128, 32, 8), (64, 32, 32), (256, 16, 4), (96, 12, 12), (96, 32, 8)])
 def test_long_prompts(hip_lib, dim, heads, kv_heads, how):
     """Some thousands of tokens of all heads, against 64 bits on the card; the bound is tests/kv8_ref.py's."""
     n, new = 4221, 4090
