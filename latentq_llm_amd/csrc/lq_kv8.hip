@@ -11,6 +11,7 @@
 // Bound: memory. Appending 8192 tokens of 32 + 8 heads of 128 and turning their queries moves 185 MB in 39 us, 4.7 TB/s, where a copy
 // of 1 GiB reaches 5.0. One token of 32 heads, 4.8 us, is the launch and loads that wait for each other: length, table, scale.
 #include "lq_kv8.h"
+#include "lq_kv8_place.h"
 
 namespace {
 
@@ -156,14 +157,12 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
     int start, n;
     kv8_span(a.cu, a.batch, a.tokens, seq, start, n);
     if (n == 0) return;
-    const int len = max(kv8_uniform(a.lens + seq), 0), first = len - n;
-    const int place = max(first, 0) / KV8_BLOCK + jb;  // which block of the sequence
-    const int begin = place * KV8_BLOCK, hi = min(len, begin + KV8_BLOCK);
+    const auto [first, place, begin, hi, from, lo] = kv8_place(max(kv8_uniform(a.lens + seq), 0), n, jb);
     const int64_t row0 = (int64_t)start - first;  // row of the operands that position 0 would have
 
-    if (role < 0) {  // queries of kQHeads heads: positions of this block, and with its first block any before position 0
+    if (role < 0) {  // queries of kQHeads heads
         constexpr int kPairs = D / 16;
-        const int h0 = (role + a.q_groups) * kQHeads, heads = min(kQHeads, a.heads - h0), from = jb ? begin : first, count = hi - from;
+        const int h0 = (role + a.q_groups) * kQHeads, heads = min(kQHeads, a.heads - h0), count = hi - from;
         const uint16_t *src = (const uint16_t *)a.q + h0 * a.q_head;
         uint16_t *dst = (uint16_t *)a.q_out + h0 * a.qo_head;
         if constexpr (kThreads == 64) {  // few tokens: heads side by side
@@ -195,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
         return;
     }
 
-    const int lo = max(first, begin), count = hi - lo;
+    const int count = hi - lo;
     if (count <= 0 || place >= a.width) return;
     const int block = kv8_uniform(a.table + (int64_t)seq * a.width + place);
     if (block < 0 || block >= a.blocks) return;
