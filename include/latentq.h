@@ -515,7 +515,7 @@ int lq_weight_grad_plan(int form, int64_t M, int64_t N, int64_t K, int compute_u
  * The cache is a pool of num_blocks blocks of LQ_KV_BLOCK tokens, for kv_heads heads of dim dimensions (64, 96, 128 or 256):
  *   k_codes  uint8 [num_blocks][kv_heads][64][dim]
  *   v_codes  uint8 [num_blocks][kv_heads][16][dim][4]    token t of a block at [t / 4][d][t % 4]
- *   k_scale, v_scale  float [num_blocks][kv_heads]       value = (code - 128) * scale, codes 1 .. 255
+ *   k_scale, v_scale  float [num_blocks][kv_heads]       value = (code - 128) * scale, codes 1 .. 255, scales finite and not negative
  * block_table int32 [batch][table_width] lists the blocks of each sequence in order, seq_lens int32 [batch] the tokens
  * of each sequence in the cache INCLUDING the new ones. Operands hold the new tokens of all sequences one after the
  * other, `tokens` rows in all: cu_tokens int32 [batch + 1] has each sequence's first row and, last, the number of
@@ -557,7 +557,9 @@ int lq_kv8_read(const void *k_codes, const void *v_codes, const float *k_scale, 
  * none at positions <= the row's own less `window`. A row that sees nothing gives zeros. lse (null, or float
  * [tokens][heads]): the natural logarithm of the softmax's denominator, -inf for such a row. scale > 0.
  * q becomes f16 by a power of two for each row (exact but for elements under 2^-37 of the row's largest), codes are exact, scores,
- * softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits) relative to the largest contribution so far.
+ * softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits) relative to the largest contribution so far
+ * (weight times v_scale; keys under 2^-126 of it count for nothing). A block whose v_scale is under 2^-97, as 0, has values of zero: its keys
+ * have their weight and add nothing.
  * workspace (16-byte aligned, or null): with it, long keys are shared among more workgroups, whose partial results a
  * second launch joins in order; lq_kv8_attention_plan says how many and the bytes they take. Calls sharing a workspace are
  * ordered on one stream. */

@@ -84,6 +84,12 @@ __device__ __forceinline__ f16x8_t kv8_operand(unsigned a, unsigned b) {
     return __builtin_bit_cast(f16x8_t, u32x4_t{x[0], x[1], y[0], y[1]});
 }
 
+// The value scale goes into the exponent as its logarithm and into the denominator as its reciprocal, so it may not be 0 there: a scale under
+// 2^-97 (the least that appending makes is 2^-90 / 127, just above it; a quantiser that takes the largest magnitude gives 0 to a block of
+// zeros) counts as 2^-97, which the weight in the denominator does not see, and the block's values as zeros.
+constexpr float kLeastScale = 0x1p-97f;
+__device__ __forceinline__ bool kv8_no_values(float scale) { return __float_as_uint(scale) << 1 < __builtin_bit_cast(unsigned, kLeastScale) << 1; }
+
 // Maximum over lanes i, i ^ 32 and over i, i ^ 16 (v_permlane32_swap / v_permlane16_swap with both operands the same value
 // leave the two lanes' values in the two results): vector instructions, where a shuffle would go through shared memory.
 __device__ __forceinline__ float kv8_max32(float x) {

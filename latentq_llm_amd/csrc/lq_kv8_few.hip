@@ -242,7 +242,9 @@ __global__ __launch_bounds__(256, kv8_few_waves(D, RT)) void few_kernel(const Kv
             __builtin_amdgcn_sched_barrier(0);
         }
         const int key0 = t * KV8_BLOCK;
-        const float lv = __builtin_amdgcn_logf(vs), rv = 1.0f / vs;
+        const bool no_values = kv8_no_values(vs);
+        const float vs_least = no_values ? kLeastScale : vs, lv = __builtin_amdgcn_logf(vs_least), rv = 1.0f / vs_least;
+        const unsigned kept = no_values ? 0u : ~0u;  // of the weights' bits, once they are in the denominator
         f16x8_t p[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(256, kv8_few_waves(D, RT)) void few_kernel(const Kv
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const f32x4_t x = c[rt][2 * e], y = c[rt][2 * e + 1];
-                p[rt][e] = __builtin_bit_cast(f16x8_t, u32x4_t{kv8_pack_f16(x[0], x[1]), kv8_pack_f16(x[2], x[3]), kv8_pack_f16(y[0], y[1]), kv8_pack_f16(y[2], y[3])});
+                p[rt][e] = __builtin_bit_cast(f16x8_t, u32x4_t{kv8_pack_f16(x[0], x[1]) & kept, kv8_pack_f16(x[2], x[3]) & kept, kv8_pack_f16(y[0], y[1]) & kept, kv8_pack_f16(y[2], y[3]) & kept});
             }
         }
 #pragma unroll

@@ -37,3 +37,40 @@ def test_appending_at_the_largest_lengths(hip_lib, tokens, back):
     codes = ref.from_layout(*tensors[:2])
     assert all(np.array_equal(a, b) for a, b in zip(codes, cache.codes))
     assert all(np.array_equal(a.cpu().numpy(), b) for a, b in zip(tensors[2:], cache.scale))
+
+
+def call(tensors, q, table, lens, news, **more):
+    from latentq_llm_amd import ops
+    cu = None if len(set(news)) == 1 else i32(np.concatenate([[0], np.cumsum(news)]))
+    return ops.kv8_attention(q.cuda(), *tensors, i32(table), i32(lens), cu_tokens=cu, **more)
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("lens, tokens", [([400], 1), ([1900], 3), ([400], 90), ([700], 500), ([8300], 70)])
+def test_value_scales_of_zero(hip_lib, lens, tokens, dim):
+    """Blocks whose value scale is 0, negative zero, subnormal or under 2^-97, as of blocks of zeros: their keys have their weight, their values
+    add nothing. One workgroup to a row, shares, one tile, two sides and slices of the keys."""
+    pool = -(-lens[0] // 64) + 2
+    table = ref.blocks_of(lens, pool, seed=1)
+    q = rows((tokens, 4, dim), BF16, 6)
+    for seed, scales in ((0, [0.0]), (1, [0.0, -0.0, 1e-40, 2.0 ** -126, 2.0 ** -98]), (2, [2.0 ** -97])):
+        cache = ref.Cache(pool, 2, dim, seed=5 + seed)
+        rng = np.random.default_rng(seed)
+        for h in range(2):
+            for b in range(pool):
+                if rng.random() < 0.5:
+                    cache.scale[1][b, h] = np.float32(rng.choice(scales))
+        cache.scale[1][table[0, 0]] = scales[0]  # among them the first tile
+        want, (want_lse, lse_bound), bound = ref.attention(cache, q, table, lens, [tokens])
+        out, lse = call(cache.tensors(), q, table, lens, [tokens], return_lse=True)
+        got, off = out.cpu().double().numpy(), np.abs(out.cpu().double().numpy() - want)
+        assert np.isfinite(got).all() and (off <= bound + 127 * 2.0 ** -97).all(), (seed, float((off / bound).max()))
+        assert (np.abs(lse.cpu().double().numpy() - want_lse) <= lse_bound).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+def test_value_scales_that_are_all_zero(hip_lib, tokens):
+    cache = ref.Cache(6, 2, 64, seed=5)
+    cache.scale[1][:] = 0
+    table = ref.blocks_of([300], 6)
+    assert not call(cache.tensors(), rows((tokens, 4, 64), BF16, 6), table, [300], [tokens]).any()
