@@ -35,7 +35,10 @@ class KVCache8:
         return self.k_codes, self.v_codes, self.k_scale, self.v_scale
 
     def append(self, k, v, step: "Step", q=None, cos=None, sin=None):
-        """ops.kv8_append of a step's new tokens; returns the rotated q, or None."""
+        """ops.kv8_append of a step's new tokens; returns the rotated q, or None. Raises, and appends nothing, where a sequence has outgrown the
+        rotation tables."""
+        if cos is not None and step.longest > cos.shape[0]:  # (the kernel would turn what lies beyond by the last row)
+            raise ValueError(f"the rotation tables have {cos.shape[0]} positions, a sequence {step.longest} tokens")
         return ops.kv8_append(k, v, *self.tensors(), step.block_table, step.seq_lens, q=q, cos=cos, sin=sin, cu_tokens=step.cu_tokens,
                               max_tokens=step.max_tokens)
 
@@ -52,7 +55,7 @@ class KVCache8:
 @dataclass
 class Step:
     """The new tokens of a pass: tensors on the device and the host's bounds that size the launches. Rows of the operands are the
-    sequences' new tokens one after the other."""
+    sequences' new tokens one after the other. longest is what the host knows exactly, for checks."""
     block_table: torch.Tensor  # int32 [sequences, blocks of the longest]
     seq_lens: torch.Tensor     # int32 [sequences], new tokens included
     cu_tokens: torch.Tensor | None
@@ -60,6 +63,7 @@ class Step:
     max_len: int
     last: torch.Tensor         # int64 [sequences]: the row of each one's last new token
     positions: torch.Tensor    # int64 [rows]
+    longest: int = 0           # tokens of the longest sequence (0: not known, not checked)
 
 
 class Sequences:
@@ -108,7 +112,8 @@ class Sequences:
                     seq_lens=torch.tensor([lens[s] for s in new], **i32),
                     cu_tokens=None if len(set(counts)) == 1 else torch.tensor(starts, **i32), max_tokens=max(counts), max_len=max(lens.values()),
                     last=torch.tensor(starts[1:], device=self.device) - 1,
-                    positions=torch.cat([torch.arange(lens[s] - n, lens[s]) for s, n in new.items()]).to(self.device))
+                    positions=torch.cat([torch.arange(lens[s] - n, lens[s]) for s, n in new.items()]).to(self.device),
+                    longest=max(lens.values()))
 
 
 def rotation_tables(positions: int, head_dim: int, base: float = 10000.0, device="cuda"):
