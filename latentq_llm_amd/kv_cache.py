@@ -34,9 +34,14 @@ class KVCache8:
     def tensors(self):
         return self.k_codes, self.v_codes, self.k_scale, self.v_scale
 
+    def _holds(self, step: "Step") -> None:
+        if step.pool > self.num_blocks:  # (the kernels would drop its tokens and read another block)
+            raise ValueError(f"the pass uses block {step.pool - 1} of a cache of {self.num_blocks} blocks")
+
     def append(self, k, v, step: "Step", q=None, cos=None, sin=None):
         """ops.kv8_append of a step's new tokens; returns the rotated q, or None. Raises, and appends nothing, where a sequence has outgrown the
-        rotation tables."""
+        rotation tables or its blocks are not of this cache."""
+        self._holds(step)
         if cos is not None and step.longest > cos.shape[0]:  # (the kernel would turn what lies beyond by the last row)
             raise ValueError(f"the rotation tables have {cos.shape[0]} positions, a sequence {step.longest} tokens")
         return ops.kv8_append(k, v, *self.tensors(), step.block_table, step.seq_lens, q=q, cos=cos, sin=sin, cu_tokens=step.cu_tokens,
@@ -44,6 +49,7 @@ class KVCache8:
 
     def attend(self, q, step: "Step", scale=None, window=0):
         """ops.kv8_attention of a step's new tokens over what the cache holds of their sequences."""
+        self._holds(step)
         return ops.kv8_attention(q, *self.tensors(), step.block_table, step.seq_lens, cu_tokens=step.cu_tokens, max_tokens=step.max_tokens,
                                  max_len=step.max_len, scale=scale, window=window)
 
@@ -55,7 +61,7 @@ class KVCache8:
 @dataclass
 class Step:
     """The new tokens of a pass: tensors on the device and the host's bounds that size the launches. Rows of the operands are the
-    sequences' new tokens one after the other. longest is what the host knows exactly, for checks."""
+    sequences' new tokens one after the other. longest and pool are what the host knows exactly, for checks."""
     block_table: torch.Tensor  # int32 [sequences, blocks of the longest]
     seq_lens: torch.Tensor     # int32 [sequences], new tokens included
     cu_tokens: torch.Tensor | None
@@ -64,6 +70,7 @@ class Step:
     last: torch.Tensor         # int64 [sequences]: the row of each one's last new token
     positions: torch.Tensor    # int64 [rows]
     longest: int = 0           # tokens of the longest sequence (0: not known, not checked)
+    pool: int = 0              # blocks that a cache must have: the highest one named, and 1 (0: as above)
 
 
 class Sequences:
@@ -113,7 +120,7 @@ class Sequences:
                     cu_tokens=None if len(set(counts)) == 1 else torch.tensor(starts, **i32), max_tokens=max(counts), max_len=max(lens.values()),
                     last=torch.tensor(starts[1:], device=self.device) - 1,
                     positions=torch.cat([torch.arange(lens[s] - n, lens[s]) for s, n in new.items()]).to(self.device),
-                    longest=max(lens.values()))
+                    longest=max(lens.values()), pool=1 + max(max(self._blocks[s]) for s in new))
 
 
 def rotation_tables(positions: int, head_dim: int, base: float = 10000.0, device="cuda"):

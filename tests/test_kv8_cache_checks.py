@@ -1,4 +1,4 @@
-"""What the cache of a layer refuses on the host, before anything is launched: passes beyond the rotation tables."""
+"""What the cache of a layer refuses on the host, before anything is launched: passes beyond the rotation tables, and blocks that it has not."""
 import pytest
 import torch
 
@@ -23,6 +23,19 @@ def test_a_sequence_longer_than_the_rotation_tables():
     with pytest.raises(ValueError, match="a sequence 101 tokens"):
         attention(x[:1], cache, seqs.extend({"b": 1}))
     assert (cache.k_codes == 128).all() and (cache.v_codes == 128).all()
+
+
+def test_a_pool_larger_than_the_cache():
+    """Sequences may be of more blocks than a cache has, as long as none of those is used."""
+    attention, cache, seqs = layer(1000), KVCache8(3, 1, 64, device="cpu"), Sequences(5, device="cpu")
+    x = torch.zeros((192, 64), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        attention(x, cache, seqs.extend({"a": 192}))
+    step = seqs.extend({"b": 1})
+    assert step.pool == 4
+    for call in (lambda: attention(x[:1], cache, step), lambda: cache.attend(x[:1].view(1, 1, 64), step), lambda: cache.append(x[:1].view(1, 1, 64), x[:1].view(1, 1, 64), step)):
+        with pytest.raises(ValueError, match="block 3 of a cache of 3 blocks"):
+            call()
 
 
 def test_a_step_made_by_hand_is_taken_as_it_is():
