@@ -68,7 +68,12 @@ struct W4 {
 
 int64_t integer(PyObject *o) { return PyLong_AsLongLong(o); }
 
-PyObject *none() { Py_RETURN_NONE; }
+// The wrapper is to look at the call. An argument that could not be converted has left its error, which the wrapper's own conversions
+// and checks take the place of.
+PyObject *none() {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
 
 PyObject *fail(const char *who, int rc) {
     PyErr_Format(g_error ? g_error : PyExc_RuntimeError, "%s failed (%d): %s", who, rc, lq_last_error());
