@@ -630,9 +630,12 @@ struct Rows16 {
         dtype = f16;
         return true;
     }
-    // rows of their own, to be written
+    // rows of their own, to be written: the heads of a token beside each other, or the tokens of a head (the wrapper looks at others)
     bool separate() const {
-        return (t->size(0) == 1 || t->stride(0) >= t->size(2)) && (t->size(1) == 1 || t->stride(1) >= t->size(2));
+        const auto within = [this](int inner, int outer) {
+            return (t->size(inner) == 1 || t->stride(inner) >= t->size(2)) && (t->size(outer) == 1 || t->stride(outer) >= t->stride(inner) * (t->size(inner) - 1) + t->size(2));
+        };
+        return within(1, 0) || within(0, 1);
     }
 };
 

@@ -13,6 +13,8 @@
 #include "lq_kv8.h"
 #include "lq_kv8_place.h"
 
+#include <utility>
+
 namespace {
 
 constexpr float kLeast = 0x1p-90f;  // so that scales, their reciprocals and their logarithms are all normal numbers
@@ -379,6 +381,23 @@ void launch_read(const void *k_codes, const void *v_codes, const float *k_scale,
     else read_kernel<D, 2><<<grid, 256, 0, s>>>(k, v, k_scale, v_scale, blocks, k_out, v_out, kv_heads, pool);
 }
 
+// Whether rows of dim elements, at multiples of two strides, lie apart: outputs, which are written in no order. Strides in which one index goes
+// round within a step of the other do; any others are looked at row by row.
+bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int dim) {
+    if ((n0 > 1 && s0 < dim) || (n1 > 1 && s1 < dim)) return false;
+    if (n0 <= 1 || n1 <= 1) return true;
+    if (s0 > s1) {
+        std::swap(n0, n1);
+        std::swap(s0, s1);
+    }
+    const __int128 end = (__int128)(n0 - 1) * s0 + dim;  // of the rows of one outer index
+    for (int64_t j = 1; j < n1 && (__int128)j * s1 < end; ++j) {
+        const __int128 at = (__int128)j * s1, i = at / s0;
+        if ((i < n0 && at - i * s0 < dim) || (i + 1 < n0 && (i + 1) * s0 - at < dim)) return false;
+    }
+    return true;
+}
+
 bool good_dim(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 256; }
 
 // How a call is cut.
@@ -491,6 +510,7 @@ extern "C" int lq_kv8_append(const void *k, int64_t k_token_stride, int64_t k_he
         LQ_REQUIRE(s >= 0 && s % 8 == 0, "kv8_append: strides must be multiples of 8 elements, got %lld", (long long)s);
     for (const void *p : {k, v, q, (const void *)q_out, (const void *)cos_table, (const void *)sin_table, (const void *)k_codes, (const void *)v_codes})
         LQ_REQUIRE(lq_aligned(p, 16), "kv8_append: k, v, q, the tables and the codes must be 16-byte aligned");
+    LQ_REQUIRE(!q || rows_apart(tokens, q_out_token_stride, heads, q_out_head_stride, dim), "kv8_append: rows of q_out overlap");
     Append a{k, v, q, q_out, cos_table, sin_table, (uint8_t *)k_codes, (uint8_t *)v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens,
              k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride,
              (int)positions, cos_table ? rot_dim : 0, (int)num_blocks, (int)table_width, (int)batch, (int)tokens, heads, kv_heads, 0, q ? (heads + kQHeads - 1) / kQHeads : 0};
@@ -572,6 +592,7 @@ extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q
         LQ_REQUIRE(s >= 0 && s % 8 == 0, "kv8_attention: strides must be multiples of 8 elements, got %lld", (long long)s);
     for (const void *p : {q, k_codes, v_codes, (const void *)out, (const void *)workspace})
         LQ_REQUIRE(lq_aligned(p, 16), "kv8_attention: q, codes, output and workspace must be 16-byte aligned");
+    LQ_REQUIRE(rows_apart(tokens, out_token_stride, heads, out_head_stride, dim), "kv8_attention: rows of the output overlap");
     LQ_REQUIRE(workspace_bytes >= 0, "kv8_attention: the workspace's size must not be negative");
     if (max_tokens > tokens) max_tokens = tokens;
     if (max_len > table_width * KV8_BLOCK) max_len = table_width * KV8_BLOCK;

@@ -1003,12 +1003,21 @@ def _kv8_layout(t):
     return t if not t.numel() or _kv8_in_form(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def _kv8_apart(t):
+    """Whether the rows [tokens, heads] of t lie apart."""
+    (s0, n0), (s1, n1) = sorted(zip(t.stride(), t.shape[:2]))
+    dim, end = t.shape[2], (n0 - 1) * s0 + t.shape[2]
+    if (n0 > 1 and s0 < dim) or (n1 > 1 and s1 < dim):
+        return False
+    return n0 <= 1 or not any(j * s1 % s0 < dim and j * s1 // s0 < n0 or -(j * s1) % s0 < dim and -(-j * s1 // s0) < n0 for j in range(1, min(n1, -(-end // s1))))
+
+
 def _kv8_result(t, name, like):
     """An output given by the caller: rows like `like`, none of them in another's place."""
     _kv8_rows(t, name, like.shape[1], like.shape[2], like, like.dtype)
     if t.shape != like.shape:
         raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(t.shape)}")
-    if t.numel() and (not _kv8_in_form(t) or any(t.shape[i] > 1 and t.stride(i) < t.shape[2] for i in (0, 1))):
+    if t.numel() and not (_kv8_in_form(t) and _kv8_apart(t)):
         raise ValueError(f"{name} must have a contiguous last dimension and 16-byte aligned heads of their own")
     return t
 

@@ -74,3 +74,27 @@ def test_value_scales_that_are_all_zero(hip_lib, tokens):
     cache.scale[1][:] = 0
     table = ref.blocks_of([300], 6)
     assert not call(cache.tensors(), rows((tokens, 4, 64), BF16, 6), table, [300], [tokens]).any()
+
+
+def test_outputs_whose_rows_overlap(hip_lib):
+    """Refused in every entry; rows that lie apart in unusual strides are not."""
+    from latentq_llm_amd import ops
+    dim, lens = 64, [70]
+    cache = ref.Cache(3, 2, dim)
+    t, table, n = cache.tensors(), i32(ref.blocks_of(lens, 3)), i32(lens)
+    q, k = rows((6, 4, dim), BF16, 1).cuda(), rows((6, 2, dim), BF16, 2).cuda()
+    cos, sin = (torch.from_numpy(x).cuda() for x in ref.tables(70, dim))
+    room = torch.zeros(20000, dtype=BF16, device="cuda")
+    want = ops.kv8_attention(q, *t, table, n)
+    turned = ops.kv8_append(k, k, *ref.Cache(3, 2, dim).tensors(), table, n, q=q, cos=cos, sin=sin)
+    for strides, apart in (((64, 64), False), ((128, 64), False), ((64, 128), False), ((0, 64), False), ((256, 64), True), ((64, 384), True), ((192, 128), False),
+                           ((192, 64), False), ((512, 64), True), ((320, 1600), False), ((96, 576), True), ((192, 704), True)):
+        out = room.as_strided((6, 4, dim), (*strides, 1))
+        if apart:
+            assert torch.equal(ops.kv8_attention(q, *t, table, n, out=out), want), strides
+            assert torch.equal(ops.kv8_append(k, k, *ref.Cache(3, 2, dim).tensors(), table, n, q=q, cos=cos, sin=sin, q_out=out), turned), strides
+        else:
+            with pytest.raises(ValueError, match="heads of their own"):
+                ops.kv8_attention(q, *t, table, n, out=out)
+            with pytest.raises(ValueError, match="heads of their own"):
+                ops.kv8_append(k, k, *t, table, n, q=q, cos=cos, sin=sin, q_out=out)
