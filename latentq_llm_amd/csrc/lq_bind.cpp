@@ -615,6 +615,10 @@ PyObject *adam8_w8(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
 }
 
 // ---- paged 8-bit cache of keys and values
+// Its calls have no derivative: an operand that requires a gradient, and any call under an open forward-mode level, are the wrapper's,
+// which refuses those that would lose one.
+bool wants_gradient(const at::Tensor *t) { return t->requires_grad() && c10::GradMode::is_enabled(); }
+
 // Rows [tokens, heads, dim] of a 16-bit type in the strides the kernels take, without a gradient to keep
 struct Rows16 {
     const at::Tensor *t = nullptr;
@@ -625,7 +629,7 @@ struct Rows16 {
         const bool f16 = x.scalar_type() == at::kHalf;
         if (!x.is_cuda() || (!f16 && x.scalar_type() != at::kBFloat16) || x.dim() != 3 || x.numel() == 0 || !x.has_storage()) return false;
         if (x.key_set().has_any(kWrappedKeys) || x.stride(2) != 1 || x.stride(0) % 8 || x.stride(1) % 8 || !aligned16(&x)) return false;
-        if (x.requires_grad() && c10::GradMode::is_enabled()) return false;
+        if (wants_gradient(&x)) return false;
         t = &x;
         dtype = f16;
         return true;
@@ -653,7 +657,8 @@ struct Cache8 {
         dim = kc->size(3);
         return blocks > 0 && heads > 0 && kc->size(2) == LQ_KV_BLOCK && (dim == 64 || dim == 96 || dim == 128 || dim == 256) &&
                vc->sizes() == at::IntArrayRef({blocks, heads, LQ_KV_BLOCK / 4, dim, 4}) && ks->sizes() == at::IntArrayRef({blocks, heads}) &&
-               vs->sizes() == ks->sizes() && same_device(kc, vc) && same_device(kc, ks) && same_device(kc, vs) && aligned16(kc) && aligned16(vc);
+               vs->sizes() == ks->sizes() && same_device(kc, vc) && same_device(kc, ks) && same_device(kc, vs) && aligned16(kc) && aligned16(vc) && !wants_gradient(ks) &&
+               !wants_gradient(vs);
     }
 };
 
@@ -689,6 +694,7 @@ struct Sequences {
 // k, v, cache (4), block_table, seq_lens, q, cos, sin, cu_tokens, max_tokens, q_out -> the rotated q, or True without one
 PyObject *kv8_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     LQ_ARGS(14)
+    if (watched()) return none();
     Rows16 k, v, q, o;
     Cache8 c;
     Sequences s;
@@ -701,7 +707,7 @@ PyObject *kv8_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (!s.load(a[6], a[7], a[11], a[12], tokens, c.kc)) return none();
     const at::Tensor *cos = rotates ? plain(a[9], at::kFloat) : nullptr, *sin = rotates ? plain(a[10], at::kFloat) : nullptr;
     if (rotates && (!cos || !sin || cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->numel() == 0 || cos->size(1) % 8 || 2 * cos->size(1) > c.dim ||
-                    !same_device(cos, c.kc) || !same_device(sin, c.kc) || !aligned16(cos) || !aligned16(sin)))
+                    !same_device(cos, c.kc) || !same_device(sin, c.kc) || !aligned16(cos) || !aligned16(sin) || wants_gradient(cos) || wants_gradient(sin)))
         return none();
     if (with_q && (!q.load(a[8]) || !same_device(q.t, c.kc) || q.dtype != k.dtype || q.t->size(0) != tokens || q.t->size(2) != c.dim)) return none();
     if (a[13] != Py_None && (!o.load(a[13]) || !same_device(o.t, c.kc) || o.dtype != k.dtype || o.t->sizes() != q.t->sizes() || !o.separate())) return none();
@@ -727,6 +733,7 @@ PyObject *kv8_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
 // without a workspace where one is wanted: its bytes, and nothing is done
 PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     LQ_ARGS(15)
+    if (watched()) return none();
     Rows16 q;
     Cache8 c;
     Sequences s;
@@ -767,6 +774,7 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
 // cache (4), blocks, dtype as the C entry points number them -> (k, v)
 PyObject *kv8_read(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     LQ_ARGS(6)
+    if (watched()) return none();
     Cache8 c;
     const at::Tensor *b = plain(a[4], at::kInt);
     const int64_t dtype = integer(a[5]);

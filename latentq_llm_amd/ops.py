@@ -9,6 +9,7 @@ from __future__ import annotations
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _C
 
@@ -959,6 +960,14 @@ KV_DIMS = (64, 96, 128, 256)
 _KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+def _kv8_no_derivative(t, name):
+    """Refuses an operand whose derivative something waits for."""
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError(f"the operators of the 8-bit cache have no backward, and {name} requires a gradient")
+    if t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"the operators of the 8-bit cache have no derivative, and {name} has a tangent")
+
+
 def _kv8_cache(k_codes, v_codes, k_scale, v_scale):
     """(blocks, kv heads, dim) of a cache, checked."""
     for t, dtype, name in ((k_codes, torch.uint8, "k_codes"), (v_codes, torch.uint8, "v_codes"), (k_scale, torch.float32, "k_scale"),
@@ -974,6 +983,7 @@ def _kv8_cache(k_codes, v_codes, k_scale, v_scale):
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         if tuple(t.shape) != (n, heads):
             raise ValueError(f"{name} must be {(n, heads)}, got {tuple(t.shape)}")
+        _kv8_no_derivative(t, name)
     if n == 0 or heads == 0:
         raise ValueError("the cache needs at least one block and one kv head")
     return n, heads, dim
@@ -989,8 +999,7 @@ def _kv8_rows(t, name, heads, dim, like, dtype=None):
         raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
     if t.device != like.device:
         raise ValueError(f"{name} must be on the device of the cache")
-    if torch.is_grad_enabled() and t.requires_grad:
-        raise RuntimeError(f"the operators of the 8-bit cache have no backward, and {name} requires a gradient")
+    _kv8_no_derivative(t, name)
     return t
 
 
@@ -1074,6 +1083,7 @@ def kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
                 raise ValueError(f"{name} must be on the device of the cache")
             if t.data_ptr() % 16:
                 raise ValueError(f"{name} must be 16-byte aligned")
+            _kv8_no_derivative(t, name)
         if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[0] == 0 or cos.shape[1] % 8 or not 0 < 2 * cos.shape[1] <= dim:
             raise ValueError(f"cos and sin must be [positions, rotated dims / 2] with a multiple of 16 rotated dims up to {dim}, got {tuple(cos.shape)} and {tuple(sin.shape)}")
         rot = 2 * cos.shape[1]
