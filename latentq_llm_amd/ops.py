@@ -970,6 +970,8 @@ def _kv8_no_derivative(t, name):
 
 def _kv8_cache(k_codes, v_codes, k_scale, v_scale):
     """(blocks, kv heads, dim) of a cache, checked."""
+    if torch.jit.is_tracing():  # (it would keep this call's results as constants)
+        raise RuntimeError("the operators of the 8-bit cache cannot be recorded in a trace")
     for t, dtype, name in ((k_codes, torch.uint8, "k_codes"), (v_codes, torch.uint8, "v_codes"), (k_scale, torch.float32, "k_scale"),
                            (v_scale, torch.float32, "v_scale")):
         _chk(t, dtype, name)
