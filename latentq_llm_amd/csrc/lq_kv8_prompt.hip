@@ -22,13 +22,11 @@ constexpr float kLazy = 8.0f;
 // 541 -> 569 us).
 struct Values {
     unsigned lo, hi, off;
-    float scale;
     __device__ __forceinline__ explicit Values(float s) {
         const bool none = kv8_no_values(s);
         lo = none ? 0x04040404u : 0x04010400u;
         hi = none ? 0x04040404u : 0x04030402u;
         off = none ? 0xE464E464u : 0xE480E480u;  // -1124, -1152
-        scale = none ? kLeastScale : s;
     }
     __device__ __forceinline__ u32x2_t halves(unsigned w) const {
         const f16x2_t o = __builtin_bit_cast(f16x2_t, off);
@@ -234,10 +232,9 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
     const int steps = (t_hi - t_lo + kSides - 1) / kSides;  // of every side; in the last one a side may be without a tile
     if (steps > 0) {
         request_tile(min(t_lo + side, t_hi - 1));
-        const Values values(vs_next);
-        store_all(0, values);
+        store_all(0, Values(vs_next));
         ks = ks_next;
-        vs = values.scale;
+        vs = vs_next;
         request_tile(min(t_lo + side + kSides, t_hi - 1));
     }
     __syncthreads();
@@ -246,8 +243,7 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
         const int key0 = t * KV8_BLOCK;
         const bool mine = (kSides == 1 || t < t_hi) && key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before;
         // (the tile after the last one is the last one again, stored and not used)
-        const Values values(vs_next);
-        if (!mine) store_all(buffer ^ 1, values);
+        if (!mine) store_all(buffer ^ 1, Values(vs_next));
         f32x16_t c[2];
         if (mine) {
             // Two chains of products at a time (keys 0 .. 31 and 32 .. 63), operands read two steps ahead of them.
@@ -264,6 +260,7 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
 #pragma unroll
                 for (int j = 0; j < 16; ++j) c[x][j] = 0.0f;
             read_k(0, 0);
+            const Values values(vs_next);  // (under the keys' way: in front of it, slices of few rows were 3 % slower)
             constexpr int kPairs = kSteps / 2;
 #pragma unroll
             for (int i = 0; i < kSteps; i += 2) {
@@ -281,9 +278,9 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        const float ks_now = ks, vs_now = vs;
+        const float ks_now = ks, vs_now = kv8_no_values(vs) ? kLeastScale : vs;
         ks = ks_next;
-        vs = values.scale;
+        vs = vs_next;
         if (n + 1 < steps) request_tile(min(t + 2 * kSides, t_hi - 1));
         if (mine) {
             // values of the first 16 keys: under the softmax
