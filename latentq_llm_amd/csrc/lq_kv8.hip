@@ -415,7 +415,7 @@ struct Plan {
 // registers (45 rows of 128 dimensions 14.4 / 6.3, 33.2 / 14.4, 68.1 / 64.1, 62.5 / 60.2).
 bool takes_few(int64_t rows, int64_t tiles, int dim) { return rows <= 16 || (tiles >= 24 && rows <= (dim <= 96 ? 64 : dim == 128 ? 32 : 16)); }
 
-Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t width, int64_t workspace, int cus) {
+Plan plan_within(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t width, int64_t workspace, int cus) {
     Plan p{};
     const int64_t rows = max_tokens * (heads / kv_heads), units = batch * kv_heads;
     int64_t keys = max_len;
@@ -477,6 +477,20 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
         p.slot_rows = tokens * heads;
     }
     return p;
+}
+
+int64_t plan_bytes(const Plan &p, int dim) { return p.slots * p.slot_rows * (dim + 1) * 4; }
+
+// The plan within a workspace, and within the bytes that it takes of it: a captured call is given no more, and is to be cut as any other is.
+// (A number of slices whose last ones would be empty counts for fewer, which may not win among themselves. Each turn takes fewer bytes
+// than the one before, so this ends: the second one as a rule.)
+Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t window, int64_t width, int64_t workspace, int cus) {
+    for (;;) {
+        const Plan p = plan_within(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, width, workspace, cus);
+        const int64_t bytes = plan_bytes(p, dim);
+        if (p.few || bytes == 0 || bytes == workspace) return p;
+        workspace = bytes;
+    }
 }
 
 }  // namespace
@@ -569,7 +583,7 @@ extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_
                        : Plan{true, 0, 1, 0, 0, 0, 0, 0, 0};
     *kernel = p.few ? 0 : 1;
     *parts = p.few ? p.workgroups : p.slices;
-    *needed = p.slots * p.slot_rows * (dim + 1) * 4;
+    *needed = plan_bytes(p, dim);
     return LQ_OK;
 }
 
