@@ -572,7 +572,8 @@ int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_strid
 
 /* What lq_kv8_attention does with a call of these sizes (launches nothing; compute_units <= 0: the current device's): *kernel 0 = few
  * rows, 1 = prompt; *parts = few rows: workgroups that share the keys (0: one for each sequence and kv head, nothing to join), prompt: slices of
- * the keys (1: nothing to join); *needed = the bytes of workspace that they take, no more than workspace_bytes. */
+ * the keys (1: nothing to join); *needed = the bytes of workspace that they take, no more than workspace_bytes. The call is taken to be causal:
+ * one with causal = 0 and a window is planned as one without a window, on min(max_len, window + max_tokens + LQ_KV_BLOCK) keys. */
 int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
                           int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *parts, int64_t *needed);
 

@@ -757,7 +757,9 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (!ws) {
         int kernel, parts;
         int64_t needed;
-        if (const int rc = lq_kv8_attention_plan(s.batch, tokens, s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, window, kWorkspaceBytes, 0, &kernel, &parts, &needed))
+        const bool ahead = window && !causal;
+        if (const int rc = lq_kv8_attention_plan(s.batch, tokens, s.most, ahead ? std::min(max_len, window + s.most + LQ_KV_BLOCK) : max_len, (int)heads, (int)c.heads,
+                                                 (int)c.dim, ahead ? 0 : window, kWorkspaceBytes, 0, &kernel, &parts, &needed))
             return fail("lq_kv8_attention_plan", rc);
         if (needed) return PyLong_FromLongLong(needed);
     }

@@ -1141,6 +1141,7 @@ def kv8_attention_plan(batch: int, tokens: int, max_tokens: int, max_len: int, h
                        workspace_bytes: int = WORKSPACE_MAX_BYTES, compute_units: int = 0):
     """(kernel name, parts, bytes of workspace these take) kv8_attention would use for a call of these sizes (lq_kv8_attention_plan):
     parts are workgroups that share the keys ("few"; 0: one for each sequence and kv head) or slices of the keys ("prompt"; 1: whole).
+    For a causal call; one with causal=False and a window is planned as one without, on min(max_len, window + max_tokens + KV_BLOCK) keys.
     Launches nothing, as a16w4_plan."""
     import ctypes
     kernel, parts, needed = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
@@ -1186,7 +1187,8 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
     if tokens and batch:
         q = _kv8_layout(q)
         with torch.cuda.device(k_codes.device):
-            needed = kv8_attention_plan(batch, tokens, most, max_len, heads, kv_heads, dim, window)[2]
+            ahead = window and not causal
+            needed = kv8_attention_plan(batch, tokens, most, min(max_len, window + most + KV_BLOCK) if ahead else max_len, heads, kv_heads, dim, 0 if ahead else window)[2]
             keep, ws, ws_bytes = _workspace(q, 1, -(-needed // 32)) if needed else (None, None, 0)
             _C.call("lq_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
                     v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(), None if cu_tokens is None else cu_tokens.data_ptr(),

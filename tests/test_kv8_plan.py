@@ -27,3 +27,25 @@ def test_the_workspace_that_a_plan_names_gives_the_same_plan(hip_lib):
         assert again == first, case
         cut += first[0] == "prompt" and first[1] > 1
     assert cut > 1000
+
+
+def test_no_slice_beyond_what_a_window_shows(hip_lib):
+    """Slices of the keys are of what the rows of a workgroup see: of 128 or 256 rows, their tokens' windows."""
+    def plan(tokens, length, heads, kv_heads, dim, window, **more):
+        return ops.kv8_attention_plan(1, tokens, tokens, length, heads, kv_heads, dim, window, compute_units=256, **more)
+
+    for case in ((2048, 2048, 12, 12, 96, 128), (2048, 2048, 8, 1, 128, 64), (4096, 4096, 8, 1, 128, 16), (4096, 4096, 8, 1, 128, 128), (1024, 8192, 12, 12, 96, 256)):
+        assert plan(*case) == ("prompt", 1, 0), case
+    assert plan(512, 16384, 32, 8, 128, 0)[1] > 1 and plan(512, 16384, 32, 8, 128, 8192)[1] > 1
+    seen = 0
+    for case in shapes(2, 40000):
+        kernel, parts, _ = ops.kv8_attention_plan(**case)
+        if kernel != "prompt" or not case["window"]:
+            continue
+        group = case["heads"] // case["kv_heads"]
+        tiles = (case["window"] + min(case["max_tokens"], 256 // group + 1) - 1 + 62) // 64 + 1
+        assert parts <= tiles, case
+        seen += parts > 1
+        wide = dict(case, window=case["max_len"] + 1)  # a window that hides nothing
+        assert ops.kv8_attention_plan(**wide) == ops.kv8_attention_plan(**dict(case, window=0)), case
+    assert seen > 300
