@@ -143,6 +143,15 @@ class CachedAttention(nn.Module):
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        """The rotation tables go where the module goes and stay float32, which the kernels take, when it is cast."""
+        tables = {"cos": self.cos, "sin": self.sin}
+        super()._apply(fn, recurse)
+        for name, t in tables.items():
+            if t is not None and not t.is_meta:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
     @torch.no_grad()
     def forward(self, x, cache: KVCache8, step: Step):
         rows = x.shape[0]
