@@ -564,7 +564,7 @@ extern "C" int lq_kv8_read(const void *k_codes, const void *v_codes, const float
     if (n == 0) return LQ_OK;
     LQ_REQUIRE(k_codes && v_codes && k_scale && v_scale && blocks && k_out && v_out, "kv8_read: null pointer");
     LQ_REQUIRE(num_blocks > 0 && num_blocks <= INT32_MAX, "kv8_read: a pool of blocks is needed");
-    LQ_REQUIRE(n * kv_heads <= INT32_MAX, "kv8_read: too many blocks");
+    LQ_REQUIRE(n <= INT32_MAX / kv_heads, "kv8_read: too many blocks");
     for (const void *p : {k_codes, v_codes, (const void *)k_out, (const void *)v_out})
         LQ_REQUIRE(lq_aligned(p, 16), "kv8_read: codes and outputs must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
@@ -581,7 +581,7 @@ int attention_sizes(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t m
     LQ_REQUIRE(good_dim(dim), "kv8_attention: head dimension must be 64, 96, 128 or 256, got %d", dim);
     LQ_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "kv8_attention: heads must be a multiple of kv heads, got %d and %d", heads, kv_heads);
     LQ_REQUIRE(window >= 0, "kv8_attention: the window must not be negative");
-    LQ_REQUIRE(tokens * heads <= INT32_MAX && batch * kv_heads <= INT32_MAX, "kv8_attention: too many tokens or sequences");
+    LQ_REQUIRE(tokens <= INT32_MAX / heads && batch <= INT32_MAX / kv_heads, "kv8_attention: too many tokens or sequences");
     return LQ_OK;
 }
 }  // namespace
@@ -591,6 +591,8 @@ extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_
     if (const int rc = attention_sizes(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window)) return rc;
     LQ_REQUIRE(kernel && parts && needed, "kv8_attention_plan: null pointer");
     if (max_tokens > tokens) max_tokens = tokens;
+    if (max_len > INT32_MAX) max_len = INT32_MAX;
+    if (window > INT32_MAX) window = 0;
     const Plan p = batch && tokens && max_tokens
                        ? plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window, (max_len + KV8_BLOCK - 1) / KV8_BLOCK, workspace_bytes, compute_units > 0 ? compute_units : lq_device_cu_count())
                        : Plan{true, 0, 1, 0, 0, 0, 0, 0, 0};
@@ -623,6 +625,7 @@ extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q
     LQ_REQUIRE(workspace_bytes >= 0, "kv8_attention: the workspace's size must not be negative");
     if (max_tokens > tokens) max_tokens = tokens;
     if (max_len > table_width * KV8_BLOCK) max_len = table_width * KV8_BLOCK;
+    if (window > INT32_MAX) window = 0;  // positions are less
     // (rows that also see what follows them see all the call's keys from their windows' beginnings on)
     const bool ahead = !causal && window;
     const Plan p = plan_of(batch, tokens, max_tokens, ahead ? std::min(max_len, window + max_tokens + KV8_BLOCK) : max_len, heads, kv_heads, dim, ahead ? 0 : window,

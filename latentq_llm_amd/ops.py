@@ -1173,7 +1173,7 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 3.4e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    window = int(window or 0)
+    window = min(int(window or 0), 1 << 31)  # (positions are less)
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
     max_len = width * KV_BLOCK if max_len is None else min(int(max_len), width * KV_BLOCK)

@@ -60,3 +60,17 @@ def test_sizes_of_a_layer_that_are_not_integers(hip_lib):
     with pytest.raises(Exception) as e:
         ops.a16w4_forward(x, codes, s, s, (128.0, 256))
     assert not isinstance(e.value, SystemError)
+
+
+def test_windows_of_any_size(hip_lib, call):
+    """Beyond every position: as none, also for sequences with fewer tokens than new ones."""
+    from latentq_llm_amd import ops
+    want = call()
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 5, 2 ** 70):
+        assert torch.equal(call(window=window), want), window
+    q = call.q.repeat(20, 1, 1)
+    short = dict(cu_tokens=i32([0, 100, 120]), max_tokens=100)
+    lens = i32([40, 20])
+    want = ops.kv8_attention(q, *call.tensors, call.table, lens, **short)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1):
+        assert torch.equal(ops.kv8_attention(q, *call.tensors, call.table, lens, window=window, **short), want), window
