@@ -17,27 +17,22 @@ namespace {
 
 constexpr float kLazy = 8.0f;
 
-// A tile's values on their way from codes to halves: the bytes and the offset of kv8_halves, which are scalar registers, and others that make
-// every half 0x6464 less 1124 where the tile has no values (zeros put in the codes' place under a branch: 8192 tokens of 32 heads
-// 541 -> 569 us).
-struct Values {
-    unsigned lo, hi, off;
-    __device__ __forceinline__ explicit Values(float s) {
-        const bool none = kv8_no_values(s);
-        lo = none ? 0x04040404u : 0x04010400u;
-        hi = none ? 0x04040404u : 0x04030402u;
-        off = none ? 0xE464E464u : 0xE480E480u;  // -1124, -1152
+// How a tile's codes become halves (kv8_halves): the bytes that are put beside 0x64, and what is taken off. Those are scalar registers, and so
+// they can be others where the tile has no values, which make every half 0x6464 less 1124 (zeros put in the codes' place under a
+// branch: 8192 tokens of 32 heads 541 -> 569 us). An instruction takes one scalar register, so 0x64 is a vector's.
+struct Halves {
+    unsigned lo = 0x04010400u, hi = 0x04030402u, off = 0xE480E480u;  // -1152
+    Halves() = default;
+    __device__ __forceinline__ explicit Halves(float v_scale) {
+        const bool none = kv8_no_values(v_scale);
+        lo = none ? 0x04040404u : lo;
+        hi = none ? 0x04040404u : hi;
+        off = none ? 0xE464E464u : off;  // -1124
     }
-    __device__ __forceinline__ u32x2_t halves(unsigned w) const {
-        const f16x2_t o = __builtin_bit_cast(f16x2_t, off);
-        const f16x2_t x = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, w, lo)) + o;
-        const f16x2_t y = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, w, hi)) + o;
-        return u32x2_t{__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y)};
+    __device__ __forceinline__ unsigned two(unsigned w, unsigned bytes, unsigned x64) const {
+        return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(x64, w, bytes)) + __builtin_bit_cast(f16x2_t, off));
     }
-    __device__ __forceinline__ u32x4_t operand(unsigned a, unsigned b) const {
-        const u32x2_t x = halves(a), y = halves(b);
-        return u32x4_t{x[0], x[1], y[0], y[1]};
-    }
+    __device__ __forceinline__ u32x4_t operand(unsigned a, unsigned b, unsigned x64) const { return u32x4_t{two(a, lo, x64), two(a, hi, x64), two(b, lo, x64), two(b, hi, x64)}; }
 };
 
 // Sum over the lanes (in rows of 16 by lane shifts, then the four rows)
@@ -199,13 +194,16 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
     };
     // The way into shared memory, in pieces that go between the products of the scores
     constexpr int kParts = kNk + 2 * kNv;
-    const auto store = [&](int buffer, int part, const Values &values) {
+    unsigned x64 = 0x64646464u;
+    asm("" : "+v"(x64));
+    const Halves keys;
+    const auto store = [&](int buffer, int part, const Halves &values) {
         if (part < kNk) {
             const int u = tid + part * kThreads, t = u / (D / 16), piece = u % (D / 16) * 2;
             if (kKeys % kThreads == 0 || u < kKeys) {
                 u32x4_t *row_at = lds[side][buffer] + t * kPieces;
-                row_at[placed(piece, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[part][0], kr[part][1]));
-                row_at[placed(piece + 1, t)] = __builtin_bit_cast(u32x4_t, kv8_operand(kr[part][2], kr[part][3]));
+                row_at[placed(piece, t)] = keys.operand(kr[part][0], kr[part][1], x64);
+                row_at[placed(piece + 1, t)] = keys.operand(kr[part][2], kr[part][3], x64);
             }
         } else {
             const int i = (part - kNk) >> 1, u = tid + i * kThreads, pair = u / (D / 4), d = u % (D / 4) * 4;
@@ -213,11 +211,11 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
                 u32x4_t *v_at = lds[side][buffer] + kHalf + pair * D;
 #pragma unroll
                 for (int j = 2 * ((part - kNk) & 1); j < 2 * ((part - kNk) & 1) + 2; ++j)
-                    v_at[dim_at(d + j)] = values.operand(vr[i][0][j], vr[i][1][j]);
+                    v_at[dim_at(d + j)] = values.operand(vr[i][0][j], vr[i][1][j], x64);
             }
         }
     };
-    const auto store_all = [&](int buffer, const Values &values) {
+    const auto store_all = [&](int buffer, const Halves &values) {
 #pragma unroll
         for (int part = 0; part < kParts; ++part) store(buffer, part, values);
     };
@@ -232,7 +230,7 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
     const int steps = (t_hi - t_lo + kSides - 1) / kSides;  // of every side; in the last one a side may be without a tile
     if (steps > 0) {
         request_tile(min(t_lo + side, t_hi - 1));
-        store_all(0, Values(vs_next));
+        store_all(0, Halves(vs_next));
         ks = ks_next;
         vs = vs_next;
         request_tile(min(t_lo + side + kSides, t_hi - 1));
@@ -243,7 +241,7 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
         const int key0 = t * KV8_BLOCK;
         const bool mine = (kSides == 1 || t < t_hi) && key0 <= wave_last && key0 + KV8_BLOCK - 1 > wave_before;
         // (the tile after the last one is the last one again, stored and not used)
-        if (!mine) store_all(buffer ^ 1, Values(vs_next));
+        if (!mine) store_all(buffer ^ 1, Halves(vs_next));
         f32x16_t c[2];
         if (mine) {
             // Two chains of products at a time (keys 0 .. 31 and 32 .. 63), operands read two steps ahead of them.
@@ -260,7 +258,7 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
 #pragma unroll
                 for (int j = 0; j < 16; ++j) c[x][j] = 0.0f;
             read_k(0, 0);
-            const Values values(vs_next);  // (under the keys' way: in front of it, slices of few rows were 3 % slower)
+            const Halves values(vs_next);  // (under the keys' way)
             constexpr int kPairs = kSteps / 2;
 #pragma unroll
             for (int i = 0; i < kSteps; i += 2) {
