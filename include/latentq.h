@@ -556,9 +556,9 @@ int lq_kv8_read(const void *k_codes, const void *v_codes, const float *k_scale, 
  * the sequence's tokens in the cache: those at positions <= the row's own (causal = 0: all), and with window > 0
  * none at positions <= the row's own less `window`. A row that sees nothing gives zeros. lse (null, or float
  * [tokens][heads]): the natural logarithm of the softmax's denominator, -inf for such a row. scale > 0.
- * q becomes f16 by a power of two for each row (exact but for elements under 2^-37 of the row's largest), codes are exact, scores,
- * softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits) relative to the largest contribution so far
- * (weight times v_scale; keys under 2^-126 of it count for nothing). A block whose v_scale is under 2^-97, as 0, has values of zero: its keys
+ * q becomes f16 by a power of two for each row (elements from 2^-29, of f16 2^-26, of the row's largest on exactly, smaller ones
+ * within 2^-37 of it), codes are exact, scores, softmax and sums are fp32, the weights of the values are rounded to f16 (11 bits)
+ * relative to the largest contribution so far (weight times v_scale; keys under 2^-126 of it count for nothing). A block whose v_scale is under 2^-97, as 0, has values of zero: its keys
  * have their weight and add nothing.
  * workspace (16-byte aligned, or null): with it, long keys are shared among more workgroups, whose partial results a
  * second launch joins in order; lq_kv8_attention_plan says how many and the bytes they take. Calls sharing a workspace are

@@ -101,8 +101,9 @@ __device__ __forceinline__ float kv8_max16(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// A row of queries becomes f16 with its largest element in [2^12, 2^13), by a power of two: exact for 16-bit inputs but for
-// elements under 2^-37 of the largest. The power goes back into the row's factor of the scores.
+// A row of queries becomes f16 with its largest element in [2^12, 2^13), by a power of two: bf16 elements are exact down to 2^-29 of the
+// largest one's power of two, f16 elements down to 2^-26, and smaller ones within 2^-37 of it. The power goes back into the row's
+// factor of the scores.
 __device__ __forceinline__ void kv8_row_power(float most, float &to, float &back) {
     const int e = max((int)((__float_as_uint(most) >> 23) & 0xFF) - 127, -100);
     to = __uint_as_float((unsigned)(127 + 12 - e) << 23);

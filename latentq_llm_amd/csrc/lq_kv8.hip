@@ -6,7 +6,8 @@
 //
 // One workgroup owns a (block, head) of the keys or of the values, so nothing is shared and nothing depends on an order: the new
 // tokens' values stay in registers between the maximum and the rounding, and a block's old codes are touched only when its scale
-// grows. The rotation of the queries needs no maximum and is spread over workgroups of the same launch.
+// grows. (Tokens of a standard normal that come one by one have an rms error of 0.38 steps of the last scale, at once 0.29.) The rotation
+// of the queries needs no maximum and is spread over workgroups of the same launch.
 //
 // Bound: memory. Appending 8192 tokens of 32 + 8 heads of 128 and turning their queries moves 185 MB in 39 us, 4.7 TB/s, where a copy
 // of 1 GiB reaches 5.0. One token of 32 heads, 4.8 us, is the launch and loads that wait for each other: length, table, scale.
@@ -427,9 +428,11 @@ Plan plan_within(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_
         // One workgroup for a (sequence, kv head) and one launch, or the tiles of all of them in equal shares and a launch that
         // joins (2 to 3 us): a unit up to 16 KiB of keys and values for each of its tiles goes through a compute unit at some 40 GB/s, so
         // long keys are shared where units leave compute units idle, and, lengths in a batch being what they are, where
-        // that costs little for equal ones. us by units / by shares, 128 dimensions: 32 units of 16 tiles 10.3 / 9.4, 32 tiles 16.9 / 10.6; 128 of 32
-        // 18.7 / 18.1, of 64 33.7 / 27.6; 256 of 64 42.0 / 46.8 (lengths down to a quarter 35.9 / 35.2), of 128 79.9 / 85.5 (67.6 / 59.9); 384 of 64
-        // 72.0 / 68.5 (60.2 / 49.4); 512 of 64 80.6 / 83.7 (64.4 / 61.7). 64 dimensions are level at twice the tiles.
+        // that costs little for equal ones. us by units / by shares, 128 dimensions: 32 units of 16 tiles 8.8 to 10.3 (as
+        // what runs before them is short or long) / 9.2 to 9.4, of 20 10.4 to 12.0 / 9.3 to 9.7, of 32 16.9 / 10.6; 64 of 20 12.5 / 12.7; 128 of 20 13.2 / 14.3,
+        // of 32 18.7 / 18.1, of 64 33.7 / 27.6; 256 of 64 42.0 / 46.8 (lengths down to a quarter 35.9 / 35.2), of 128 79.9 / 85.5 (67.6 / 59.9); 384 of 64
+        // 72.0 / 68.5 (60.2 / 49.4); 512 of 64 80.6 / 83.7 (64.4 / 61.7). 64 dimensions are level at twice the tiles. The line at 24 is where 64
+        // units gain as well; up to 32 units would from 17 on.
         const int64_t rounds = (units + cus - 1) / cus, equal = tiles * dim / 128;  // tiles of 16 KiB
         const bool split = equal >= 24 && equal * rounds * cus >= 80 * units && batch <= 512 && units * width <= INT32_MAX;
         int64_t share = (int64_t)cus * kv8_few_workgroups(dim, (int)rows);

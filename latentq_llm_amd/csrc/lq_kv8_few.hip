@@ -13,7 +13,7 @@
 // shared evenly and the pieces of a unit go through the workspace and a second launch.
 //
 // Bound: memory. 64 sequences of 2048 to 8192 keys, 32 heads on 8, 111 us: 6.1 TB/s, where a plain read of 1 GiB reaches 7.1; one
-// sequence of 131072 keys 50 us, 5.4 TB/s (268 MB, the second launch among them). One token on 1019 keys of 32 heads, 8.7 us, is
+// sequence of 131072 keys 47.5 us, 5.7 TB/s (268 MB, the second launch among them). One token on 1019 keys of 32 heads, 9.2 us, is
 // latency: the sequence's length, the table, the block and its codes are four loads that wait for each other, four
 // tiles to a wave, and the launch.
 #include "lq_kv8.h"

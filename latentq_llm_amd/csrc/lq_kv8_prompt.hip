@@ -9,8 +9,9 @@
 //
 // Bound: the matrix units, at the clock that they leave (2.17 GHz under this kernel). 8192 causal tokens of 32 heads of 128
 // in 554 us, 993 TFLOP/s of the visible half, where a large f16 product of the tensor library reaches 1162; 512 tokens on 16384 keys, 32 heads on
-// 8, 148 us, 915. A wave alone on its tile waits for its own products and weights in turn, so short prompts are bound by the
-// way of one workgroup through its tiles, 1.45 us each (1024 tokens of 32 heads 24 us).
+// 8, 144 us, 944. 64 dimensions have twice the weights to a product (8192 tokens 341 us, vector units 73 % busy), 256 one wave on a SIMD,
+// beside which nothing runs (16 heads on 4, 644 us). A wave alone on its tile waits for its own products and weights in turn, so short prompts are bound by the
+// way of one workgroup through its tiles, 1.45 us each (1024 tokens of 32 heads 24.7 us).
 #include "lq_kv8.h"
 
 namespace {
@@ -168,7 +169,8 @@ __global__ __launch_bounds__(64 * kWaves * kSides, D <= 128 ? 2 : 1) void prompt
     // Shared memory gives 16 lanes their 16 bytes at a time from 64 banks, so the lanes of such a group go to 16 different places of
     // 256 bytes. Keys: 16 rows at one piece; pieces are exchanged by bits of the row. Values: 16 dimensions that follow each other
     // (read) or are 4 apart (written); a dimension moves on within its 16 by the number of the 16. (Without: 63 % of the cycles
-    // that shared memory was busy were conflicts, 650 us for 8192 tokens of 32 heads.)
+    // that shared memory was busy were conflicts, 650 us for 8192 tokens of 32 heads. The 17 % that are counted with eight waves and the 25 % with
+    // four, whose stores are the same and whose loads are half as many, fit loads without any and half of the stores' cycles.)
     const auto placed = [](int piece, int row) { return piece ^ (D == 64 ? row >> 1 & 7 : D == 96 ? row >> 2 & 3 : row & 15); };
     const auto dim_at = [](int d) { return d ^ (d >> 4 & 3); };
     // A thread's part of a tile: 16 bytes of keys (16 dimensions of a token) at a time; of values 4 dimensions of the 8 tokens that

@@ -132,7 +132,8 @@ def rotation_tables(positions: int, head_dim: int, base: float = 10000.0, device
 
 class CachedAttention(nn.Module):
     """o_proj(attention(rotate(q_proj(x)), cache)) of a decoder layer: keys and values of x's rows are appended to the cache on the way.
-    The projections are this package's quantised layers (or any with their shapes); cos and sin None: nothing is rotated."""
+    The projections are this package's quantised layers (or any with their shapes); cos and sin None: nothing is rotated.
+    For inference: nothing is recorded for a backward."""
 
     def __init__(self, q_proj, k_proj, v_proj, o_proj, heads: int, kv_heads: int, head_dim: int, cos=None, sin=None, window: int = 0):
         super().__init__()
