@@ -400,6 +400,9 @@ bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int dim) {
     return true;
 }
 
+// A launch has fewer than 2^32 threads in each direction
+bool launchable(int64_t workgroups, int threads) { return workgroups <= UINT32_MAX / threads; }
+
 bool good_dim(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 256; }
 
 // How a call is cut.
@@ -546,10 +549,11 @@ extern "C" int lq_kv8_append(const void *k, int64_t k_token_stride, int64_t k_he
              (int)positions, cos_table ? rot_dim : 0, (int)num_blocks, (int)table_width, (int)batch, (int)tokens, heads, kv_heads, 0, q ? (heads + kQHeads - 1) / kQHeads : 0};
     if (max_tokens > tokens) max_tokens = tokens;
     const int64_t per = (max_tokens + KV8_BLOCK - 2) / KV8_BLOCK + 1;
-    LQ_REQUIRE(per * batch <= INT32_MAX, "kv8_append: too many tokens or sequences");
+    const bool few = max_tokens <= kFew;
+    LQ_REQUIRE(launchable(per * batch, few ? 64 : 256), "kv8_append: too many workgroups: %lld sequences of up to %lld new tokens (max_tokens, the most of any, sizes the launch)",
+               (long long)batch, (long long)max_tokens);
     a.per_seq = (int)per;
     const dim3 grid((unsigned)(per * batch), (unsigned)(2 * kv_heads + a.q_groups));
-    const bool few = max_tokens <= kFew;
     hipStream_t s = (hipStream_t)stream;
     if (dim == 64) launch_append<64>(a, few, dtype == 1, grid, s);
     else if (dim == 96) launch_append<96>(a, few, dtype == 1, grid, s);
@@ -567,7 +571,7 @@ extern "C" int lq_kv8_read(const void *k_codes, const void *v_codes, const float
     if (n == 0) return LQ_OK;
     LQ_REQUIRE(k_codes && v_codes && k_scale && v_scale && blocks && k_out && v_out, "kv8_read: null pointer");
     LQ_REQUIRE(num_blocks > 0 && num_blocks <= INT32_MAX, "kv8_read: a pool of blocks is needed");
-    LQ_REQUIRE(n <= INT32_MAX / kv_heads, "kv8_read: too many blocks");
+    LQ_REQUIRE(n <= INT32_MAX / kv_heads && launchable(n * kv_heads, 256), "kv8_read: too many blocks");
     for (const void *p : {k_codes, v_codes, (const void *)k_out, (const void *)v_out})
         LQ_REQUIRE(lq_aligned(p, 16), "kv8_read: codes and outputs must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
@@ -648,6 +652,7 @@ extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q
     // is some 0.5 us in every workgroup, which few short ones do not get back (7 x 580 tokens, 32 heads: 27.9 / 28.5, 30 x 130, 32 on 8:
     // 19.1 / 20.6; 40 x 600, 12 heads: 58.8 / 44.8). With as many new tokens each (no cu_tokens) there is nothing to gain.
     a.ranked = cu_tokens && batch > 1 && batch <= 64 && (p.row_tiles >= 8 || batch * kv_heads * p.row_tiles >= 2048);
-    LQ_REQUIRE(p.few || (int64_t)p.slices * batch * kv_heads * p.row_tiles <= INT32_MAX, "kv8_attention: too many tokens or sequences");
+    LQ_REQUIRE(launchable(p.few ? batch * kv_heads : (int64_t)p.slices * batch * kv_heads * p.row_tiles, p.few ? 256 : 64 * p.waves * p.sides),
+               "kv8_attention: too many workgroups: %lld sequences of up to %lld new tokens (max_tokens, the most of any, sizes the launch)", (long long)batch, (long long)max_tokens);
     return p.few ? kv8_launch_few(a, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
 }

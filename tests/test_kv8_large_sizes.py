@@ -30,3 +30,16 @@ def test_lengths_and_windows_of_any_size_have_a_plan(hip_lib):
         assert plan(top, tokens=tokens) == plan((1 << 31) - 1, tokens=tokens)
         for window in ((1 << 31) - 1, 1 << 31, 1 << 40, top - 64, top):
             assert plan(16384, window, tokens) == plan(16384, 0, tokens), window
+
+
+def test_launches_that_are_too_large_are_refused_with_the_reason(hip_lib, p):  # noqa: F811
+    """Many sequences whose number of new tokens is not given: every one may have them all. (A null stream and host pointers: nothing may be
+    launched here.)"""
+    from tests.test_kv8_abi import append_args
+    ptr = p[0]
+    assert hip_lib.lq_kv8_attention(*attention_args(ptr, cu=ptr, batch=512, tokens=1 << 17, most=1 << 17, len=512, heads=32, kv=8, width=8, ot=32 * 64)) == -1
+    assert b"max_tokens" in hip_lib.lq_last_error() and b"512 sequences" in hip_lib.lq_last_error(), hip_lib.lq_last_error()
+    assert hip_lib.lq_kv8_append(*append_args(ptr, cu=ptr, batch=4096, tokens=1 << 20, most=1 << 20)) == -1
+    assert b"max_tokens" in hip_lib.lq_last_error(), hip_lib.lq_last_error()
+    import ctypes as C
+    assert hip_lib.lq_kv8_read(ptr, ptr, ptr, ptr, 4, ptr, 1 << 22, 8, 64, 0, ptr, C.c_void_p(ptr.value), None) == -1 and b"too many blocks" in hip_lib.lq_last_error()
