@@ -40,7 +40,7 @@ class KVCache8:
 
     def append(self, k, v, step: "Step", q=None, cos=None, sin=None):
         """ops.kv8_append of a step's new tokens; returns the rotated q, or None. Raises, and appends nothing, where a sequence has outgrown the
-        rotation tables or its blocks are not of this cache."""
+        rotation tables or its blocks are not of this cache (Sequences has counted the tokens by then: such a sequence is to be dropped)."""
         self._holds(step)
         if cos is not None and step.longest > cos.shape[0]:  # (the kernel would turn what lies beyond by the last row)
             raise ValueError(f"the rotation tables have {cos.shape[0]} positions, a sequence {step.longest} tokens")
