@@ -577,6 +577,51 @@ int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_strid
 int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
                           int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *parts, int64_t *needed);
 
+/* Bookkeeping of such a cache on the device: the sequences' lengths become max(seq_lens[i] + change[i], 0), the blocks that they no
+ * longer need go onto the list of free blocks, and those they need are taken from it (of those that are given back in the call,
+ * too). A sequence of n tokens has max(ceil(n / 64), shared) blocks: the first `shared` blocks of every sequence, which a batch may have in
+ * common, are never taken or given back, and entries of block_table behind a sequence's blocks stay as they are.
+ * free_blocks int32 [capacity], of which the first *free_count are free; the last of these is the first to be taken, in the order of the sequences and of
+ * their blocks; blocks given back lie so that the first of them is taken first. So what is taken and given back again leaves the list as it was.
+ * cu_tokens int32 [batch + 1]: sums of the new tokens, max(change[i], 0) and no more than fit (written). rows >= 0: position and slot
+ * (block * 64 + place in it) of each new token, int64 [rows], in the order of the sequences; 0 and -1 in rows behind them.
+ * rows < 0: neither is written. *status: 0, or what cannot be done, and then lengths, table and list stay as they are and cu_tokens is zeros: the
+ * number of blocks that are missing, LQ_KV_NARROW: a sequence has or would have more than table_width blocks, LQ_KV_ROWS: more new
+ * tokens than rows (or than 2^31 - 1), LQ_KV_LIST: the list would hold more than capacity, or *free_count is none of its sizes.
+ * Up to 4096 sequences; calls on the same list or tables are ordered on one stream. */
+#define LQ_KV_NARROW (-1)
+#define LQ_KV_ROWS (-2)
+#define LQ_KV_LIST (-3)
+int lq_kv8_resize(int32_t *block_table, int64_t table_width, int32_t *seq_lens, int32_t *free_blocks, int64_t capacity, int32_t *free_count,
+                  const int32_t *change, int64_t batch, int64_t shared, int64_t rows, int32_t *cu_tokens, int64_t *positions, int64_t *slots,
+                  int32_t *status, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Drafted tokens checked against the target's logits (an addition; the reference generates with its model library). Row r of
+ * logits [rows][vocab] is what the target gave for tokens[r]; the rows of a sequence follow each other (cu_tokens as above; null:
+ * rows / batch each), the first of its tokens is known, the others are drafts: tokens[r + 1] was drafted behind row r, drawn from
+ * softmax(draft_logits[r] / temperature), or (draft_logits null) chosen in any way that does not depend on the target's logits.
+ *   p = softmax(logits[r] / temperature), q = softmax(draft_logits[r] / temperature), or 1 at the draft and 0 elsewhere
+ * In order, draft x of row r is taken if accept_draws[r] * q(x) < p(x). Behind the taken ones follows one token more: drawn from what is left of the
+ * row whose draft was refused, max(p - q, 0) (where that is zero everywhere, from p), or from p of the last row: the first j at which the sum of the
+ * first j + 1 values passes sample_draws[i] times the sum of all, and no j whose value is 0. Numbers are uniform in [0, 1). A sequence of one row has no
+ * draft: its token is drawn. temperature 0: p is 1 at the largest logit (the first of equal ones) and 0 elsewhere, no numbers are used.
+ * A NaN is a masked logit (-inf), +inf counts as 2^128 (1 - 2^-24); drafts outside the vocabulary are refused; a row whose logits are all masked
+ * gives -1. Logits are of dtype 0 = bf16, 1 = f16, 2 = f32, rows at any distance (in elements), their entries beside each other and aligned to their
+ * size; exponentials and sums are 64 bits. accept_draws float [rows] (a sequence's last one is not used; may be null if max_tokens is 1), sample_draws
+ * float [batch].
+ * out int64 [batch][max_tokens]: the taken drafts, the token behind them, then -1 (a sequence without rows: all -1); accepted int32 [batch]: how many drafts
+ * were taken. Rows of a sequence beyond max_tokens are not looked at. Up to 65535 rows and sequences. workspace: 16-byte aligned, the
+ * bytes that lq_verify_drafts_plan says; calls sharing one are ordered on one stream. No result depends on an order.
+ * ------------------------------------------------------------------------- */
+int lq_verify_drafts(const void *logits, int64_t row_stride, const void *draft_logits, int64_t draft_row_stride, const int64_t *tokens,
+                     const int32_t *cu_tokens, int64_t batch, int64_t rows, int64_t vocab, int64_t max_tokens, int dtype, double temperature,
+                     const float *accept_draws, const float *sample_draws, int64_t *out, int32_t *accepted, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+/* Into how many slices the above cuts a row, and the bytes of workspace that it needs (launches nothing; compute_units <= 0: the current device's). */
+int lq_verify_drafts_plan(int64_t batch, int64_t rows, int64_t vocab, int greedy, int with_draft_logits, int compute_units, int *slices,
+                          int64_t *needed);
+
 /* ---------------------------------------------------------------------------
  * Layout converters (device side).
  * GPTQ layout (reference PTQ/quant/quant_linear.py:343-389): qweight is

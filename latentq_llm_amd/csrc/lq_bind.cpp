@@ -789,6 +789,96 @@ PyObject *kv8_read(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     return Py_BuildValue("NN", wrap(std::move(k)), wrap(std::move(v)));
 }
 
+// block_table, seq_lens, free_blocks, free_count, change, rows (None: no positions and slots), shared -> (cu_tokens, positions, slots, status)
+PyObject *kv8_resize(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    LQ_ARGS(7)
+    if (watched()) return none();
+    const at::Tensor *t[5];
+    for (int i = 0; i < 5; ++i) {
+        t[i] = plain(a[i], at::kInt);
+        if (!t[i] || !same_device(t[i], t[0])) return none();
+    }
+    if (t[0]->dim() != 2 || t[0]->numel() == 0 || t[1]->dim() != 1 || t[2]->dim() != 1 || t[3]->sizes() != at::IntArrayRef({1}) || t[4]->sizes() != t[1]->sizes() ||
+        t[1]->size(0) != t[0]->size(0))
+        return none();
+    const int64_t batch = t[0]->size(0), rows = a[5] == Py_None ? -1 : integer(a[5]), shared = integer(a[6]);
+    if (PyErr_Occurred() || (a[5] != Py_None && rows < 0) || rows > INT32_MAX || shared < 0 || shared > t[0]->size(1)) return none();
+    On on(*t[0]);
+    at::Tensor cu = make({batch + 1}, at::kInt, *t[0]), status = make({1}, at::kInt, *t[0]), positions, slots;
+    if (rows >= 0) {
+        positions = make({rows}, at::kLong, *t[0]);
+        slots = make({rows}, at::kLong, *t[0]);
+    }
+    LQ_CALL(lq_kv8_resize, (int32_t *)t[0]->data_ptr(), t[0]->size(1), (int32_t *)t[1]->data_ptr(), (int32_t *)t[2]->data_ptr(), t[2]->size(0), (int32_t *)t[3]->data_ptr(),
+            (const int32_t *)t[4]->data_ptr(), batch, shared, rows, (int32_t *)cu.data_ptr(), rows >= 0 ? (int64_t *)positions.data_ptr() : nullptr,
+            rows >= 0 ? (int64_t *)slots.data_ptr() : nullptr, (int32_t *)status.data_ptr(), on.stream);
+    if (rows < 0) return Py_BuildValue("NOON", wrap(std::move(cu)), Py_None, Py_None, wrap(std::move(status)));
+    return Py_BuildValue("NNNN", wrap(std::move(cu)), wrap(std::move(positions)), wrap(std::move(slots)), wrap(std::move(status)));
+}
+
+// Rows [rows, vocab] of logits with their entries beside each other
+struct Logits {
+    const at::Tensor *t = nullptr;
+    int dtype = 0;
+    bool load(PyObject *o) {
+        if (!THPVariable_CheckExact(o)) return false;
+        const at::Tensor &x = THPVariable_Unpack(o);
+        if (!x.is_cuda() || x.dim() != 2 || x.numel() == 0 || !x.has_storage() || x.key_set().has_any(kWrappedKeys) || x.stride(1) != 1) return false;
+        dtype = x.scalar_type() == at::kBFloat16 ? 0 : x.scalar_type() == at::kHalf ? 1 : x.scalar_type() == at::kFloat ? 2 : -1;
+        t = &x;
+        return dtype >= 0;
+    }
+};
+
+// logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws (None or tensors), temperature, batch, max_tokens (None), workspace -> (out, accepted);
+// without a workspace: the bytes that it needs, and nothing is done
+PyObject *verify_drafts(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    LQ_ARGS(10)
+    if (watched()) return none();
+    Logits l, d;
+    const at::Tensor *tokens = plain(a[1], at::kLong), *cu = nullptr, *accept = nullptr, *sample = nullptr;
+    if (!l.load(a[0]) || !tokens || !same_device(tokens, l.t)) return none();
+    const int64_t rows = l.t->size(0), vocab = l.t->size(1);
+    if (tokens->sizes() != at::IntArrayRef({rows}) || rows > 65535) return none();
+    int64_t batch = rows;
+    if (a[2] != Py_None) {
+        cu = plain(a[2], at::kInt);
+        if (!cu || cu->dim() != 1 || cu->size(0) < 2 || !same_device(cu, l.t) || a[7] != Py_None) return none();
+        batch = cu->size(0) - 1;
+    } else if (a[7] != Py_None) {
+        batch = integer(a[7]);
+        if (batch <= 0 || rows % batch) return none();
+    }
+    int64_t most = cu ? rows : rows / batch;
+    if (a[8] != Py_None) {
+        const int64_t given = integer(a[8]);
+        if (given <= 0 || (!cu && given < most)) return none();
+        most = std::min(most, given);
+    }
+    const double temperature = PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred() || !(temperature == 0.0 || (temperature >= 0x1p-60 && temperature <= 0x1p60))) return none();
+    const bool draws = temperature != 0.0;
+    if (a[3] != Py_None && (!d.load(a[3]) || d.dtype != l.dtype || d.t->sizes() != l.t->sizes() || !same_device(d.t, l.t))) return none();
+    if (a[4] != Py_None && (!(accept = plain(a[4], at::kFloat)) || accept->sizes() != at::IntArrayRef({rows}) || !same_device(accept, l.t))) return none();
+    if (a[5] != Py_None && (!(sample = plain(a[5], at::kFloat)) || sample->sizes() != at::IntArrayRef({batch}) || !same_device(sample, l.t))) return none();
+    if (draws && (!sample || (!accept && most > 1))) return none();
+    void *ws;
+    int64_t ws_bytes;
+    if (!workspace(a[9], l.t, &ws, &ws_bytes)) return none();
+    On on(*l.t);
+    if (!ws) {
+        int slices;
+        int64_t needed;
+        if (const int rc = lq_verify_drafts_plan(batch, rows, vocab, !draws, d.t != nullptr, 0, &slices, &needed)) return fail("lq_verify_drafts_plan", rc);
+        return PyLong_FromLongLong(needed);
+    }
+    at::Tensor out = make({batch, most}, at::kLong, *l.t), accepted = make({batch}, at::kInt, *l.t);
+    LQ_CALL(lq_verify_drafts, l.t->data_ptr(), l.t->stride(0), d.t ? d.t->data_ptr() : nullptr, d.t ? d.t->stride(0) : 0, (const int64_t *)tokens->data_ptr(),
+            cu ? (const int32_t *)cu->data_ptr() : nullptr, batch, rows, vocab, most, l.dtype, temperature, accept ? (const float *)accept->data_ptr() : nullptr,
+            sample ? (const float *)sample->data_ptr() : nullptr, (int64_t *)out.data_ptr(), (int32_t *)accepted.data_ptr(), ws, ws_bytes, on.stream);
+    return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(accepted)));
+}
+
 // device index -> the current stream's handle
 PyObject *current_stream(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     LQ_ARGS(1)
@@ -837,7 +927,7 @@ PyMethodDef methods[] = {
     LQ_METHOD(linear4), LQ_METHOD(linear4_eval), LQ_METHOD(dx4), LQ_METHOD(gate_up), LQ_METHOD(dx_silu), LQ_METHOD(dx_pair), LQ_METHOD(linear8), LQ_METHOD(infer8),
     LQ_METHOD(infer8_eval), LQ_METHOD(dx8), LQ_METHOD(quant8), LQ_METHOD(quant8_token), LQ_METHOD(dequant8), LQ_METHOD(weight_grad),
     LQ_METHOD(weight_grad_acc), LQ_METHOD(weight_grad_acc8), LQ_METHOD(gradq8), LQ_METHOD(adam8_param), LQ_METHOD(adam8_sr),
-    LQ_METHOD(adam8_queue), LQ_METHOD(adam8_run), LQ_METHOD(adam8_w4), LQ_METHOD(adam8_w8), LQ_METHOD(kv8_append), LQ_METHOD(kv8_attention), LQ_METHOD(kv8_read), LQ_METHOD(current_stream),
+    LQ_METHOD(adam8_queue), LQ_METHOD(adam8_run), LQ_METHOD(adam8_w4), LQ_METHOD(adam8_w8), LQ_METHOD(kv8_append), LQ_METHOD(kv8_attention), LQ_METHOD(kv8_read), LQ_METHOD(kv8_resize), LQ_METHOD(verify_drafts), LQ_METHOD(current_stream),
     LQ_METHOD(records_plainly), LQ_METHOD(set_error), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lqbind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -957,6 +957,7 @@ def latent_w8_requant(latent, qscales, residual_int, k1, b1, k2, b2, k3):
 # ---- paged 8-bit cache of keys and values (include/latentq.h, lq_kv8_*) ----------------------------------------------
 KV_BLOCK = 64
 KV_DIMS = (64, 96, 128, 256)
+KV_NARROW, KV_ROWS, KV_LIST = -1, -2, -3  # of kv8_resize's status
 _KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -1196,3 +1197,121 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
                     out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws, ws_bytes, _stream(q))
             del keep
     return (out, lse) if return_lse else out
+
+
+def kv8_resize(block_table, seq_lens, free_blocks, free_count, change, *, rows=None, shared=0):
+    """Change the lengths of the sequences of a paged 8-bit cache on the device (lq_kv8_resize): seq_lens[i] becomes max(seq_lens[i] + change[i], 0),
+    blocks that are no longer needed go back to free_blocks (int32, the first free_count[0] of them free) and those that are needed
+    come from it, into block_table; all int32, in place. The first `shared` blocks of every sequence are left alone. Returns (cu_tokens int32
+    [batch + 1], positions, slots, status int32 [1]): the first rows of the sequences' new tokens, and with `rows` given, which has to be as many
+    as there are new tokens or more, each one's position and slot block * 64 + place (int64 [rows]; 0 and -1 behind the last), else None.
+    status 0, or nothing has changed: the number of blocks that are missing, or KV_NARROW, KV_ROWS, KV_LIST."""
+    done = (_native or _fast()).kv8_resize(block_table, seq_lens, free_blocks, free_count, change, rows, shared)
+    if done is not None:
+        return done
+    if torch.jit.is_tracing():
+        raise RuntimeError("the operators of the 8-bit cache cannot be recorded in a trace")
+    for t, name in ((block_table, "block_table"), (seq_lens, "seq_lens"), (free_blocks, "free_blocks"), (free_count, "free_count"), (change, "change")):
+        _chk(t, torch.int32, name)
+        if t.device != block_table.device:
+            raise ValueError(f"{name} must be on the device of block_table")
+    if block_table.dim() != 2 or block_table.shape[1] == 0 or tuple(seq_lens.shape) != (block_table.shape[0],):
+        raise ValueError(f"block_table must be [batch, blocks of a sequence] and seq_lens [batch], got {tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
+    batch, width = block_table.shape
+    if tuple(change.shape) != (batch,):
+        raise ValueError(f"change must be {(batch,)}, got {tuple(change.shape)}")
+    if free_blocks.dim() != 1 or tuple(free_count.shape) != (1,):
+        raise ValueError(f"free_blocks must be one-dimensional and free_count [1], got {tuple(free_blocks.shape)} and {tuple(free_count.shape)}")
+    if rows is not None and not 0 <= int(rows) < 1 << 31:
+        raise ValueError(f"rows must be 0 to 2^31 - 1, got {rows}")
+    if not 0 <= int(shared) <= width:
+        raise ValueError(f"shared must be 0 to {width}, the columns of block_table, got {shared}")
+    dev = block_table.device
+    cu, status = torch.empty(batch + 1, dtype=torch.int32, device=dev), torch.empty(1, dtype=torch.int32, device=dev)
+    positions, slots = (None, None) if rows is None else (torch.empty(int(rows), dtype=torch.int64, device=dev) for _ in range(2))
+    with torch.cuda.device(dev):
+        _C.call("lq_kv8_resize", block_table.data_ptr(), width, seq_lens.data_ptr(), free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(), change.data_ptr(),
+                batch, int(shared), -1 if rows is None else int(rows), cu.data_ptr(), None if rows is None else positions.data_ptr(),
+                None if rows is None else slots.data_ptr(), status.data_ptr(), _stream(block_table))
+    return cu, positions, slots, status
+
+
+def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0, batch=None, max_tokens=None):
+    """Check drafted tokens against the target's logits and draw the token that follows the accepted ones (lq_verify_drafts; the rule:
+    include/latentq.h). logits [rows, vocab] (bfloat16, float16, float32) are what the target gave for tokens (int64 [rows]); cu_tokens
+    (int32 [batch + 1]) has each sequence's first row (without it: `batch` sequences of as many rows each, default one row each). Of a sequence's
+    rows the first is a known token and the others are drafts, drawn from softmax(draft_logits / temperature) of the row before, or without draft_logits
+    chosen in any other way. accept_draws (float32 [rows]) and sample_draws (float32 [batch]) are uniform numbers in [0, 1); temperature 0 takes the
+    largest logit and needs none. max_tokens: the largest number of rows of a sequence (default: what the rows allow). Returns (int64 [batch,
+    max_tokens]: accepted drafts, the token behind them, -1; int32 [batch]: how many drafts were accepted)."""
+    args = (logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws, temperature, batch, max_tokens)
+    r = (_native or _fast()).verify_drafts(*args, None)
+    if type(r) is int:  # the bytes of its workspace
+        r = _native.verify_drafts(*args, _verify_workspace(logits, r))
+    if r is not None:
+        return r
+    if torch.jit.is_tracing():
+        raise RuntimeError("verify_drafts cannot be recorded in a trace")
+    if not logits.is_cuda:
+        raise _C.LatentQError("logits must be a GPU tensor: the HIP kernels have no CPU fallback")
+    if logits.dtype not in _KV_TYPES:
+        raise TypeError(f"logits: expected bfloat16, float16 or float32, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    for t, dtype, name, shape in ((tokens, torch.int64, "tokens", (rows,)), (cu_tokens, torch.int32, "cu_tokens", None)):
+        if t is not None:
+            _chk(t, dtype, name)
+            if t.device != logits.device:
+                raise ValueError(f"{name} must be on the device of logits")
+            if shape is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if cu_tokens is not None:
+        if batch is not None:
+            raise ValueError("batch goes without cu_tokens, which has it")
+        if cu_tokens.dim() != 1 or cu_tokens.numel() == 0:
+            raise ValueError(f"cu_tokens must be [batch + 1], got {tuple(cu_tokens.shape)}")
+        batch, most = cu_tokens.numel() - 1, rows
+    else:
+        batch = rows if batch is None else int(batch)
+        if batch < 0 or (rows % batch if batch else rows):
+            raise ValueError(f"without cu_tokens every sequence has the same number of rows: {rows} for {batch} sequences")
+        most = rows // batch if batch else 0
+    if max_tokens is not None and (max_tokens < 0 or (cu_tokens is None and max_tokens < most) or (max_tokens == 0 and rows)):
+        raise ValueError(f"max_tokens is the largest number of rows of a sequence, got {max_tokens} for {rows} rows of {batch} sequences")
+    most = most if max_tokens is None else min(int(max_tokens), most)
+    temperature = float(temperature)
+    if not (temperature == 0.0 or 2.0 ** -60 <= temperature <= 2.0 ** 60):
+        raise ValueError(f"the temperature must be 0 or a positive number, got {temperature}")
+    if draft_logits is not None:
+        if not draft_logits.is_cuda or draft_logits.device != logits.device:
+            raise ValueError("draft_logits must be on the device of logits")
+        if draft_logits.dtype != logits.dtype or draft_logits.shape != logits.shape:
+            raise ValueError(f"draft_logits must be {logits.dtype} {tuple(logits.shape)}, as logits, got {draft_logits.dtype} {tuple(draft_logits.shape)}")
+    for t, n, name, needed in ((accept_draws, rows, "accept_draws", most > 1), (sample_draws, batch, "sample_draws", rows > 0)):
+        if t is not None:
+            _chk(t, torch.float32, name)
+            if t.device != logits.device or tuple(t.shape) != (n,):
+                raise ValueError(f"{name} must be {(n,)} on the device of logits, got {tuple(t.shape)}")
+        elif temperature > 0 and needed:
+            raise ValueError(f"a temperature above 0 needs {name}")
+    out = torch.full((batch, most), -1, dtype=torch.int64, device=logits.device)
+    accepted = torch.zeros(batch, dtype=torch.int32, device=logits.device)
+    if rows and batch:
+        import ctypes
+        logits, draft_logits = (t if t is None or t.stride(1) == 1 else t.contiguous() for t in (logits, draft_logits))
+        with torch.cuda.device(logits.device):
+            slices, needed = ctypes.c_int(), ctypes.c_int64()
+            _C.call("lq_verify_drafts_plan", batch, rows, vocab, int(temperature == 0), int(draft_logits is not None), 0, ctypes.addressof(slices), ctypes.addressof(needed))
+            ws = _verify_workspace(logits, needed.value)
+            ptr = [None if t is None else t.data_ptr() for t in (draft_logits, cu_tokens, accept_draws, sample_draws)]
+            _C.call("lq_verify_drafts", logits.data_ptr(), logits.stride(0), ptr[0], 0 if draft_logits is None else draft_logits.stride(0), tokens.data_ptr(), ptr[1], batch, rows,
+                    vocab, most, _KV_TYPES[logits.dtype], temperature, ptr[2], ptr[3], out.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(logits))
+            del ws
+    return out, accepted
+
+
+def _verify_workspace(t, needed):
+    if needed > WORKSPACE_MAX_BYTES:
+        return torch.empty(needed, dtype=torch.uint8, device=t.device)
+    return _workspace(t, 1, -(-needed // 32))[0]
