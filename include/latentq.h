@@ -577,6 +577,20 @@ int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_strid
 int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim,
                           int64_t window, int64_t workspace_bytes, int compute_units, int *kernel, int *parts, int64_t *needed);
 
+/* lq_kv8_attention (without a window) of a batch whose sequences all begin with the same `shared` blocks: the first `shared` columns of
+ * block_table are the same in every row, which is the caller's promise (which row's entries are read is not said). Those keys are
+ * read once for all rows, where that is faster, and the result is that of lq_kv8_attention but for roundings. A sequence may be shorter than the shared blocks: its rows
+ * see what is theirs. workspace as there, and without one, or with too little, every sequence is read by itself. */
+int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes, const float *k_scale,
+                            const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width, const int32_t *seq_lens,
+                            const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int64_t shared, int heads, int kv_heads,
+                            int dim, int dtype, float scale, int causal, void *out, int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+/* What the above does with a call of these sizes, as lq_kv8_attention_plan: slices of the shared keys and of a sequence's own (0 and 0: the call is
+ * one of lq_kv8_attention), and the bytes of workspace that they take. */
+int lq_kv8_attention_shared_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t shared,
+                                 int64_t workspace_bytes, int compute_units, int *prefix_slices, int *own_slices, int64_t *needed);
+
 /* Bookkeeping of such a cache on the device: the sequences' lengths become max(seq_lens[i] + change[i], 0), the blocks that they no
  * longer need go onto the list of free blocks, and those they need are taken from it (of those that are given back in the call,
  * too). A sequence of n tokens has max(ceil(n / 64), shared) blocks: the first `shared` blocks of every sequence, which a batch may have in

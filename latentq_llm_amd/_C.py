@@ -61,6 +61,9 @@ SIGNATURES = {
     "lq_kv8_attention": [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
                          _f32, _i32, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _vp],
     "lq_kv8_attention_plan": [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i32, _vp, _vp, _vp],
+    "lq_kv8_attention_shared": [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+                                _f32, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _vp],
+    "lq_kv8_attention_shared_plan": [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i32, _vp, _vp, _vp],
     "lq_kv8_resize": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
     "lq_verify_drafts": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _f64, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "lq_verify_drafts_plan": [_i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp],

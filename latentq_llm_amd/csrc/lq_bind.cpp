@@ -773,6 +773,47 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
 }
 
+// q, cache (4), block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse, workspace -> as kv8_attention
+PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    LQ_ARGS(15)
+    if (watched()) return none();
+    Rows16 q;
+    Cache8 c;
+    Sequences s;
+    if (!q.load(a[0]) || !c.load(a + 1) || !same_device(q.t, c.kc) || q.t->size(2) != c.dim || q.t->size(1) % c.heads) return none();
+    const int64_t tokens = q.t->size(0), heads = q.t->size(1);
+    if (!s.load(a[5], a[6], a[8], a[9], tokens, c.kc)) return none();
+    const int64_t shared = integer(a[7]);
+    int64_t max_len = s.width * LQ_KV_BLOCK;
+    if (a[10] != Py_None) {
+        const int64_t given = integer(a[10]);
+        if (given < 0) return none();
+        max_len = std::min(max_len, given);
+    }
+    const double scale = a[11] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(a[11]);
+    const int causal = PyObject_IsTrue(a[12]), with_lse = PyObject_IsTrue(a[13]);
+    if (PyErr_Occurred() || !(scale > 0.0 && scale <= 3.4e38) || shared < 0 || shared > s.width) return none();
+    void *ws;
+    int64_t ws_bytes;
+    if (!workspace(a[14], q.t, &ws, &ws_bytes)) return none();
+    On on(*c.kc);
+    if (!ws) {
+        int prefix, own;
+        int64_t needed;
+        if (const int rc = lq_kv8_attention_shared_plan(s.batch, tokens, s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, shared, kWorkspaceBytes, 0, &prefix, &own, &needed))
+            return fail("lq_kv8_attention_shared_plan", rc);
+        if (needed) return PyLong_FromLongLong(needed);
+    }
+    at::Tensor out = make(q.t->sizes(), q.t->scalar_type(), *q.t), lse;
+    if (with_lse) lse = make({tokens, heads}, at::kFloat, *q.t);
+    LQ_CALL(lq_kv8_attention_shared, q.t->data_ptr(), q.t->stride(0), q.t->stride(1), c.kc->data_ptr(), c.vc->data_ptr(), (const float *)c.ks->data_ptr(),
+            (const float *)c.vs->data_ptr(), c.blocks, (const int32_t *)s.table->data_ptr(), s.width, (const int32_t *)s.lens->data_ptr(), s.cu, s.batch, tokens,
+            s.most, max_len, shared, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, out.data_ptr(), out.stride(0), out.stride(1),
+            with_lse ? (float *)lse.data_ptr() : nullptr, ws, ws_bytes, on.stream);
+    if (!with_lse) return wrap(std::move(out));
+    return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
+}
+
 // cache (4), blocks, dtype as the C entry points number them -> (k, v)
 PyObject *kv8_read(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     LQ_ARGS(6)
@@ -927,7 +968,7 @@ PyMethodDef methods[] = {
     LQ_METHOD(linear4), LQ_METHOD(linear4_eval), LQ_METHOD(dx4), LQ_METHOD(gate_up), LQ_METHOD(dx_silu), LQ_METHOD(dx_pair), LQ_METHOD(linear8), LQ_METHOD(infer8),
     LQ_METHOD(infer8_eval), LQ_METHOD(dx8), LQ_METHOD(quant8), LQ_METHOD(quant8_token), LQ_METHOD(dequant8), LQ_METHOD(weight_grad),
     LQ_METHOD(weight_grad_acc), LQ_METHOD(weight_grad_acc8), LQ_METHOD(gradq8), LQ_METHOD(adam8_param), LQ_METHOD(adam8_sr),
-    LQ_METHOD(adam8_queue), LQ_METHOD(adam8_run), LQ_METHOD(adam8_w4), LQ_METHOD(adam8_w8), LQ_METHOD(kv8_append), LQ_METHOD(kv8_attention), LQ_METHOD(kv8_read), LQ_METHOD(kv8_resize), LQ_METHOD(verify_drafts), LQ_METHOD(current_stream),
+    LQ_METHOD(adam8_queue), LQ_METHOD(adam8_run), LQ_METHOD(adam8_w4), LQ_METHOD(adam8_w8), LQ_METHOD(kv8_append), LQ_METHOD(kv8_attention), LQ_METHOD(kv8_attention_shared), LQ_METHOD(kv8_read), LQ_METHOD(kv8_resize), LQ_METHOD(verify_drafts), LQ_METHOD(current_stream),
     LQ_METHOD(records_plainly), LQ_METHOD(set_error), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lqbind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -221,5 +221,30 @@ constexpr int kv8_few_workgroups(int dim, int rows) {
     return waves < 2 ? waves : 2;
 }
 
+// The arguments of lq_kv8_attention, in its order
+struct Kv8Call {
+    const void *q;
+    int64_t q_token_stride, q_head_stride;
+    const void *k_codes, *v_codes;
+    const float *k_scale, *v_scale;
+    int64_t num_blocks;
+    const int32_t *block_table;
+    int64_t table_width;
+    const int32_t *seq_lens, *cu_tokens;
+    int64_t batch, tokens, max_tokens, max_len;
+    int heads, kv_heads, dim, dtype;
+    float scale;
+    int causal;
+    int64_t window;
+    void *out;
+    int64_t out_token_stride, out_head_stride;
+    float *lse;
+    void *workspace;
+    int64_t workspace_bytes;
+    void *stream;
+};
+int kv8_attention_arguments(Kv8Attn &a, bool &any, const Kv8Call &c);
+int kv8_attention_call(const Kv8Call &c);
+
 int kv8_launch_few(const Kv8Attn &a, int dim, bool f16, void *stream);
 int kv8_launch_prompt(const Kv8Attn &a, int dim, bool f16, void *stream);

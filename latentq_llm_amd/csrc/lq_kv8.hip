@@ -609,50 +609,65 @@ extern "C" int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_
     return LQ_OK;
 }
 
-extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes,
-                                const float *k_scale, const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width,
-                                const int32_t *seq_lens, const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens,
-                                int64_t max_len, int heads, int kv_heads, int dim, int dtype, float scale, int causal, int64_t window, void *out,
-                                int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
-    if (const int rc = attention_sizes(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, window)) return rc;
-    LQ_REQUIRE(dtype == 0 || dtype == 1, "kv8_attention: dtype must be 0 (bf16) or 1 (f16), got %d", dtype);
-    LQ_REQUIRE(scale > 0.0f && scale <= 3.402823466e38f, "kv8_attention: the scale of the scores must be positive and finite");
-    if (batch == 0 || tokens == 0) return LQ_OK;
-    LQ_REQUIRE(max_tokens > 0, "kv8_attention: max_tokens must be the largest number of tokens of a sequence, got 0");
-    LQ_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && block_table && seq_lens && out, "kv8_attention: null pointer");
-    LQ_REQUIRE(num_blocks > 0 && num_blocks <= INT32_MAX && table_width > 0 && table_width <= INT32_MAX / KV8_BLOCK,
+// The arguments of an attention call, checked; false in `any`: there is nothing to be done
+int kv8_attention_arguments(Kv8Attn &a, bool &any, const Kv8Call &c) {
+    any = false;
+    if (const int rc = attention_sizes(c.batch, c.tokens, c.max_tokens, c.max_len, c.heads, c.kv_heads, c.dim, c.window)) return rc;
+    LQ_REQUIRE(c.dtype == 0 || c.dtype == 1, "kv8_attention: dtype must be 0 (bf16) or 1 (f16), got %d", c.dtype);
+    LQ_REQUIRE(c.scale > 0.0f && c.scale <= 3.402823466e38f, "kv8_attention: the scale of the scores must be positive and finite");
+    if (c.batch == 0 || c.tokens == 0) return LQ_OK;
+    LQ_REQUIRE(c.max_tokens > 0, "kv8_attention: max_tokens must be the largest number of tokens of a sequence, got 0");
+    LQ_REQUIRE(c.q && c.k_codes && c.v_codes && c.k_scale && c.v_scale && c.block_table && c.seq_lens && c.out, "kv8_attention: null pointer");
+    LQ_REQUIRE(c.num_blocks > 0 && c.num_blocks <= INT32_MAX && c.table_width > 0 && c.table_width <= INT32_MAX / KV8_BLOCK,
                "kv8_attention: a pool of blocks and a block table of 1 to %d columns are needed", INT32_MAX / KV8_BLOCK);
-    LQ_REQUIRE(cu_tokens || tokens % batch == 0, "kv8_attention: without cu_tokens every sequence has the same number of tokens: %lld do not divide by %lld",
-               (long long)tokens, (long long)batch);
-    for (int64_t s : {q_token_stride, q_head_stride, out_token_stride, out_head_stride})
+    LQ_REQUIRE(c.cu_tokens || c.tokens % c.batch == 0, "kv8_attention: without cu_tokens every sequence has the same number of tokens: %lld do not divide by %lld",
+               (long long)c.tokens, (long long)c.batch);
+    for (int64_t s : {c.q_token_stride, c.q_head_stride, c.out_token_stride, c.out_head_stride})
         LQ_REQUIRE(s >= 0 && s % 8 == 0, "kv8_attention: strides must be multiples of 8 elements, got %lld", (long long)s);
-    for (const void *p : {q, k_codes, v_codes, (const void *)out, (const void *)workspace})
+    for (const void *p : {c.q, c.k_codes, c.v_codes, (const void *)c.out, (const void *)c.workspace})
         LQ_REQUIRE(lq_aligned(p, 16), "kv8_attention: q, codes, output and workspace must be 16-byte aligned");
-    LQ_REQUIRE(rows_apart(tokens, out_token_stride, heads, out_head_stride, dim), "kv8_attention: rows of the output overlap");
-    LQ_REQUIRE(workspace_bytes >= 0, "kv8_attention: the workspace's size must not be negative");
-    if (max_tokens > tokens) max_tokens = tokens;
-    if (max_len > table_width * KV8_BLOCK) max_len = table_width * KV8_BLOCK;
-    if (window > INT32_MAX) window = 0;  // positions are less
+    LQ_REQUIRE(rows_apart(c.tokens, c.out_token_stride, c.heads, c.out_head_stride, c.dim), "kv8_attention: rows of the output overlap");
+    LQ_REQUIRE(c.workspace_bytes >= 0, "kv8_attention: the workspace's size must not be negative");
+    any = true;
+    a = Kv8Attn{};
+    a.q = c.q; a.k = (const uint8_t *)c.k_codes; a.v = (const uint8_t *)c.v_codes; a.ks = c.k_scale; a.vs = c.v_scale;
+    a.table = c.block_table; a.lens = c.seq_lens; a.cu = c.cu_tokens; a.out = c.out; a.lse = c.lse;
+    a.part = (float *)c.workspace;
+    a.q_token = c.q_token_stride; a.q_head = c.q_head_stride; a.o_token = c.out_token_stride; a.o_head = c.out_head_stride;
+    a.window = c.window > INT32_MAX ? 0 : c.window;  // positions are less
+    a.scale = c.scale * 1.442695040888963f;
+    a.blocks = (int)c.num_blocks; a.width = (int)c.table_width; a.batch = (int)c.batch; a.tokens = (int)c.tokens; a.heads = c.heads; a.kv_heads = c.kv_heads;
+    a.causal = c.causal != 0; a.rows = (int)(std::min(c.max_tokens, c.tokens) * (c.heads / c.kv_heads));
+    return LQ_OK;
+}
+
+int kv8_attention_call(const Kv8Call &c) {
+    Kv8Attn a;
+    bool any;
+    if (const int rc = kv8_attention_arguments(a, any, c); rc || !any) return rc;
+    const int64_t max_tokens = std::min(c.max_tokens, c.tokens), max_len = std::min(c.max_len, c.table_width * KV8_BLOCK), window = a.window, batch = c.batch;
     // (rows that also see what follows them see all the call's keys from their windows' beginnings on)
-    const bool ahead = !causal && window;
-    const Plan p = plan_of(batch, tokens, max_tokens, ahead ? std::min(max_len, window + max_tokens + KV8_BLOCK) : max_len, heads, kv_heads, dim, ahead ? 0 : window,
-                           table_width, workspace ? workspace_bytes : 0, lq_device_cu_count());
-    Kv8Attn a{};
-    a.q = q; a.k = (const uint8_t *)k_codes; a.v = (const uint8_t *)v_codes; a.ks = k_scale; a.vs = v_scale;
-    a.table = block_table; a.lens = seq_lens; a.cu = cu_tokens; a.out = out; a.lse = lse;
-    a.part = (float *)workspace;
-    a.part_lse = a.part + p.slots * p.slot_rows * dim;
-    a.q_token = q_token_stride; a.q_head = q_head_stride; a.o_token = out_token_stride; a.o_head = out_head_stride;
-    a.window = window; a.scale = scale * 1.442695040888963f;
-    a.blocks = (int)num_blocks; a.width = (int)table_width; a.batch = (int)batch; a.tokens = (int)tokens; a.heads = heads; a.kv_heads = kv_heads;
-    a.causal = causal != 0; a.workgroups = p.workgroups; a.rows = (int)(max_tokens * (heads / kv_heads));
+    const bool ahead = !a.causal && window;
+    const Plan p = plan_of(batch, c.tokens, max_tokens, ahead ? std::min(max_len, window + max_tokens + KV8_BLOCK) : max_len, c.heads, c.kv_heads, c.dim, ahead ? 0 : window,
+                           c.table_width, c.workspace ? c.workspace_bytes : 0, lq_device_cu_count());
+    a.part_lse = a.part + p.slots * p.slot_rows * c.dim;
+    a.workgroups = p.workgroups;
     a.slices = p.slices; a.tiles = p.tiles; a.row_tiles = p.row_tiles; a.waves = p.waves; a.sides = p.sides;
     // Sequences of different lengths, one after the other, leave compute units to those that got the long ones: in the order of what they
     // see, 4 x 4096 tokens (32 heads on 8 of 128; shortest 1473) 524 -> 295 us, 16 x 1024 (12 heads of 96) 72 -> 39. Finding a place in that order
     // is some 0.5 us in every workgroup, which few short ones do not get back (7 x 580 tokens, 32 heads: 27.9 / 28.5, 30 x 130, 32 on 8:
     // 19.1 / 20.6; 40 x 600, 12 heads: 58.8 / 44.8). With as many new tokens each (no cu_tokens) there is nothing to gain.
-    a.ranked = cu_tokens && batch > 1 && batch <= 64 && (p.row_tiles >= 8 || batch * kv_heads * p.row_tiles >= 2048);
-    LQ_REQUIRE(launchable(p.few ? batch * kv_heads : (int64_t)p.slices * batch * kv_heads * p.row_tiles, p.few ? 256 : 64 * p.waves * p.sides),
+    a.ranked = c.cu_tokens && batch > 1 && batch <= 64 && (p.row_tiles >= 8 || batch * c.kv_heads * p.row_tiles >= 2048);
+    LQ_REQUIRE(launchable(p.few ? batch * c.kv_heads : (int64_t)p.slices * batch * c.kv_heads * p.row_tiles, p.few ? 256 : 64 * p.waves * p.sides),
                "kv8_attention: too many workgroups: %lld sequences of up to %lld new tokens (max_tokens, the most of any, sizes the launch)", (long long)batch, (long long)max_tokens);
-    return p.few ? kv8_launch_few(a, dim, dtype == 1, stream) : kv8_launch_prompt(a, dim, dtype == 1, stream);
+    return p.few ? kv8_launch_few(a, c.dim, c.dtype == 1, c.stream) : kv8_launch_prompt(a, c.dim, c.dtype == 1, c.stream);
+}
+
+extern "C" int lq_kv8_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes,
+                                const float *k_scale, const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width,
+                                const int32_t *seq_lens, const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens,
+                                int64_t max_len, int heads, int kv_heads, int dim, int dtype, float scale, int causal, int64_t window, void *out,
+                                int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
+    return kv8_attention_call(Kv8Call{q, q_token_stride, q_head_stride, k_codes, v_codes, k_scale, v_scale, num_blocks, block_table, table_width, seq_lens, cu_tokens, batch, tokens,
+                                      max_tokens, max_len, heads, kv_heads, dim, dtype, scale, causal, window, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream});
 }

@@ -1151,6 +1151,27 @@ def kv8_attention_plan(batch: int, tokens: int, max_tokens: int, max_len: int, h
     return KV8_KERNELS[kernel.value], parts.value, needed.value
 
 
+def _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, out):
+    """(blocks, kv heads, dim, batch, table width, max_tokens, scale, max_len, out) of an attention call, checked; out made where there is none."""
+    n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    _kv8_rows(q, "q", None, dim, k_codes)
+    tokens, heads = q.shape[0], q.shape[1]
+    if heads == 0 or heads % kv_heads:
+        raise ValueError(f"the number of query heads must be a multiple of {kv_heads}, got {heads}")
+    batch, width, most = _kv8_sequences(block_table, seq_lens, cu_tokens, max_tokens, tokens, k_codes)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 3.4e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    max_len = width * KV_BLOCK if max_len is None else min(int(max_len), width * KV_BLOCK)
+    if max_len < 0:
+        raise ValueError(f"max_len must not be negative, got {max_len}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _kv8_result(out, "out", q)
+    return n, kv_heads, dim, batch, width, most, scale, max_len, out
+
+
 def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,
                   causal=True, window=0, out=None, return_lse=False):
     """Attention of the last tokens of each sequence, q [tokens, heads, dim], over its blocks of a paged 8-bit cache (lq_kv8_attention):
@@ -1165,25 +1186,12 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
             r = _native.kv8_attention(*args, _workspace(q, 1, -(-r // 32))[0])
         if r is not None:
             return r
-    n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
-    _kv8_rows(q, "q", None, dim, k_codes)
+    n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
+                                                                                       scale, out)
     tokens, heads = q.shape[0], q.shape[1]
-    if heads == 0 or heads % kv_heads:
-        raise ValueError(f"the number of query heads must be a multiple of {kv_heads}, got {heads}")
-    batch, width, most = _kv8_sequences(block_table, seq_lens, cu_tokens, max_tokens, tokens, k_codes)
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale <= 3.4e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
     window = min(int(window or 0), 1 << 31)  # (positions are less)
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
-    max_len = width * KV_BLOCK if max_len is None else min(int(max_len), width * KV_BLOCK)
-    if max_len < 0:
-        raise ValueError(f"max_len must not be negative, got {max_len}")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _kv8_result(out, "out", q)
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if tokens and batch:
         q = _kv8_layout(q)
@@ -1194,6 +1202,48 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
             _C.call("lq_kv8_attention", q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
                     v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(), None if cu_tokens is None else cu_tokens.data_ptr(),
                     batch, tokens, most, max_len, heads, kv_heads, dim, _KV_TYPES[q.dtype], scale, int(bool(causal)), window, out.data_ptr(),
+                    out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws, ws_bytes, _stream(q))
+            del keep
+    return (out, lse) if return_lse else out
+
+
+def kv8_attention_shared_plan(batch: int, tokens: int, max_tokens: int, max_len: int, heads: int, kv_heads: int, dim: int, shared: int,
+                              workspace_bytes: int = WORKSPACE_MAX_BYTES, compute_units: int = 0):
+    """(slices of the shared keys, of a sequence's own, bytes of workspace these take) kv8_attention_shared would use for a call of these sizes
+    (lq_kv8_attention_shared_plan); (0, 0, bytes): the call is one of kv8_attention. Launches nothing."""
+    import ctypes
+    prefix, own, needed = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
+    _C.call("lq_kv8_attention_shared_plan", batch, tokens, max_tokens, max_len, heads, kv_heads, dim, shared, workspace_bytes, compute_units,
+            ctypes.addressof(prefix), ctypes.addressof(own), ctypes.addressof(needed))
+    return prefix.value, own.value, needed.value
+
+
+def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,
+                         causal=True, out=None, return_lse=False):
+    """kv8_attention of a batch whose sequences all begin with the same `shared` blocks (lq_kv8_attention_shared): the first `shared` columns of
+    block_table are the same in every row. Their keys and values are read once for all rows. Arguments and results otherwise as
+    kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
+    if out is None:
+        args = (q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse)
+        r = (_native or _fast()).kv8_attention_shared(*args, None)
+        if type(r) is int:  # the bytes that its parts want
+            r = _native.kv8_attention_shared(*args, _workspace(q, 1, -(-r // 32))[0])
+        if r is not None:
+            return r
+    n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
+                                                                                       scale, out)
+    tokens, heads, shared = q.shape[0], q.shape[1], int(shared)
+    if not 0 <= shared <= width:
+        raise ValueError(f"shared must be 0 to {width}, the columns of block_table, got {shared}")
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    if tokens and batch:
+        q = _kv8_layout(q)
+        with torch.cuda.device(k_codes.device):
+            needed = kv8_attention_shared_plan(batch, tokens, most, max_len, heads, kv_heads, dim, shared)[2]
+            keep, ws, ws_bytes = _workspace(q, 1, -(-needed // 32)) if needed else (None, None, 0)
+            _C.call("lq_kv8_attention_shared", q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
+                    v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(), None if cu_tokens is None else cu_tokens.data_ptr(),
+                    batch, tokens, most, max_len, shared, heads, kv_heads, dim, _KV_TYPES[q.dtype], scale, int(bool(causal)), out.data_ptr(),
                     out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws, ws_bytes, _stream(q))
             del keep
     return (out, lse) if return_lse else out
