@@ -10,17 +10,23 @@
 // this device's vector units do at the rate of 32.
 //   2^y = 2^(k/32) 2^r,  k = rint(32 y),  |r| <= 1/64:  a table of 32 and the series of 2^r to r^6 (what is cut off: 4e-18)
 //
-// Three launches, each a pass that needs a sum of the one before: maximum and sum of every row in slices; the rows' tests, and the
-// sums of what is left of one row of each sequence in blocks of 2048; the block in which the sum passes the number.
+// Every row's maximum and sum is taken in slices first, by as many workgroups. Without the drafter's logits a second launch, a workgroup for each
+// sequence, makes the rows' tests, finds the slice in which the sum passes the number by the slices' sums, and the entry in it. With them what is left of a
+// row needs both rows' sums first: one launch more takes the sums of max(p - q, 0) in blocks of the one row of each sequence.
 #include "lq_common.h"
+
+#include <algorithm>
 
 namespace {
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kSpan = 2048;  // entries of a block of the row that a token is drawn from
+constexpr int kStats = 256;             // threads of a workgroup on a slice
+constexpr int kThreads = 512, kWaves = 8;  // on a sequence
+constexpr int kEach = 8, kBlock = kThreads * kEach;  // entries of a thread, and of a block of the row that a token is drawn from
+constexpr int kRound = 32;              // rows of a sequence that are tested together
 constexpr float kMost = 3.402823466e38f;
 
-enum { kBf16, kF16, kF32 };
+enum { kBf16, kF16, kF32 };             // of the logits
+enum { kGreedy, kAlone, kBoth };        // the largest logit; by the target's logits alone; by both
 
 struct Stat {  // of a slice: sum of 2^((l - m) c); of the greedy choice: the maximum's place
     union {
@@ -36,7 +42,7 @@ struct Left {  // of a block: sums of max(p - q, 0) and of p
 struct Chosen {  // the row that a sequence's token is drawn from
     double p_sum, q_sum;
     float p_m, q_m;
-    int row, draft;  // draft: the token that was refused, -1: none was; row -1: nothing to be drawn
+    int row, draft;  // draft: the token that was refused, -1: none was, -2: one outside the vocabulary; row -1: nothing to be drawn
     int64_t *to;
 };
 
@@ -65,31 +71,48 @@ struct Row {
     static constexpr int kVec = kType == kF32 ? 4 : 8;  // entries of 16 bytes
     const void *at;
     __device__ __forceinline__ float one(int64_t j) const {
-        if constexpr (kType == kF32) return counted(((const float *)at)[j]);
-        else if constexpr (kType == kF16) return counted((float)((const _Float16 *)at)[j]);
-        else return counted(lq_bf16_bits_to_f32(((const unsigned short *)at)[j]));
+        if constexpr (kType == kF32) return ((const float *)at)[j];
+        else if constexpr (kType == kF16) return (float)((const _Float16 *)at)[j];
+        else return lq_bf16_bits_to_f32(((const unsigned short *)at)[j]);
     }
-    // entries j .. j + kVec - 1, those from `end` on as masked ones
-    __device__ __forceinline__ void some(int j, int end, float f[kVec]) const {
-        if (j + kVec <= end) {
-            const u32x4_t w = kType == kF32 ? *(const piece_t *)((const float *)at + j) : *(const piece_t *)((const unsigned short *)at + j);
+    // entries j .. j + kVec - 1, as they lie there and as they count
+    __device__ __forceinline__ u32x4_t piece(int j) const { return kType == kF32 ? *(const piece_t *)((const float *)at + j) : *(const piece_t *)((const unsigned short *)at + j); }
+    static __device__ __forceinline__ void values(const u32x4_t w, float *f) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned x = w[i];
-                if constexpr (kType == kF32) {
-                    f[i] = counted(__uint_as_float(x));
-                } else if constexpr (kType == kF16) {
-                    f[2 * i] = counted((float)__builtin_bit_cast(_Float16, (unsigned short)x));
-                    f[2 * i + 1] = counted((float)__builtin_bit_cast(_Float16, (unsigned short)(x >> 16)));
-                } else {
-                    f[2 * i] = counted(lq_bf16_lo(x));
-                    f[2 * i + 1] = counted(lq_bf16_hi(x));
-                }
+        for (int i = 0; i < 4; ++i) {
+            const unsigned x = w[i];
+            if constexpr (kType == kF32) {
+                f[i] = __uint_as_float(x);
+            } else if constexpr (kType == kF16) {
+                f[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)x);
+                f[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(x >> 16));
+            } else {
+                f[2 * i] = lq_bf16_lo(x);
+                f[2 * i + 1] = lq_bf16_hi(x);
             }
+        }
+    }
+    template <int kCount>
+    static __device__ __forceinline__ void count(float (&f)[kCount]) {
+        bool plain = true;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) plain &= f[i] <= kMost;
+        if (!plain) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) f[i] = counted(f[i]);
+        }
+    }
+    // kCount entries from j on, those from `end` on masked
+    template <int kCount>
+    __device__ __forceinline__ void some(int j, int end, float (&f)[kCount]) const {
+        if (j + kCount <= end) {
+#pragma unroll
+            for (int v = 0; v < kCount; v += kVec) values(piece(j + v), f + v);
         } else {
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) f[i] = j + i < end ? one(j + i) : -__builtin_inff();
+            for (int i = 0; i < kCount; ++i) f[i] = j + i < end ? one(j + i) : -__builtin_inff();
         }
+        count(f);
     }
 };
 
@@ -102,18 +125,19 @@ __device__ __forceinline__ Row<kType> row_at(const void *base, int64_t stride, i
 // 2^((l - m) c), l <= m; 0 where nothing of it is left in 64 bits. The table is in shared memory, one bank pair to an entry.
 struct Exp2 {
     const double *table;
-    double c;
-    __device__ __forceinline__ double operator()(float l, float m) const {
-        const double y = fmax(((double)l - (double)m) * c, -1100.0), magic = 0x1.8p52;
-        const double t = fma(y, 32.0, magic);
+    double c32;  // 32 c
+    __device__ __forceinline__ Exp2(const double *table, double c) : table(table), c32(32.0 * c) {}
+    __device__ __forceinline__ double operator()(float l, double m) const {
+        const double y = fmax(((double)l - m) * c32, -32.0 * 1100), magic = 0x1.8p52;
+        const double t = y + magic;
         const int k = (int)__builtin_bit_cast(uint64_t, t);
-        const double r = fma(t - magic, -0x1p-5, y), e = table[k & 31];
-        double s = 0x1.430912f86c787p-13;      // ln(2)^6 / 6!
-        s = fma(s, r, 0x1.5d87fe78a6731p-10);  // ln(2)^5 / 5!
-        s = fma(s, r, 0x1.3b2ab6fba4e77p-7);
-        s = fma(s, r, 0x1.c6b08d704a0c0p-5);
-        s = fma(s, r, 0x1.ebfbdff82c58fp-3);
-        s = fma(s, r, 0x1.62e42fefa39efp-1);   // ln(2)
+        const double r = y - (t - magic), e = table[k & 31];  // |r| <= 1/2, in 32nds
+        double s = 0x1.430912f86c787p-43;      // (ln(2) / 32)^6 / 6!
+        s = fma(s, r, 0x1.5d87fe78a6731p-35);  // (ln(2) / 32)^5 / 5!
+        s = fma(s, r, 0x1.3b2ab6fba4e77p-27);
+        s = fma(s, r, 0x1.c6b08d704a0c0p-20);
+        s = fma(s, r, 0x1.ebfbdff82c58fp-13);
+        s = fma(s, r, 0x1.62e42fefa39efp-6);   // ln(2) / 32
         return ldexp(fma(e, s * r, e), k >> 5);
     }
 };
@@ -124,16 +148,31 @@ __device__ __forceinline__ void fill_table(double *table) {
 // The reference of a row's exponents: its maximum, or anything where the row is masked as a whole
 __device__ __forceinline__ float reference(float m) { return m == -__builtin_inff() ? 0.0f : m; }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+// Over the lanes of a wave by lane shifts (row_shr:1, 2, 4, 8, then row_bcast:15 and 31): sums up to each lane, and the largest of the lanes up to it; lanes
+// 31 and 63 have those of the wave's halves before the last step, lane 63 that of all after it.
+template <int kShift, int kRows>
+__device__ __forceinline__ int shifted(int x, int none) { return __builtin_amdgcn_update_dpp(none, x, kShift, kRows, 0xf, false); }
+template <int kShift, int kRows>
+__device__ __forceinline__ double plus(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const unsigned lo = shifted<kShift, kRows>((int)b, 0), hi = shifted<kShift, kRows>((int)(b >> 32), 0);
+    return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+template <int kShift, int kRows>
+__device__ __forceinline__ float most_of(float x) {
+    return fmaxf(x, __int_as_float(shifted<kShift, kRows>(__float_as_int(x), (int)0xFF800000)));
 }
+__device__ __forceinline__ double halves_scan(double x) { return plus<0x142, 0xa>(plus<0x118, 0xf>(plus<0x114, 0xf>(plus<0x112, 0xf>(plus<0x111, 0xf>(x))))); }
+__device__ __forceinline__ double wave_scan(double x) { return plus<0x143, 0xc>(halves_scan(x)); }
+__device__ __forceinline__ float halves_most(float x) { return most_of<0x142, 0xa>(most_of<0x118, 0xf>(most_of<0x114, 0xf>(most_of<0x112, 0xf>(most_of<0x111, 0xf>(x))))); }
+__device__ __forceinline__ double at_lane(double x, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const unsigned lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float at_lane(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+__device__ __forceinline__ float wave_max(float x) { return at_lane(most_of<0x143, 0xc>(halves_most(x)), 63); }
+__device__ __forceinline__ double wave_sum(double x) { return at_lane(wave_scan(x), 63); }
 
 // Rows of a sequence: start .. start + n - 1, no more than max_tokens of them
 __device__ __forceinline__ void rows_of(const Verify &a, int seq, int &start, int &n) {
@@ -148,28 +187,30 @@ __device__ __forceinline__ void rows_of(const Verify &a, int seq, int &start, in
 }
 
 // ---- every row: blockIdx.x for a slice, .y for a row, .z: 0 the target's, 1 the drafter's
-template <int kType, bool kGreedy>
-__global__ __launch_bounds__(kThreads) void stats_kernel(const Verify a) {
-    constexpr int kVec = Row<kType>::kVec;
-    __shared__ double table[32], sums[kWaves];
-    __shared__ float tops[kWaves];
-    __shared__ int places[kWaves];
+template <int kType, bool kLargest>
+__global__ __launch_bounds__(kStats) void stats_kernel(const Verify a) {
+    constexpr int kMine = 16;  // entries of a thread at a time
+    __shared__ double table[32], sums[kStats / 64];
+    __shared__ float tops[kStats / 64];
+    __shared__ int places[kStats / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.y, slice = blockIdx.x;
     const bool of_draft = blockIdx.z;
-    if (of_draft) {  // a sequence's last row has no draft behind it
+    const auto unused = [&] {  // a sequence's last row has no draft behind it
+        if (!of_draft) return false;
         bool last = row + 1 >= a.rows;
         if (a.cu)
             for (int i = lane; i < a.batch; i += 64) last |= a.cu[i + 1] == row + 1;
         else last |= (row + 1) % (a.rows / a.batch) == 0;
-        if (__any(last)) return;
-    }
+        return (bool)__any(last);
+    };
     const Row<kType> x = of_draft ? row_at<kType>(a.draft, a.draft_stride, row) : row_at<kType>(a.logits, a.stride, row);
     const int begin = slice * a.span, end = min(begin + a.span, a.vocab);
     Stat &to = a.stats[((int64_t)row * 2 + of_draft) * a.slices + slice];
-    if constexpr (kGreedy) {
-        float m = -__builtin_inff();
+    constexpr int kVec = Row<kType>::kVec;
+    float m = -__builtin_inff();
+    if constexpr (kLargest) {
         int at = INT32_MAX;
-        for (int j = begin + (int)threadIdx.x * kVec; j < end; j += kThreads * kVec) {
+        for (int j = begin + (int)threadIdx.x * kVec; j < end; j += kStats * kVec) {
             float f[kVec];
             x.some(j, end, f);
 #pragma unroll
@@ -192,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const Verify a) {
             Stat s;
             s.m = tops[0];
             int best = places[0];
-            for (int w = 1; w < kWaves; ++w)
+            for (int w = 1; w < kStats / 64; ++w)
                 if (tops[w] > s.m || (tops[w] == s.m && places[w] < best)) {
                     s.m = tops[w];
                     best = places[w];
@@ -202,23 +243,48 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const Verify a) {
             to = s;
         }
     } else {
+        // kMine entries at a time, in pieces that the workgroup has side by side, requested a turn ahead; then what is left piece by piece
+        constexpr int kPieces = kMine / kVec, kTurn = kMine * kStats;
+        int j = begin + (int)threadIdx.x * kVec;
+        u32x4_t w[kPieces];
+        const auto request = [&] {
+#pragma unroll
+            for (int v = 0; v < kPieces; ++v) w[v] = x.piece(j + v * kStats * kVec);
+        };
+        bool whole = j + kTurn - kStats * kVec + kVec <= end;
+        if (whole) request();
+        if (unused()) return;  // (under the first pieces' way)
         fill_table(table);
         __syncthreads();
-        const Exp2 power{table, a.c};
-        float m = -__builtin_inff();
+        const Exp2 power(table, a.c);
         double sum = 0.0;
-        for (int j = begin + (int)threadIdx.x * kVec; j < end; j += kThreads * kVec) {
-            float f[kVec], most = m;
-            x.some(j, end, f);
+        const auto add = [&](auto &f) {
+            constexpr int kCount = sizeof(f) / sizeof(f[0]);
+            x.count(f);
+            float most = f[0];
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) most = fmaxf(most, f[i]);
+            for (int i = 1; i < kCount; ++i) most = fmaxf(most, f[i]);
             if (most > m) {
                 sum *= power(m, reference(most));
                 m = most;
             }
-            const float ref = reference(m);
+            const double ref = reference(m);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) sum += power(f[i], ref);
+            for (int i = 0; i < kCount; ++i) sum += power(f[i], ref);
+        };
+        while (whole) {
+            float f[kMine];
+#pragma unroll
+            for (int v = 0; v < kPieces; ++v) x.values(w[v], f + v * kVec);
+            j += kTurn;
+            whole = j + kTurn - kStats * kVec + kVec <= end;
+            if (whole) request();
+            add(f);
+        }
+        for (; j < end; j += kVec * kStats) {
+            float f[kVec];
+            x.some(j, end, f);
+            add(f);
         }
         const float top = wave_max(m);
         sum = wave_sum(sum * power(m, reference(top)));
@@ -227,265 +293,407 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(const Verify a) {
             sums[wave] = sum;
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            Stat s;
-            s.m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-            s.sum = 0.0;
-            for (int w = 0; w < kWaves; ++w) s.sum += sums[w] * power(tops[w], reference(s.m));
-            s.pad = 0;
-            to = s;
+        if (threadIdx.x < 4) {
+            static_assert(kStats / 64 == 4, "");
+            const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+            const double all = plus<0x112, 0xf>(plus<0x111, 0xf>(sums[lane] * power(tops[lane], reference(most))));
+            if (lane == 3) {
+                Stat s;
+                s.m = most;
+                s.sum = all;
+                s.pad = 0;
+                to = s;
+            }
         }
     }
 }
 
-// The slices of a row put together
-__device__ __forceinline__ void joined(const Verify &a, const Exp2 &power, int row, int which, float &m, double &sum) {
-    const Stat *s = a.stats + ((int64_t)row * 2 + which) * a.slices;
-    m = -__builtin_inff();
-    for (int i = 0; i < a.slices; ++i) m = fmaxf(m, s[i].m);
-    sum = 0.0;
-    for (int i = 0; i < a.slices; ++i) sum += s[i].sum * power(s[i].m, reference(m));
-}
-
-// What is left of a row's probabilities for the token that is drawn
-template <int kType>
+// Entries of what is left of a row's probabilities, or of the probabilities themselves, for the token that is drawn
+template <int kType, bool kQ>
 struct Rest {
     Row<kType> p, q;
     Exp2 power;
-    float p_m, q_m;
-    double p_by, q_by;  // 1 / sum
-    int draft;          // -1: none; without q its entry alone is taken off
-    bool with_q;
+    double p_m, q_m, p_by, q_by;  // references and 1 / sums
+    int draft;                    // -1: none; without q its entry alone is taken off
     __device__ __forceinline__ Rest(const Verify &a, const Exp2 &power, const Chosen &c)
         : p(row_at<kType>(a.logits, a.stride, c.row)), q(row_at<kType>(a.draft, a.draft_stride, c.row)), power(power), p_m(reference(c.p_m)), q_m(reference(c.q_m)),
-          p_by(c.p_sum > 0.0 ? 1.0 / c.p_sum : 0.0), q_by(c.q_sum > 0.0 ? 1.0 / c.q_sum : 0.0), draft(c.draft), with_q(a.draft && c.draft != -1) {}
-    __device__ __forceinline__ void some(int j, int end, double rest[Row<kType>::kVec], double all[Row<kType>::kVec]) const {
-        constexpr int kVec = Row<kType>::kVec;
-        float f[kVec], g[kVec];
-        p.some(j, end, f);
-        if (with_q) q.some(j, end, g);
+          p_by(c.p_sum > 0.0 ? 1.0 / c.p_sum : 0.0), q_by(c.q_sum > 0.0 ? 1.0 / c.q_sum : 0.0), draft(c.draft) {}
+    template <int kCount>
+    __device__ __forceinline__ void some(int j, int end, double (&rest)[kCount], double (&all)[kCount]) const {
+        float f[kCount], g[kCount];
+        const bool both = kQ && draft != -1;
+        constexpr int kVec = Row<kType>::kVec, kPieces = kCount / kVec;
+        if (both && j + kCount <= end) {
+            u32x4_t v[kPieces], w[kPieces];
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+            for (int i = 0; i < kPieces; ++i) {
+                v[i] = p.piece(j + i * kVec);
+                w[i] = q.piece(j + i * kVec);
+            }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                p.values(v[i], f + i * kVec);
+                q.values(w[i], g + i * kVec);
+            }
+            p.count(f);
+            q.count(g);
+        } else {
+            p.some(j, end, f);
+            if (both) q.some(j, end, g);
+        }
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
             all[i] = power(f[i], p_m) * p_by;
-            if (with_q) rest[i] = fmax(all[i] - power(g[i], q_m) * q_by, 0.0);
-            else rest[i] = j + i == draft ? 0.0 : all[i];
+            rest[i] = !kQ && j + i == draft ? 0.0 : all[i];
+        }
+        if (both) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) rest[i] = fmax(all[i] - power(g[i], q_m) * q_by, 0.0);
         }
     }
 };
 
-// ---- every sequence: blockIdx.y; blockIdx.x for a block of its row
-template <int kType, bool kGreedy>
-__global__ __launch_bounds__(kThreads) void decide_kernel(const Verify a) {
-    constexpr int kVec = Row<kType>::kVec, kAtOnce = kThreads / 2;
-    __shared__ double table[32], row_sum[2][kAtOnce], sums[2][kWaves];
-    __shared__ float row_m[2][kAtOnce];
-    __shared__ int64_t best[kAtOnce];
-    __shared__ int refused;
-    const int tid = threadIdx.x, seq = blockIdx.y;
-    int start, n;
-    rows_of(a, seq, start, n);
-    int64_t *out = a.out + (int64_t)seq * a.most;
-    const bool writes = blockIdx.x == 0;
-    if (n == 0) {
-        if (writes) {
-            for (int i = tid; i < a.most; i += kThreads) out[i] = -1;
-            if (tid == 0) {
-                a.accepted[seq] = 0;
-                if constexpr (!kGreedy) a.chosen[seq].row = -1;
-            }
-        }
-        return;
-    }
-    if constexpr (!kGreedy) fill_table(table);
-    const Exp2 power{table, a.c};
-    int first = n - 1, base = 0;  // the first row whose draft is not taken
-    for (;; base += kAtOnce) {
-        const int count = min(kAtOnce, n - base);
-        if (tid == 0) refused = INT32_MAX;
+struct Board {  // in shared memory
+    double row_sum[2][kRound];
+    float row_m[2][kRound];
+    int64_t best[kRound];
+    int refused;
+};
+
+// The rows' tests, by all waves of a workgroup: the first row of the sequence whose draft is not taken, or its last one. A wave has a row at a time: its
+// slices lie in the lanes of a half, the drafter's in the other, and what the test needs besides is on its way with them.
+template <int kType, int kMode>
+__device__ __forceinline__ int first_refused(const Verify &a, const Exp2 &power, Board &b, int start, int n, int &base) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    for (base = 0;; base += kRound) {
+        if (threadIdx.x == 0) b.refused = INT32_MAX;
         __syncthreads();
-        const int i = tid >> 1, which = tid & 1, row = start + base + i;
-        if (i < count) {
-            if constexpr (kGreedy) {
-                if (which == 0) {
-                    const Stat *s = a.stats + (int64_t)row * 2 * a.slices;
-                    float m = -__builtin_inff();
-                    int64_t at = -1;
-                    for (int k = 0; k < a.slices; ++k)
-                        if (s[k].m > m) {
-                            m = s[k].m;
-                            at = s[k].at;
-                        }
-                    best[i] = at;
-                    if (base + i == n - 1 || a.tokens[row + 1] != at || at < 0) atomicMin(&refused, base + i);
+        const int count = min(kRound, n - base);
+        for (int i = wave; i < count; i += kWaves) {
+            const int row = start + base + i;
+            const bool drafted = base + i < n - 1;
+            const int64_t token = drafted ? a.tokens[row + 1] : -1;
+            const bool inside = token >= 0 && token < a.vocab;
+            if constexpr (kMode == kGreedy) {
+                const Stat *s = a.stats + (int64_t)row * 2 * a.slices;
+                float m = -__builtin_inff();
+                int at = INT32_MAX;
+                for (int k = lane; k < a.slices; k += 64)
+                    if (s[k].m > m) {
+                        m = s[k].m;
+                        at = (int)s[k].at;
+                    }
+                const float top = wave_max(m);
+                at = m == top ? at : INT32_MAX;
+#pragma unroll
+                for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+                const int64_t best = top == -__builtin_inff() ? -1 : at;
+                if (lane == 0) {
+                    b.best[i] = best;
+                    if (!inside || token != best) atomicMin(&b.refused, base + i);
                 }
             } else {
-                float m = 0.0f;
-                double sum = 0.0;
-                if (which == 0 || (a.draft && base + i < n - 1)) joined(a, power, row, which, m, sum);
-                row_m[which][i] = m;
-                row_sum[which][i] = sum;
-            }
-        }
-        __syncthreads();
-        if constexpr (!kGreedy) {
-            if (tid < count) {
-                bool taken = false;
-                if (base + tid < n - 1) {
-                    const int r = start + base + tid;
-                    const int64_t token = a.tokens[r + 1];
-                    if (token >= 0 && token < a.vocab) {
-                        const double p = power(row_at<kType>(a.logits, a.stride, r).one(token), reference(row_m[0][tid])), sp = row_sum[0][tid];
-                        double q = 1.0, sq = 1.0;
-                        if (a.draft) {
-                            q = power(row_at<kType>(a.draft, a.draft_stride, r).one(token), reference(row_m[1][tid]));
-                            sq = row_sum[1][tid];
-                        }
-                        taken = sp > 0.0 && (double)a.accept[r] * (sq > 0.0 ? q / sq : 0.0) < p / sp;
-                    }
+                float of_p = 0.0f, of_q = 0.0f, u = 0.0f;
+                if (inside) {
+                    of_p = row_at<kType>(a.logits, a.stride, row).one(token);
+                    if constexpr (kMode == kBoth) of_q = row_at<kType>(a.draft, a.draft_stride, row).one(token);
+                    u = a.accept[row];
                 }
-                if (!taken) atomicMin(&refused, base + tid);
-            }
-            __syncthreads();
-        }
-        if (refused != INT32_MAX) {
-            first = refused;
-            break;
-        }
-        __syncthreads();
-    }
-    const int row = start + first, at = first - base;
-    if (writes) {
-        if (tid == 0) a.accepted[seq] = first;
-        for (int i = tid; i < a.most; i += kThreads) {
-            if constexpr (kGreedy) out[i] = i < first ? a.tokens[start + i + 1] : i == first ? best[at] : -1;
-            else if (i != first) out[i] = i < first ? a.tokens[start + i + 1] : -1;
-        }
-    }
-    if constexpr (!kGreedy) {
-        Chosen c{row_sum[0][at], row_sum[1][at], row_m[0][at], row_m[1][at], row, -1, out + first};
-        if (first < n - 1) {
-            const int64_t token = a.tokens[row + 1];
-            c.draft = token >= 0 && token < a.vocab ? (int)token : -2;  // -2: one that has no entry
-        }
-        if (writes && tid == 0) a.chosen[seq] = c;
-        const Rest<kType> rest(a, power, c);
-        const int begin = blockIdx.x * kSpan, end = min(begin + kSpan, a.vocab);
-        double mine = 0.0, whole = 0.0;
-        for (int j = begin + tid * kVec; j < end; j += kThreads * kVec) {
-            double x[kVec], y[kVec];
-            rest.some(j, end, x, y);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                mine += x[i];
-                whole += y[i];
+                const bool mine = half == 0 || (kMode == kBoth && drafted);
+                const Stat *s = a.stats + ((int64_t)row * 2 + half) * a.slices;
+                float m = -__builtin_inff();
+                double sum = 0.0;
+                if (mine && (lane & 31) < a.slices) {
+                    m = s[lane & 31].m;
+                    sum = s[lane & 31].sum;
+                }
+                for (int k = (lane & 31) + 32; mine && k < a.slices; k += 32) {
+                    const float more = fmaxf(m, s[k].m);
+                    sum = sum * power(m, reference(more)) + s[k].sum * power(s[k].m, reference(more));
+                    m = more;
+                }
+                const float tops = halves_most(m), p_m = at_lane(tops, 31), q_m = at_lane(tops, 63);
+                const double sums = halves_scan(sum * power(m, reference(half ? q_m : p_m))), p_sum = at_lane(sums, 31), q_sum = at_lane(sums, 63);
+                bool taken = false;
+                if (inside) {
+                    const double p = power(counted(of_p), reference(p_m));
+                    const double q = kMode == kBoth ? power(counted(of_q), reference(q_m)) : 1.0, all = kMode == kBoth ? q_sum : 1.0;
+                    taken = p_sum > 0.0 && (double)u * (all > 0.0 ? q / all : 0.0) < p / p_sum;
+                }
+                if (lane == 0) {
+                    b.row_m[0][i] = p_m;
+                    b.row_m[1][i] = q_m;
+                    b.row_sum[0][i] = p_sum;
+                    b.row_sum[1][i] = q_sum;
+                    if (!taken) atomicMin(&b.refused, base + i);
+                }
             }
         }
-        mine = wave_sum(mine);
-        whole = wave_sum(whole);
-        if ((tid & 63) == 0) {
-            sums[0][tid >> 6] = mine;
-            sums[1][tid >> 6] = whole;
-        }
         __syncthreads();
-        if (tid == 0) a.left[(int64_t)seq * a.blocks + blockIdx.x] = Left{(sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]), (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3])};
+        const int refused = b.refused;
+        if (refused != INT32_MAX) return refused;
+        __syncthreads();
     }
 }
 
-// ---- every sequence: the block in which the sum passes the number, and the entry in it
+// A sequence without rows
+__device__ __forceinline__ void nothing(const Verify &a, int seq) {
+    for (int i = threadIdx.x; i < a.most; i += kThreads) a.out[(int64_t)seq * a.most + i] = -1;
+    if (threadIdx.x == 0) a.accepted[seq] = 0;
+}
+// Its taken drafts, and nothing behind the token that is drawn
+__device__ __forceinline__ void write_taken(const Verify &a, int seq, int start, int first) {
+    int64_t *out = a.out + (int64_t)seq * a.most;
+    if (threadIdx.x == 0) a.accepted[seq] = first;
+    for (int i = threadIdx.x; i < a.most; i += kThreads)
+        if (i != first) out[i] = i < first ? a.tokens[start + i + 1] : -1;
+}
+__device__ __forceinline__ Chosen chosen_row(const Verify &a, const Board &b, int seq, int start, int n, int first, int at) {
+    Chosen c{b.row_sum[0][at], b.row_sum[1][at], b.row_m[0][at], b.row_m[1][at], start + first, -1, a.out + (int64_t)seq * a.most + first};
+    if (first < n - 1) {
+        const int64_t token = a.tokens[c.row + 1];
+        c.draft = token >= 0 && token < a.vocab ? (int)token : -2;
+    }
+    return c;
+}
+
 template <int kType>
-__global__ __launch_bounds__(kThreads) void draw_kernel(const Verify a) {
-    constexpr int kVec = Row<kType>::kVec, kEach = kSpan / kThreads;
-    __shared__ double table[32], sums[kWaves], below_at;
-    __shared__ int block_at, token, fallback, of_rest;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seq = blockIdx.x;
-    const Chosen c = a.chosen[seq];
-    if (c.row < 0) return;
+__global__ __launch_bounds__(kThreads) void greedy_kernel(const Verify a) {
+    __shared__ Board board;
+    const int seq = blockIdx.x;
+    int start, n, base;
+    rows_of(a, seq, start, n);
+    if (n == 0) return nothing(a, seq);
+    const int first = first_refused<kType, kGreedy>(a, Exp2(nullptr, 0.0), board, start, n, base);
+    write_taken(a, seq, start, first);
+    if (threadIdx.x == 0) a.out[(int64_t)seq * a.most + first] = board.best[first - base];
+}
+
+// ---- with the drafter's logits: blockIdx.y for a sequence, .x for a block of the row that its token is drawn from
+template <int kType>
+__global__ __launch_bounds__(kThreads) void rest_kernel(const Verify a) {
+    __shared__ Board board;
+    __shared__ double table[32], sums[2][kWaves];
+    const int tid = threadIdx.x, seq = blockIdx.y;
+    int start, n, base;
+    rows_of(a, seq, start, n);
     fill_table(table);
-    const Left *left = a.left + (int64_t)seq * a.blocks;
-    const double u = a.sample[seq];
-    if (wave == 0) {
-        double rest = 0.0, all = 0.0;
-        for (int i = lane; i < a.blocks; i += 64) {
-            rest += left[i].rest;
-            all += left[i].all;
+    if (n == 0) {
+        if (blockIdx.x == 0) {
+            nothing(a, seq);
+            if (tid == 0) a.chosen[seq].row = -1;
         }
-        rest = wave_sum(rest);
-        all = wave_sum(all);
-        const bool use = rest > 0.0;  // (the drafter's share is all of it where roundings make it so)
-        const double limit = u * (use ? rest : all);
-        double before = 0.0, below = 0.0;
-        int found = -1, last = -1;
-        for (int base = 0; base < a.blocks && found < 0; base += 64) {
-            const int i = base + lane;
-            const double x = i < a.blocks ? (use ? left[i].rest : left[i].all) : 0.0;
-            double upto = x;
+        return;
+    }
+    const Exp2 power(table, a.c);
+    const int first = first_refused<kType, kBoth>(a, power, board, start, n, base);
+    const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
+    const Rest<kType, true> rest(a, power, c);
+    constexpr int kVec = Row<kType>::kVec;
+    const int begin = blockIdx.x * kBlock, end = min(begin + kBlock, a.vocab);
+    double mine = 0.0, whole = 0.0;
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(upto, o);
-                if (lane >= o) upto += y;
-            }
-            const uint64_t passed = __ballot(x > 0.0 && before + upto > limit), some = __ballot(x > 0.0);
-            if (passed) {
-                const int l = __builtin_ctzll(passed);
-                found = base + l;
-                below = before + (l ? __shfl(upto, l - 1) : 0.0);
-            } else if (some) {
-                last = base + 63 - __builtin_clzll(some);
-            }
-            before += __shfl(upto, 63);
-        }
-        if (lane == 0) {
-            block_at = found >= 0 ? found : last;
-            below_at = found >= 0 ? limit - below : __builtin_inf();  // none passed it: the last entry that is left
-            of_rest = use;
-            token = INT32_MAX;
-            fallback = -1;
+    for (int v = 0; v < kEach; v += kVec) {
+        const int j = begin + v * kThreads + tid * kVec;
+        if (j >= end) break;
+        double x[kVec], y[kVec];
+        rest.some(j, end, x, y);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            mine += x[i];
+            whole += y[i];
         }
     }
+    if (blockIdx.x == 0) {
+        write_taken(a, seq, start, first);
+        if (tid == 0) a.chosen[seq] = c;
+    }
+    mine = wave_sum(mine);
+    whole = wave_sum(whole);
+    if ((tid & 63) == 0) {
+        sums[0][tid >> 6] = mine;
+        sums[1][tid >> 6] = whole;
+    }
     __syncthreads();
-    const int block = block_at;
-    if (block < 0) {  // a row that is masked as a whole
+    if (tid == 0) {
+        Left l{0.0, 0.0};
+        for (int w = 0; w < kWaves; ++w) {
+            l.rest += sums[0][w];
+            l.all += sums[1][w];
+        }
+        a.left[(int64_t)seq * a.blocks + blockIdx.x] = l;
+    }
+}
+
+struct Draw {  // in shared memory
+    double sums[kWaves], below;
+    int part, of_rest, first[kWaves], last[kWaves];
+};
+
+// The part of a row in which the sum passes the number, of parts whose sums one wave has in its lanes (part(i): of what is left, and of all), and how
+// much of the number is left in it. Where roundings leave none, the last one that has any; -1: no part has any.
+template <typename Part>
+__device__ __forceinline__ void find_part(Draw &d, int parts, double u, const Part &part) {
+    const int lane = threadIdx.x & 63;
+    double rest = 0.0, all = 0.0;
+    for (int i = lane; i < parts; i += 64) {
+        const Left l = part(i);
+        rest += l.rest;
+        all += l.all;
+    }
+    rest = wave_sum(rest);
+    const bool use = rest > 0.0;  // (the drafter's share is all of it where roundings make it so)
+    if (!use) rest = wave_sum(all);
+    const double limit = u * rest;
+    double before = 0.0, below = 0.0;
+    int found = -1, last = -1;
+    for (int base = 0; base < parts && found < 0; base += 64) {
+        Left l{0.0, 0.0};
+        if (base + lane < parts) l = part(base + lane);
+        const double x = use ? l.rest : l.all, upto = wave_scan(x);
+        const uint64_t passed = __ballot(x > 0.0 && before + upto > limit), some = __ballot(x > 0.0);
+        if (passed) {
+            const int i = __builtin_ctzll(passed);
+            found = base + i;
+            below = before + (i ? at_lane(upto, i - 1) : 0.0);
+        } else if (some) {
+            last = base + 63 - __builtin_clzll(some);
+        }
+        before += at_lane(upto, 63);
+    }
+    if (lane == 0) {
+        d.part = found >= 0 ? found : last;
+        d.below = found >= 0 ? limit - below : __builtin_inf();  // none passed it: the last entry that is left
+        d.of_rest = use;
+    }
+}
+
+// The entry of begin .. end - 1 at which the sum passes what is left of the number, or the last one that has any
+template <int kType, bool kQ>
+__device__ __forceinline__ void find_entry(Draw &d, const Rest<kType, kQ> &rest, int begin, int end, int64_t *to) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const bool of_rest = d.of_rest;
+    const double below = d.below;
+    double before = 0.0;
+    int token = -1;
+    for (int at = begin; at < end; at += kBlock) {
+        const int j0 = at + tid * kEach;
+        double x[kEach], all[kEach], mine = 0.0;
+        rest.some(j0, end, x, all);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (!of_rest) x[i] = all[i];
+            mine += x[i];
+        }
+        const double upto = wave_scan(mine);
+        if (lane == 63) d.sums[wave] = upto;
+        __syncthreads();
+        double run = before + (upto - mine);
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) run += d.sums[w];
+            before += d.sums[w];
+        }
+        int first = -1, last = -1;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            run += x[i];
+            if (x[i] > 0.0) {
+                last = j0 + i;
+                if (run > below && first < 0) first = j0 + i;
+            }
+        }
+        // the lowest of the first ones, the highest of the last ones: entries go up with the lanes and the waves
+        const uint64_t passed = __ballot(first >= 0), some = __ballot(last >= 0);
+        if (lane == 0) {
+            d.first[wave] = passed ? __builtin_amdgcn_readlane(first, __builtin_ctzll(passed)) : -1;
+            d.last[wave] = some ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(some)) : -1;
+        }
+        __syncthreads();
+        bool done = false;
+        for (int w = 0; w < kWaves && !done; ++w) {
+            if (d.first[w] >= 0) {
+                token = d.first[w];
+                done = true;
+            } else if (d.last[w] >= 0) {
+                token = d.last[w];
+            }
+        }
+        if (done) break;
+    }
+    if (tid == 0) *to = token;
+}
+
+template <int kType>
+__global__ __launch_bounds__(kThreads) void draw_kernel(const Verify a) {
+    __shared__ double table[32];
+    __shared__ Draw draw;
+    const int seq = blockIdx.x;
+    const Chosen c = a.chosen[seq];
+    const Left *left = a.left + (int64_t)seq * a.blocks;
+    fill_table(table);
+    if (c.row < 0) return;
+    if (threadIdx.x < 64) find_part(draw, a.blocks, a.sample[seq], [&](int i) { return left[i]; });
+    __syncthreads();
+    if (draw.part < 0) {  // a row that is masked as a whole
+        if (threadIdx.x == 0) *c.to = -1;
+        return;
+    }
+    const int begin = draw.part * kBlock;
+    find_entry(draw, Rest<kType, true>(a, Exp2(table, a.c), c), begin, min(begin + kBlock, a.vocab), c.to);
+}
+
+// ---- without them: a workgroup for a sequence
+template <int kType>
+__global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
+    __shared__ Board board;
+    __shared__ double table[32];
+    __shared__ Draw draw;
+    const int tid = threadIdx.x, seq = blockIdx.x;
+    int start, n, base;
+    rows_of(a, seq, start, n);
+    fill_table(table);
+    if (n == 0) return nothing(a, seq);
+    const double u = a.sample[seq];
+    const Exp2 power(table, a.c);
+    const int first = first_refused<kType, kAlone>(a, power, board, start, n, base);
+    const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
+    write_taken(a, seq, start, first);
+    const Rest<kType, false> rest(a, power, c);
+    // the slice that had the draft, without it
+    const int without = c.draft >= 0 ? c.draft / a.span : -1;
+    if (without >= 0) {
+        const int end = min((without + 1) * a.span, a.vocab);
+        double mine = 0.0;
+        for (int j = without * a.span + tid * kEach; j < end; j += kBlock) {
+            double x[kEach], all[kEach];
+            rest.some(j, end, x, all);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) mine += x[i];
+        }
+        mine = wave_sum(mine);
+        if ((tid & 63) == 0) draw.sums[tid >> 6] = mine;
+        __syncthreads();
+    }
+    if (tid < 64) {
+        double other = 0.0;
+        if (without >= 0)
+            for (int w = 0; w < kWaves; ++w) other += draw.sums[w];
+        const Stat *s = a.stats + (int64_t)c.row * 2 * a.slices;
+        find_part(draw, a.slices, u, [&](int i) {
+            const double all = s[i].sum * power(s[i].m, rest.p_m) * rest.p_by;
+            return Left{i == without ? other : all, all};
+        });
+    }
+    __syncthreads();
+    if (draw.part < 0) {
         if (tid == 0) *c.to = -1;
         return;
     }
-    const Exp2 power{table, a.c};
-    const Rest<kType> rest(a, power, c);
-    const int begin = block * kSpan, end = min(begin + kSpan, a.vocab), j0 = begin + tid * kEach;
-    double x[kEach], mine = 0.0;
-#pragma unroll
-    for (int v = 0; v < kEach; v += kVec) {
-        double r[kVec], all[kVec];
-        rest.some(j0 + v, end, r, all);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            x[v + i] = of_rest ? r[i] : all[i];
-            mine += x[v + i];
-        }
-    }
-    double upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(upto, o);
-        if (lane >= o) upto += y;
-    }
-    if (lane == 63) sums[wave] = upto;
-    __syncthreads();
-    double run = upto - mine;
-    for (int w = 0; w < wave; ++w) run += sums[w];
-    int first = INT32_MAX, last = -1;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        run += x[i];
-        if (x[i] > 0.0) {
-            last = j0 + i;
-            if (run > below_at && first == INT32_MAX) first = j0 + i;
-        }
-    }
-    if (first != INT32_MAX) atomicMin(&token, first);
-    if (last >= 0) atomicMax(&fallback, last);
-    __syncthreads();
-    if (tid == 0) *c.to = token != INT32_MAX ? token : fallback;
+    const int begin = draw.part * a.span;
+    find_entry(draw, rest, begin, min(begin + a.span, a.vocab), c.to);
 }
+
+constexpr int kPiece = 2048;  // entries of the smallest slice
 
 struct Plan {
     int slices, span, blocks;
@@ -494,12 +702,11 @@ struct Plan {
 
 Plan plan_of(int64_t batch, int64_t rows, int64_t vocab, bool greedy, bool draft, int cus) {
     Plan p{};
-    p.blocks = (int)((vocab + kSpan - 1) / kSpan);
-    const int64_t items = rows * (draft && !greedy ? 2 : 1), wanted = ((int64_t)cus * 8 + items - 1) / items;
-    int64_t per = (p.blocks + wanted - 1) / wanted;
-    p.span = (int)(per * kSpan);
+    p.blocks = draft && !greedy ? (int)((vocab + kBlock - 1) / kBlock) : 0;
+    const int64_t items = rows * (draft && !greedy ? 2 : 1), wanted = ((int64_t)cus * 4 + items - 1) / items, pieces = (vocab + kPiece - 1) / kPiece;
+    p.span = (int)(std::min((pieces + wanted - 1) / wanted, (int64_t)4) * kPiece);
     p.slices = (int)((vocab + p.span - 1) / p.span);
-    p.bytes = rows * 2 * p.slices * (int64_t)sizeof(Stat) + (greedy ? 0 : batch * (p.blocks * (int64_t)sizeof(Left) + (int64_t)sizeof(Chosen)));
+    p.bytes = rows * 2 * p.slices * (int64_t)sizeof(Stat) + (p.blocks ? batch * (p.blocks * (int64_t)sizeof(Left) + (int64_t)sizeof(Chosen)) : 0);
     return p;
 }
 
@@ -511,18 +718,22 @@ int sizes(int64_t batch, int64_t rows, int64_t vocab) {
 
 template <int kType>
 int launch(const Verify &a, bool greedy, hipStream_t s) {
-    const dim3 grid((unsigned)a.slices, (unsigned)a.rows, a.draft && !greedy ? 2u : 1u), decide(greedy ? 1u : (unsigned)a.blocks, (unsigned)a.batch);
     if (a.rows) {
-        if (greedy) stats_kernel<kType, true><<<grid, kThreads, 0, s>>>(a);
-        else stats_kernel<kType, false><<<grid, kThreads, 0, s>>>(a);
+        const dim3 grid((unsigned)a.slices, (unsigned)a.rows, a.draft ? 2u : 1u);
+        if (greedy) stats_kernel<kType, true><<<grid, kStats, 0, s>>>(a);
+        else stats_kernel<kType, false><<<grid, kStats, 0, s>>>(a);
         if (const int rc = lq_check_launch("verify_drafts (rows)")) return rc;
     }
-    if (greedy) decide_kernel<kType, true><<<decide, kThreads, 0, s>>>(a);
-    else decide_kernel<kType, false><<<decide, kThreads, 0, s>>>(a);
-    if (const int rc = lq_check_launch("verify_drafts")) return rc;
-    if (greedy) return LQ_OK;
-    draw_kernel<kType><<<(unsigned)a.batch, kThreads, 0, s>>>(a);
-    return lq_check_launch("verify_drafts (draw)");
+    if (greedy) {
+        greedy_kernel<kType><<<(unsigned)a.batch, kThreads, 0, s>>>(a);
+    } else if (!a.draft) {
+        alone_kernel<kType><<<(unsigned)a.batch, kThreads, 0, s>>>(a);
+    } else {
+        rest_kernel<kType><<<dim3((unsigned)a.blocks, (unsigned)a.batch), kThreads, 0, s>>>(a);
+        if (const int rc = lq_check_launch("verify_drafts")) return rc;
+        draw_kernel<kType><<<(unsigned)a.batch, kThreads, 0, s>>>(a);
+    }
+    return lq_check_launch("verify_drafts");
 }
 
 }  // namespace
