@@ -69,14 +69,14 @@ def run(shared, own, news, heads, kv_heads, dim, dtype, seed=0, split=True, lens
 def test_one_token(hip_lib, heads, kv_heads, batch, dim, dtype):
     """Rows of the prefix for every form of the kernel (to 16, to 64, more), own keys around the tiles of 64."""
     own = ([1, 2, 63, 64, 65, 127, 300] * 6)[:batch]
-    run(8, own, [1] * batch, heads, kv_heads, dim, dtype, seed=dim + heads)
+    run(14, own, [1] * batch, heads, kv_heads, dim, dtype, seed=dim + heads)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("dim", [64, 96, 128, 256])
 @pytest.mark.parametrize("tokens, group, batch", [(2, 1, 3), (5, 3, 2), (8, 2, 9), (3, 4, 30), (8, 8, 2), (33, 1, 2), (64, 1, 3)])
 def test_few_tokens(hip_lib, tokens, group, batch, dim, dtype):
-    run(9, ([tokens, tokens + 1, 64 + tokens, 257] * 8)[:batch], [tokens] * batch, 2 * group, 2, dim, dtype, seed=tokens)
+    run(15, ([tokens, tokens + 1, 64 + tokens, 257] * 8)[:batch], [tokens] * batch, 2 * group, 2, dim, dtype, seed=tokens)
 
 
 @pytest.mark.parametrize("how", [{}, {"causal": False}, {"scale": 0.3}])
@@ -85,17 +85,17 @@ def test_sequences_of_all_lengths(hip_lib, batch, how):
     """Different numbers of new tokens, none among them; sequences shorter than what they share, to nothing at all, and rows before position 0."""
     rng = np.random.default_rng(batch)
     news = [int(n) for n in rng.integers(0, 6, batch)]
-    lens = [int(n) for n in rng.integers(0, 900, batch)]
-    news[0], lens[0] = 5, 5 * 64
+    lens = [int(n) for n in rng.integers(0, 1500, batch)]
+    news[0], lens[0] = 5, 14 * 64
     news[1], lens[1] = 3, 0
     if batch > 2:
         news[2], lens[2] = 4, 2
-        news[-1], lens[-1] = 2, 5 * 64 + 1
-    run(5, None, news, 8, 2, 64, BF16, seed=batch, lens=lens, **how)
-    run(5, None, news, 3, 3, 128, F16, seed=batch, lens=lens, **how)
+        news[-1], lens[-1] = 2, 14 * 64 + 1
+    run(14, None, news, 8, 2, 64, BF16, seed=batch, lens=lens, **how)
+    run(14, None, news, 3, 3, 128, F16, seed=batch, lens=lens, **how)
 
 
-@pytest.mark.parametrize("shared, width", [(1, 9), (2, 9), (63, 70), (64, 66), (65, 66), (300, 301)])
+@pytest.mark.parametrize("shared, width", [(14, 20), (15, 16), (16, 19), (63, 70), (64, 66), (65, 66), (300, 301)])
 @pytest.mark.parametrize("dim, batch", [(128, 3), (64, 30), (96, 70)])
 def test_shared_lengths(hip_lib, shared, width, dim, batch):
     run(shared, [1 + i % 60 for i in range(batch)], [1] * batch, 4, 2, dim, BF16, seed=shared, width=width)
@@ -103,13 +103,13 @@ def test_shared_lengths(hip_lib, shared, width, dim, batch):
 
 def test_nothing_of_their_own(hip_lib):
     """Rows that are in the shared blocks themselves, and a table with no other columns."""
-    run(4, None, [3, 3, 3], 4, 2, 64, BF16, lens=[256, 200, 3])
-    run(4, None, [1, 2], 4, 2, 128, F16, lens=[256, 2])
+    run(14, None, [3, 3, 3], 4, 2, 64, BF16, lens=[896, 700, 3])
+    run(14, None, [1, 2], 4, 2, 128, F16, lens=[896, 2])
 
 
-@pytest.mark.parametrize("shared, batch, tokens, heads", [(0, 3, 1, 4), (5, 1, 3, 4), (5, 2, 17, 8)])
+@pytest.mark.parametrize("shared, batch, tokens, heads", [(0, 3, 1, 4), (5, 1, 3, 4), (5, 2, 17, 8), (5, 4, 1, 4)])
 def test_left_to_ordinary_attention(hip_lib, shared, batch, tokens, heads):
-    """Nothing shared, nobody to share with, and rows enough in every sequence: as kv8_attention gives it, bit for bit."""
+    """Nothing shared, nobody to share with, rows enough in every sequence, and little to be shared: as kv8_attention gives it, bit for bit."""
     from latentq_llm_amd import ops
     lens = [400] * batch
     cache = ref.Cache(40, 2, 64, seed=3)
@@ -132,7 +132,7 @@ def test_scales_far_apart(hip_lib, dim, batch):
         c.scale[0][rng.random(c.scale[0].shape) < 0.2] = 0.0
         c.scale[0][0] *= 8
         return c
-    run(7, [1 + 37 * (i % 5) for i in range(batch)], [1] * batch, 4, 2, dim, BF16, seed=dim + batch, cache=cache)
+    run(14, [1 + 37 * (i % 5) for i in range(batch)], [1] * batch, 4, 2, dim, BF16, seed=dim + batch, cache=cache)
 
 
 def test_scores_far_apart(hip_lib):
@@ -142,11 +142,11 @@ def test_scores_far_apart(hip_lib):
         c.scale[0] *= np.float32(30) * np.random.default_rng(3).random(c.scale[0].shape).astype(np.float32)
         return c
     for batch in (3, 40, 90):
-        run(6, [1 + 11 * i for i in range(batch)], [1] * batch, 2, 1, 128, F16, seed=5, cache=cache)
+        run(14, [1 + 11 * i for i in range(batch)], [1] * batch, 2, 1, 128, F16, seed=5, cache=cache)
 
 
 def test_strides_and_a_given_output(hip_lib):
-    lens, shared, heads, dim = [900, 700, 640], 10, 4, 128
+    lens, shared, heads, dim = [1160, 960, 900], 14, 4, 128
     cache = ref.Cache(30, 2, dim, seed=9)
     table = table_of(lens, shared, 30, 9)
     q = rows((6, heads, dim), BF16, 10)
@@ -166,7 +166,7 @@ def test_strides_and_a_given_output(hip_lib):
 
 def test_rows_that_no_sequence_has(hip_lib):
     """Rows behind the last sequence, and beyond max_tokens of one, are left as they were."""
-    lens, news, shared = [700, 400, 330], [2, 0, 3], 5
+    lens, news, shared = [1276, 976, 906], [2, 0, 3], 14
     cache = ref.Cache(30, 2, 64, seed=11)
     table, q = table_of(lens, shared, 30, 11), rows((9, 4, 64), BF16, 12)
     want, _, bound = ref.attention(cache, q[:5], table, lens, news)
@@ -182,8 +182,8 @@ def test_rows_that_no_sequence_has(hip_lib):
 
 def test_bounds_that_are_too_small(hip_lib):
     """A max_len below the sequences' lengths costs time, not correctness: below their shared blocks, too."""
-    for max_len in (1, 64, 300, 320, 400):
-        run(5, [300, 100, 20, 64], [1] * 4, 4, 2, 64, BF16, seed=13, max_len=max_len, split=True)
+    for max_len in (1, 64, 890, 896, 900, 1000):
+        run(14, [300, 100, 20, 64], [1] * 4, 4, 2, 64, BF16, seed=13, max_len=max_len, split=max_len > 832)
 
 
 def test_what_the_device_holds_is_kept_inside(hip_lib):
@@ -191,17 +191,17 @@ def test_what_the_device_holds_is_kept_inside(hip_lib):
     cache = ref.Cache(12, 2, 64, seed=14)
     q = rows((8, 4, 64), BF16, 15)
     t = cache.tensors()
-    table = table_of([400] * 4, 3, 40, 14)
-    table[:, 1], table[2, 5], table[3, 4] = 1 << 30, -5, 99
-    for lens in ([400] * 4, [2 ** 31 - 1, -2 ** 31, 449, -1]):
+    table = table_of([1104] * 4, 14, 40, 14)
+    table[:, 1], table[2, 16], table[3, 15] = 1 << 30, -5, 99
+    for lens in ([1104] * 4, [2 ** 31 - 1, -2 ** 31, 1153, -1]):
         for cu in (None, [0, 2, 4, 6, 8], [-9, 1 << 30, 3, 2, 8], [8, 0, 8, 0, 8]):
-            out = call(t, q, table, lens, [2] * 4, 3, cu_tokens=None if cu is None else i32(cu))
+            out = call(t, q, table, lens, [2] * 4, 14, cu_tokens=None if cu is None else i32(cu))
             assert out.shape == q.shape
 
 
 def test_another_stream_and_graphs(hip_lib):
     from latentq_llm_amd import ops
-    lens, shared = [900, 1200, 700, 641, 650], 10
+    lens, shared = [1156, 1456, 956, 897, 906], 14
     cache = ref.Cache(60, 4, 128, seed=16)
     t, table = cache.tensors(), i32(table_of(lens, shared, 60, 16))
     length = i32(lens)
