@@ -38,102 +38,105 @@ __device__ __forceinline__ int holder(const int *at, int n, int x) {
     return lo;
 }
 
-// Position and slot of a row, or 0 and -1 behind the last sequence's
-__device__ __forceinline__ void place_row(const Resize &a, const int *at_row, int row) {
-    int64_t position = 0, slot = -1;
-    if (row < at_row[a.batch]) {
-        const int i = holder(at_row, a.batch, row);
-        position = (int64_t)a.lens[i] - (at_row[i + 1] - row);
-        slot = (int64_t)a.table[(int64_t)i * a.width + position / KV8_BLOCK] * KV8_BLOCK + position % KV8_BLOCK;
-    }
+__device__ __forceinline__ void write_row(const Resize &a, int row, int64_t position, int64_t block) {
     a.positions[row] = position;
-    a.slots[row] = slot;
+    a.slots[row] = block * KV8_BLOCK + position % KV8_BLOCK;
+}
+__device__ __forceinline__ void write_no_row(const Resize &a, int row) {
+    a.positions[row] = 0;
+    a.slots[row] = -1;
 }
 
 struct Sums {
     int64_t more, less, rows;
+    __device__ __forceinline__ Sums operator+(const Sums &s) const { return Sums{more + s.more, less + s.less, rows + s.rows}; }
+    __device__ __forceinline__ Sums operator-(const Sums &s) const { return Sums{more - s.more, less - s.less, rows - s.rows}; }
 };
 
-// Inclusive sums over the lanes of a wave
-__device__ __forceinline__ Sums scanned(Sums s) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t more = __shfl_up(s.more, o), less = __shfl_up(s.less, o), rows = __shfl_up(s.rows, o);
-        if (lane >= o) {
-            s.more += more;
-            s.less += less;
-            s.rows += rows;
-        }
-    }
-    return s;
+// Sums up to each lane of a wave, by lane shifts (row_shr:1, 2, 4, 8, row_bcast:15 and 31)
+template <int kShift, int kRows>
+__device__ __forceinline__ int64_t plus(int64_t x) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)x, kShift, kRows, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), kShift, kRows, 0xf, false);
+    return x + (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t scanned(int64_t x) {
+    return plus<0x143, 0xc>(plus<0x142, 0xa>(plus<0x118, 0xf>(plus<0x114, 0xf>(plus<0x112, 0xf>(plus<0x111, 0xf>(x))))));
+}
+__device__ __forceinline__ int64_t last_lane(int64_t x) {
+    const unsigned lo = __builtin_amdgcn_readlane((int)x, 63), hi = __builtin_amdgcn_readlane((int)(x >> 32), 63);
+    return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 template <int kThreads, int kMost>
 __global__ __launch_bounds__(kThreads) void resize_kernel(const Resize a) {
     constexpr int kWaves = kThreads / 64;
-    __shared__ int at_more[kMost + 1], at_less[kMost + 1], at_row[kMost + 1], base[kMost];
+    __shared__ int at_more[kMost + 1], at_less[kMost + 1], at_row[kMost + 1], base[kMost], after[kMost];
     __shared__ Sums of_wave[kWaves];
-    __shared__ int wide;
+    __shared__ int wide[kWaves];
     const int tid = threadIdx.x, wave = tid >> 6;
-    const int per = (a.batch + kThreads - 1) / kThreads, begin = min(tid * per, a.batch), end = min(begin + per, a.batch);
-    const int count = *a.free_count;
-    if (tid == 0) wide = 0;
-    if constexpr (kWaves > 1) __syncthreads();
+    const int per = kMost == kThreads ? 1 : (a.batch + kThreads - 1) / kThreads, begin = min(tid * per, a.batch), end = min(begin + per, a.batch);
 
     struct Part {
         int have, need;
         int64_t after, rows;
     };
     const auto part = [&](int i) {
-        const int64_t len = max(a.lens[i], 0), after = max(len + a.change[i], (int64_t)0);
+        const int64_t len = max(a.lens[i], 0), to = max(len + a.change[i], (int64_t)0);
         const auto blocks = [&](int64_t n) { return max((int)((n + KV8_BLOCK - 1) / KV8_BLOCK), a.shared); };
-        return Part{blocks(len), blocks(after), after, max(after - len, (int64_t)0)};
+        return Part{blocks(len), blocks(to), to, max(to - len, (int64_t)0)};
     };
+    const auto sums = [](const Part &p) { return Sums{max(p.need - p.have, 0), max(p.have - p.need, 0), p.rows}; };
+    const int count = *a.free_count;
     Sums mine{0, 0, 0};
+    Part first{0, 0, 0, 0};
+    bool too_wide = false;
     for (int i = begin; i < end; ++i) {
         const Part p = part(i);
-        if (max(p.have, p.need) > a.width) wide = 1;
-        mine.more += max(p.need - p.have, 0);
-        mine.less += max(p.have - p.need, 0);
-        mine.rows += p.rows;
+        if (i == begin) first = p;
+        too_wide |= max(p.have, p.need) > a.width;
+        mine = mine + sums(p);
     }
-    Sums upto = scanned(mine);
-    if ((tid & 63) == 63) of_wave[wave] = upto;
-    __syncthreads();
-    Sums all{0, 0, 0};
+    Sums upto{scanned(mine.more), scanned(mine.less), scanned(mine.rows)};
+    Sums all{last_lane(upto.more), last_lane(upto.less), last_lane(upto.rows)};
+    bool any_wide = __any(too_wide);
+    if constexpr (kWaves > 1) {
+        if ((tid & 63) == 0) {
+            of_wave[wave] = all;
+            wide[wave] = any_wide;
+        }
+        __syncthreads();
+        all = Sums{0, 0, 0};
+        any_wide = false;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wave) upto = Sums{upto.more + all.more, upto.less + all.less, upto.rows + all.rows};
-        all = Sums{all.more + of_wave[w].more, all.less + of_wave[w].less, all.rows + of_wave[w].rows};
+        for (int w = 0; w < kWaves; ++w) {
+            if (w == wave) upto = upto + all;
+            all = all + of_wave[w];
+            any_wide |= wide[w];
+        }
     }
     // what cannot be done is not begun
     int status = 0;
-    if (wide) status = LQ_KV_NARROW;
+    if (any_wide) status = LQ_KV_NARROW;
     else if (all.rows > a.limit) status = LQ_KV_ROWS;
     else if (count < 0 || (int64_t)count + all.less > a.capacity) status = LQ_KV_LIST;
     else if (all.more > (int64_t)count + all.less) status = (int)(all.more - all.less - count);
     if (tid == 0) *a.status = status;
     if (status) {
         for (int i = tid; i <= a.batch; i += kThreads) a.cu[i] = 0;
-        for (int row = tid; row < a.rows; row += kThreads) {
-            a.positions[row] = 0;
-            a.slots[row] = -1;
-        }
+        for (int row = tid; row < a.rows; row += kThreads) write_no_row(a, row);
         return;
     }
-    Sums s{upto.more - mine.more, upto.less - mine.less, upto.rows - mine.rows};
+    Sums s = upto - mine;
     for (int i = begin; i < end; ++i) {
-        const Part p = part(i);
+        const Part p = i == begin ? first : part(i);
         at_more[i] = (int)s.more;
         at_less[i] = (int)s.less;
         at_row[i] = (int)s.rows;
         base[i] = min(p.have, p.need);
+        after[i] = (int)p.after;
         a.cu[i] = (int)s.rows;
         a.lens[i] = (int)p.after;  // (the thread's own)
-        s.more += max(p.need - p.have, 0);
-        s.less += max(p.have - p.need, 0);
-        s.rows += p.rows;
+        s = s + sums(p);
     }
     const int more = (int)all.more, less = (int)all.less, top = count + less - 1;
     if (tid == 0) {
@@ -147,12 +150,22 @@ __global__ __launch_bounds__(kThreads) void resize_kernel(const Resize a) {
         const int i = holder(at, a.batch, r);
         return a.table + (int64_t)i * a.width + base[i] + (r - at[i]);
     };
-    for (int r = tid; r < less; r += kThreads) a.free_blocks[top - r] = *entry(at_less, r);
-    if (less) __syncthreads();
+    if (less) {
+        for (int r = tid; r < less; r += kThreads) a.free_blocks[top - r] = *entry(at_less, r);
+        __syncthreads();  // what is given back may be taken
+    }
     for (int r = tid; r < more; r += kThreads) *entry(at_more, r) = a.free_blocks[top - r];
-    if (a.rows == 0) return;
-    __syncthreads();
-    for (int row = tid; row < a.rows; row += kThreads) place_row(a, at_row, row);
+    // A row's block is one that its sequence had, or is being taken: from the list in that case, which does not wait for the table
+    for (int row = tid; row < a.rows; row += kThreads) {
+        if (row < at_row[a.batch]) {
+            const int i = holder(at_row, a.batch, row);
+            const int64_t position = (int64_t)after[i] - (at_row[i + 1] - row);
+            const int block = (int)(position / KV8_BLOCK), taken = block - base[i];
+            write_row(a, row, position, taken >= 0 ? a.free_blocks[top - (at_more[i] + taken)] : a.table[(int64_t)i * a.width + block]);
+        } else {
+            write_no_row(a, row);
+        }
+    }
 }
 
 // Positions and slots of many rows, after the lengths and tables
@@ -160,7 +173,15 @@ __global__ __launch_bounds__(256) void rows_kernel(const Resize a) {
     __shared__ int at_row[kMostSequences + 1];
     for (int i = threadIdx.x; i <= a.batch; i += 256) at_row[i] = a.cu[i];
     __syncthreads();
-    for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) place_row(a, at_row, (int)row);
+    for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
+        if (row < at_row[a.batch]) {
+            const int i = holder(at_row, a.batch, (int)row);
+            const int64_t position = (int64_t)a.lens[i] - (at_row[i + 1] - row);
+            write_row(a, (int)row, position, a.table[(int64_t)i * a.width + position / KV8_BLOCK]);
+        } else {
+            write_no_row(a, (int)row);
+        }
+    }
 }
 
 }  // namespace
@@ -182,7 +203,9 @@ extern "C" int lq_kv8_resize(int32_t *block_table, int64_t table_width, int32_t 
     Resize a{block_table, seq_lens, free_blocks, free_count, change, cu_tokens, positions, slots, status, rows < 0 ? INT32_MAX : rows,
              (int)table_width, (int)capacity, (int)batch, (int)shared, rows > 0 && rows <= kFewRows ? (int)rows : 0};
     hipStream_t s = (hipStream_t)stream;
-    resize_kernel<1024, kMostSequences><<<1, 1024, 0, s>>>(a);
+    if (batch <= 64 && a.rows <= 256) resize_kernel<64, 64><<<1, 64, 0, s>>>(a);
+    else if (batch <= 256 && a.rows <= 1024) resize_kernel<256, 256><<<1, 256, 0, s>>>(a);
+    else resize_kernel<1024, kMostSequences><<<1, 1024, 0, s>>>(a);
     if (const int rc = lq_check_launch("kv8_resize")) return rc;
     if (rows <= kFewRows) return LQ_OK;
     a.rows = (int)rows;
