@@ -103,6 +103,17 @@ at::Tensor make_rows(const at::Tensor &x, int64_t last, at::ScalarType type) {
     return make(shape, type, x);
 }
 
+// Several results of a call in one allocation, each a tensor by itself: an allocation is a microsecond of the host's time. `at`: the bytes before it,
+// moved past it; those of 8 bytes an element first.
+at::Tensor take(const at::Tensor &bytes, int64_t &at, at::IntArrayRef shape, at::ScalarType type) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(), c10::scalarTypeToTypeMeta(type));
+    const int64_t size = (int64_t)c10::elementSize(type);
+    t.unsafeGetTensorImpl()->set_storage_offset(at / size);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    at += c10::multiply_integers(shape) * size;
+    return t;
+}
+
 // Token rows of an operand whose last dimension is `width`: 0 if there are none or the width differs
 int64_t rows_of(const at::Tensor *x, int64_t width) {
     return x && x->dim() >= 1 && width > 0 && x->size(-1) == width ? x->numel() / width : 0;
@@ -773,9 +784,9 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
 }
 
-// q, cache (4), block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse, workspace -> as kv8_attention
+// q, cache (4), block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse -> out, or (out, lse)
 PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    LQ_ARGS(15)
+    LQ_ARGS(14)
     if (watched()) return none();
     Rows16 q;
     Cache8 c;
@@ -793,23 +804,19 @@ PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     const double scale = a[11] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(a[11]);
     const int causal = PyObject_IsTrue(a[12]), with_lse = PyObject_IsTrue(a[13]);
     if (PyErr_Occurred() || !(scale > 0.0 && scale <= 3.4e38) || shared < 0 || shared > s.width) return none();
-    void *ws;
-    int64_t ws_bytes;
-    if (!workspace(a[14], q.t, &ws, &ws_bytes)) return none();
     On on(*c.kc);
-    if (!ws) {
-        int prefix, own;
-        int64_t needed;
-        if (const int rc = lq_kv8_attention_shared_plan(s.batch, tokens, s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, shared, kWorkspaceBytes, 0, &prefix, &own, &needed))
-            return fail("lq_kv8_attention_shared_plan", rc);
-        if (needed) return PyLong_FromLongLong(needed);
-    }
+    int prefix, own;
+    int64_t needed;
+    if (const int rc = lq_kv8_attention_shared_plan(s.batch, tokens, s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, shared, kWorkspaceBytes, 0, &prefix, &own, &needed))
+        return fail("lq_kv8_attention_shared_plan", rc);
+    at::Tensor ws;
+    if (needed) ws = make({needed}, at::kByte, *q.t);
     at::Tensor out = make(q.t->sizes(), q.t->scalar_type(), *q.t), lse;
     if (with_lse) lse = make({tokens, heads}, at::kFloat, *q.t);
     LQ_CALL(lq_kv8_attention_shared, q.t->data_ptr(), q.t->stride(0), q.t->stride(1), c.kc->data_ptr(), c.vc->data_ptr(), (const float *)c.ks->data_ptr(),
             (const float *)c.vs->data_ptr(), c.blocks, (const int32_t *)s.table->data_ptr(), s.width, (const int32_t *)s.lens->data_ptr(), s.cu, s.batch, tokens,
             s.most, max_len, shared, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, out.data_ptr(), out.stride(0), out.stride(1),
-            with_lse ? (float *)lse.data_ptr() : nullptr, ws, ws_bytes, on.stream);
+            with_lse ? (float *)lse.data_ptr() : nullptr, needed ? ws.data_ptr() : nullptr, needed, on.stream);
     if (!with_lse) return wrap(std::move(out));
     return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
 }
@@ -845,11 +852,15 @@ PyObject *kv8_resize(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     const int64_t batch = t[0]->size(0), rows = a[5] == Py_None ? -1 : integer(a[5]), shared = integer(a[6]);
     if (PyErr_Occurred() || (a[5] != Py_None && rows < 0) || rows > INT32_MAX || shared < 0 || shared > t[0]->size(1)) return none();
     On on(*t[0]);
-    at::Tensor cu = make({batch + 1}, at::kInt, *t[0]), status = make({1}, at::kInt, *t[0]), positions, slots;
+    const int64_t n = std::max(rows, (int64_t)0);
+    const at::Tensor all = make({16 * n + 4 * (batch + 2)}, at::kByte, *t[0]);
+    int64_t at = 0;
+    at::Tensor positions, slots;
     if (rows >= 0) {
-        positions = make({rows}, at::kLong, *t[0]);
-        slots = make({rows}, at::kLong, *t[0]);
+        positions = take(all, at, {rows}, at::kLong);
+        slots = take(all, at, {rows}, at::kLong);
     }
+    at::Tensor cu = take(all, at, {batch + 1}, at::kInt), status = take(all, at, {1}, at::kInt);
     LQ_CALL(lq_kv8_resize, (int32_t *)t[0]->data_ptr(), t[0]->size(1), (int32_t *)t[1]->data_ptr(), (int32_t *)t[2]->data_ptr(), t[2]->size(0), (int32_t *)t[3]->data_ptr(),
             (const int32_t *)t[4]->data_ptr(), batch, shared, rows, (int32_t *)cu.data_ptr(), rows >= 0 ? (int64_t *)positions.data_ptr() : nullptr,
             rows >= 0 ? (int64_t *)slots.data_ptr() : nullptr, (int32_t *)status.data_ptr(), on.stream);
@@ -871,10 +882,9 @@ struct Logits {
     }
 };
 
-// logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws (None or tensors), temperature, batch, max_tokens (None), workspace -> (out, accepted);
-// without a workspace: the bytes that it needs, and nothing is done
+// logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws (None or tensors), temperature, batch, max_tokens (None) -> (out, accepted)
 PyObject *verify_drafts(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    LQ_ARGS(10)
+    LQ_ARGS(9)
     if (watched()) return none();
     Logits l, d;
     const at::Tensor *tokens = plain(a[1], at::kLong), *cu = nullptr, *accept = nullptr, *sample = nullptr;
@@ -903,20 +913,16 @@ PyObject *verify_drafts(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (a[4] != Py_None && (!(accept = plain(a[4], at::kFloat)) || accept->sizes() != at::IntArrayRef({rows}) || !same_device(accept, l.t))) return none();
     if (a[5] != Py_None && (!(sample = plain(a[5], at::kFloat)) || sample->sizes() != at::IntArrayRef({batch}) || !same_device(sample, l.t))) return none();
     if (draws && (!sample || (!accept && most > 1))) return none();
-    void *ws;
-    int64_t ws_bytes;
-    if (!workspace(a[9], l.t, &ws, &ws_bytes)) return none();
     On on(*l.t);
-    if (!ws) {
-        int slices;
-        int64_t needed;
-        if (const int rc = lq_verify_drafts_plan(batch, rows, vocab, !draws, d.t != nullptr, 0, &slices, &needed)) return fail("lq_verify_drafts_plan", rc);
-        return PyLong_FromLongLong(needed);
-    }
-    at::Tensor out = make({batch, most}, at::kLong, *l.t), accepted = make({batch}, at::kInt, *l.t);
+    int slices;
+    int64_t needed;
+    if (const int rc = lq_verify_drafts_plan(batch, rows, vocab, !draws, d.t != nullptr, 0, &slices, &needed)) return fail("lq_verify_drafts_plan", rc);
+    const at::Tensor all = make({8 * batch * most + 4 * batch}, at::kByte, *l.t), ws = make({needed}, at::kByte, *l.t);
+    int64_t at = 0;
+    at::Tensor out = take(all, at, {batch, most}, at::kLong), accepted = take(all, at, {batch}, at::kInt);
     LQ_CALL(lq_verify_drafts, l.t->data_ptr(), l.t->stride(0), d.t ? d.t->data_ptr() : nullptr, d.t ? d.t->stride(0) : 0, (const int64_t *)tokens->data_ptr(),
             cu ? (const int32_t *)cu->data_ptr() : nullptr, batch, rows, vocab, most, l.dtype, temperature, accept ? (const float *)accept->data_ptr() : nullptr,
-            sample ? (const float *)sample->data_ptr() : nullptr, (int64_t *)out.data_ptr(), (int32_t *)accepted.data_ptr(), ws, ws_bytes, on.stream);
+            sample ? (const float *)sample->data_ptr() : nullptr, (int64_t *)out.data_ptr(), (int32_t *)accepted.data_ptr(), ws.data_ptr(), needed, on.stream);
     return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(accepted)));
 }
 

@@ -1224,10 +1224,8 @@ def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq
     block_table are the same in every row. Their keys and values are read once for all rows. Arguments and results otherwise as
     kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
     if out is None:
-        args = (q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse)
-        r = (_native or _fast()).kv8_attention_shared(*args, None)
-        if type(r) is int:  # the bytes that its parts want
-            r = _native.kv8_attention_shared(*args, _workspace(q, 1, -(-r // 32))[0])
+        r = (_native or _fast()).kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal,
+                                                      return_lse)
         if r is not None:
             return r
     n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
@@ -1240,12 +1238,11 @@ def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq
         q = _kv8_layout(q)
         with torch.cuda.device(k_codes.device):
             needed = kv8_attention_shared_plan(batch, tokens, most, max_len, heads, kv_heads, dim, shared)[2]
-            keep, ws, ws_bytes = _workspace(q, 1, -(-needed // 32)) if needed else (None, None, 0)
+            ws = torch.empty(needed, dtype=torch.uint8, device=q.device)
             _C.call("lq_kv8_attention_shared", q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
                     v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(), None if cu_tokens is None else cu_tokens.data_ptr(),
                     batch, tokens, most, max_len, shared, heads, kv_heads, dim, _KV_TYPES[q.dtype], scale, int(bool(causal)), out.data_ptr(),
-                    out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws, ws_bytes, _stream(q))
-            del keep
+                    out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr() if needed else None, needed, _stream(q))
     return (out, lse) if return_lse else out
 
 
@@ -1294,10 +1291,7 @@ def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_d
     chosen in any other way. accept_draws (float32 [rows]) and sample_draws (float32 [batch]) are uniform numbers in [0, 1); temperature 0 takes the
     largest logit and needs none. max_tokens: the largest number of rows of a sequence (default: what the rows allow). Returns (int64 [batch,
     max_tokens]: accepted drafts, the token behind them, -1; int32 [batch]: how many drafts were accepted)."""
-    args = (logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws, temperature, batch, max_tokens)
-    r = (_native or _fast()).verify_drafts(*args, None)
-    if type(r) is int:  # the bytes of its workspace
-        r = _native.verify_drafts(*args, _verify_workspace(logits, r))
+    r = (_native or _fast()).verify_drafts(logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws, temperature, batch, max_tokens)
     if r is not None:
         return r
     if torch.jit.is_tracing():
@@ -1353,15 +1347,8 @@ def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_d
         with torch.cuda.device(logits.device):
             slices, needed = ctypes.c_int(), ctypes.c_int64()
             _C.call("lq_verify_drafts_plan", batch, rows, vocab, int(temperature == 0), int(draft_logits is not None), 0, ctypes.addressof(slices), ctypes.addressof(needed))
-            ws = _verify_workspace(logits, needed.value)
+            ws = torch.empty(needed.value, dtype=torch.uint8, device=logits.device)
             ptr = [None if t is None else t.data_ptr() for t in (draft_logits, cu_tokens, accept_draws, sample_draws)]
             _C.call("lq_verify_drafts", logits.data_ptr(), logits.stride(0), ptr[0], 0 if draft_logits is None else draft_logits.stride(0), tokens.data_ptr(), ptr[1], batch, rows,
                     vocab, most, _KV_TYPES[logits.dtype], temperature, ptr[2], ptr[3], out.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(logits))
-            del ws
     return out, accepted
-
-
-def _verify_workspace(t, needed):
-    if needed > WORKSPACE_MAX_BYTES:
-        return torch.empty(needed, dtype=torch.uint8, device=t.device)
-    return _workspace(t, 1, -(-needed // 32))[0]
