@@ -2,7 +2,9 @@
 
 ``KVCache8`` holds the blocks of one layer (layout and rounding: include/latentq.h, lq_kv8_*), ``Sequences`` which blocks each
 sequence has (one for all layers), ``CachedAttention`` the four projections of a layer with the operators between them:
-rotation and appending in one launch, attention over the cache in one or two. The reference's counterparts are the rotation of
+rotation and appending in one launch, attention over the cache in one or two. ``DeviceSequences`` keeps the same books on the
+device, for a batch that may begin with blocks in common and whose lengths follow from what the device computed (drafted tokens that
+were accepted): a pass can be captured into a graph. The reference's counterparts are the rotation of
 PTQ/quant/fused_attn.py:8-93 and the tensor library's cache and attention, in 16 bits. Inference only.
 """
 from __future__ import annotations
@@ -48,8 +50,12 @@ class KVCache8:
                               max_tokens=step.max_tokens)
 
     def attend(self, q, step: "Step", scale=None, window=0):
-        """ops.kv8_attention of a step's new tokens over what the cache holds of their sequences."""
+        """ops.kv8_attention of a step's new tokens over what the cache holds of their sequences (kv8_attention_shared of sequences that
+        begin with blocks in common)."""
         self._holds(step)
+        if step.shared and not window:
+            return ops.kv8_attention_shared(q, *self.tensors(), step.block_table, step.seq_lens, step.shared, cu_tokens=step.cu_tokens, max_tokens=step.max_tokens,
+                                            max_len=step.max_len, scale=scale)
         return ops.kv8_attention(q, *self.tensors(), step.block_table, step.seq_lens, cu_tokens=step.cu_tokens, max_tokens=step.max_tokens,
                                  max_len=step.max_len, scale=scale, window=window)
 
@@ -71,6 +77,9 @@ class Step:
     positions: torch.Tensor    # int64 [rows]
     longest: int = 0           # tokens of the longest sequence (0: not known, not checked)
     pool: int = 0              # blocks that a cache must have: the highest one named, and 1 (0: as above)
+    shared: int = 0            # blocks that all the sequences begin with
+    slots: torch.Tensor | None = None   # int64 [rows]: block * 64 + place of each new token (of DeviceSequences; -1 behind the last)
+    status: torch.Tensor | None = None  # int32 [1]: of ops.kv8_resize (of DeviceSequences)
 
 
 class Sequences:
@@ -121,6 +130,59 @@ class Sequences:
                     last=torch.tensor(starts[1:], device=self.device) - 1,
                     positions=torch.cat([torch.arange(lens[s] - n, lens[s]) for s, n in new.items()]).to(self.device),
                     longest=max(lens.values()), pool=1 + max(max(self._blocks[s]) for s in new))
+
+
+class DeviceSequences:
+    """Which blocks of a pool a fixed batch of sequences has, kept on the device (ops.kv8_resize): no pass asks the host. `capacity` is the most tokens of
+    a sequence. The first `shared` blocks of the pool are every sequence's first ones: their tokens are appended once, by the pass
+    that prompt() describes, and a sequence without tokens of its own has those."""
+
+    def __init__(self, num_blocks: int, batch: int, capacity: int, shared: int = 0, device="cuda"):
+        width = -(-capacity // BLOCK)
+        if batch < 1 or capacity < 1 or not 0 <= shared <= min(num_blocks, width):
+            raise ValueError(f"needs a sequence, a token for it, and no more shared blocks than the pool and a sequence have, got {batch}, {capacity} and {shared}")
+        self.num_blocks, self.batch, self.shared, self.capacity = num_blocks, batch, shared, width * BLOCK
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.zeros((batch, width), **i32)
+        self.block_table[:, :shared] = torch.arange(shared, **i32)
+        self.seq_lens = torch.full((batch,), shared * BLOCK, **i32)
+        self.free_blocks = torch.zeros(num_blocks, **i32)  # the last free one is the next to be taken
+        self.free_blocks[:num_blocks - shared] = torch.arange(num_blocks - 1, shared - 1, -1, **i32)
+        self.free_count = torch.full((1,), num_blocks - shared, **i32)
+
+    def _books(self):
+        return self.block_table, self.seq_lens, self.free_blocks, self.free_count
+
+    def prompt(self) -> Step:
+        """The pass that appends the shared blocks' tokens, as those of one sequence."""
+        if not self.shared:
+            raise ValueError("the sequences share no blocks")
+        n, dev = self.shared * BLOCK, self.block_table.device
+        return Step(block_table=self.block_table[:1], seq_lens=torch.full((1,), n, dtype=torch.int32, device=dev), cu_tokens=None, max_tokens=n, max_len=n,
+                    last=torch.full((1,), n - 1, device=dev), positions=torch.arange(n, device=dev), longest=n, pool=self.num_blocks)
+
+    def extend(self, new, rows: int, max_tokens: int | None = None, max_len: int | None = None) -> Step:
+        """Make room for new[i] more tokens of sequence i (int32 [batch] on the device, none negative) and describe the pass that appends them. `rows`
+        is the number of rows that the pass has, as many as there are new tokens or more; max_tokens and max_len bound a sequence's
+        new tokens and its length (defaults: rows, the capacity). Where step.status is not 0 nothing has changed and the pass has no tokens."""
+        cu, positions, slots, status = ops.kv8_resize(*self._books(), new, rows=rows, shared=self.shared)
+        return Step(block_table=self.block_table, seq_lens=self.seq_lens, cu_tokens=cu, max_tokens=rows if max_tokens is None else max_tokens,
+                    max_len=self.capacity if max_len is None else max_len, last=(cu[1:].long() - 1).clamp_min(0), positions=positions, longest=self.capacity,
+                    pool=self.num_blocks, shared=self.shared, slots=slots, status=status)
+
+    def give_back(self, tokens):
+        """Take the last tokens[i] tokens of sequence i away (int32 [batch] on the device, none negative; more than there are: all of its own). Blocks that
+        they alone had are free again."""
+        ops.kv8_resize(*self._books(), -torch.minimum(tokens, self.seq_lens - self.shared * BLOCK), shared=self.shared)
+
+    def verify(self, logits, tokens, step: Step, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0):
+        """ops.verify_drafts of a step's rows, each sequence's first one a known token and the others drafts; refused drafts leave their sequences. Returns
+        (accepted drafts, the token behind them and -1, int64 [batch, max_tokens]; how many were accepted, int32 [batch])."""
+        out, accepted = ops.verify_drafts(logits, tokens, step.cu_tokens, draft_logits=draft_logits, accept_draws=accept_draws, sample_draws=sample_draws,
+                                          temperature=temperature, max_tokens=step.max_tokens)
+        new = step.cu_tokens[1:] - step.cu_tokens[:-1]
+        self.give_back((new - accepted - 1).clamp_min(0))
+        return out, accepted
 
 
 def rotation_tables(positions: int, head_dim: int, base: float = 10000.0, device="cuda"):
