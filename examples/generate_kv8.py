@@ -1,7 +1,9 @@
 """Generation with int4 layers and a paged 8-bit cache of keys and values: prompts of different lengths go in together, then every
-sequence gives one token a pass; one that is done gives its blocks back.
+sequence gives one token a pass; one that is done gives its blocks back. With --drafts, the same prompts as questions behind --shared
+tokens that they have in common: tokens that followed the last one earlier are drafted, checked in one pass, and the books stay on the device.
 
     python examples/generate_kv8.py [--layers 4] [--hidden 4096] [--inter 11008] [--heads 32] [--kv-heads 32] [--new 32]
+                                    [--drafts 3] [--shared 1024]
 
 Weights are random (the sizes of a 7B decoder by default), so the tokens mean nothing; it shows the calls and prints their speed.
 """
@@ -15,7 +17,7 @@ import torch.nn as nn
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from latentq_llm_amd.fused_mlp import QuantLlamaMLP  # noqa: E402
-from latentq_llm_amd.kv_cache import CachedAttention, KVCache8, Sequences, rotation_tables  # noqa: E402
+from latentq_llm_amd.kv_cache import BLOCK, CachedAttention, DeviceSequences, KVCache8, Sequences, rotation_tables  # noqa: E402
 from latentq_llm_amd.quant import QLinearA16W4  # noqa: E402
 
 BF16 = torch.bfloat16
@@ -58,13 +60,13 @@ class Decoder(nn.Module):
             self.layers.append(nn.ModuleList([Norm(hidden), attention, Norm(hidden), mlp]))
 
     @torch.no_grad()
-    def forward(self, tokens, caches, step):
-        """Logits of each sequence's last new token."""
+    def forward(self, tokens, caches, step, every=False):
+        """Logits of each sequence's last new token, or of every one."""
         x = self.embed[tokens]
         for (norm1, attention, norm2, mlp), cache in zip(self.layers, caches):
             x = x + attention(norm1(x), cache, step)
             x = x + mlp(norm2(x))
-        return self.norm(x[step.last]) @ self.head.t()
+        return self.norm(x if every else x[step.last]) @ self.head.t()
 
 
 def generate(model, caches, sequences, prompts, new):
@@ -91,12 +93,63 @@ def generate(model, caches, sequences, prompts, new):
     return out, middle - begin, time.perf_counter() - middle
 
 
+def looked_up(history, lengths, drafts):
+    """The tokens that followed the last token of each row where it was before, the latest time: int64 [rows, drafts]."""
+    place = torch.arange(history.shape[1], device=history.device)
+    last = history.gather(1, lengths[:, None] - 1)
+    at = torch.where((history == last) & (place < lengths[:, None] - 1), place, -1).amax(1, keepdim=True)
+    return history.gather(1, (at + 1 + torch.arange(drafts, device=history.device)).clamp(max=history.shape[1] - 1))
+
+
+def generate_drafted(model, caches, sequences, prompt, questions, new, drafts):
+    """Greedy continuation of each question by `new` tokens behind the prompt that they share (whole blocks), `drafts` tokens looked up in what it has so far in
+    every pass; returns (tokens, seconds of the prompts, of the rest, passes). The host waits for the device every 8 passes."""
+    batch, width = len(questions), drafts + 1
+    torch.cuda.synchronize()
+    begin = time.perf_counter()
+    if prompt:
+        model(torch.tensor(prompt).cuda(), caches, sequences.prompt())
+    counts = torch.tensor([len(p) for p in questions])
+    history = torch.zeros((batch, int(counts.max()) + new + 2 * width), dtype=torch.int64)
+    for i, p in enumerate(questions):
+        history[i, :len(p)] = torch.tensor(p)
+    history, first = history.cuda(), counts.cuda()
+    lengths, place, row = first.clone(), torch.arange(width, device="cuda"), torch.full((1,), batch * width, device="cuda")
+    step = sequences.extend(lengths.int(), int(counts.sum()), max_tokens=int(counts.max()))
+    out = model(torch.cat([torch.tensor(p) for p in questions]).cuda(), caches, step).argmax(-1)[:, None].expand(-1, width)
+    gave = torch.ones_like(lengths)
+    torch.cuda.synchronize()
+    middle, passes = time.perf_counter(), 0
+    while True:
+        # what the pass before gave: accepted drafts and the token behind them
+        at = lengths[:, None] + place
+        history.scatter_(1, at, torch.where(place < gave[:, None], out, history.gather(1, at)))
+        lengths += gave
+        active = lengths - first < new
+        if passes % 8 == 0 and not active.any():
+            break
+        # rows of the sequences that go on, one after the other; the others have none
+        step = sequences.extend(active.int() * width, batch * width, max_tokens=width)
+        tokens = torch.cat((history.gather(1, lengths[:, None] - 1), looked_up(history, lengths, drafts)), 1)
+        packed = torch.zeros(batch * width + 1, dtype=torch.int64, device="cuda")
+        packed.scatter_(0, torch.where(active[:, None], step.cu_tokens[:-1, None] + place, row).view(-1), tokens.view(-1))
+        out, accepted = sequences.verify(model(packed[:-1], caches, step, every=True), packed[:-1], step, temperature=0.0)
+        gave = (accepted + 1) * active
+        passes += 1
+    torch.cuda.synchronize()
+    return [history[i, n:n + new].tolist() for i, n in enumerate(counts.tolist())], middle - begin, time.perf_counter() - middle, passes
+
+
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     for name, value in (("layers", 4), ("hidden", 4096), ("inter", 11008), ("heads", 32), ("kv-heads", 32), ("vocab", 32000), ("new", 32)):
         ap.add_argument(f"--{name}", type=int, default=value)
     ap.add_argument("--prompts", type=int, nargs="+", default=[45, 512, 1019, 7], help="their lengths")
+    ap.add_argument("--drafts", type=int, default=0, help="tokens drafted in every pass")
+    ap.add_argument("--shared", type=int, default=1024, help=f"with --drafts: tokens that the prompts share, a multiple of {BLOCK}")
     a = ap.parse_args()
+    if a.drafts:
+        return drafted(a)
     positions = max(a.prompts) + a.new
     blocks = sum(-(-(n + a.new) // 64) for n in a.prompts)
     model = Decoder(a.layers, a.hidden, a.inter, a.heads, a.kv_heads, a.vocab, positions).eval()
@@ -109,6 +162,26 @@ def main():
     out, first, rest = generate(model, caches, sequences, prompts, new)
     print(f"{sum(a.prompts)} prompt tokens in {first * 1e3:.2f} ms, then {a.new - 1} passes of {len(prompts)} tokens, {rest / max(1, a.new - 1) * 1e3:.3f} ms each "
           f"({a.layers} layers); cache {sum(t.numel() * t.element_size() for c in caches for t in c.tensors()) >> 20} MiB")
+    for p, o in zip(a.prompts, out):
+        print(f"prompt of {p}: {o[:8]} ...")
+
+
+def drafted(a):
+    if a.shared % BLOCK:
+        raise SystemExit(f"--shared must be a multiple of {BLOCK}")
+    room = a.new + 2 * (a.drafts + 1)
+    capacity = a.shared + max(a.prompts) + room
+    blocks = a.shared // BLOCK + sum(-(-(n + room) // BLOCK) for n in a.prompts)
+    model = Decoder(a.layers, a.hidden, a.inter, a.heads, a.kv_heads, a.vocab, -(-capacity // BLOCK) * BLOCK).eval()
+    caches = [KVCache8(blocks, a.kv_heads, a.hidden // a.heads) for _ in range(a.layers)]
+    gen = torch.Generator().manual_seed(1)
+    shared = torch.randint(0, a.vocab, (a.shared,), generator=gen).tolist()
+    prompts = [torch.randint(0, a.vocab, (n,), generator=gen).tolist() for n in a.prompts]
+    for _ in range(2):  # first calls load code
+        sequences = DeviceSequences(blocks, len(prompts), capacity, a.shared // BLOCK)
+        out, first, rest, passes = generate_drafted(model, caches, sequences, shared, prompts, a.new, a.drafts)
+    print(f"{a.shared} shared and {sum(a.prompts)} prompt tokens in {first * 1e3:.2f} ms, then {passes} passes of {len(prompts)} x {a.drafts + 1} tokens, {rest / passes * 1e3:.3f} ms each "
+          f"({a.layers} layers): {a.new - 1} tokens and more of each")
     for p, o in zip(a.prompts, out):
         print(f"prompt of {p}: {o[:8]} ...")
 

@@ -160,3 +160,31 @@ def test_refusals(hip_lib):
     table = torch.zeros((100, 32), device="cuda")
     with pytest.raises(ValueError, match="100 positions"):
         KVCache8(10, 1, 64).append(x, x, step, q=x, cos=table, sin=table)
+
+
+def test_example(hip_lib):
+    """The example's drafted generation runs and gives as many tokens as asked, all of the vocabulary, and the same ones again."""
+    import importlib.util
+    import os
+
+    from latentq_llm_amd.kv_cache import DeviceSequences, KVCache8
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "generate_kv8.py")
+    spec = importlib.util.spec_from_file_location("generate_kv8", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    shared, new, drafts = 15, 9, 3
+    model = m.Decoder(2, 512, 1024, 8, 2, 1000, 64 * shared + 320).eval()
+    caches = [KVCache8(60, 2, 64) for _ in range(2)]
+    gen = torch.Generator().manual_seed(1)
+    prompt = torch.randint(0, 1000, (64 * shared,), generator=gen).tolist()
+    questions = [torch.randint(0, 1000, (n,), generator=gen).tolist() for n in (200, 33, 1)]
+    questions[1] = questions[1][:3] * 11  # (something to look up)
+    runs = []
+    for _ in range(2):
+        sequences = DeviceSequences(60, 3, 64 * shared + 260, shared)
+        out, _, _, passes = m.generate_drafted(model, caches, sequences, prompt, questions, new, drafts)
+        assert [len(o) for o in out] == [new] * 3 and all(0 <= t < 1000 for o in out for t in o)
+        assert passes % 8 == 0 and passes >= (new - 1) / (drafts + 1)
+        assert all(64 * shared + len(q) + new - 1 <= n <= 64 * shared + len(q) + new + drafts for q, n in zip(questions, sequences.seq_lens.tolist()))
+        runs.append(out)
+    assert runs[0] == runs[1]
