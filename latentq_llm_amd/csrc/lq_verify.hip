@@ -34,7 +34,7 @@ struct Stat {  // of a slice: sum of 2^((l - m) c); of the greedy choice: the ma
         int64_t at;
     };
     float m;
-    int pad;
+    float drafted;  // of a row's first slice: the logit of the token drafted behind the row
 };
 struct Left {  // of a block: sums of max(p - q, 0) and of p
     double rest, all;
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kStats) void stats_kernel(const Verify a) {
                     best = places[w];
                 }
             s.at = best;
-            s.pad = 0;
+            s.drafted = 0.0f;
             to = s;
         }
     } else {
@@ -253,6 +253,11 @@ __global__ __launch_bounds__(kStats) void stats_kernel(const Verify a) {
         };
         bool whole = j + kTurn - kStats * kVec + kVec <= end;
         if (whole) request();
+        float drafted = -__builtin_inff();
+        if (slice == 0 && threadIdx.x == 3 && row + 1 < a.rows) {  // for the tests, which then need not wait for a token and its logit in turn
+            const int64_t token = a.tokens[row + 1];
+            if (token >= 0 && token < a.vocab) drafted = counted(x.one(token));
+        }
         if (unused()) return;  // (under the first pieces' way)
         fill_table(table);
         __syncthreads();
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(kStats) void stats_kernel(const Verify a) {
                 Stat s;
                 s.m = most;
                 s.sum = all;
-                s.pad = 0;
+                s.drafted = drafted;
                 to = s;
             }
         }
@@ -355,7 +360,7 @@ struct Rest {
 
 struct Board {  // in shared memory
     double row_sum[2][kRound];
-    float row_m[2][kRound];
+    float row_m[2][kRound];  // (without the drafter's logits, the second one: the logit of the draft)
     int64_t best[kRound];
     int refused;
 };
@@ -393,19 +398,15 @@ __device__ __forceinline__ int first_refused(const Verify &a, const Exp2 &power,
                     if (!inside || token != best) atomicMin(&b.refused, base + i);
                 }
             } else {
-                float of_p = 0.0f, of_q = 0.0f, u = 0.0f;
-                if (inside) {
-                    of_p = row_at<kType>(a.logits, a.stride, row).one(token);
-                    if constexpr (kMode == kBoth) of_q = row_at<kType>(a.draft, a.draft_stride, row).one(token);
-                    u = a.accept[row];
-                }
+                const float u = drafted ? a.accept[row] : 0.0f;
                 const bool mine = half == 0 || (kMode == kBoth && drafted);
                 const Stat *s = a.stats + ((int64_t)row * 2 + half) * a.slices;
-                float m = -__builtin_inff();
+                float m = -__builtin_inff(), of_draft = m;
                 double sum = 0.0;
                 if (mine && (lane & 31) < a.slices) {
                     m = s[lane & 31].m;
                     sum = s[lane & 31].sum;
+                    of_draft = s[lane & 31].drafted;
                 }
                 for (int k = (lane & 31) + 32; mine && k < a.slices; k += 32) {
                     const float more = fmaxf(m, s[k].m);
@@ -414,15 +415,16 @@ __device__ __forceinline__ int first_refused(const Verify &a, const Exp2 &power,
                 }
                 const float tops = halves_most(m), p_m = at_lane(tops, 31), q_m = at_lane(tops, 63);
                 const double sums = halves_scan(sum * power(m, reference(half ? q_m : p_m))), p_sum = at_lane(sums, 31), q_sum = at_lane(sums, 63);
+                const float of_p = at_lane(of_draft, 0), of_q = at_lane(of_draft, 32);
                 bool taken = false;
                 if (inside) {
-                    const double p = power(counted(of_p), reference(p_m));
-                    const double q = kMode == kBoth ? power(counted(of_q), reference(q_m)) : 1.0, all = kMode == kBoth ? q_sum : 1.0;
+                    const double p = power(of_p, reference(p_m));
+                    const double q = kMode == kBoth ? power(of_q, reference(q_m)) : 1.0, all = kMode == kBoth ? q_sum : 1.0;
                     taken = p_sum > 0.0 && (double)u * (all > 0.0 ? q / all : 0.0) < p / p_sum;
                 }
                 if (lane == 0) {
                     b.row_m[0][i] = p_m;
-                    b.row_m[1][i] = q_m;
+                    b.row_m[1][i] = kMode == kBoth ? q_m : of_p;
                     b.row_sum[0][i] = p_sum;
                     b.row_sum[1][i] = q_sum;
                     if (!taken) atomicMin(&b.refused, base + i);
@@ -659,29 +661,14 @@ __global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
     const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
     write_taken(a, seq, start, first);
     const Rest<kType, false> rest(a, power, c);
-    // the slice that had the draft, without it
-    const int without = c.draft >= 0 ? c.draft / a.span : -1;
-    if (without >= 0) {
-        const int end = min((without + 1) * a.span, a.vocab);
-        double mine = 0.0;
-        for (int j = without * a.span + tid * kEach; j < end; j += kBlock) {
-            double x[kEach], all[kEach];
-            rest.some(j, end, x, all);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) mine += x[i];
-        }
-        mine = wave_sum(mine);
-        if ((tid & 63) == 0) draw.sums[tid >> 6] = mine;
-        __syncthreads();
-    }
     if (tid < 64) {
-        double other = 0.0;
-        if (without >= 0)
-            for (int w = 0; w < kWaves; ++w) other += draw.sums[w];
+        // The slice that had the draft, less the draft: what is left in all is 2^-24 and more, for a number under 1 refused it, and the difference is exact to 2^-53
+        const int without = c.draft >= 0 ? c.draft / a.span : -1;
+        const double of_draft = power(c.q_m, rest.p_m) * rest.p_by;
         const Stat *s = a.stats + (int64_t)c.row * 2 * a.slices;
         find_part(draw, a.slices, u, [&](int i) {
             const double all = s[i].sum * power(s[i].m, rest.p_m) * rest.p_by;
-            return Left{i == without ? other : all, all};
+            return Left{i == without ? fmax(all - of_draft, 0.0) : all, all};
         });
     }
     __syncthreads();
