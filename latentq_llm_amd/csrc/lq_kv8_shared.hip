@@ -21,8 +21,25 @@ namespace {
 
 constexpr float kLazy = 8.0f;
 
+// n / d of 0 <= n < 2^31 by a product: a division by a number that only the host knows is some 25 instructions that wait for each other, and a row
+// takes three before its first load
+struct Div {
+    unsigned by;
+    int shift;
+    Div() = default;
+    explicit Div(int d) {
+        int bits = 0;
+        while (((int64_t)1 << bits) < d) ++bits;
+        shift = 31 + bits;  // by = 2^shift / d, rounded up: off by less than d / 2^31 of a quotient's step, and fits 32 bits
+        by = (unsigned)((((uint64_t)1 << shift) + d - 1) / d);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)(((uint64_t)(unsigned)n * by) >> shift); }
+};
+
 struct Shared {
     Kv8Attn a;
+    int group, per_seq;         // query heads of a kv head; new tokens of a sequence, without cu
+    Div by_group, by_per_seq, by_kv_heads, by_row_tiles, by_o_slices, by_o_row_tiles, by_o_tiles;
     int common;                 // blocks that all sequences begin with
     int row_tiles;              // of the prefix's rows, each for a workgroup
     int p_slices, p_tiles;      // of the prefix: slices of the keys, tiles of 64 in each
@@ -41,10 +58,11 @@ struct Where {
         return !there ? -1 : a.causal ? min(max(len, 0) - n + (token - first), seen) : seen;
     }
 };
-__device__ __forceinline__ Where where_is(const Kv8Attn &a, int token, bool there) {
+__device__ __forceinline__ Where where_is(const Shared &s, int token, bool there) {
+    const Kv8Attn &a = s.a;
     if (!a.cu) {
-        const int n = a.tokens / a.batch, seq = min(token / n, a.batch - 1);
-        return Where{a.lens[seq], seq * n, seq * n + n, token, there};
+        const int seq = min(s.by_per_seq(token), a.batch - 1);
+        return Where{a.lens[seq], seq * s.per_seq, (seq + 1) * s.per_seq, token, there};
     }
     const int lane = threadIdx.x & 63;
     int seq = 0;
@@ -62,11 +80,28 @@ __device__ __forceinline__ Where where_is(const Kv8Attn &a, int token, bool ther
     return Where{a.lens[seq], a.cu[seq], a.cu[seq + 1], token, there};
 }
 
+// The new tokens of a sequence, rows start .. start + n - 1 of the operands, its length as it is given, and its tiles within the block table
+struct Span {
+    int start, n, len, tiles;
+};
+__device__ __forceinline__ Span span_of(const Shared &s, int seq) {
+    const Kv8Attn &a = s.a;
+    const int len = kv8_uniform(a.lens + seq);
+    int begin = seq * s.per_seq, end = begin + s.per_seq;
+    if (a.cu) {
+        begin = kv8_uniform(a.cu + seq);
+        end = kv8_uniform(a.cu + seq + 1);
+    }
+    const int start = min(max(begin, 0), a.tokens);
+    return Span{start, min(max(end, start), a.tokens) - start, len, (min(max(len, 0), a.width * KV8_BLOCK) + KV8_BLOCK - 1) / KV8_BLOCK};
+}
+
 // What an item is: rows row0 .. row0 + rows - 1 of those that begin with token `token0`, kv head h, tiles t_lo .. t_hi - 1 of the block
 // table's row, results in `slot` of the workspace
 struct Item {
     int token0, row0, rows, h, t_lo, t_hi;
     const int *table;
+    int block;  // the entry of this wave's first tile
     int64_t slot;
 };
 
@@ -92,10 +127,11 @@ constexpr int waves_of(int dim, int row_tiles) { return dim > 128 ? 1 : row_tile
 constexpr int item_lds(int dim) { return 4 * 16 * (dim + 4 + 2) * 4; }
 
 template <int D, int RT, bool kF16, bool kKept, typename Rows>
-__device__ __forceinline__ void item(const Kv8Attn &a, const Item &it, char *lds, const Rows &row_is) {
+__device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds, const Rows &row_is) {
+    const Kv8Attn &a = s.a;
     constexpr int S = D / 64, kTail = D % 64 / 32, kSteps = 2 * S + kTail, kTiles = D / 16, kWaves = 4, kPad = D + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int group = a.heads / a.kv_heads, h = it.h;
+    const int group = s.group, h = it.h;
 
     // the queries and where their rows are: requested before the first tile, so that nothing waits for that
     u32x4_t raw[RT][kSteps];
@@ -103,7 +139,7 @@ __device__ __forceinline__ void item(const Kv8Attn &a, const Item &it, char *lds
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const bool there = rt * 16 + col < it.rows;
-        const int row = it.row0 + rt * 16 + col, token = it.token0 + (there ? row / group : 0), head = there ? h * group + row % group : 0;
+        const int row = it.row0 + rt * 16 + col, at = there ? s.by_group(row) : 0, token = it.token0 + at, head = there ? h * group + row - at * group : 0;
         const uint16_t *src = (const uint16_t *)a.q + (int64_t)token * a.q_token + (int64_t)head * a.q_head;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) raw[rt][i] = *(const u32x4_t *)(src + (i < 2 * S ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 64 * S + 8 * g));
@@ -139,7 +175,7 @@ __device__ __forceinline__ void item(const Kv8Attn &a, const Item &it, char *lds
     int64_t bh = 0;
     float k_scale = 0.0f, v_scale = 0.0f;
     if (t < it.t_hi) {
-        bh = block_at(a, kv8_uniform(it.table + t), h);
+        bh = block_at(a, it.block, h);
         load_k(bh);
         k_scale = kv8_uniform(a.ks + bh);
         v_scale = kv8_uniform(a.vs + bh);
@@ -297,7 +333,8 @@ __device__ __forceinline__ void item(const Kv8Attn &a, const Item &it, char *lds
             f32x4_t x;
             kv8_join_parts<kWaves>((const f32x4_t *)&lds_o[0][c][d], &lds_m[0][c], &lds_l[0][c], 16 * kPad / 4, 16, m, total, x);
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            const int64_t at = it.slot * ((int64_t)a.tokens * a.heads) + (int64_t)(it.token0 + (it.row0 + r) / group) * a.heads + h * group + (it.row0 + r) % group;
+            const int row = it.row0 + r, y = s.by_group(row);
+            const int64_t at = it.slot * ((int64_t)a.tokens * a.heads) + (int64_t)(it.token0 + y) * a.heads + h * group + row - y * group;
             *(f32x4_t *)(a.part + at * D + d) = x * inv;
             if (d == 0) a.part_lse[at] = total == 0.0f ? -__builtin_inff() : m + __builtin_amdgcn_logf(total);
         }
@@ -309,24 +346,26 @@ template <int D, int kPrefix, int kOwn, bool kF16>
 __global__ __launch_bounds__(256, waves_of(D, kPrefix)) void shared_kernel(const Shared s) {
     __shared__ __attribute__((aligned(16))) char lds[item_lds(D)];
     const Kv8Attn &a = s.a;
-    const int group = a.heads / a.kv_heads;
-    if ((int)blockIdx.x < s.p_items) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x;
+    if (id < s.p_items) {
         // the workgroups of the same keys lie 8 apart, on one XCD: its L2 gives them to all but the first
-        const int row_tile = blockIdx.x / 8 % s.row_tiles, unit = blockIdx.x / (8 * s.row_tiles) * 8 + blockIdx.x % 8;
+        const int eight = id >> 3, units = s.by_row_tiles(eight), row_tile = eight - units * s.row_tiles, unit = units * 8 + (id & 7);
         if (unit >= a.kv_heads * s.p_slices) return;
-        const int slice = unit / a.kv_heads, row0 = row_tile * 16 * kPrefix;
-        const Item it{0, row0, min(a.tokens * group - row0, 16 * kPrefix), unit % a.kv_heads, slice * s.p_tiles, min((slice + 1) * s.p_tiles, s.common), a.table, slice};
-        item<D, kPrefix, kF16, true>(a, it, lds, [&](int token, bool there) { return where_is(a, token, there); });
+        const int slice = s.by_kv_heads(unit), row0 = row_tile * 16 * kPrefix, t_lo = slice * s.p_tiles, t_hi = min(t_lo + s.p_tiles, s.common);
+        const Item it{0, row0, min(a.tokens * s.group - row0, 16 * kPrefix), unit - slice * a.kv_heads, t_lo, t_hi, a.table, kv8_uniform(a.table + min(t_lo + wave, t_hi - 1)), slice};
+        item<D, kPrefix, kF16, true>(s, it, lds, [&](int token, bool there) { return where_is(s, token, there); });
         return;
     }
-    const int at = blockIdx.x - s.p_items, slice = at % s.o_slices, row0 = at / s.o_slices % s.o_row_tiles * 16 * kOwn, unit = at / (s.o_slices * s.o_row_tiles), seq = unit / a.kv_heads;
-    const Kv8Rows r = kv8_rows<true>(a, seq);
-    const int tiles = (r.len + KV8_BLOCK - 1) / KV8_BLOCK, t_lo = s.common + slice * s.o_tiles;
-    const int rows = min(r.n * group, a.rows) - row0;
-    if (rows <= 0 || t_lo >= tiles) return;
-    const int t_hi = slice == s.o_slices - 1 ? tiles : min(t_lo + s.o_tiles, tiles);  // (a max_len that was too small costs time)
-    const Item it{r.start, row0, min(rows, 16 * kOwn), unit % a.kv_heads, t_lo, t_hi, a.table + (int64_t)seq * a.width, s.p_slices + slice};
-    item<D, kOwn, kF16, false>(a, it, lds, [&](int token, bool there) { return Where{r.first + r.n, r.start, r.start + r.n, token, there}; });
+    const int at = id - s.p_items, part = s.by_o_slices(at), slice = at - part * s.o_slices, unit = s.by_o_row_tiles(part), row_tile = part - unit * s.o_row_tiles,
+              seq = s.by_kv_heads(unit), row0 = row_tile * 16 * kOwn, t_lo = s.common + slice * s.o_tiles;
+    const int *table = a.table + (int64_t)seq * a.width;
+    const int block = kv8_uniform(table + min(t_lo + wave, a.width - 1));  // (on its way with the sequence's length)
+    const Span r = span_of(s, seq);
+    const int rows = min(r.n * s.group, a.rows) - row0;
+    if (rows <= 0 || t_lo >= r.tiles) return;
+    const int t_hi = slice == s.o_slices - 1 ? r.tiles : min(t_lo + s.o_tiles, r.tiles);  // (a max_len that was too small costs time)
+    const Item it{r.start, row0, min(rows, 16 * kOwn), unit - seq * a.kv_heads, t_lo, t_hi, table, block, s.p_slices + slice};
+    item<D, kOwn, kF16, false>(s, it, lds, [&](int token, bool there) { return Where{r.len, r.start, r.start + r.n, token, there}; });
 }
 
 // A row's pieces joined: blockIdx.x for (sequence, kv head), .y for kRows of its rows
@@ -336,12 +375,12 @@ __global__ __launch_bounds__(256) void join_shared_kernel(const Shared s) {
     __shared__ f32x4_t lds_o[kParts][kRows * kUnits];
     __shared__ float lds_m[kParts][kRows], lds_l[kParts][kRows];
     const Kv8Attn &a = s.a;
-    const int seq = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+    const int seq = s.by_kv_heads(blockIdx.x), h = blockIdx.x - seq * a.kv_heads;
     const int unit = threadIdx.x % kUnits, at = threadIdx.x / kUnits, part = at % kParts, mine = at / kParts, r = blockIdx.y * kRows + mine;
-    const Kv8Rows q = kv8_rows<true>(a, seq);
-    const bool there = mine < kRows && r < min(q.n * group, a.rows);
-    const int own = (q.len + KV8_BLOCK - 1) / KV8_BLOCK - s.common, pieces = s.p_slices + max(min((own + s.o_tiles - 1) / s.o_tiles, s.o_slices), 0);
-    const int token = q.start + r / group, head = h * group + r % group;
+    const Span q = span_of(s, seq);
+    const bool there = mine < kRows && r < min(q.n * s.group, a.rows);
+    const int own = q.tiles - s.common, pieces = s.p_slices + max(min(s.by_o_tiles(max(own, 0) + s.o_tiles - 1), s.o_slices), 0);
+    const int y = s.by_group(r), token = q.start + y, head = h * s.group + r - y * s.group;
     float m = kNone, total = 0.0f;
     f32x4_t o = {0, 0, 0, 0};
     if (there) kv8_join<D>(a.part, a.part_lse, (int64_t)a.tokens * a.heads, (int64_t)token * a.heads + head, 4 * unit, part, kParts, pieces, [](int i) { return (int64_t)i; }, m, total, o);
@@ -406,7 +445,7 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
     p.o_row_tiles = (int)((own_rows + 16 * p.own - 1) / (16 * p.own));
     const int64_t own_tiles = std::max((max_len + KV8_BLOCK - 1) / KV8_BLOCK - common, (int64_t)0), slot = tokens * heads * ((int64_t)dim + 1) * 4;
     // Slices of the prefix, by an estimate in us: a compute unit gives a tile of an item `a_tile` (its arithmetic, or its bytes where no other row tile
-    // brings them; a tenth less with two items at a time), ways in and out are 4 us, and partial results go there and back. Items shorter than what all the work takes gain nothing. (Own keys count half: max_len is the
+    // brings them; a tenth less of several row tiles with two items at a time), ways in and out are 4 us, and partial results go there and back. Items shorter than what all the work takes gain nothing. (Own keys count half: max_len is the
     // longest sequence's.) us by slices, 128 dimensions: 12 sequences behind 2048 with up to 1019 of their own 2: 21.1, 8: 22.7, 1: 24.5; 64 behind 8192, 32 heads on 8,
     // 2: 38.9, 4: 28.0, 8: 34.8; 16 behind 131072 8: 130, 16: 63.7, 64: 73; 64 behind 32768 4: 64, 8: 59, 16: 65.
     const int64_t units = kv_heads * p.row_tiles;
@@ -416,7 +455,7 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
     double best = 0;
     for (int64_t n = 1; n <= 512 && 4 * n <= common + 3; ++n) {
         const int64_t tiles = (common + n - 1) / n, load = (n * units + cus - 1) / cus;
-        const double item = (double)(load * ((tiles + 3) / 4 * 4)) * a_tile * (load > 1 ? 0.9 : 1.0) + 4.0 * (double)((load + 1) / 2), t = std::max(item, all) + (double)(n * slot) * 2 / 4.5e6;
+        const double item = (double)(load * ((tiles + 3) / 4 * 4)) * a_tile * (load > 1 && p.row_tiles > 2 ? 0.9 : 1.0) + 4.0 * (double)((load + 1) / 2), t = std::max(item, all) + (double)(n * slot) * 2 / 4.5e6;
         if (n == 1 || t < 0.98 * best) {
             best = t;
             p_slices = n;
@@ -484,6 +523,15 @@ extern "C" int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, in
     s.p_slices = p.p_slices; s.p_tiles = p.p_tiles;
     s.o_slices = p.o_slices; s.o_tiles = p.o_tiles;
     s.o_row_tiles = p.o_row_tiles;
+    s.group = heads / kv_heads;
+    s.per_seq = cu_tokens ? 0 : (int)(tokens / batch);
+    s.by_group = Div(s.group);
+    s.by_per_seq = Div(cu_tokens ? 1 : s.per_seq);
+    s.by_kv_heads = Div(kv_heads);
+    s.by_row_tiles = Div(p.row_tiles);
+    s.by_o_slices = Div(p.o_slices);
+    s.by_o_row_tiles = Div(p.o_row_tiles);
+    s.by_o_tiles = Div(p.o_tiles);
     const int64_t p_items = (int64_t)(kv_heads * p.p_slices + 7) / 8 * 8 * p.row_tiles, items = p_items + batch * kv_heads * p.o_slices * p.o_row_tiles;
     LQ_REQUIRE(items <= UINT32_MAX / 256, "kv8_attention_shared: too many workgroups: %lld sequences", (long long)batch);
     s.p_items = (int)p_items;
