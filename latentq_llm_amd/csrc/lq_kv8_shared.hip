@@ -124,6 +124,16 @@ struct TileLoads {
 // Waves that a SIMD holds: as many as the registers of operands and accumulators leave room for
 constexpr int waves_of(int dim, int row_tiles) { return dim > 128 ? 1 : row_tiles == 2 ? 2 : 3; }
 
+// Eight codes of two words as a matrix operand, u 2^-24: a byte under a zero byte is a half that is not normal, which the matrix units take as it is. Two
+// instructions for four codes, where u - 128 takes four (kv8_halves). The 128 come off once: 128 times the sum of the queries where the scores'
+// sums begin, 128 times the sum of the weights, from the same products, where the outputs' end.
+__device__ __forceinline__ f16x8_t operand(unsigned a, unsigned b) {
+    return __builtin_bit_cast(f16x8_t, u32x4_t{__builtin_amdgcn_perm(0u, a, 0x0C010C00u), __builtin_amdgcn_perm(0u, a, 0x0C030C02u), __builtin_amdgcn_perm(0u, b, 0x0C010C00u),
+                                               __builtin_amdgcn_perm(0u, b, 0x0C030C02u)});
+}
+constexpr float kUnit = 0x1p24f;
+__device__ __forceinline__ f16x8_t all_128() { return __builtin_bit_cast(f16x8_t, u32x4_t{0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u}); }
+
 constexpr int item_lds(int dim) { return 4 * 16 * (dim + 4 + 2) * 4; }
 
 template <int D, int RT, bool kF16, bool kKept, typename Rows>
@@ -185,9 +195,9 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
 
     // queries as operands: lane (row col, g) has dimensions 64 s + 16 g + 8 e .. + 7 of steps (s, e), then 64 S + 8 g ..
     f16x8_t q[RT][kSteps];
-    float factor[RT], M[RT], L[RT];
+    float factor[RT], M[RT], L[RT], begin[RT];
     int last[RT];
-    f32x4_t o[RT][kTiles];
+    f32x4_t o[RT][kTiles], taken[RT];  // taken: 128 times the sum of the weights
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         float f[kSteps][8], most = 0.0f;
@@ -200,14 +210,21 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         most = kv8_max32(kv8_max16(most));
         float to, back;
         kv8_row_power(most, to, back);
-        factor[rt] = back * a.scale;
+        factor[rt] = back * a.scale * kUnit;
+        float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             u32x4_t w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = kv8_pack_f16(f[i][2 * j] * to, f[i][2 * j + 1] * to);
             q[rt][i] = __builtin_bit_cast(f16x8_t, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += (float)q[rt][i][j];
         }
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        begin[rt] = sum * (-128.0f / kUnit);
+        taken[rt] = f32x4_t{0, 0, 0, 0};
         last[rt] = where[rt].last(a);
         M[rt] = kNone;
         L[rt] = 0.0f;
@@ -223,12 +240,12 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int tg = 0; tg < 4; ++tg) c[rt][tg] = f32x4_t{0, 0, 0, 0};
+            for (int tg = 0; tg < 4; ++tg) c[rt][tg] = f32x4_t{begin[rt], begin[rt], begin[rt], begin[rt]};
 #pragma unroll
         for (int tg = 0; tg < 4; ++tg) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                const f16x8_t k = i < 2 * S ? kv8_operand(kr[tg][i >> 1][2 * (i & 1)], kr[tg][i >> 1][2 * (i & 1) + 1]) : kv8_operand(kt[tg][0], kt[tg][1]);
+                const f16x8_t k = i < 2 * S ? operand(kr[tg][i >> 1][2 * (i & 1)], kr[tg][i >> 1][2 * (i & 1) + 1]) : operand(kt[tg][0], kt[tg][1]);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) c[rt][tg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][i], c[rt][tg], 0, 0, 0);
             }
@@ -266,6 +283,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
                 const float m = fmaxf(M[rt], most), fade = __builtin_amdgcn_exp2f(M[rt] - m);
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) o[rt][i] *= fade;
+                taken[rt] *= fade;
                 L[rt] *= fade;
                 M[rt] = m;
             }
@@ -287,13 +305,16 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         }
         if (no_values) return;  // (the keys have their weight in the denominator)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) taken[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(all_128(), p[rt][e], taken[rt], 0, 0, 0);
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
-                const f16x8_t v = i < 4 * S ? kv8_operand(vr[2 * e][i >> 2][i & 3], vr[2 * e + 1][i >> 2][i & 3]) : kv8_operand(vt[2 * e][i & 1], vt[2 * e + 1][i & 1]);
+                const f16x8_t v = i < 4 * S ? operand(vr[2 * e][i >> 2][i & 3], vr[2 * e + 1][i >> 2][i & 3]) : operand(vt[2 * e][i & 1], vt[2 * e + 1][i & 1]);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[rt][e], o[rt][i], 0, 0, 0);
             }
+        }
     };
     if (t < it.t_hi) {
         for (; t + kWaves < it.t_hi; t += kWaves) tile(std::true_type{});
@@ -306,6 +327,8 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (rt * 16 >= it.rows) break;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) o[rt][i] -= taken[rt];
         float l = L[rt];
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
@@ -332,7 +355,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
             float m, total;
             f32x4_t x;
             kv8_join_parts<kWaves>((const f32x4_t *)&lds_o[0][c][d], &lds_m[0][c], &lds_l[0][c], 16 * kPad / 4, 16, m, total, x);
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            const float inv = total == 0.0f ? 0.0f : kUnit / total;
             const int row = it.row0 + r, y = s.by_group(row);
             const int64_t at = it.slot * ((int64_t)a.tokens * a.heads) + (int64_t)(it.token0 + y) * a.heads + h * group + row - y * group;
             *(f32x4_t *)(a.part + at * D + d) = x * inv;
