@@ -195,9 +195,9 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
 
     // queries as operands: lane (row col, g) has dimensions 64 s + 16 g + 8 e .. + 7 of steps (s, e), then 64 S + 8 g ..
     f16x8_t q[RT][kSteps];
-    float factor[RT], M[RT], L[RT], begin[RT];
+    float factor[RT], M[RT], L[RT];
     int last[RT];
-    f32x4_t o[RT][kTiles], taken[RT];  // taken: 128 times the sum of the weights
+    f32x4_t o[RT][kTiles], begin[RT], taken[RT];  // of the scores' sums; 128 times the sum of the weights
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         float f[kSteps][8], most = 0.0f;
@@ -210,7 +210,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         most = kv8_max32(kv8_max16(most));
         float to, back;
         kv8_row_power(most, to, back);
-        factor[rt] = back * a.scale * kUnit;
+        factor[rt] = back * a.scale;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -223,7 +223,8 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
-        begin[rt] = sum * (-128.0f / kUnit);
+        sum *= -128.0f / kUnit;
+        begin[rt] = f32x4_t{sum, sum, sum, sum};
         taken[rt] = f32x4_t{0, 0, 0, 0};
         last[rt] = where[rt].last(a);
         M[rt] = kNone;
@@ -238,16 +239,12 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         const float ks = k_scale, vs = v_scale;
         f32x4_t c[RT][4];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int tg = 0; tg < 4; ++tg) c[rt][tg] = f32x4_t{begin[rt], begin[rt], begin[rt], begin[rt]};
-#pragma unroll
         for (int tg = 0; tg < 4; ++tg) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 const f16x8_t k = i < 2 * S ? operand(kr[tg][i >> 1][2 * (i & 1)], kr[tg][i >> 1][2 * (i & 1) + 1]) : operand(kt[tg][0], kt[tg][1]);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) c[rt][tg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][i], c[rt][tg], 0, 0, 0);
+                for (int rt = 0; rt < RT; ++rt) c[rt][tg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rt][i], i ? c[rt][tg] : begin[rt], 0, 0, 0);
             }
         }
         if constexpr (decltype(more)::value) {
@@ -271,7 +268,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
                     for (int i = 0; i < 4; ++i)
                         if (key0 + tg * 16 + 4 * g + i > last[rt]) c[rt][tg][i] = -__builtin_inff();
             }
-            const float f = fmaxf(ks * factor[rt], 0x1p-100f);  // (a factor of 0 would make hidden keys NaN)
+            const float f = fmaxf(ks * factor[rt], 0x1p-100f) * kUnit;  // (a factor of 0 would make hidden keys NaN; the unit last, or large queries would pass 2^128 here)
             float most = c[rt][0][0];
 #pragma unroll
             for (int tg = 0; tg < 4; ++tg)
@@ -469,10 +466,10 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
     const int64_t own_tiles = std::max((max_len + KV8_BLOCK - 1) / KV8_BLOCK - common, (int64_t)0), slot = tokens * heads * ((int64_t)dim + 1) * 4;
     // Slices of the prefix, by an estimate in us: a compute unit gives a tile of an item `a_tile` (its arithmetic, or its bytes where no other row tile
     // brings them; a tenth less of several row tiles with two items at a time), ways in and out are 4 us, and partial results go there and back. Items shorter than what all the work takes gain nothing. (Own keys count half: max_len is the
-    // longest sequence's.) us by slices, 128 dimensions: 12 sequences behind 2048 with up to 1019 of their own 2: 21.1, 8: 22.7, 1: 24.5; 64 behind 8192, 32 heads on 8,
-    // 2: 38.9, 4: 28.0, 8: 34.8; 16 behind 131072 8: 130, 16: 63.7, 64: 73; 64 behind 32768 4: 64, 8: 59, 16: 65.
+    // longest sequence's.) us by slices, 128 dimensions: 12 sequences behind 2048 with up to 1019 of their own 2: 20.0, 4: 20.0, 8: 21.5; 64 behind 8192, 32 heads on 8,
+    // 3: 30.0, 4: 26.9, 8: 31.5; 16 behind 131072 16: 58, 32: 59, 48: 63; 64 behind 32768 4: 56, 8: 55, 16: 57; 8 x 5 behind 4096, 32 heads of 64, 2: 16.4, 4: 12.6, 8: 13.5.
     const int64_t units = kv_heads * p.row_tiles;
-    const double arithmetic = (dim == 64 ? 0.25 : dim == 96 ? 0.36 : dim == 128 ? 0.42 : 0.6) * (prefix == 2 ? 1.0 : 0.6), memory = dim * 128 / 25e3;
+    const double arithmetic = (dim == 64 ? 0.21 : dim == 96 ? 0.3 : dim == 128 ? 0.37 : 0.5) * (prefix == 2 ? 1.0 : 0.6), memory = dim * 128 / 25e3;
     const double a_tile = std::max(arithmetic, memory / p.row_tiles), all = ((double)(units * common) * a_tile + (double)(batch * kv_heads * p.o_row_tiles * own_tiles) * memory / 2) / cus;
     int64_t p_slices = 1;
     double best = 0;

@@ -164,6 +164,14 @@ def test_what_cannot_be_done_changes_nothing(resize, what, by, rows, status):
     assert all(torch.equal(a, b) for a, b in zip(state, before))
 
 
+def test_many_rows_of_a_call_that_cannot_be_done(resize):
+    books = Books(3, 200, 100, seed=9, lens=[64, 64, 100])
+    state = books.tensors()
+    want = books.change([5000, 4000, 0], 9001)
+    assert want[3] > 0
+    check(resize(*state, i32([5000, 4000, 0]), rows=9001), want, state, books, 9001)
+
+
 @pytest.mark.parametrize("count, by", [(-1, [0]), (9, [0]), (8, [-64]), (2 ** 31 - 1, [-64]), (-2 ** 31, [64])])
 def test_a_broken_list(resize, count, by):
     table, lens, stack = i32([[3, 4]]), i32([64]), i32(list(range(8)))
@@ -228,6 +236,8 @@ def test_refusals(resize):
                                ((TypeError, ValueError), {}, dict(rows="x"))):
         with pytest.raises(kind):
             resize(*args(**change), **more)
+    with pytest.raises(RuntimeError, match="cannot be recorded in a trace"):
+        torch.jit.trace(lambda x: resize(*args(change=x))[0], i32([0] * 3), check_trace=False)
     same = i32([0] * 3)
     from latentq_llm_amd import _C
     with pytest.raises(_C.LatentQError, match="overlap"):

@@ -1,5 +1,8 @@
 """lq_kv8_attention_shared: attention of sequences that begin with the same blocks, against attention in 64 bits. The bounds are those of
-tests/kv8_ref.py, derived from what the kernels round; joining two parts more is among the sums in 32 bits that they hold."""
+tests/kv8_ref.py, derived from what the kernels round, and what this kernel adds to them: codes go into the products as u = 1 .. 255, so the sums that 128 times
+the queries, or the weights, come off are up to 255 sum |q| and 255 max(v_scale), in steps of 32 terms that round to 24 bits each. For a score these are
+(dim / 32 + 2) 2^-24 255 sum |q| k_scale, less than (dim + 8) 2^-24 sum |q k| while codes are 14 from 128 on average (they are 27 here); for an output (keys / 32 + 4) 2^-24 255
+max(v_scale), added below."""
 import numpy as np
 import pytest
 import torch
@@ -55,7 +58,7 @@ def run(shared, own, news, heads, kv_heads, dim, dtype, seed=0, split=True, lens
     assert (took[0] > 0) == split, took  # (a plan that leaves the call to kv8_attention)
     out, lse = call(cache.tensors(), q, table, lens, news, shared, return_lse=True, **how)
     want, (want_lse, lse_bound), bound = ref.attention(cache, q, table, lens, news, **{k: how[k] for k in ("scale", "causal") if k in how})
-    holds(out, want, bound)
+    holds(out, want, bound + (max(lens) / 32 + 4) * 2.0 ** -24 * 255 * cache.scale[1].max())
     lse = lse.cpu().double().numpy()
     assert np.array_equal(np.isinf(lse), np.isinf(want_lse))
     fine = np.isfinite(want_lse)
@@ -143,6 +146,24 @@ def test_scores_far_apart(hip_lib):
         return c
     for batch in (3, 40, 90):
         run(14, [1 + 11 * i for i in range(batch)], [1] * batch, 2, 1, 128, F16, seed=5, cache=cache)
+
+
+@pytest.mark.parametrize("size, scale", [(1e30, 1e-30), (3e34, 1e-35), (1e-30, 1e30), (1.0, 1e3), (1.0, 1e5), (1e-30, 1.0), (1e-38, 1.0), (0.0, 1.0)])
+def test_queries_of_any_size(hip_lib, size, scale):
+    """As ordinary attention gives them, queries and their factor at the ends of 32 bits; scores of 1e6 pick a key (from some 2^26 on a step of 32 bits is an exponent's range,
+    and there neither kernel has a result), small ones average."""
+    from latentq_llm_amd import ops
+    lens, shared = [1000, 1300, 960, 900], 14
+    cache = ref.Cache(40, 2, 64, seed=21)
+    t, table, length = cache.tensors(), i32(table_of(lens, shared, 40, 21)), i32(lens)
+    q = (rows((4, 4, 64), BF16, 22).float() * size).to(BF16).cuda()
+    got = ops.kv8_attention_shared(q, *t, table, length, shared, scale=scale)
+    assert ops.kv8_attention_shared_plan(4, 4, 1, table.shape[1] * 64, 4, 2, 64, shared)[0] > 0
+    want = ops.kv8_attention(q, *t, table, length, scale=scale)
+    assert torch.isfinite(got).all()
+    # each is within its bound of the value: ulp and weights (2^-11 |o| + 2^-11 sum p |v|, |v| <= 127 v_scale), and one step of bf16 of either
+    slack = (2.0 ** -10 + 2.0 ** -12) * 127 * float(cache.scale[1].max()) * 2 + 2.0 ** -7 * want.float().abs()
+    assert ((got.float() - want.float()).abs() <= slack).all()
 
 
 def test_strides_and_a_given_output(hip_lib):

@@ -340,3 +340,26 @@ def test_refusals(verify):
         verify(logits, tokens, torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda"), **good)
     with pytest.raises(RuntimeError):
         verify(logits.cpu(), tokens, **good)
+    with pytest.raises(RuntimeError, match="cannot be recorded in a trace"):
+        torch.jit.trace(lambda x: verify(x, tokens, **good)[0], logits, check_trace=False)
+
+
+def test_numbers_that_are_none(verify):
+    """NaN and 1 in the place of uniform numbers: tokens of the vocabulary all the same, the last one left for them."""
+    (logits, tokens, draft, accept), gen = inputs(12, 300, "f32", 15, True)
+    logits[:, 250:] = -float("inf")
+    for u in (float("nan"), 1.0, 2.0, float("inf")):
+        for d in (draft, None):
+            out, accepted = verify(logits, tokens, batch=6, draft_logits=d, accept_draws=torch.full((12,), u, device="cuda"), sample_draws=torch.full((6,), u, device="cuda"))
+            given = out[out >= 0]
+            assert given.numel() >= 6 and (given < 250).all()
+
+
+def test_a_row_that_is_one_token(verify):
+    """p is 1 at the draft and 0 elsewhere: whatever the number, nothing else can come."""
+    logits = torch.full((4, 5000), -float("inf"), device="cuda")
+    logits[:, 4321] = 2.0
+    tokens = torch.full((4,), 4321, device="cuda")
+    for u in (0.0, 0.999999, 1.0):
+        out, accepted = verify(logits, tokens, batch=2, accept_draws=torch.full((4,), u, device="cuda"), sample_draws=torch.full((2,), min(u, 0.5), device="cuda"))
+        assert (out[out >= 0] == 4321).all() and (out[:, 0] == 4321).all()
