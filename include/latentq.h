@@ -625,12 +625,13 @@ int lq_kv8_resize(int32_t *block_table, int64_t table_width, int32_t *seq_lens, 
  * size; exponentials and sums are 64 bits. accept_draws float [rows] (a sequence's last one is not used; may be null if max_tokens is 1), sample_draws
  * float [batch].
  * out int64 [batch][max_tokens]: the taken drafts, the token behind them, then -1 (a sequence without rows: all -1); accepted int32 [batch]: how many drafts
- * were taken. Rows of a sequence beyond max_tokens are not looked at. Up to 65535 rows and sequences. workspace: 16-byte aligned, the
+ * were taken; change int32 [batch] (or null): accepted + 1 - its rows (0 without rows), by which lq_kv8_resize gives refused drafts back. Rows of a
+ * sequence beyond max_tokens are not looked at. Up to 65535 rows and sequences. workspace: 16-byte aligned, the
  * bytes that lq_verify_drafts_plan says; calls sharing one are ordered on one stream. No result depends on an order.
  * ------------------------------------------------------------------------- */
 int lq_verify_drafts(const void *logits, int64_t row_stride, const void *draft_logits, int64_t draft_row_stride, const int64_t *tokens,
                      const int32_t *cu_tokens, int64_t batch, int64_t rows, int64_t vocab, int64_t max_tokens, int dtype, double temperature,
-                     const float *accept_draws, const float *sample_draws, int64_t *out, int32_t *accepted, void *workspace,
+                     const float *accept_draws, const float *sample_draws, int64_t *out, int32_t *accepted, int32_t *change, void *workspace,
                      int64_t workspace_bytes, void *stream);
 /* Into how many slices the above cuts a row, and the bytes of workspace that it needs (launches nothing; compute_units <= 0: the current device's). */
 int lq_verify_drafts_plan(int64_t batch, int64_t rows, int64_t vocab, int greedy, int with_draft_logits, int compute_units, int *slices,

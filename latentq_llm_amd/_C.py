@@ -65,7 +65,7 @@ SIGNATURES = {
                                 _f32, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _vp],
     "lq_kv8_attention_shared_plan": [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i32, _vp, _vp, _vp],
     "lq_kv8_resize": [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
-    "lq_verify_drafts": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _f64, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "lq_verify_drafts": [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _f64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "lq_verify_drafts_plan": [_i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp],
     "lq_repack_gptq_to_native": [_vp, _vp, _i64, _i64, _vp],
     "lq_repack_native_to_gptq": [_vp, _vp, _i64, _i64, _vp],

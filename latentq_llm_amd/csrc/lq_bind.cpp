@@ -882,12 +882,12 @@ struct Logits {
     }
 };
 
-// logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws (None or tensors), temperature, batch, max_tokens (None) -> (out, accepted)
+// logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws (None or tensors), temperature, batch, max_tokens (None), change (None or a tensor) -> (out, accepted)
 PyObject *verify_drafts(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    LQ_ARGS(9)
+    LQ_ARGS(10)
     if (watched()) return none();
     Logits l, d;
-    const at::Tensor *tokens = plain(a[1], at::kLong), *cu = nullptr, *accept = nullptr, *sample = nullptr;
+    const at::Tensor *tokens = plain(a[1], at::kLong), *cu = nullptr, *accept = nullptr, *sample = nullptr, *change = nullptr;
     if (!l.load(a[0]) || !tokens || !same_device(tokens, l.t)) return none();
     const int64_t rows = l.t->size(0), vocab = l.t->size(1);
     if (tokens->sizes() != at::IntArrayRef({rows}) || rows > 65535) return none();
@@ -912,6 +912,7 @@ PyObject *verify_drafts(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (a[3] != Py_None && (!d.load(a[3]) || d.dtype != l.dtype || d.t->sizes() != l.t->sizes() || !same_device(d.t, l.t))) return none();
     if (a[4] != Py_None && (!(accept = plain(a[4], at::kFloat)) || accept->sizes() != at::IntArrayRef({rows}) || !same_device(accept, l.t))) return none();
     if (a[5] != Py_None && (!(sample = plain(a[5], at::kFloat)) || sample->sizes() != at::IntArrayRef({batch}) || !same_device(sample, l.t))) return none();
+    if (a[9] != Py_None && (!(change = plain(a[9], at::kInt)) || change->sizes() != at::IntArrayRef({batch}) || !same_device(change, l.t))) return none();
     if (draws && (!sample || (!accept && most > 1))) return none();
     On on(*l.t);
     int slices;
@@ -922,7 +923,8 @@ PyObject *verify_drafts(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     at::Tensor out = take(all, at, {batch, most}, at::kLong), accepted = take(all, at, {batch}, at::kInt);
     LQ_CALL(lq_verify_drafts, l.t->data_ptr(), l.t->stride(0), d.t ? d.t->data_ptr() : nullptr, d.t ? d.t->stride(0) : 0, (const int64_t *)tokens->data_ptr(),
             cu ? (const int32_t *)cu->data_ptr() : nullptr, batch, rows, vocab, most, l.dtype, temperature, accept ? (const float *)accept->data_ptr() : nullptr,
-            sample ? (const float *)sample->data_ptr() : nullptr, (int64_t *)out.data_ptr(), (int32_t *)accepted.data_ptr(), ws.data_ptr(), needed, on.stream);
+            sample ? (const float *)sample->data_ptr() : nullptr, (int64_t *)out.data_ptr(), (int32_t *)accepted.data_ptr(),
+            change ? (int32_t *)change->data_ptr() : nullptr, ws.data_ptr(), needed, on.stream);
     return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(accepted)));
 }
 

@@ -53,7 +53,7 @@ struct Verify {
     const int *cu;
     const float *accept, *sample;
     int64_t *out;
-    int *accepted;
+    int *accepted, *change;
     Stat *stats;
     Left *left;
     Chosen *chosen;
@@ -212,16 +212,16 @@ __device__ __forceinline__ float at_lane(float x, int lane) { return __int_as_fl
 __device__ __forceinline__ float wave_max(float x) { return at_lane(most_of<0x143, 0xc>(halves_most(x)), 63); }
 __device__ __forceinline__ double wave_sum(double x) { return at_lane(wave_scan(x), 63); }
 
-// Rows of a sequence: start .. start + n - 1, no more than max_tokens of them
-__device__ __forceinline__ void rows_of(const Verify &a, int seq, int &start, int &n) {
+// Rows of a sequence: start .. start + all - 1, the first n of them, no more than max_tokens, looked at
+__device__ __forceinline__ void rows_of(const Verify &a, int seq, int &start, int &n, int &all) {
     if (a.cu) {
         start = min(max(a.cu[seq], 0), a.rows);
-        n = min(max(a.cu[seq + 1], start), a.rows) - start;
+        all = min(max(a.cu[seq + 1], start), a.rows) - start;
     } else {
-        n = a.rows / a.batch;
-        start = seq * n;
+        all = a.rows / a.batch;
+        start = seq * all;
     }
-    n = min(n, a.most);
+    n = min(all, a.most);
 }
 
 // ---- every row: blockIdx.x for a slice, .y for a row, .z: 0 the target's, 1 the drafter's
@@ -478,12 +478,18 @@ __device__ __forceinline__ int first_refused(const Verify &a, const Exp2 &power,
 // A sequence without rows
 __device__ __forceinline__ void nothing(const Verify &a, int seq) {
     for (int i = threadIdx.x; i < a.most; i += kThreads) a.out[(int64_t)seq * a.most + i] = -1;
-    if (threadIdx.x == 0) a.accepted[seq] = 0;
+    if (threadIdx.x == 0) {
+        a.accepted[seq] = 0;
+        if (a.change) a.change[seq] = 0;
+    }
 }
 // Its taken drafts, and nothing behind the token that is drawn
-__device__ __forceinline__ void write_taken(const Verify &a, int seq, int start, int first) {
+__device__ __forceinline__ void write_taken(const Verify &a, int seq, int start, int all, int first) {
     int64_t *out = a.out + (int64_t)seq * a.most;
-    if (threadIdx.x == 0) a.accepted[seq] = first;
+    if (threadIdx.x == 0) {
+        a.accepted[seq] = first;
+        if (a.change) a.change[seq] = first + 1 - all;
+    }
     for (int i = threadIdx.x; i < a.most; i += kThreads)
         if (i != first) out[i] = i < first ? a.tokens[start + i + 1] : -1;
 }
@@ -500,11 +506,11 @@ template <int kType>
 __global__ __launch_bounds__(kThreads) void greedy_kernel(const Verify a) {
     __shared__ Board board;
     const int seq = blockIdx.x;
-    int start, n, base;
-    rows_of(a, seq, start, n);
+    int start, n, all, base;
+    rows_of(a, seq, start, n, all);
     if (n == 0) return nothing(a, seq);
     const int first = first_refused<kType, kGreedy>(a, Exp2(nullptr, 0.0), board, start, n, base);
-    write_taken(a, seq, start, first);
+    write_taken(a, seq, start, all, first);
     if (threadIdx.x == 0) a.out[(int64_t)seq * a.most + first] = board.best[first - base];
 }
 
@@ -514,8 +520,8 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(const Verify a) {
     __shared__ Board board;
     __shared__ double table[32], sums[2][kWaves];
     const int tid = threadIdx.x, seq = blockIdx.y;
-    int start, n, base;
-    rows_of(a, seq, start, n);
+    int start, n, all, base;
+    rows_of(a, seq, start, n, all);
     fill_table(table);
     if (n == 0) {
         if (blockIdx.x == 0) {
@@ -544,7 +550,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(const Verify a) {
         }
     }
     if (blockIdx.x == 0) {
-        write_taken(a, seq, start, first);
+        write_taken(a, seq, start, all, first);
         if (tid == 0) a.chosen[seq] = c;
     }
     mine = wave_sum(mine);
@@ -688,15 +694,15 @@ __global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
     __shared__ double table[32];
     __shared__ Draw draw;
     const int tid = threadIdx.x, seq = blockIdx.x;
-    int start, n, base;
-    rows_of(a, seq, start, n);
+    int start, n, all, base;
+    rows_of(a, seq, start, n, all);
     fill_table(table);
     if (n == 0) return nothing(a, seq);
     const double u = a.sample[seq];
     const Exp2 power(table, a.c);
     const int first = first_refused<kType, kAlone>(a, power, board, start, n, base);
     const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
-    write_taken(a, seq, start, first);
+    write_taken(a, seq, start, all, first);
     const Rest<kType, false> rest(a, power, c);
     if (tid < 64) {
         // The slice that had the draft, less the draft: what is left in all is 2^-24 and more, for a number under 1 refused it, and the difference is exact to 2^-53
@@ -773,7 +779,7 @@ extern "C" int lq_verify_drafts_plan(int64_t batch, int64_t rows, int64_t vocab,
 
 extern "C" int lq_verify_drafts(const void *logits, int64_t row_stride, const void *draft_logits, int64_t draft_row_stride, const int64_t *tokens, const int32_t *cu_tokens,
                                 int64_t batch, int64_t rows, int64_t vocab, int64_t max_tokens, int dtype, double temperature, const float *accept_draws, const float *sample_draws,
-                                int64_t *out, int32_t *accepted, void *workspace, int64_t workspace_bytes, void *stream) {
+                                int64_t *out, int32_t *accepted, int32_t *change, void *workspace, int64_t workspace_bytes, void *stream) {
     if (const int rc = sizes(batch, rows, vocab)) return rc;
     LQ_REQUIRE(dtype >= 0 && dtype <= 2, "verify_drafts: dtype must be 0 (bf16), 1 (f16) or 2 (f32), got %d", dtype);
     const bool greedy = temperature == 0.0;
@@ -790,7 +796,7 @@ extern "C" int lq_verify_drafts(const void *logits, int64_t row_stride, const vo
     LQ_REQUIRE(batch <= 65535, "verify_drafts: up to 65535 sequences, got %lld", (long long)batch);
     const Plan p = plan_of(batch, rows > 0 ? rows : 1, vocab, greedy, draft_logits != nullptr, lq_device_cu_count());
     LQ_REQUIRE(workspace && workspace_bytes >= p.bytes, "verify_drafts: needs a workspace of %lld bytes, got %lld", (long long)p.bytes, (long long)workspace_bytes);
-    Verify a{logits, greedy ? nullptr : draft_logits, row_stride, draft_row_stride, tokens, cu_tokens, accept_draws, sample_draws, out, accepted, (Stat *)workspace, nullptr, nullptr,
+    Verify a{logits, greedy ? nullptr : draft_logits, row_stride, draft_row_stride, tokens, cu_tokens, accept_draws, sample_draws, out, accepted, change, (Stat *)workspace, nullptr, nullptr,
              greedy ? 0.0 : 1.4426950408889634 / temperature, (int)batch, (int)rows, (int)vocab, (int)max_tokens, p.slices, p.span, p.blocks};
     a.left = (Left *)(a.stats + (rows > 0 ? rows : 1) * 2 * p.slices);
     a.chosen = (Chosen *)(a.left + batch * p.blocks);

@@ -178,10 +178,10 @@ class DeviceSequences:
     def verify(self, logits, tokens, step: Step, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0):
         """ops.verify_drafts of a step's rows, each sequence's first one a known token and the others drafts; refused drafts leave their sequences. Returns
         (accepted drafts, the token behind them and -1, int64 [batch, max_tokens]; how many were accepted, int32 [batch])."""
+        change = torch.empty_like(self.seq_lens)
         out, accepted = ops.verify_drafts(logits, tokens, step.cu_tokens, draft_logits=draft_logits, accept_draws=accept_draws, sample_draws=sample_draws,
-                                          temperature=temperature, max_tokens=step.max_tokens)
-        new = step.cu_tokens[1:] - step.cu_tokens[:-1]
-        self.give_back((new - accepted - 1).clamp_min(0))
+                                          temperature=temperature, max_tokens=step.max_tokens, change=change)
+        ops.kv8_resize(*self._books(), change, shared=self.shared)
         return out, accepted
 
 

@@ -1283,15 +1283,15 @@ def kv8_resize(block_table, seq_lens, free_blocks, free_count, change, *, rows=N
     return cu, positions, slots, status
 
 
-def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0, batch=None, max_tokens=None):
+def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0, batch=None, max_tokens=None, change=None):
     """Check drafted tokens against the target's logits and draw the token that follows the accepted ones (lq_verify_drafts; the rule:
     include/latentq.h). logits [rows, vocab] (bfloat16, float16, float32) are what the target gave for tokens (int64 [rows]); cu_tokens
     (int32 [batch + 1]) has each sequence's first row (without it: `batch` sequences of as many rows each, default one row each). Of a sequence's
     rows the first is a known token and the others are drafts, drawn from softmax(draft_logits / temperature) of the row before, or without draft_logits
     chosen in any other way. accept_draws (float32 [rows]) and sample_draws (float32 [batch]) are uniform numbers in [0, 1); temperature 0 takes the
-    largest logit and needs none. max_tokens: the largest number of rows of a sequence (default: what the rows allow). Returns (int64 [batch,
-    max_tokens]: accepted drafts, the token behind them, -1; int32 [batch]: how many drafts were accepted)."""
-    r = (_native or _fast()).verify_drafts(logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws, temperature, batch, max_tokens)
+    largest logit and needs none. max_tokens: the largest number of rows of a sequence (default: what the rows allow). change (int32 [batch], or
+    None) is filled with accepted + 1 - rows of each sequence, by which kv8_resize gives refused drafts back. Returns (int64 [batch, max_tokens]: accepted drafts, the token behind them, -1; int32 [batch]: how many drafts were accepted)."""
+    r = (_native or _fast()).verify_drafts(logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws, temperature, batch, max_tokens, change)
     if r is not None:
         return r
     if torch.jit.is_tracing():
@@ -1339,6 +1339,11 @@ def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_d
                 raise ValueError(f"{name} must be {(n,)} on the device of logits, got {tuple(t.shape)}")
         elif temperature > 0 and needed:
             raise ValueError(f"a temperature above 0 needs {name}")
+    if change is not None:
+        _chk(change, torch.int32, "change")
+        if change.device != logits.device or tuple(change.shape) != (batch,):
+            raise ValueError(f"change must be {(batch,)} on the device of logits, got {tuple(change.shape)}")
+        change.zero_()
     out = torch.full((batch, most), -1, dtype=torch.int64, device=logits.device)
     accepted = torch.zeros(batch, dtype=torch.int32, device=logits.device)
     if rows and batch:
@@ -1348,7 +1353,7 @@ def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_d
             slices, needed = ctypes.c_int(), ctypes.c_int64()
             _C.call("lq_verify_drafts_plan", batch, rows, vocab, int(temperature == 0), int(draft_logits is not None), 0, ctypes.addressof(slices), ctypes.addressof(needed))
             ws = torch.empty(needed.value, dtype=torch.uint8, device=logits.device)
-            ptr = [None if t is None else t.data_ptr() for t in (draft_logits, cu_tokens, accept_draws, sample_draws)]
+            ptr = [None if t is None else t.data_ptr() for t in (draft_logits, cu_tokens, accept_draws, sample_draws, change)]
             _C.call("lq_verify_drafts", logits.data_ptr(), logits.stride(0), ptr[0], 0 if draft_logits is None else draft_logits.stride(0), tokens.data_ptr(), ptr[1], batch, rows,
-                    vocab, most, _KV_TYPES[logits.dtype], temperature, ptr[2], ptr[3], out.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel(), _stream(logits))
+                    vocab, most, _KV_TYPES[logits.dtype], temperature, ptr[2], ptr[3], out.data_ptr(), accepted.data_ptr(), ptr[4], ws.data_ptr(), ws.numel(), _stream(logits))
     return out, accepted

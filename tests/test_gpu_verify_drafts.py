@@ -88,13 +88,14 @@ def check(verify, logits, tokens, cu, draft, accept, sample, heat, most=None, gi
     longest = max((b - a for a, b in zip(cu, cu[1:])), default=0)
     most = longest if most is None else most
     where = dict(batch=len(cu) - 1) if uniform else dict(max_tokens=most)
-    args = given or (logits, draft)
+    args, change = given or (logits, draft), torch.full((len(cu) - 1,), 99, dtype=torch.int32, device="cuda")
     out, accepted = verify(args[0], tokens, None if uniform else torch.tensor(cu, dtype=torch.int32, device="cuda"), draft_logits=args[1], accept_draws=accept, sample_draws=sample,
-                           temperature=heat, **where)
+                           temperature=heat, change=change, **where)
     want, counts = reference(logits, tokens, cu, draft, accept, sample, heat, most)
     assert out.dtype == torch.int64 and accepted.dtype == torch.int32
     assert accepted.tolist() == counts
     assert out.tolist() == want.tolist()
+    assert change.tolist() == [c + 1 - (b - a) if b > a else 0 for c, a, b in zip(counts, cu, cu[1:])]
     return counts
 
 
@@ -266,8 +267,9 @@ def test_tokens_are_distributed_as_the_targets(verify):
 def test_nothing_to_do(verify):
     empty = torch.empty((0, 10), device="cuda")
     none = torch.empty(0, dtype=torch.int64, device="cuda")
-    out, accepted = verify(empty, none, torch.zeros(4, dtype=torch.int32, device="cuda"), sample_draws=torch.rand(3, device="cuda"))
-    assert out.shape == (3, 0) and accepted.tolist() == [0, 0, 0]
+    change = torch.full((3,), 99, dtype=torch.int32, device="cuda")
+    out, accepted = verify(empty, none, torch.zeros(4, dtype=torch.int32, device="cuda"), sample_draws=torch.rand(3, device="cuda"), change=change)
+    assert out.shape == (3, 0) and accepted.tolist() == change.tolist() == [0, 0, 0]
     out, accepted = verify(empty, none)
     assert out.shape == (0, 0) and accepted.shape == (0,)
 
@@ -325,7 +327,8 @@ def test_refusals(verify):
     for kind, change in ((ValueError, dict(batch=4)), (ValueError, dict(batch=0)), (ValueError, dict(temperature=-1.0)), (ValueError, dict(temperature=float("nan"))),
                          (ValueError, dict(temperature=float("inf"))), (ValueError, dict(sample_draws=None)), (ValueError, dict(accept_draws=None)), (ValueError, dict(max_tokens=2)),
                          (ValueError, dict(draft_logits=draft[:, :99])), (ValueError, dict(draft_logits=draft.float())), (TypeError, dict(sample_draws=sample.double())),
-                         (ValueError, dict(sample_draws=sample[:1])), (ValueError, dict(accept_draws=accept[:5])), (ValueError, dict(draft_logits=draft.cpu()))):
+                         (ValueError, dict(sample_draws=sample[:1])), (ValueError, dict(accept_draws=accept[:5])), (ValueError, dict(draft_logits=draft.cpu())),
+                         (ValueError, dict(change=torch.zeros(3, dtype=torch.int32, device="cuda"))), (TypeError, dict(change=tokens[:2]))):
         with pytest.raises(kind):
             verify(logits, tokens, **{**good, **change})
     with pytest.raises(TypeError):

@@ -35,7 +35,7 @@ def test_resize_refuses(hip_lib, p, change, message):
 
 
 def verify_args(p, **change):
-    a = dict(logits=p, stride=100, draft=p, draft_stride=100, tokens=p, cu=None, batch=2, rows=6, vocab=100, most=3, dtype=0, temperature=1.0, accept=p, sample=p, out=p, accepted=p, ws=p,
+    a = dict(logits=p, stride=100, draft=p, draft_stride=100, tokens=p, cu=None, batch=2, rows=6, vocab=100, most=3, dtype=0, temperature=1.0, accept=p, sample=p, out=p, accepted=p, change=None, ws=p,
              ws_bytes=1 << 20, stream=None)
     a.update(change)
     return list(a.values())
