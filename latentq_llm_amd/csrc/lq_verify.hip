@@ -141,9 +141,6 @@ struct Exp2 {
         return ldexp(fma(e, s * r, e), k >> 5);
     }
 };
-__device__ __forceinline__ void fill_table(double *table) {
-    if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x * 0x1p-5);
-}
 
 // The same for whole rows, with a table of 1024 in device memory and a copy in shared memory: 2^(k/1024) 2^r to r^3, and the exponent added to the entry
 // at once (the table has k's lower bits taken off its upper words, so k << 10 needs no mask). Sixteen instructions an entry where Exp2 takes 21: the largest
@@ -181,6 +178,10 @@ template <int kCount>
 __device__ __forceinline__ void fill_powers(uint64_t *table) {
 #pragma unroll
     for (int i = 0; i < kPowers; i += 2 * kCount) *(ulonglong2 *)(table + i + 2 * threadIdx.x) = *(const ulonglong2 *)(kPowersOfTwo.of + i + 2 * threadIdx.x);
+}
+
+__device__ __forceinline__ void fill_table(double *table) {
+    if (threadIdx.x < 32) table[threadIdx.x] = __builtin_bit_cast(double, kPowersOfTwo.of[threadIdx.x * (kPowers / 32)] + ((uint64_t)threadIdx.x * (kPowers / 32) << 42));
 }
 
 // The reference of a row's exponents: its maximum, or anything where the row is masked as a whole
@@ -400,16 +401,18 @@ struct Board {  // in shared memory
     float row_m[2][kRound];  // (without the drafter's logits, the second one: the logit of the draft)
     int64_t best[kRound];
     int refused;
+    __device__ __forceinline__ void begin() {
+        if (threadIdx.x == 0) refused = INT32_MAX;
+        __syncthreads();
+    }
 };
 
 // The rows' tests, by all waves of a workgroup: the first row of the sequence whose draft is not taken, or its last one. A wave has a row at a time: its
-// slices lie in the lanes of a half, the drafter's in the other, and what the test needs besides is on its way with them.
+// slices lie in the lanes of a half, the drafter's in the other, and what the test needs besides is on its way with them. (b.refused: nobody's, as begin() leaves it.)
 template <int kType, int kMode>
 __device__ __forceinline__ int first_refused(const Verify &a, const Exp2 &power, Board &b, int start, int n, int &base) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     for (base = 0;; base += kRound) {
-        if (threadIdx.x == 0) b.refused = INT32_MAX;
-        __syncthreads();
         const int count = min(kRound, n - base);
         for (int i = wave; i < count; i += kWaves) {
             const int row = start + base + i;
@@ -509,6 +512,7 @@ __global__ __launch_bounds__(kThreads) void greedy_kernel(const Verify a) {
     int start, n, all, base;
     rows_of(a, seq, start, n, all);
     if (n == 0) return nothing(a, seq);
+    board.begin();
     const int first = first_refused<kType, kGreedy>(a, Exp2(nullptr, 0.0), board, start, n, base);
     write_taken(a, seq, start, all, first);
     if (threadIdx.x == 0) a.out[(int64_t)seq * a.most + first] = board.best[first - base];
@@ -530,6 +534,7 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(const Verify a) {
         }
         return;
     }
+    board.begin();
     const Exp2 power(table, a.c);
     const int first = first_refused<kType, kBoth>(a, power, board, start, n, base);
     const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
@@ -575,13 +580,13 @@ struct Draw {  // in shared memory
     int part, of_rest, first[kWaves], last[kWaves];
 };
 
-// The part of a row in which the sum passes the number, of parts whose sums one wave has in its lanes (part(i): of what is left, and of all), and how
+// The part of a row in which the sum passes the number, of parts whose sums one wave has in its lanes (own: of what is left, and of all; part(i) beyond the first 64), and how
 // much of the number is left in it. Where roundings leave none, the last one that has any; -1: no part has any.
 template <typename Part>
-__device__ __forceinline__ void find_part(Draw &d, int parts, double u, const Part &part) {
+__device__ __forceinline__ void find_part(Draw &d, int parts, double u, const Left &own, const Part &part) {
     const int lane = threadIdx.x & 63;
-    double rest = 0.0, all = 0.0;
-    for (int i = lane; i < parts; i += 64) {
+    double rest = own.rest, all = own.all;
+    for (int i = lane + 64; i < parts; i += 64) {
         const Left l = part(i);
         rest += l.rest;
         all += l.all;
@@ -593,8 +598,8 @@ __device__ __forceinline__ void find_part(Draw &d, int parts, double u, const Pa
     double before = 0.0, below = 0.0;
     int found = -1, last = -1;
     for (int base = 0; base < parts && found < 0; base += 64) {
-        Left l{0.0, 0.0};
-        if (base + lane < parts) l = part(base + lane);
+        Left l = own;
+        if (base) l = base + lane < parts ? part(base + lane) : Left{0.0, 0.0};
         const double x = use ? l.rest : l.all, upto = wave_scan(x);
         const uint64_t passed = __ballot(x > 0.0 && before + upto > limit), some = __ballot(x > 0.0);
         if (passed) {
@@ -675,9 +680,11 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const Verify a) {
     const int seq = blockIdx.x;
     const Chosen c = a.chosen[seq];
     const Left *left = a.left + (int64_t)seq * a.blocks;
+    Left own{0.0, 0.0};
+    if (threadIdx.x < 64 && (int)threadIdx.x < a.blocks) own = left[threadIdx.x];  // (on its way with the row)
     fill_table(table);
     if (c.row < 0) return;
-    if (threadIdx.x < 64) find_part(draw, a.blocks, a.sample[seq], [&](int i) { return left[i]; });
+    if (threadIdx.x < 64) find_part(draw, a.blocks, a.sample[seq], own, [&](int i) { return left[i]; });
     __syncthreads();
     if (draw.part < 0) {  // a row that is masked as a whole
         if (threadIdx.x == 0) *c.to = -1;
@@ -699,6 +706,7 @@ __global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
     fill_table(table);
     if (n == 0) return nothing(a, seq);
     const double u = a.sample[seq];
+    board.begin();
     const Exp2 power(table, a.c);
     const int first = first_refused<kType, kAlone>(a, power, board, start, n, base);
     const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
@@ -709,10 +717,11 @@ __global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
         const int without = c.draft >= 0 ? c.draft / a.span : -1;
         const double of_draft = power(c.q_m, rest.p_m) * rest.p_by;
         const Stat *s = a.stats + (int64_t)c.row * 2 * a.slices;
-        find_part(draw, a.slices, u, [&](int i) {
+        const auto part = [&](int i) {
             const double all = s[i].sum * power(s[i].m, rest.p_m) * rest.p_by;
             return Left{i == without ? fmax(all - of_draft, 0.0) : all, all};
-        });
+        };
+        find_part(draw, a.slices, u, tid < a.slices ? part(tid) : Left{0.0, 0.0}, part);
     }
     __syncthreads();
     if (draw.part < 0) {
