@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kStats = 256;             // threads of a workgroup on a slice
 constexpr int kThreads = 512, kWaves = 8;  // on a sequence
-constexpr int kEach = 8, kBlock = kThreads * kEach;  // entries of a thread, and of a block of the row that a token is drawn from
+constexpr int kEach = 8, kTurn = kThreads * kEach;  // entries of a thread, and of all of them
 constexpr int kRound = 32;              // rows of a sequence that are tested together
 constexpr float kMost = 3.402823466e38f;
 
@@ -58,7 +58,7 @@ struct Verify {
     Left *left;
     Chosen *chosen;
     double c;  // log2(e) / T
-    int batch, rows, vocab, most, slices, span, blocks;
+    int batch, rows, vocab, most, slices, span, block, blocks;  // block: entries of a block of the row that a token is drawn from
 };
 
 // A logit as it counts: NaN is masked, infinity the largest number
@@ -540,10 +540,10 @@ __global__ __launch_bounds__(kThreads) void rest_kernel(const Verify a) {
     const Chosen c = chosen_row(a, board, seq, start, n, first, first - base);
     const Rest<kType, true> rest(a, power, c);
     constexpr int kVec = Row<kType>::kVec;
-    const int begin = blockIdx.x * kBlock, end = min(begin + kBlock, a.vocab);
+    const int begin = blockIdx.x * a.block, end = min(begin + a.block, a.vocab);
     double mine = 0.0, whole = 0.0;
 #pragma unroll
-    for (int v = 0; v < kEach; v += kVec) {
+    for (int v = 0; v < kEach; v += kVec) {  // (a block is kTurn entries at most)
         const int j = begin + v * kThreads + tid * kVec;
         if (j >= end) break;
         double x[kVec], y[kVec];
@@ -626,14 +626,16 @@ __device__ __forceinline__ void find_entry(Draw &d, const Rest<kType, kQ> &rest,
     const double below = d.below;
     double before = 0.0;
     int token = -1;
-    for (int at = begin; at < end; at += kBlock) {
+    for (int at = begin; at < end; at += kTurn) {
         const int j0 = at + tid * kEach;
-        double x[kEach], all[kEach], mine = 0.0;
-        rest.some(j0, end, x, all);
+        double x[kEach] = {}, all[kEach], mine = 0.0;
+        if (j0 < end) {
+            rest.some(j0, end, x, all);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (!of_rest) x[i] = all[i];
-            mine += x[i];
+            for (int i = 0; i < kEach; ++i) {
+                if (!of_rest) x[i] = all[i];
+                mine += x[i];
+            }
         }
         const double upto = wave_scan(mine);
         if (lane == 63) d.sums[wave] = upto;
@@ -690,8 +692,8 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(const Verify a) {
         if (threadIdx.x == 0) *c.to = -1;
         return;
     }
-    const int begin = draw.part * kBlock;
-    find_entry(draw, Rest<kType, true>(a, Exp2(table, a.c), c), begin, min(begin + kBlock, a.vocab), c.to);
+    const int begin = draw.part * a.block;
+    find_entry(draw, Rest<kType, true>(a, Exp2(table, a.c), c), begin, min(begin + a.block, a.vocab), c.to);
 }
 
 // ---- without them: a workgroup for a sequence
@@ -735,13 +737,16 @@ __global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
 constexpr int kPiece = 2048;  // entries of the smallest slice
 
 struct Plan {
-    int slices, span, blocks;
+    int slices, span, block, blocks;
     int64_t bytes;
 };
 
 Plan plan_of(int64_t batch, int64_t rows, int64_t vocab, bool greedy, bool draft, int cus) {
     Plan p{};
-    p.blocks = draft && !greedy ? (int)((vocab + kBlock - 1) / kBlock) : 0;
+    // Blocks of the rows that tokens are drawn from: half as long where that leaves three workgroups to a compute unit or fewer, for the last launch has one of them to a
+    // sequence, and its exponentials in turn. us with 2048 / 4096, 5 rows a sequence: 8 sequences of 32000 13.7 / 15.1, 48 25.2 / 26.5, 64 30.8 / 29.6; 16 of 100003 27.6 / 27.1.
+    p.block = batch * ((vocab + kTurn / 2 - 1) / (kTurn / 2)) <= 3 * cus ? kTurn / 2 : kTurn;
+    p.blocks = draft && !greedy ? (int)((vocab + p.block - 1) / p.block) : 0;
     const int64_t items = rows * (draft && !greedy ? 2 : 1), wanted = ((int64_t)cus * 4 + items - 1) / items, pieces = (vocab + kPiece - 1) / kPiece;
     p.span = (int)(std::min((pieces + wanted - 1) / wanted, (int64_t)4) * kPiece);
     p.slices = (int)((vocab + p.span - 1) / p.span);
@@ -806,7 +811,7 @@ extern "C" int lq_verify_drafts(const void *logits, int64_t row_stride, const vo
     const Plan p = plan_of(batch, rows > 0 ? rows : 1, vocab, greedy, draft_logits != nullptr, lq_device_cu_count());
     LQ_REQUIRE(workspace && workspace_bytes >= p.bytes, "verify_drafts: needs a workspace of %lld bytes, got %lld", (long long)p.bytes, (long long)workspace_bytes);
     Verify a{logits, greedy ? nullptr : draft_logits, row_stride, draft_row_stride, tokens, cu_tokens, accept_draws, sample_draws, out, accepted, change, (Stat *)workspace, nullptr, nullptr,
-             greedy ? 0.0 : 1.4426950408889634 / temperature, (int)batch, (int)rows, (int)vocab, (int)max_tokens, p.slices, p.span, p.blocks};
+             greedy ? 0.0 : 1.4426950408889634 / temperature, (int)batch, (int)rows, (int)vocab, (int)max_tokens, p.slices, p.span, p.block, p.blocks};
     a.left = (Left *)(a.stats + (rows > 0 ? rows : 1) * 2 * p.slices);
     a.chosen = (Chosen *)(a.left + batch * p.blocks);
     hipStream_t s = (hipStream_t)stream;
