@@ -734,8 +734,6 @@ __global__ __launch_bounds__(kThreads) void alone_kernel(const Verify a) {
     find_entry(draw, rest, begin, min(begin + a.span, a.vocab), c.to);
 }
 
-constexpr int kPiece = 2048;  // entries of the smallest slice
-
 struct Plan {
     int slices, span, block, blocks;
     int64_t bytes;
@@ -747,8 +745,14 @@ Plan plan_of(int64_t batch, int64_t rows, int64_t vocab, bool greedy, bool draft
     // sequence, and its exponentials in turn. us with 2048 / 4096, 5 rows a sequence: 8 sequences of 32000 13.7 / 15.1, 48 25.2 / 26.5, 64 30.8 / 29.6; 16 of 100003 27.6 / 27.1.
     p.block = batch * ((vocab + kTurn / 2 - 1) / (kTurn / 2)) <= 3 * cus ? kTurn / 2 : kTurn;
     p.blocks = draft && !greedy ? (int)((vocab + p.block - 1) / p.block) : 0;
-    const int64_t items = rows * (draft && !greedy ? 2 : 1), wanted = ((int64_t)cus * 4 + items - 1) / items, pieces = (vocab + kPiece - 1) / kPiece;
-    p.span = (int)(std::min((pieces + wanted - 1) / wanted, (int64_t)4) * kPiece);
+    // Slices of the rows: half as long or a quarter while the workgroups are not too many. Without the drafter's logits the last launch has one to a sequence, which looks
+    // through a slice by itself, so more of them pay. us with 2048 / 4096 / 8192, 5 rows a sequence, without: 16 sequences of 32000 10.5 / 10.9, 32 13.1 / 12.5,
+    // 64 - / 17.1 / 18.7, 128 - / 27.4 / 25.4; of 100003 8 12.0 / 11.7, 16 16.6 / 15.2 / 17.6, 32 - / 21.1 / 23.5; with: 32 of 32000 - / 21.2 / 20.9, 64 - / 31.5 / 29.6; of 100003
+    // 4 15.7 / 15.0, 8 21.3 / 19.4 / 19.0.
+    const bool both = draft && !greedy;
+    const int64_t items = rows * (both ? 2 : 1);
+    const auto within = [&](int span, int units) { return items * ((vocab + span - 1) / span) <= (int64_t)units * cus; };
+    p.span = within(2048, both ? 5 : 7) ? 2048 : within(4096, both ? 6 : 16) ? 4096 : 8192;
     p.slices = (int)((vocab + p.span - 1) / p.span);
     p.bytes = rows * 2 * p.slices * (int64_t)sizeof(Stat) + (p.blocks ? batch * (p.blocks * (int64_t)sizeof(Left) + (int64_t)sizeof(Chosen)) : 0);
     return p;

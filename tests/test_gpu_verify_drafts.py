@@ -229,8 +229,8 @@ def test_drafts_outside_the_vocabulary(verify):
 @pytest.mark.parametrize("with_draft", [False, True])
 def test_many_sequences(verify, with_draft):
     """Rows enough for the longest slices and blocks, of 8192 and 4096 entries, and a vocabulary that ends inside one."""
-    (logits, tokens, draft, accept), gen = inputs(390, 20001, "bf16", 15, with_draft)
-    check(verify, logits, tokens, list(range(0, 391, 3)), draft, accept, torch.rand(130, generator=gen).cuda(), 1.0)
+    (logits, tokens, draft, accept), gen = inputs(900, 20001, "bf16", 15, with_draft)
+    check(verify, logits, tokens, list(range(0, 901, 3)), draft, accept, torch.rand(300, generator=gen).cuda(), 1.0)
 
 
 @pytest.mark.parametrize("heat", [0.0, 1.0])
