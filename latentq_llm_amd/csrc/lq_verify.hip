@@ -283,14 +283,14 @@ __global__ __launch_bounds__(kStats) void stats_kernel(const Verify a) {
         }
     } else {
         // kMine entries at a time, in pieces that the workgroup has side by side, requested a turn ahead; then what is left piece by piece
-        constexpr int kPieces = 2, kMine = kPieces * kVec, kTurn = kMine * kStats;
+        constexpr int kPieces = 2, kMine = kPieces * kVec, kAtOnce = kMine * kStats;
         int j = begin + (int)threadIdx.x * kVec;
         u32x4_t w[kPieces];
         const auto request = [&] {
 #pragma unroll
             for (int v = 0; v < kPieces; ++v) w[v] = x.piece(j + v * kStats * kVec);
         };
-        bool whole = j + kTurn - kStats * kVec + kVec <= end;
+        bool whole = j + kAtOnce - kStats * kVec + kVec <= end;
         if (whole) request();
         const bool names = slice == 0 && threadIdx.x == 3 && row + 1 < a.rows;
         const int64_t token = names ? a.tokens[row + 1] : -1;
@@ -319,8 +319,8 @@ __global__ __launch_bounds__(kStats) void stats_kernel(const Verify a) {
             float f[kMine];
 #pragma unroll
             for (int v = 0; v < kPieces; ++v) x.values(w[v], f + v * kVec);
-            j += kTurn;
-            whole = j + kTurn - kStats * kVec + kVec <= end;
+            j += kAtOnce;
+            whole = j + kAtOnce - kStats * kVec + kVec <= end;
             if (whole) request();
             add(f);
         }
