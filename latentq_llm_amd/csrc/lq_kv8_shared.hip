@@ -12,6 +12,9 @@
 // keys, 32 heads on 8: 268 MB became 536, 93 us, 65 with). Tiles that become halves once in shared memory for 128 rows, as in lq_kv8_prompt.hip, have a third fewer vector
 // instructions and were slower or level at all sizes: 64 rows of 128 dimensions 71 / 64 us, 64 x 8192 of 64 dimensions 31.6 / 24.2, of 96 37 / 33, 1024 rows of 128 48.8 / 50.2. 64 rows to a
 // wave do not fit (80 bytes spilled; 93 us).
+//
+// Bound: 64 rows of 128 dimensions on 131072 keys 59 us, 4.7 TB/s, with the vector units 52 % and the matrix units 30 % busy; 12 sequences behind 2048 keys with up to
+// 1019 of their own, 32 heads of 128, 18.4 us, 4.6 TB/s; 64 behind 8192, 32 heads on 8, 23.8 us, the vector units 56 % and the matrix units 22 %. The join is 4 to 5.
 #include "lq_kv8.h"
 
 #include <algorithm>
