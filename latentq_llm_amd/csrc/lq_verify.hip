@@ -151,7 +151,7 @@ struct Exp2 {
 // r^4/24, which is cut off, is taken as r^2 h^2/24 (|r| <= h = ln(2)/2048): what is left is within 1.4e-16.
 constexpr int kPowers = 1024;
 struct Powers {
-    uint64_t of[kPowers];
+    alignas(16) uint64_t of[kPowers];
     constexpr Powers() : of() {
         for (int j = 0; j < kPowers; ++j) {
             const double x = j * (0x1.62e42fefa39efp-1 / kPowers);  // e^x by its series

@@ -164,7 +164,8 @@ class DeviceSequences:
     def extend(self, new, rows: int, max_tokens: int | None = None, max_len: int | None = None) -> Step:
         """Make room for new[i] more tokens of sequence i (int32 [batch] on the device, none negative) and describe the pass that appends them. `rows`
         is the number of rows that the pass has, as many as there are new tokens or more; max_tokens and max_len bound a sequence's
-        new tokens and its length (defaults: rows, the capacity). Where step.status is not 0 nothing has changed and the pass has no tokens."""
+        new tokens and its length (defaults: rows, the capacity). Where step.status is not 0 nothing has changed and the pass has no tokens. The
+        step names the tables themselves: it describes the pass until they are changed again."""
         cu, positions, slots, status = ops.kv8_resize(*self._books(), new, rows=rows, shared=self.shared)
         return Step(block_table=self.block_table, seq_lens=self.seq_lens, cu_tokens=cu, max_tokens=rows if max_tokens is None else max_tokens,
                     max_len=self.capacity if max_len is None else max_len, last=(cu[1:].long() - 1).clamp_min(0), positions=positions, longest=self.capacity,
