@@ -260,11 +260,13 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         }
         const int key0 = t * KV8_BLOCK;
         const bool no_values = kv8_no_values(vs);
-        const float vs_least = no_values ? kLeastScale : vs, lv = __builtin_amdgcn_logf(vs_least), rv = __builtin_amdgcn_rcpf(vs_least);
+        const float vs_least = no_values ? kLeastScale : vs, log_scale = __builtin_amdgcn_logf(vs_least), reciprocal = __builtin_amdgcn_rcpf(vs_least);
         f16x8_t p[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            float lv = log_scale, rv = reciprocal;
             if (__any(key0 + KV8_BLOCK - 1 > last[rt])) {
+                if (key0 > last[rt]) lv = rv = 0.0f;  // nothing of the tile is the row's, whatever its scale is
 #pragma unroll
                 for (int tg = 0; tg < 4; ++tg)
 #pragma unroll

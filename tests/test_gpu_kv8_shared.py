@@ -138,6 +138,38 @@ def test_scales_far_apart(hip_lib, dim, batch):
     run(14, [1 + 37 * (i % 5) for i in range(batch)], [1] * batch, 4, 2, dim, BF16, seed=dim + batch, cache=cache)
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("batch, tokens", [(4, 1), (30, 1), (6, 5)])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_blocks_that_a_sequence_does_not_see(hip_lib, kind, batch, tokens, dim):
+    """Scales that are no numbers, of shared blocks behind a sequence's end and of own blocks behind a token's last key, are nothing to it."""
+    lens = [64 * 16 + 70 if i % 3 == 0 else 64 * 14 + i - 1 for i in range(batch)]
+    cache = ref.Cache(18 + 2 * batch, 2, dim, seed=dim)
+    table = table_of(lens, 16, 18 + 2 * batch, 1)
+    q = rows((batch * tokens, 4, dim), BF16, 2)
+    want, (want_lse, lse_bound), bound = ref.attention(cache, q, table, lens, [tokens] * batch)
+    bound = bound + (max(lens) / 32 + 4) * 2.0 ** -24 * 255 * cache.scale[1].max()
+    short = [i * tokens + j for i in range(batch) if lens[i] <= 64 * 15 for j in range(tokens)]
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        tensors = cache.tensors()
+        tensors[2 + kind][i32(table[0, 15:16]).long()] = bad
+        out, lse = call(tensors, q, table, lens, [tokens] * batch, 16, return_lse=True)
+        holds(out[short], want[short], bound[short])
+        assert (np.abs(lse.cpu().double().numpy() - want_lse)[short] <= lse_bound[short]).all()
+    # five tokens of which the last one alone sees the third own block
+    lens = [64 * 18 + 1] * batch
+    table = table_of(lens, 15, 18 + 4 * batch, 1)
+    cache = ref.Cache(18 + 4 * batch, 2, dim, seed=dim)
+    q = rows((batch * 5, 4, dim), BF16, 2)
+    want, _, bound = ref.attention(cache, q, table, lens, [5] * batch)
+    bound = bound + (max(lens) / 32 + 4) * 2.0 ** -24 * 255 * cache.scale[1].max()
+    tensors = cache.tensors()
+    tensors[2 + kind][i32(table[:, 18]).long()] = float("nan")
+    out = call(tensors, q, table, lens, [5] * batch, 15)
+    seen = [i for i in range(5 * batch) if i % 5 < 4]
+    holds(out[seen], want[seen], bound[seen])
+
+
 def test_scores_far_apart(hip_lib):
     """Scores to some hundreds: the largest ones in the prefix for some rows, among their own keys for others."""
     def cache(pool):
