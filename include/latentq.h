@@ -522,7 +522,7 @@ int lq_weight_grad_plan(int form, int64_t M, int64_t N, int64_t K, int compute_u
  * rows (null: every sequence has tokens / batch). The new tokens of sequence i are its last n_i =
  * cu_tokens[i + 1] - cu_tokens[i]; token t of them is at position seq_lens[i] - n_i + t. max_tokens >= every n_i and max_len >= every
  * seq_lens[i] are host values that size the launch (rows beyond max_tokens of a sequence are not computed; a max_len
- * that is too small costs time, not correctness).
+ * that is too small costs time, not correctness). What the outputs hold in those rows, and in rows that no sequence has, stays as it is.
  * dtype: 0 = bf16, 1 = f16. Strides are in elements, multiples of 8; the last dimension is contiguous; q, k, v, outputs,
  * rotation tables and codes are 16-byte aligned. What the kernels read on the device is kept inside the operands: a
  * block_table entry outside the pool is read as the last block and never written to, tokens beyond table_width blocks or before

@@ -740,12 +740,23 @@ PyObject *kv8_append(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     return a[13];
 }
 
-// q, cache (4), block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, causal, window, return_lse, workspace -> out, or (out, lse);
+// What attention writes: the caller's rows (o, from an operand that is not None), or some that are made
+bool given_rows(PyObject *o_out, Rows16 &o, const Rows16 &q) {
+    return o_out == Py_None || (o.load(o_out) && same_device(o.t, q.t) && o.dtype == q.dtype && o.t->sizes() == q.t->sizes() && o.separate());
+}
+PyObject *attended(PyObject *o_out, at::Tensor &made, at::Tensor &lse) {
+    PyObject *out = o_out;
+    if (made.defined()) out = wrap(std::move(made));
+    else Py_INCREF(out);
+    return lse.defined() ? Py_BuildValue("NN", out, wrap(std::move(lse))) : out;
+}
+
+// q, cache (4), block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, causal, window, return_lse, out, workspace -> out, or (out, lse);
 // without a workspace where one is wanted: its bytes, and nothing is done
 PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    LQ_ARGS(15)
+    LQ_ARGS(16)
     if (watched()) return none();
-    Rows16 q;
+    Rows16 q, o;
     Cache8 c;
     Sequences s;
     if (!q.load(a[0]) || !c.load(a + 1) || !same_device(q.t, c.kc) || q.t->size(2) != c.dim || q.t->size(1) % c.heads) return none();
@@ -763,7 +774,7 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     if (PyErr_Occurred() || !(scale > 0.0 && scale <= 3.4e38) || window < 0) return none();
     void *ws;
     int64_t ws_bytes;
-    if (!workspace(a[14], q.t, &ws, &ws_bytes)) return none();
+    if (!given_rows(a[14], o, q) || !workspace(a[15], q.t, &ws, &ws_bytes)) return none();
     On on(*c.kc);
     if (!ws) {
         int kernel, parts;
@@ -774,21 +785,24 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
             return fail("lq_kv8_attention_plan", rc);
         if (needed) return PyLong_FromLongLong(needed);
     }
-    at::Tensor out = make(q.t->sizes(), q.t->scalar_type(), *q.t), lse;
+    at::Tensor made, lse;
+    if (!o.t) {
+        made = make(q.t->sizes(), q.t->scalar_type(), *q.t);
+        o.t = &made;
+    }
     if (with_lse) lse = make({tokens, heads}, at::kFloat, *q.t);
     LQ_CALL(lq_kv8_attention, q.t->data_ptr(), q.t->stride(0), q.t->stride(1), c.kc->data_ptr(), c.vc->data_ptr(), (const float *)c.ks->data_ptr(),
             (const float *)c.vs->data_ptr(), c.blocks, (const int32_t *)s.table->data_ptr(), s.width, (const int32_t *)s.lens->data_ptr(), s.cu, s.batch, tokens,
-            s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, window, out.data_ptr(), out.stride(0), out.stride(1),
+            s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, window, o.t->data_ptr(), o.t->stride(0), o.t->stride(1),
             with_lse ? (float *)lse.data_ptr() : nullptr, ws, ws_bytes, on.stream);
-    if (!with_lse) return wrap(std::move(out));
-    return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
+    return attended(a[14], made, lse);
 }
 
-// q, cache (4), block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse -> out, or (out, lse)
+// q, cache (4), block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse, out -> out, or (out, lse)
 PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
-    LQ_ARGS(14)
+    LQ_ARGS(15)
     if (watched()) return none();
-    Rows16 q;
+    Rows16 q, o;
     Cache8 c;
     Sequences s;
     if (!q.load(a[0]) || !c.load(a + 1) || !same_device(q.t, c.kc) || q.t->size(2) != c.dim || q.t->size(1) % c.heads) return none();
@@ -803,7 +817,7 @@ PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     }
     const double scale = a[11] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(a[11]);
     const int causal = PyObject_IsTrue(a[12]), with_lse = PyObject_IsTrue(a[13]);
-    if (PyErr_Occurred() || !(scale > 0.0 && scale <= 3.4e38) || shared < 0 || shared > s.width) return none();
+    if (PyErr_Occurred() || !(scale > 0.0 && scale <= 3.4e38) || shared < 0 || shared > s.width || !given_rows(a[14], o, q)) return none();
     On on(*c.kc);
     int prefix, own;
     int64_t needed;
@@ -811,14 +825,17 @@ PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs)
         return fail("lq_kv8_attention_shared_plan", rc);
     at::Tensor ws;
     if (needed) ws = make({needed}, at::kByte, *q.t);
-    at::Tensor out = make(q.t->sizes(), q.t->scalar_type(), *q.t), lse;
+    at::Tensor made, lse;
+    if (!o.t) {
+        made = make(q.t->sizes(), q.t->scalar_type(), *q.t);
+        o.t = &made;
+    }
     if (with_lse) lse = make({tokens, heads}, at::kFloat, *q.t);
     LQ_CALL(lq_kv8_attention_shared, q.t->data_ptr(), q.t->stride(0), q.t->stride(1), c.kc->data_ptr(), c.vc->data_ptr(), (const float *)c.ks->data_ptr(),
             (const float *)c.vs->data_ptr(), c.blocks, (const int32_t *)s.table->data_ptr(), s.width, (const int32_t *)s.lens->data_ptr(), s.cu, s.batch, tokens,
-            s.most, max_len, shared, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, out.data_ptr(), out.stride(0), out.stride(1),
+            s.most, max_len, shared, (int)heads, (int)c.heads, (int)c.dim, q.dtype, (float)scale, causal, o.t->data_ptr(), o.t->stride(0), o.t->stride(1),
             with_lse ? (float *)lse.data_ptr() : nullptr, needed ? ws.data_ptr() : nullptr, needed, on.stream);
-    if (!with_lse) return wrap(std::move(out));
-    return Py_BuildValue("NN", wrap(std::move(out)), wrap(std::move(lse)));
+    return attended(a[14], made, lse);
 }
 
 // cache (4), blocks, dtype as the C entry points number them -> (k, v)

@@ -51,13 +51,15 @@ class KVCache8:
 
     def attend(self, q, step: "Step", scale=None, window=0):
         """ops.kv8_attention of a step's new tokens over what the cache holds of their sequences (kv8_attention_shared of sequences that
-        begin with blocks in common)."""
+        begin with blocks in common). Rows that have no token are zeros."""
         self._holds(step)
+        # (what follows may look at all rows, as a projection does that finds one scale for all of them)
+        out = torch.zeros_like(q, memory_format=torch.contiguous_format) if step.padded and step.cu_tokens is not None else None
         if step.shared and not window:
             return ops.kv8_attention_shared(q, *self.tensors(), step.block_table, step.seq_lens, step.shared, cu_tokens=step.cu_tokens, max_tokens=step.max_tokens,
-                                            max_len=step.max_len, scale=scale)
+                                            max_len=step.max_len, scale=scale, out=out)
         return ops.kv8_attention(q, *self.tensors(), step.block_table, step.seq_lens, cu_tokens=step.cu_tokens, max_tokens=step.max_tokens,
-                                 max_len=step.max_len, scale=scale, window=window)
+                                 max_len=step.max_len, scale=scale, window=window, out=out)
 
     def read(self, blocks, dtype=torch.bfloat16):
         """ops.kv8_read: (keys, values) [n, 64, kv_heads, head_dim] of blocks."""
@@ -79,6 +81,7 @@ class Step:
     pool: int = 0              # blocks that a cache must have: the highest one named, and 1 (0: as above)
     shared: int = 0            # blocks that all the sequences begin with
     slots: torch.Tensor | None = None   # int64 [rows]: block * 64 + place of each new token (of DeviceSequences; -1 behind the last)
+    padded: bool = True        # with cu_tokens: there may be rows that no sequence has, behind the last one's
     status: torch.Tensor | None = None  # int32 [1]: of ops.kv8_resize (of DeviceSequences)
 
 
@@ -129,7 +132,7 @@ class Sequences:
                     cu_tokens=None if len(set(counts)) == 1 else torch.tensor(starts, **i32), max_tokens=max(counts), max_len=max(lens.values()),
                     last=torch.tensor(starts[1:], device=self.device) - 1,
                     positions=torch.cat([torch.arange(lens[s] - n, lens[s]) for s, n in new.items()]).to(self.device),
-                    longest=max(lens.values()), pool=1 + max(max(self._blocks[s]) for s in new))
+                    longest=max(lens.values()), pool=1 + max(max(self._blocks[s]) for s in new), padded=False)
 
 
 class DeviceSequences:
@@ -163,7 +166,8 @@ class DeviceSequences:
 
     def extend(self, new, rows: int, max_tokens: int | None = None, max_len: int | None = None) -> Step:
         """Make room for new[i] more tokens of sequence i (int32 [batch] on the device, none negative) and describe the pass that appends them. `rows`
-        is the number of rows that the pass has, as many as there are new tokens or more; max_tokens and max_len bound a sequence's
+        is the number of rows that the pass has, as many as there are new tokens or more: those behind them belong to no sequence, but a layer that finds one scale for all rows
+        of its input (QLinearA8W8 as constructed) sees what the caller puts there. max_tokens and max_len bound a sequence's
         new tokens and its length (defaults: rows, the capacity). Where step.status is not 0 nothing has changed and the pass has no tokens. The
         step names the tables themselves: it describes the pass until they are changed again."""
         cu, positions, slots, status = ops.kv8_resize(*self._books(), new, rows=rows, shared=self.shared)

@@ -1178,14 +1178,15 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
     softmax(scale * q K^T) V, scale 1 / sqrt(dim) by default, query head j on kv head j // (heads // kv_heads). A row sees
     the positions up to its own (causal=False: the whole sequence), with window > 0 none before the last `window` up to its own; one that sees
     nothing gives zeros. max_tokens and max_len, the largest numbers of new tokens and of tokens of a sequence, size the launch
-    (defaults: what the rows and the block table allow). return_lse: also the logarithm of the softmax's denominator, float32 [tokens, heads]."""
-    if out is None:
-        args = (q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, causal, window, return_lse)
-        r = (_native or _fast()).kv8_attention(*args, None)
-        if type(r) is int:  # the bytes that its parts want
-            r = _native.kv8_attention(*args, _workspace(q, 1, -(-r // 32))[0])
-        if r is not None:
-            return r
+    (defaults: what the rows and the block table allow). return_lse: also the logarithm of the softmax's denominator, float32 [tokens, heads].
+    Rows that no sequence has, as behind cu_tokens[batch], and a sequence's beyond max_tokens are not written: they are as `out` had them, and without `out` whatever the
+    memory held."""
+    args = (q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, causal, window, return_lse, out)
+    r = (_native or _fast()).kv8_attention(*args, None)
+    if type(r) is int:  # the bytes that its parts want
+        r = _native.kv8_attention(*args, _workspace(q, 1, -(-r // 32))[0])
+    if r is not None:
+        return r
     n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
                                                                                        scale, out)
     tokens, heads = q.shape[0], q.shape[1]
@@ -1223,11 +1224,10 @@ def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq
     """kv8_attention of a batch whose sequences all begin with the same `shared` blocks (lq_kv8_attention_shared): the first `shared` columns of
     block_table are the same in every row. Their keys and values are read once for all rows. Arguments and results otherwise as
     kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
-    if out is None:
-        r = (_native or _fast()).kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal,
-                                                      return_lse)
-        if r is not None:
-            return r
+    r = (_native or _fast()).kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse,
+                                                  out)
+    if r is not None:
+        return r
     n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
                                                                                        scale, out)
     tokens, heads, shared = q.shape[0], q.shape[1], int(shared)
