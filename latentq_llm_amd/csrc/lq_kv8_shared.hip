@@ -48,6 +48,9 @@ struct Shared {
     int p_slices, p_tiles;      // of the prefix: slices of the keys, tiles of 64 in each
     int o_slices, o_tiles;      // of a sequence's own keys
     int o_row_tiles;            // and of its rows
+    int direct, j_direct;       // workgroups of the own keys with a place for each (sequence, kv head, one of o_row_tiles), of the join in blockIdx.y; the others have place_beyond()
+    int j_rows, j_turns;        // rows of a place there in the join, in so many turns
+    Div by_o_rows, by_j_rows;
     int p_items;                // workgroups of the prefix, with those that pad its units to a multiple of 8
 };
 
@@ -97,6 +100,33 @@ __device__ __forceinline__ Span span_of(const Shared &s, int seq) {
     }
     const int start = min(max(begin, 0), a.tokens);
     return Span{start, min(max(end, start), a.tokens) - start, len, (min(max(len, 0), a.width * KV8_BLOCK) + KV8_BLOCK - 1) / KV8_BLOCK};
+}
+
+// Where a workgroup on a sequence's rows is: the sequence, and the first row of its tile
+struct Place {
+    int seq, row0;
+    Span span;
+};
+
+// Tiles of `per` rows from each sequence's row `from` on (per or more), the sequences' one after the other: those of one that begins with row r of all are r / per and on, which leaves
+// room for as many as it can have. Where the one at `at` is: one look at 64 sequences, two at 4096. (First rows that are no sums put it at other rows of the operands, or at none.)
+__device__ __forceinline__ Place place_beyond(const Shared &s, int at, const Div &by_per, int per, int from) {
+    const Kv8Attn &a = s.a;
+    const int lane = threadIdx.x & 63;
+    const auto begin_of = [&](int seq) { return min(max(a.cu ? a.cu[seq] : seq * s.per_seq, 0), a.tokens); };
+    int lo = 0, n = a.batch;
+    while (n > 64) {  // the last sequence that has begun, of 64 that lie evenly, then of those up to the next
+        const int step = (n + 63) >> 6, seq = lo + min(lane * step, n - 1);
+        const int i = max(__builtin_popcountll(__ballot(lane * step < n && by_per(begin_of(seq) * s.group) <= at)) - 1, 0);
+        lo += i * step;
+        n = min(step, n - i * step);
+    }
+    const int seq = lo + min(lane, n - 1), begin = begin_of(seq), len = a.lens[seq];
+    const int end = min(max(a.cu ? a.cu[seq + 1] : begin + s.per_seq, begin), a.tokens), first = by_per(begin * s.group);
+    const int i = max(__builtin_popcountll(__ballot(lane < n && first <= at)) - 1, 0);
+    const int of_seq = __builtin_amdgcn_readlane(len, i), start = __builtin_amdgcn_readlane(begin, i);
+    return Place{lo + i, from + (at - __builtin_amdgcn_readlane(first, i)) * per,
+                 Span{start, __builtin_amdgcn_readlane(end, i) - start, of_seq, (min(max(of_seq, 0), a.width * KV8_BLOCK) + KV8_BLOCK - 1) / KV8_BLOCK}};
 }
 
 // What an item is: rows row0 .. row0 + rows - 1 of those that begin with token `token0`, kv head h, tiles t_lo .. t_hi - 1 of the block
@@ -382,89 +412,132 @@ __global__ __launch_bounds__(256, waves_of(D, kPrefix)) void shared_kernel(const
         return;
     }
     const int at = id - s.p_items, part = s.by_o_slices(at), slice = at - part * s.o_slices, unit = s.by_o_row_tiles(part), row_tile = part - unit * s.o_row_tiles,
-              seq = s.by_kv_heads(unit), row0 = row_tile * 16 * kOwn, t_lo = s.common + slice * s.o_tiles;
-    const int *table = a.table + (int64_t)seq * a.width;
+              t_lo = s.common + slice * s.o_tiles;
+    Place place{s.by_kv_heads(unit), row_tile * 16 * kOwn, {}};
+    int h = unit - place.seq * a.kv_heads;
+    if (part >= s.direct) {
+        const int beyond = s.by_kv_heads(part - s.direct);
+        h = part - s.direct - beyond * a.kv_heads;
+        place = place_beyond(s, beyond, s.by_o_rows, 16 * kOwn, s.o_row_tiles * 16 * kOwn);
+    }
+    const int *table = a.table + (int64_t)place.seq * a.width;
     const int block = kv8_uniform(table + min(t_lo + wave, a.width - 1));  // (on its way with the sequence's length)
-    const Span r = span_of(s, seq);
-    const int rows = min(r.n * s.group, a.rows) - row0;
-    if (rows <= 0 || t_lo >= r.tiles) return;
+    if (part < s.direct) place.span = span_of(s, place.seq);
+    const Span r = place.span;
+    const int row0 = place.row0, rows = min(r.n * s.group, a.rows) - row0;
+    if (row0 < 0 || rows <= 0 || t_lo >= r.tiles) return;
     const int t_hi = slice == s.o_slices - 1 ? r.tiles : min(t_lo + s.o_tiles, r.tiles);  // (a max_len that was too small costs time)
-    const Item it{r.start, row0, min(rows, 16 * kOwn), unit - seq * a.kv_heads, t_lo, t_hi, table, block, s.p_slices + slice};
+    const Item it{r.start, row0, min(rows, 16 * kOwn), h, t_lo, t_hi, table, block, s.p_slices + slice};
     item<D, kOwn, kF16, false>(s, it, lds, [&](int token, bool there) { return Where{r.len, r.start, r.start + r.n, token, there}; });
 }
 
-// A row's pieces joined: blockIdx.x for (sequence, kv head), .y for kRows of its rows
+// A row's pieces joined: blockIdx.x for (sequence, kv head), .y for kRows of its rows; beyond j_direct of those for j_rows rows of any sequence
 template <int D, int kParts, bool kF16>
 __global__ __launch_bounds__(256) void join_shared_kernel(const Shared s) {
     constexpr int kUnits = D / 4, kRows = 256 / (kUnits * kParts);
     __shared__ f32x4_t lds_o[kParts][kRows * kUnits];
     __shared__ float lds_m[kParts][kRows], lds_l[kParts][kRows];
     const Kv8Attn &a = s.a;
-    const int seq = s.by_kv_heads(blockIdx.x), h = blockIdx.x - seq * a.kv_heads;
-    const int unit = threadIdx.x % kUnits, at = threadIdx.x / kUnits, part = at % kParts, mine = at / kParts, r = blockIdx.y * kRows + mine;
-    const Span q = span_of(s, seq);
-    const bool there = mine < kRows && r < min(q.n * s.group, a.rows);
-    const int own = q.tiles - s.common, pieces = s.p_slices + max(min(s.by_o_tiles(max(own, 0) + s.o_tiles - 1), s.o_slices), 0);
-    const int y = s.by_group(r), token = q.start + y, head = h * s.group + r - y * s.group;
-    float m = kNone, total = 0.0f;
-    f32x4_t o = {0, 0, 0, 0};
-    if (there) kv8_join<D>(a.part, a.part_lse, (int64_t)a.tokens * a.heads, (int64_t)token * a.heads + head, 4 * unit, part, kParts, pieces, [](int i) { return (int64_t)i; }, m, total, o);
-    if constexpr (kParts > 1) {
-        if (there) {
-            lds_o[part][mine * kUnits + unit] = o;
-            if (unit == 0) {
-                lds_m[part][mine] = m;
-                lds_l[part][mine] = total;
+    const int seq = s.by_kv_heads(blockIdx.x), h = blockIdx.x - seq * a.kv_heads, y_beyond = (int)blockIdx.y - s.j_direct;
+    const int unit = threadIdx.x % kUnits, at = threadIdx.x / kUnits, part = at % kParts, mine = at / kParts;
+    const Place place = y_beyond < 0 ? Place{seq, (int)blockIdx.y * kRows, span_of(s, seq)} : place_beyond(s, y_beyond * a.batch + seq, s.by_j_rows, s.j_rows, s.j_direct * kRows);
+    const Span q = place.span;
+    const int rows = min(q.n * s.group, a.rows), own = q.tiles - s.common, pieces = s.p_slices + max(min(s.by_o_tiles(max(own, 0) + s.o_tiles - 1), s.o_slices), 0);
+    for (int turn = 0; turn < (y_beyond < 0 ? 1 : s.j_turns); ++turn) {
+        const int row0 = place.row0 + turn * kRows, r = row0 + mine;
+        if (row0 < 0 || row0 >= rows) return;
+        const bool there = mine < kRows && r < rows;
+        const int y = s.by_group(r), token = q.start + y, head = h * s.group + r - y * s.group;
+        float m = kNone, total = 0.0f;
+        f32x4_t o = {0, 0, 0, 0};
+        if (there) kv8_join<D>(a.part, a.part_lse, (int64_t)a.tokens * a.heads, (int64_t)token * a.heads + head, 4 * unit, part, kParts, pieces, [](int i) { return (int64_t)i; }, m, total, o);
+        if constexpr (kParts > 1) {
+            if (turn) __syncthreads();  // the parts of the rows before are read
+            if (there) {
+                lds_o[part][mine * kUnits + unit] = o;
+                if (unit == 0) {
+                    lds_m[part][mine] = m;
+                    lds_l[part][mine] = total;
+                }
             }
+            __syncthreads();
+            if (!there || part) continue;
+            kv8_join_parts<kParts>(&lds_o[0][mine * kUnits + unit], &lds_m[0][mine], &lds_l[0][mine], kRows * kUnits, kRows, m, total, o);
         }
-        __syncthreads();
-        if (!there || part) return;
-        kv8_join_parts<kParts>(&lds_o[0][mine * kUnits + unit], &lds_m[0][mine], &lds_l[0][mine], kRows * kUnits, kRows, m, total, o);
+        if (there) kv8_finish<kF16>(a, token, head, 4 * unit, m, total, o);
     }
-    if (there) kv8_finish<kF16>(a, token, head, 4 * unit, m, total, o);
 }
 
 template <int D, int kPrefix, int kOwn, bool kF16>
-int launch(const Shared &s, int64_t items, hipStream_t stream) {
+int launch(Shared s, int64_t planned, hipStream_t stream) {
+    // Rows of a sequence beyond `planned`: a place for every tile of them that there can be, where there can be some
+    const int64_t all = s.a.rows > planned ? (int64_t)s.a.tokens * s.group : 0;
+    const int64_t direct = (int64_t)s.a.batch * s.a.kv_heads * s.o_row_tiles, beyond = all / (16 * kOwn) * s.a.kv_heads, items = s.p_items + (direct + beyond) * s.o_slices;
+    constexpr int kParts = D <= 128 ? 4 : 2, kRows = 256 / (D / 4 * kParts);
+    const int64_t j_direct = (planned + kRows - 1) / kRows;
+    // Several turns in a place there (2 us each) only where the places, most of them empty, are more than the compute units hold at a time: 300 sequences of 4 rows with all rows for a
+    // bound 11.2 -> 7.4 us
+    int64_t j_turns = 1;
+    while (2 * j_turns <= std::min(j_direct, (int64_t)4) && all / (j_turns * kRows) * s.a.kv_heads > 8 * lq_device_cu_count()) j_turns *= 2;
+    const int64_t j_beyond = all / (j_turns * kRows);
+    LQ_REQUIRE(items <= UINT32_MAX / 256 && j_direct + j_beyond / s.a.batch < 65535, "kv8_attention_shared: too many workgroups: %d tokens of %d sequences", s.a.tokens, s.a.batch);
+    s.direct = (int)direct;
+    s.by_o_rows = Div(16 * kOwn);
+    s.j_direct = (int)j_direct;
+    s.j_turns = (int)j_turns;
+    s.j_rows = (int)(j_turns * kRows);
+    s.by_j_rows = Div(s.j_rows);
     shared_kernel<D, kPrefix, kOwn, kF16><<<(unsigned)items, 256, 0, stream>>>(s);
     if (const int rc = lq_check_launch("kv8_attention_shared")) return rc;
-    constexpr int kParts = D <= 128 ? 4 : 2, kRows = 256 / (D / 4 * kParts);
-    const dim3 grid((unsigned)(s.a.batch * s.a.kv_heads), (unsigned)((s.a.rows + kRows - 1) / kRows));
+    const dim3 grid((unsigned)(s.a.batch * s.a.kv_heads), (unsigned)(j_direct + (j_beyond + s.a.batch - 1) / s.a.batch));
     join_shared_kernel<D, kParts, kF16><<<grid, 256, 0, stream>>>(s);
     return lq_check_launch("kv8_attention_shared (join)");
 }
 
 template <int D, bool kF16>
-int launch_rows(const Shared &s, int prefix, int own, int64_t items, hipStream_t stream) {
+int launch_rows(const Shared &s, int prefix, int own, int64_t planned, hipStream_t stream) {
     if constexpr (D <= 128) {
-        if (own == 2) return launch<D, 2, 2, kF16>(s, items, stream);
-        if (prefix == 2) return launch<D, 2, 1, kF16>(s, items, stream);
+        if (own == 2) return launch<D, 2, 2, kF16>(s, planned, stream);
+        if (prefix == 2) return launch<D, 2, 1, kF16>(s, planned, stream);
     }
-    return launch<D, 1, 1, kF16>(s, items, stream);
+    return launch<D, 1, 1, kF16>(s, planned, stream);
 }
 
 // How a call is cut; prefix 0: as one without a shared prefix
 struct Plan {
-    int prefix, own, row_tiles, o_row_tiles, p_slices, p_tiles, o_slices, o_tiles;
+    int own_rows, prefix, own, row_tiles, o_row_tiles, p_slices, p_tiles, o_slices, o_tiles;
     int64_t bytes;
 };
+
+constexpr int64_t kFewRows = 64;
 
 // Whether reading the shared blocks once is worth a second launch and partial results: with enough of them, or with enough that would be read again
 // from the caches. us shared / each by itself, 32 heads of 128 and a page of tokens of their own: 2 sequences behind 256 8.1 / 6.5, behind 512 8.2 / 7.7,
 // behind 1024 8.2 / 10.2; 8 behind 512 9.4 / 8.1; 16 behind 512 10.3 / 11.3; 64 behind 512 24.8 / 29.7; 32 behind 256 15.2 / 13.1; on 8 kv heads 32 behind 512 11.3 / 8.0, 16
-// behind 1024 12.4 / 12.2, 64 behind 1024 15.9 / 17.1. Rows that fill matrix tiles by themselves have little to share (beyond 64 the prompt kernel's).
+// behind 1024 12.4 / 12.2, 64 behind 1024 15.9 / 17.1. Rows that fill matrix tiles by themselves have little to share: shared / each by itself with 32, 64, 96, 128 rows of a sequence, 8 behind
+// 8192 on 8 kv heads .64, .77, 1.05, 1.07, on 32 .75, .82, 1.15, 1.30; 2 behind 65536 on 32 .70, .79, .98, 1.10. (Behind 1024, where many workgroups run, 64 rows lose already: 8 on 32 1.38.)
 bool pays(int64_t batch, int64_t own_rows, int kv_heads, int dim, int64_t common) {
-    if (batch < 2 || own_rows > 64) return false;
+    if (batch < 2 || own_rows > kFewRows) return false;
     const int64_t again = (batch - 1) * kv_heads * common * 2 * KV8_BLOCK * dim;
     return common >= 14 || (common >= 8 && again >= 48000000);
 }
 
+// The rows that a sequence is taken to have: as many as it may have, but where that is far from what the pass has for each (it may be a bound that nobody looked for, or that of one
+// sequence alone) the latter; those beyond are found in place_beyond(). us with the bound exact / all rows of the pass / each sequence by itself, 32 heads on 8 of 128: 64 x 1 behind 8192 29.1 / 29.4 /
+// 94, 17 x 1 behind 131072 83 / 86 / 660, 300 x 1 behind 4096 62 / 63 / 200; 8 x 5 behind 4096, 32 heads of 64, 13.5 / 13.5 / 21. With one sequence of more rows, taken to have as many as
+// it / as the others: 15 x 1 and one of 12 behind 4096 17.9 / 15.0, 63 x 1 and one of 512 behind 8192 631 / 155 (each by itself 690).
+int64_t rows_of_a_sequence(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t group) {
+    const int64_t most = max_tokens * group, average = (tokens + batch - 1) / batch * group;
+    return most > kFewRows || (most + 15) / 16 >= 3 * ((average + 15) / 16) ? std::min(average, most) : most;
+}
+
 Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t common, int64_t workspace, int cus) {
     Plan p{};
-    const int64_t group = heads / kv_heads, rows = tokens * group, own_rows = max_tokens * group;
+    const int64_t group = heads / kv_heads, rows = tokens * group, own_rows = rows_of_a_sequence(batch, tokens, max_tokens, group);
     if (!pays(batch, own_rows, kv_heads, dim, common)) return p;
     // 32 rows to an item where there are as many, and registers for them (up to 128 dimensions)
     const int prefix = rows > 16 && dim <= 128 ? 2 : 1;
+    p.own_rows = (int)own_rows;
     p.own = own_rows > 16 && dim <= 128 ? 2 : 1;
     p.row_tiles = (int)((rows + 16 * prefix - 1) / (16 * prefix));
     p.o_row_tiles = (int)((own_rows + 16 * p.own - 1) / (16 * p.own));
@@ -555,15 +628,15 @@ extern "C" int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, in
     s.by_kv_heads = Div(kv_heads);
     s.by_row_tiles = Div(p.row_tiles);
     s.by_o_slices = Div(p.o_slices);
-    s.by_o_row_tiles = Div(p.o_row_tiles);
+    s.by_o_row_tiles = Div(s.o_row_tiles);
     s.by_o_tiles = Div(p.o_tiles);
-    const int64_t p_items = (int64_t)(kv_heads * p.p_slices + 7) / 8 * 8 * p.row_tiles, items = p_items + batch * kv_heads * p.o_slices * p.o_row_tiles;
-    LQ_REQUIRE(items <= UINT32_MAX / 256, "kv8_attention_shared: too many workgroups: %lld sequences", (long long)batch);
+    const int64_t p_items = (int64_t)(kv_heads * p.p_slices + 7) / 8 * 8 * p.row_tiles;
+    LQ_REQUIRE(p_items <= UINT32_MAX / 256, "kv8_attention_shared: too many workgroups: %lld tokens", (long long)tokens);
     s.p_items = (int)p_items;
     hipStream_t on = (hipStream_t)stream;
     const auto run = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return dtype == 1 ? launch_rows<D, true>(s, p.prefix, p.own, items, on) : launch_rows<D, false>(s, p.prefix, p.own, items, on);
+        return dtype == 1 ? launch_rows<D, true>(s, p.prefix, p.own, p.own_rows, on) : launch_rows<D, false>(s, p.prefix, p.own, p.own_rows, on);
     };
     if (dim == 64) return run(std::integral_constant<int, 64>());
     if (dim == 96) return run(std::integral_constant<int, 96>());

@@ -1222,8 +1222,8 @@ def kv8_attention_shared_plan(batch: int, tokens: int, max_tokens: int, max_len:
 def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,
                          causal=True, out=None, return_lse=False):
     """kv8_attention of a batch whose sequences all begin with the same `shared` blocks (lq_kv8_attention_shared): the first `shared` columns of
-    block_table are the same in every row. Their keys and values are read once for all rows. Arguments and results otherwise as
-    kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
+    block_table are the same in every row. Their keys and values are read once for all rows, where that is faster (the pass has up to 64 rows for a sequence and kv head on average, ...:
+    kv8_attention_shared_plan says). Arguments and results otherwise as kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
     r = (_native or _fast()).kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse,
                                                   out)
     if r is not None:
