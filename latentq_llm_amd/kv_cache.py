@@ -138,7 +138,8 @@ class Sequences:
 class DeviceSequences:
     """Which blocks of a pool a fixed batch of sequences has, kept on the device (ops.kv8_resize): no pass asks the host. `capacity` is the most tokens of
     a sequence. The first `shared` blocks of the pool are every sequence's first ones: their tokens are appended once, by the pass
-    that prompt() describes, and a sequence without tokens of its own has those."""
+    that prompt() describes, and a sequence without tokens of its own has those. Every change of the books names its success in a tensor on the device, `status` of the latest one
+    (int32 [1], ops.kv8_resize's: 0, or the books are as they were)."""
 
     def __init__(self, num_blocks: int, batch: int, capacity: int, shared: int = 0, device="cuda"):
         width = -(-capacity // BLOCK)
@@ -152,6 +153,7 @@ class DeviceSequences:
         self.free_blocks = torch.zeros(num_blocks, **i32)  # the last free one is the next to be taken
         self.free_blocks[:num_blocks - shared] = torch.arange(num_blocks - 1, shared - 1, -1, **i32)
         self.free_count = torch.full((1,), num_blocks - shared, **i32)
+        self.status = torch.zeros(1, **i32)
 
     def _books(self):
         return self.block_table, self.seq_lens, self.free_blocks, self.free_count
@@ -171,23 +173,25 @@ class DeviceSequences:
         new tokens and its length (defaults: rows, the capacity); attention over shared blocks is as fast with the default, without them a bound close to what the
         sequences have is faster, and verify() gives as many columns. Where step.status is not 0 nothing has changed and the pass has no tokens. The
         step names the tables themselves: it describes the pass until they are changed again."""
-        cu, positions, slots, status = ops.kv8_resize(*self._books(), new, rows=rows, shared=self.shared)
+        cu, positions, slots, self.status = ops.kv8_resize(*self._books(), new, rows=rows, shared=self.shared)
         return Step(block_table=self.block_table, seq_lens=self.seq_lens, cu_tokens=cu, max_tokens=rows if max_tokens is None else max_tokens,
                     max_len=self.capacity if max_len is None else max_len, last=(cu[1:].long() - 1).clamp_min(0), positions=positions, longest=self.capacity,
-                    pool=self.num_blocks, shared=self.shared, slots=slots, status=status)
+                    pool=self.num_blocks, shared=self.shared, slots=slots, status=self.status)
 
     def give_back(self, tokens):
         """Take the last tokens[i] tokens of sequence i away (int32 [batch] on the device, none negative; more than there are: all of its own). Blocks that
-        they alone had are free again."""
-        ops.kv8_resize(*self._books(), -torch.minimum(tokens, self.seq_lens - self.shared * BLOCK), shared=self.shared)
+        they alone had are free again. Returns the status."""
+        self.status = ops.kv8_resize(*self._books(), -torch.minimum(tokens, self.seq_lens - self.shared * BLOCK), shared=self.shared)[3]
+        return self.status
 
     def verify(self, logits, tokens, step: Step, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0):
         """ops.verify_drafts of a step's rows, each sequence's first one a known token and the others drafts; refused drafts leave their sequences. Returns
-        (accepted drafts, the token behind them and -1, int64 [batch, max_tokens]; how many were accepted, int32 [batch])."""
+        (accepted drafts, the token behind them and -1, int64 [batch, max_tokens]; how many were accepted, int32 [batch]); where self.status is not 0 then, the books were none (changed by
+        others, say) and the refused drafts are still in them."""
         change = torch.empty_like(self.seq_lens)
         out, accepted = ops.verify_drafts(logits, tokens, step.cu_tokens, draft_logits=draft_logits, accept_draws=accept_draws, sample_draws=sample_draws,
                                           temperature=temperature, max_tokens=step.max_tokens, change=change)
-        ops.kv8_resize(*self._books(), change, shared=self.shared)
+        self.status = ops.kv8_resize(*self._books(), change, shared=self.shared)[3]
         return out, accepted
 
 
