@@ -537,7 +537,8 @@ int lq_weight_grad_plan(int form, int64_t M, int64_t N, int64_t K, int compute_u
  * tables [positions][rot_dim / 2], in fp32; q_out is rounded once, keys go to 8 bits unrounded.
  * A (block, head)'s scale is max(A, 2^-90) / 127, A the largest finite |x| of its new tokens, or what it was where
  * that is larger and the block held tokens of the sequence (then also: where it grows, the codes c that are there become
- * rint(c * (old / new))). New codes: 128 + clamp(rint(x * (1 / scale)), -127, 127), NaN -> 128 (zero). Slots of a block
+ * rint(c * (old / new))). So tokens that are taken back (a shorter seq_lens later) leave their mark in a block of which tokens stay: its scale, and the
+ * codes that were rounded again for it. A block that none of them stays in begins anew. New codes: 128 + clamp(rint(x * (1 / scale)), -127, 127), NaN -> 128 (zero). Slots of a block
  * beyond the sequence's tokens stay as they are. A block that takes tokens belongs to one sequence of the call. */
 int lq_kv8_append(const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
                   int64_t v_head_stride, const void *q, int64_t q_token_stride, int64_t q_head_stride, void *q_out,
@@ -579,7 +580,8 @@ int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int
 
 /* lq_kv8_attention (without a window) of a batch whose sequences all begin with the same `shared` blocks: the first `shared` columns of
  * block_table are the same in every row, which is the caller's promise (which row's entries are read is not said). Those keys are
- * read once for all rows, where that is faster, and the result is that of lq_kv8_attention but for roundings. A sequence may be shorter than the shared blocks: its rows
+ * read once for all rows, where that is faster, and the result is that of lq_kv8_attention but for roundings: codes enter the products as 1 .. 255, and 128 times the sum of the queries, or of
+ * the weights, is taken off, so that the fp32 sums are of numbers up to 255 where they are up to 127 there. A sequence may be shorter than the shared blocks: its rows
  * see what is theirs. What is faster goes by the rows that the pass has for a sequence on average (up to 64, query heads of a kv head counted), so that max_tokens may be a bound far above what the sequences
  * have. workspace as there, and without one, or with too little, every sequence is read by itself. */
 int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes, const float *k_scale,
@@ -629,6 +631,8 @@ int lq_kv8_resize(int32_t *block_table, int64_t table_width, int32_t *seq_lens, 
  * were taken; change int32 [batch] (or null): accepted + 1 - its rows (0 without rows), by which lq_kv8_resize gives refused drafts back. Rows of a
  * sequence beyond max_tokens are not looked at. Up to 65535 rows and sequences. workspace: 16-byte aligned, the
  * bytes that lq_verify_drafts_plan says; calls sharing one are ordered on one stream. No result depends on an order.
+ * Tokens are distributed as the target's for the logits given. Generation with drafts need not be, bit for bit or in distribution, that without: drafts are in the cache when the logits are
+ * made, and refused ones leave their blocks' scales there (lq_kv8_append).
  * ------------------------------------------------------------------------- */
 int lq_verify_drafts(const void *logits, int64_t row_stride, const void *draft_logits, int64_t draft_row_stride, const int64_t *tokens,
                      const int32_t *cu_tokens, int64_t batch, int64_t rows, int64_t vocab, int64_t max_tokens, int dtype, double temperature,

@@ -3,7 +3,7 @@
 //   p = softmax(l / T) of a row's logits, q the same of the drafter's;  draft x of row r is taken where u_r q(x) < p(x)
 //   the first one refused, at row a: the token is drawn from max(p - q, 0);  none refused: from p of the last row
 //   drawn: the first j with r_0 + .. + r_j > u (r_0 + .. + r_{V-1})
-// (Taken with probability min(1, p/q), else the rest: tokens come out distributed as the target's.)
+// (Taken with probability min(1, p/q), else the rest: tokens come out distributed as the target's, for the logits given.)
 //
 // Tokens are whole numbers, so the sums decide between neighbours: 32 bits would move a border of the cumulative sum by some 1e-8 to 1e-7 of it,
 // and of 32000 borders a number in [0, 1) meets one that moved in one row of a thousand. Exponentials and sums are 64 bits, which

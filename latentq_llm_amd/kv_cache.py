@@ -187,7 +187,8 @@ class DeviceSequences:
     def verify(self, logits, tokens, step: Step, draft_logits=None, accept_draws=None, sample_draws=None, temperature=1.0):
         """ops.verify_drafts of a step's rows, each sequence's first one a known token and the others drafts; refused drafts leave their sequences. Returns
         (accepted drafts, the token behind them and -1, int64 [batch, max_tokens]; how many were accepted, int32 [batch]); where self.status is not 0 then, the books were none (changed by
-        others, say) and the refused drafts are still in them."""
+        others, say) and the refused drafts are still in them. What they leave in the cache is the scale of the block that they ended in, and codes rounded to it, where they
+        were larger than what the block held: accepted tokens are rounded as if they had come behind the refused ones, so a generation with drafts is not, bit for bit, that without."""
         change = torch.empty_like(self.seq_lens)
         out, accepted = ops.verify_drafts(logits, tokens, step.cu_tokens, draft_logits=draft_logits, accept_draws=accept_draws, sample_draws=sample_draws,
                                           temperature=temperature, max_tokens=step.max_tokens, change=change)

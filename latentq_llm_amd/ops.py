@@ -1290,7 +1290,7 @@ def verify_drafts(logits, tokens, cu_tokens=None, *, draft_logits=None, accept_d
     rows the first is a known token and the others are drafts, drawn from softmax(draft_logits / temperature) of the row before, or without draft_logits
     chosen in any other way. accept_draws (float32 [rows]) and sample_draws (float32 [batch]) are uniform numbers in [0, 1); temperature 0 takes the
     largest logit and needs none. max_tokens: the largest number of rows of a sequence (default: what the rows allow). change (int32 [batch], or
-    None) is filled with accepted + 1 - rows of each sequence, by which kv8_resize gives refused drafts back. Returns (int64 [batch, max_tokens]:
+    None) is filled with accepted + 1 - rows of each sequence, by which kv8_resize gives refused drafts back (their blocks' scales in the cache stay: include/latentq.h). Returns (int64 [batch, max_tokens]:
     accepted drafts, the token behind them, -1; int32 [batch]: how many drafts were accepted)."""
     r = (_native or _fast()).verify_drafts(logits, tokens, cu_tokens, draft_logits, accept_draws, sample_draws, temperature, batch, max_tokens, change)
     if r is not None:
