@@ -137,7 +137,7 @@ class Sequences:
 
 class DeviceSequences:
     """Which blocks of a pool a fixed batch of sequences has, kept on the device (ops.kv8_resize): no pass asks the host. `capacity` is the most tokens of
-    a sequence. The first `shared` blocks of the pool are every sequence's first ones: their tokens are appended once, by the pass
+    a sequence, rounded up to whole blocks: sequences may have as many as the attribute then says, and rotation tables reach as far. The first `shared` blocks of the pool are every sequence's first ones: their tokens are appended once, by the pass
     that prompt() describes, and a sequence without tokens of its own has those. Every change of the books names its success in a tensor on the device, `status` of the latest one
     (int32 [1], ops.kv8_resize's: 0, or the books are as they were)."""
 
