@@ -590,7 +590,8 @@ int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, int64_t q_hea
                             int dim, int dtype, float scale, int causal, void *out, int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace,
                             int64_t workspace_bytes, void *stream);
 /* What the above does with a call of these sizes, as lq_kv8_attention_plan: slices of the shared keys and of a sequence's own (0 and 0: the call is
- * one of lq_kv8_attention), and the bytes of workspace that they take. */
+ * one of lq_kv8_attention), and the bytes of workspace that they take. A max_len above what the block table has room for (2^31 or more, here) says nothing of
+ * the sequences' lengths: the call is cut for sequences that have few keys of their own. */
 int lq_kv8_attention_shared_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t shared,
                                  int64_t workspace_bytes, int compute_units, int *prefix_slices, int *own_slices, int64_t *needed);
 

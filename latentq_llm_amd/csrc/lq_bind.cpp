@@ -808,12 +808,12 @@ PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     if (!q.load(a[0]) || !c.load(a + 1) || !same_device(q.t, c.kc) || q.t->size(2) != c.dim || q.t->size(1) % c.heads) return none();
     const int64_t tokens = q.t->size(0), heads = q.t->size(1);
     if (!s.load(a[5], a[6], a[8], a[9], tokens, c.kc)) return none();
-    const int64_t shared = integer(a[7]);
-    int64_t max_len = s.width * LQ_KV_BLOCK;
+    const int64_t shared = integer(a[7]), room = s.width * LQ_KV_BLOCK;
+    int64_t max_len = INT64_MAX;  // (not known)
     if (a[10] != Py_None) {
         const int64_t given = integer(a[10]);
         if (given < 0) return none();
-        max_len = std::min(max_len, given);
+        if (given <= room) max_len = given;
     }
     const double scale = a[11] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AsDouble(a[11]);
     const int causal = PyObject_IsTrue(a[12]), with_lse = PyObject_IsTrue(a[13]);
@@ -823,6 +823,9 @@ PyObject *kv8_attention_shared(PyObject *, PyObject *const *a, Py_ssize_t nargs)
     int64_t needed;
     if (const int rc = lq_kv8_attention_shared_plan(s.batch, tokens, s.most, max_len, (int)heads, (int)c.heads, (int)c.dim, shared, kWorkspaceBytes, 0, &prefix, &own, &needed))
         return fail("lq_kv8_attention_shared_plan", rc);
+    if (!prefix)
+        if (const int rc = lq_kv8_attention_plan(s.batch, tokens, s.most, std::min(max_len, room), (int)heads, (int)c.heads, (int)c.dim, 0, kWorkspaceBytes, 0, &prefix, &own, &needed))
+            return fail("lq_kv8_attention_plan", rc);
     at::Tensor ws;
     if (needed) ws = make({needed}, at::kByte, *q.t);
     at::Tensor made, lse;

@@ -42,11 +42,11 @@ struct Div {
 struct Shared {
     Kv8Attn a;
     int group, per_seq;         // query heads of a kv head; new tokens of a sequence, without cu
-    Div by_group, by_per_seq, by_kv_heads, by_row_tiles, by_o_slices, by_o_row_tiles, by_o_tiles;
+    Div by_group, by_per_seq, by_kv_heads, by_row_tiles, by_o_slices, by_o_row_tiles;
     int common;                 // blocks that all sequences begin with
     int row_tiles;              // of the prefix's rows, each for a workgroup
     int p_slices, p_tiles;      // of the prefix: slices of the keys, tiles of 64 in each
-    int o_slices, o_tiles;      // of a sequence's own keys
+    int o_slices;               // of a sequence's own keys, four tiles of each in turn: whatever its length is, they have as much to do
     int o_row_tiles;            // and of its rows
     int direct, j_direct;       // workgroups of the own keys with a place for each (sequence, kv head, one of o_row_tiles), of the join in blockIdx.y; the others have place_beyond()
     int j_rows, j_turns;        // rows of a place there in the join, in so many turns
@@ -129,10 +129,10 @@ __device__ __forceinline__ Place place_beyond(const Shared &s, int at, const Div
                  Span{start, __builtin_amdgcn_readlane(end, i) - start, of_seq, (min(max(of_seq, 0), a.width * KV8_BLOCK) + KV8_BLOCK - 1) / KV8_BLOCK}};
 }
 
-// What an item is: rows row0 .. row0 + rows - 1 of those that begin with token `token0`, kv head h, tiles t_lo .. t_hi - 1 of the block
-// table's row, results in `slot` of the workspace
+// What an item is: rows row0 .. row0 + rows - 1 of those that begin with token `token0`, kv head h, four tiles from t_lo, t_lo + step, ... on of the block
+// table's row, up to t_hi - 1, results in `slot` of the workspace
 struct Item {
-    int token0, row0, rows, h, t_lo, t_hi;
+    int token0, row0, rows, h, t_lo, t_hi, step;
     const int *table;
     int block;  // the entry of this wave's first tile
     int64_t slot;
@@ -174,7 +174,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
     const Kv8Attn &a = s.a;
     constexpr int S = D / 64, kTail = D % 64 / 32, kSteps = 2 * S + kTail, kTiles = D / 16, kWaves = 4, kPad = D + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int group = s.group, h = it.h;
+    const int group = s.group, h = it.h, step = kKept ? kWaves : it.step;
 
     // the queries and where their rows are: requested before the first tile, so that nothing waits for that
     u32x4_t raw[RT][kSteps];
@@ -222,7 +222,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         load_k(bh);
         k_scale = kv8_uniform(a.ks + bh);
         v_scale = kv8_uniform(a.vs + bh);
-        id_next = kv8_uniform(it.table + min(t + kWaves, it.t_hi - 1));
+        id_next = kv8_uniform(it.table + min(t + step, it.t_hi - 1));
     }
     __builtin_amdgcn_sched_barrier(0);
 
@@ -285,7 +285,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
             load_k(bh);
             k_scale = kv8_uniform(a.ks + bh);
             v_scale = kv8_uniform(a.vs + bh);
-            id_next = kv8_uniform(it.table + min(t + 2 * kWaves, it.t_hi - 1));
+            id_next = kv8_uniform(it.table + min(t + 2 * step, it.t_hi - 1));
             __builtin_amdgcn_sched_barrier(0);
         }
         const int key0 = t * KV8_BLOCK;
@@ -349,7 +349,7 @@ __device__ __forceinline__ void item(const Shared &s, const Item &it, char *lds,
         }
     };
     if (t < it.t_hi) {
-        for (; t + kWaves < it.t_hi; t += kWaves) tile(std::true_type{});
+        for (; t + step < it.t_hi; t += step) tile(std::true_type{});
         tile(std::false_type{});
     }
 
@@ -407,12 +407,12 @@ __global__ __launch_bounds__(256, waves_of(D, kPrefix)) void shared_kernel(const
         const int eight = id >> 3, units = s.by_row_tiles(eight), row_tile = eight - units * s.row_tiles, unit = units * 8 + (id & 7);
         if (unit >= a.kv_heads * s.p_slices) return;
         const int slice = s.by_kv_heads(unit), row0 = row_tile * 16 * kPrefix, t_lo = slice * s.p_tiles, t_hi = min(t_lo + s.p_tiles, s.common);
-        const Item it{0, row0, min(a.tokens * s.group - row0, 16 * kPrefix), unit - slice * a.kv_heads, t_lo, t_hi, a.table, kv8_uniform(a.table + min(t_lo + wave, t_hi - 1)), slice};
+        const Item it{0, row0, min(a.tokens * s.group - row0, 16 * kPrefix), unit - slice * a.kv_heads, t_lo, t_hi, 4, a.table, kv8_uniform(a.table + min(t_lo + wave, t_hi - 1)), slice};
         item<D, kPrefix, kF16, true>(s, it, lds, [&](int token, bool there) { return where_is(s, token, there); });
         return;
     }
     const int at = id - s.p_items, part = s.by_o_slices(at), slice = at - part * s.o_slices, unit = s.by_o_row_tiles(part), row_tile = part - unit * s.o_row_tiles,
-              t_lo = s.common + slice * s.o_tiles;
+              t_lo = s.common + slice * 4;
     Place place{s.by_kv_heads(unit), row_tile * 16 * kOwn, {}};
     int h = unit - place.seq * a.kv_heads;
     if (part >= s.direct) {
@@ -426,8 +426,7 @@ __global__ __launch_bounds__(256, waves_of(D, kPrefix)) void shared_kernel(const
     const Span r = place.span;
     const int row0 = place.row0, rows = min(r.n * s.group, a.rows) - row0;
     if (row0 < 0 || rows <= 0 || t_lo >= r.tiles) return;
-    const int t_hi = slice == s.o_slices - 1 ? r.tiles : min(t_lo + s.o_tiles, r.tiles);  // (a max_len that was too small costs time)
-    const Item it{r.start, row0, min(rows, 16 * kOwn), h, t_lo, t_hi, table, block, s.p_slices + slice};
+    const Item it{r.start, row0, min(rows, 16 * kOwn), h, t_lo, r.tiles, s.o_slices * 4, table, block, s.p_slices + slice};
     item<D, kOwn, kF16, false>(s, it, lds, [&](int token, bool there) { return Where{r.len, r.start, r.start + r.n, token, there}; });
 }
 
@@ -442,7 +441,7 @@ __global__ __launch_bounds__(256) void join_shared_kernel(const Shared s) {
     const int unit = threadIdx.x % kUnits, at = threadIdx.x / kUnits, part = at % kParts, mine = at / kParts;
     const Place place = y_beyond < 0 ? Place{seq, (int)blockIdx.y * kRows, span_of(s, seq)} : place_beyond(s, y_beyond * a.batch + seq, s.by_j_rows, s.j_rows, s.j_direct * kRows);
     const Span q = place.span;
-    const int rows = min(q.n * s.group, a.rows), own = q.tiles - s.common, pieces = s.p_slices + max(min(s.by_o_tiles(max(own, 0) + s.o_tiles - 1), s.o_slices), 0);
+    const int rows = min(q.n * s.group, a.rows), own = q.tiles - s.common, pieces = s.p_slices + min((max(own, 0) + 3) >> 2, s.o_slices);
     for (int turn = 0; turn < (y_beyond < 0 ? 1 : s.j_turns); ++turn) {
         const int row0 = place.row0 + turn * kRows, r = row0 + mine;
         if (row0 < 0 || row0 >= rows) return;
@@ -503,9 +502,11 @@ int launch_rows(const Shared &s, int prefix, int own, int64_t planned, hipStream
     return launch<D, 1, 1, kF16>(s, planned, stream);
 }
 
+int64_t blocks_of(int64_t tokens) { return tokens / KV8_BLOCK + (tokens % KV8_BLOCK != 0); }
+
 // How a call is cut; prefix 0: as one without a shared prefix
 struct Plan {
-    int own_rows, prefix, own, row_tiles, o_row_tiles, p_slices, p_tiles, o_slices, o_tiles;
+    int own_rows, prefix, own, row_tiles, o_row_tiles, p_slices, p_tiles, o_slices;
     int64_t bytes;
 };
 
@@ -541,14 +542,18 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
     p.own = own_rows > 16 && dim <= 128 ? 2 : 1;
     p.row_tiles = (int)((rows + 16 * prefix - 1) / (16 * prefix));
     p.o_row_tiles = (int)((own_rows + 16 * p.own - 1) / (16 * p.own));
-    const int64_t own_tiles = std::max((max_len + KV8_BLOCK - 1) / KV8_BLOCK - common, (int64_t)0), slot = tokens * heads * ((int64_t)dim + 1) * 4;
+    const int64_t own_tiles = std::max(blocks_of(max_len) - common, (int64_t)0), slot = tokens * heads * ((int64_t)dim + 1) * 4;
     // Slices of the prefix, by an estimate in us: a compute unit gives a tile of an item `a_tile` (its arithmetic, or its bytes where no other row tile
     // brings them; a tenth less of several row tiles with two items at a time), ways in and out are 4 us, and partial results go there and back. Items shorter than what all the work takes gain nothing. (Own keys count half: max_len is the
     // longest sequence's.) us by slices, 128 dimensions: 12 sequences behind 2048 with up to 1019 of their own 2: 20.0, 4: 20.0, 8: 21.5; 64 behind 8192, 32 heads on 8,
     // 3: 30.0, 4: 26.9, 8: 31.5; 16 behind 131072 16: 58, 32: 59, 48: 63; 64 behind 32768 4: 56, 8: 55, 16: 57; 8 x 5 behind 4096, 32 heads of 64, 2: 16.4, 4: 12.6, 8: 13.5.
     const int64_t units = kv_heads * p.row_tiles;
+    // Where max_len is not known the number is that for no own keys, which costs little where there are many: 64 behind 8192 with 512 of their own
+    // 30.9, by what the table has room for, 4096 or more, 54; 16 behind 131072 with room for 65536 60, 162; with 1500 of their own 58, of a known length 49.
+    const bool known = max_len <= INT32_MAX;
     const double arithmetic = (dim == 64 ? 0.21 : dim == 96 ? 0.3 : dim == 128 ? 0.37 : 0.5) * (prefix == 2 ? 1.0 : 0.6), memory = dim * 128 / 25e3;
-    const double a_tile = std::max(arithmetic, memory / p.row_tiles), all = ((double)(units * common) * a_tile + (double)(batch * kv_heads * p.o_row_tiles * own_tiles) * memory / 2) / cus;
+    const double a_tile = std::max(arithmetic, memory / p.row_tiles),
+                 all = ((double)(units * common) * a_tile + (known ? (double)(batch * kv_heads * p.o_row_tiles * own_tiles) * memory / 2 : 0.0)) / cus;
     int64_t p_slices = 1;
     double best = 0;
     for (int64_t n = 1; n <= 512 && 4 * n <= common + 3; ++n) {
@@ -559,15 +564,19 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
             p_slices = n;
         }
     }
-    // and of the own keys: an item for every compute unit, of 4 tiles or more
-    int64_t o_slices = std::max(std::min((cus + batch * kv_heads * p.o_row_tiles - 1) / (batch * kv_heads * p.o_row_tiles), own_tiles / 4), (int64_t)1);
+    // and of the own keys: an item for every compute unit, of four tiles or more, as many turns of four for all where the length is known
+    const int64_t turns_of_all = std::max((own_tiles + 3) / 4, (int64_t)1), most_items = (cus + batch * kv_heads * p.o_row_tiles - 1) / (batch * kv_heads * p.o_row_tiles);
+    int64_t o_slices = std::max(std::min(most_items, own_tiles / 4), (int64_t)1);
+    if (known) {
+        const int64_t turns = (turns_of_all + o_slices - 1) / o_slices;
+        o_slices = (turns_of_all + turns - 1) / turns;
+    }
     // Slices of as many tiles each, none of them empty, and fewer where the workspace holds no more: by the bytes that are taken, so that a
     // call with just those is cut in the same way
     for (;;) {
         p.p_tiles = (int)((common + p_slices - 1) / p_slices);
         p.p_slices = (int)((common + p.p_tiles - 1) / p.p_tiles);
-        p.o_tiles = (int)std::max((own_tiles + o_slices - 1) / o_slices, (int64_t)1);
-        p.o_slices = (int)std::max((own_tiles + p.o_tiles - 1) / p.o_tiles, (int64_t)1);
+        p.o_slices = (int)o_slices;
         p.bytes = (p.p_slices + p.o_slices) * slot;
         if (p.bytes <= workspace) break;
         if (p.p_slices + p.o_slices == 2) return p;
@@ -580,6 +589,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
 
 }  // namespace
 
+// A bound that says nothing of the sequences' lengths
+constexpr int64_t kNotKnown = INT64_MAX;
+
 extern "C" int lq_kv8_attention_shared_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t shared,
                                             int64_t workspace_bytes, int compute_units, int *prefix_slices, int *own_slices, int64_t *needed) {
     LQ_REQUIRE(prefix_slices && own_slices && needed, "kv8_attention_shared_plan: null pointer");
@@ -588,9 +600,9 @@ extern "C" int lq_kv8_attention_shared_plan(int64_t batch, int64_t tokens, int64
     LQ_REQUIRE(shared >= 0, "kv8_attention_shared: the number of shared blocks must not be negative");
     *prefix_slices = *own_slices = 0;
     if (max_tokens > tokens) max_tokens = tokens;
-    if (max_len > INT32_MAX) max_len = INT32_MAX;
+    if (max_len > INT32_MAX) max_len = kNotKnown;
     if (batch == 0 || tokens == 0 || max_tokens == 0) return LQ_OK;
-    const Plan p = plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, std::min(shared, (max_len + KV8_BLOCK - 1) / KV8_BLOCK), workspace_bytes,
+    const Plan p = plan_of(batch, tokens, max_tokens, max_len, heads, kv_heads, dim, std::min(shared, blocks_of(max_len)), workspace_bytes,
                            compute_units > 0 ? compute_units : lq_device_cu_count());
     if (p.prefix == 0) return LQ_OK;
     *prefix_slices = p.p_slices;
@@ -604,22 +616,23 @@ extern "C" int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, in
                                        const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int64_t shared, int heads, int kv_heads,
                                        int dim, int dtype, float scale, int causal, void *out, int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace,
                                        int64_t workspace_bytes, void *stream) {
-    const Kv8Call c{q, q_token_stride, q_head_stride, k_codes, v_codes, k_scale, v_scale, num_blocks, block_table, table_width, seq_lens, cu_tokens, batch, tokens, max_tokens, max_len, heads,
+    Kv8Call c{q, q_token_stride, q_head_stride, k_codes, v_codes, k_scale, v_scale, num_blocks, block_table, table_width, seq_lens, cu_tokens, batch, tokens, max_tokens, max_len, heads,
                     kv_heads, dim, dtype, scale, causal, 0, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, stream};
     Shared s{};
     bool any;
     if (const int rc = kv8_attention_arguments(s.a, any, c); rc) return rc;
     LQ_REQUIRE(shared >= 0 && (!any || shared <= table_width), "kv8_attention_shared: the shared blocks must be 0 to %lld, the block table's columns, got %lld", (long long)table_width, (long long)shared);
     if (!any) return LQ_OK;
-    max_len = std::min(max_len, table_width * KV8_BLOCK);
-    const int64_t common = std::min(shared, (max_len + KV8_BLOCK - 1) / KV8_BLOCK);  // (no sequence is longer)
+    if (max_len > table_width * KV8_BLOCK) max_len = kNotKnown;
+    const int64_t common = std::min(shared, blocks_of(max_len));  // (no sequence is longer)
     const Plan p = plan_of(batch, tokens, std::min(max_tokens, tokens), max_len, heads, kv_heads, dim, common, workspace ? workspace_bytes : 0, lq_device_cu_count());
+    c.max_len = std::min(max_len, table_width * KV8_BLOCK);
     if (p.prefix == 0) return kv8_attention_call(c);
     s.a.part_lse = s.a.part + (int64_t)(p.p_slices + p.o_slices) * tokens * heads * dim;
     s.common = (int)common;
     s.row_tiles = p.row_tiles;
     s.p_slices = p.p_slices; s.p_tiles = p.p_tiles;
-    s.o_slices = p.o_slices; s.o_tiles = p.o_tiles;
+    s.o_slices = p.o_slices;
     s.o_row_tiles = p.o_row_tiles;
     s.group = heads / kv_heads;
     s.per_seq = cu_tokens ? 0 : (int)(tokens / batch);
@@ -629,7 +642,6 @@ extern "C" int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, in
     s.by_row_tiles = Div(p.row_tiles);
     s.by_o_slices = Div(p.o_slices);
     s.by_o_row_tiles = Div(s.o_row_tiles);
-    s.by_o_tiles = Div(p.o_tiles);
     const int64_t p_items = (int64_t)(kv_heads * p.p_slices + 7) / 8 * 8 * p.row_tiles;
     LQ_REQUIRE(p_items <= UINT32_MAX / 256, "kv8_attention_shared: too many workgroups: %lld tokens", (long long)tokens);
     s.p_items = (int)p_items;

@@ -74,7 +74,7 @@ class Step:
     seq_lens: torch.Tensor     # int32 [sequences], new tokens included
     cu_tokens: torch.Tensor | None
     max_tokens: int
-    max_len: int
+    max_len: int | None        # None: not known
     last: torch.Tensor         # int64 [sequences]: the row of each one's last new token
     positions: torch.Tensor    # int64 [rows]
     longest: int = 0           # tokens of the longest sequence (0: not known, not checked)
@@ -170,12 +170,12 @@ class DeviceSequences:
         """Make room for new[i] more tokens of sequence i (int32 [batch] on the device, none negative) and describe the pass that appends them. `rows`
         is the number of rows that the pass has, as many as there are new tokens or more: those behind them belong to no sequence, but a layer that finds one scale for all rows
         of its input (QLinearA8W8 as constructed) sees what the caller puts there. max_tokens and max_len bound a sequence's
-        new tokens and its length (defaults: rows, the capacity); attention over shared blocks is as fast with the default, without them a bound close to what the
+        new tokens and its length (defaults: rows, the capacity); attention over shared blocks is about as fast with the defaults, without them a max_tokens close to what the
         sequences have is faster, and verify() gives as many columns. Where step.status is not 0 nothing has changed and the pass has no tokens. The
         step names the tables themselves: it describes the pass until they are changed again."""
         cu, positions, slots, self.status = ops.kv8_resize(*self._books(), new, rows=rows, shared=self.shared)
         return Step(block_table=self.block_table, seq_lens=self.seq_lens, cu_tokens=cu, max_tokens=rows if max_tokens is None else max_tokens,
-                    max_len=self.capacity if max_len is None else max_len, last=(cu[1:].long() - 1).clamp_min(0), positions=positions, longest=self.capacity,
+                    max_len=max_len, last=(cu[1:].long() - 1).clamp_min(0), positions=positions, longest=self.capacity,
                     pool=self.num_blocks, shared=self.shared, slots=slots, status=self.status)
 
     def give_back(self, tokens):

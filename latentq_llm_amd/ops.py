@@ -1152,7 +1152,7 @@ def kv8_attention_plan(batch: int, tokens: int, max_tokens: int, max_len: int, h
 
 
 def _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len, scale, out):
-    """(blocks, kv heads, dim, batch, table width, max_tokens, scale, max_len, out) of an attention call, checked; out made where there is none."""
+    """(blocks, kv heads, dim, batch, table width, max_tokens, scale, max_len, whether that was given, out) of an attention call, checked; out made where there is none."""
     n, kv_heads, dim = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     _kv8_rows(q, "q", None, dim, k_codes)
     tokens, heads = q.shape[0], q.shape[1]
@@ -1162,14 +1162,15 @@ def _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, s
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 3.4e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    max_len = width * KV_BLOCK if max_len is None else min(int(max_len), width * KV_BLOCK)
+    known = max_len is not None and max_len <= width * KV_BLOCK
+    max_len = int(max_len) if known else width * KV_BLOCK
     if max_len < 0:
         raise ValueError(f"max_len must not be negative, got {max_len}")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
         _kv8_result(out, "out", q)
-    return n, kv_heads, dim, batch, width, most, scale, max_len, out
+    return n, kv_heads, dim, batch, width, most, scale, max_len, known, out
 
 
 def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,
@@ -1187,7 +1188,7 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
         r = _native.kv8_attention(*args, _workspace(q, 1, -(-r // 32))[0])
     if r is not None:
         return r
-    n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
+    n, kv_heads, dim, batch, width, most, scale, max_len, _, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
                                                                                        scale, out)
     tokens, heads = q.shape[0], q.shape[1]
     window = min(int(window or 0), 1 << 31)  # (positions are less)
@@ -1211,7 +1212,7 @@ def kv8_attention(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
 def kv8_attention_shared_plan(batch: int, tokens: int, max_tokens: int, max_len: int, heads: int, kv_heads: int, dim: int, shared: int,
                               workspace_bytes: int = WORKSPACE_MAX_BYTES, compute_units: int = 0):
     """(slices of the shared keys, of a sequence's own, bytes of workspace these take) kv8_attention_shared would use for a call of these sizes
-    (lq_kv8_attention_shared_plan); (0, 0, bytes): the call is one of kv8_attention. Launches nothing."""
+    (lq_kv8_attention_shared_plan); (0, 0, bytes): the call is one of kv8_attention. max_len of 2^31 or more: not known, as in a call without one. Launches nothing."""
     import ctypes
     prefix, own, needed = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
     _C.call("lq_kv8_attention_shared_plan", batch, tokens, max_tokens, max_len, heads, kv_heads, dim, shared, workspace_bytes, compute_units,
@@ -1228,7 +1229,7 @@ def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq
                                                   out)
     if r is not None:
         return r
-    n, kv_heads, dim, batch, width, most, scale, max_len, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
+    n, kv_heads, dim, batch, width, most, scale, max_len, known, out = _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, cu_tokens, max_tokens, max_len,
                                                                                        scale, out)
     tokens, heads, shared = q.shape[0], q.shape[1], int(shared)
     if not 0 <= shared <= width:
@@ -1237,11 +1238,13 @@ def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq
     if tokens and batch:
         q = _kv8_layout(q)
         with torch.cuda.device(k_codes.device):
-            needed = kv8_attention_shared_plan(batch, tokens, most, max_len, heads, kv_heads, dim, shared)[2]
+            prefix, _, needed = kv8_attention_shared_plan(batch, tokens, most, max_len if known else 1 << 62, heads, kv_heads, dim, shared)
+            if not prefix:
+                needed = kv8_attention_plan(batch, tokens, most, max_len, heads, kv_heads, dim)[2]
             ws = torch.empty(needed, dtype=torch.uint8, device=q.device)
             _C.call("lq_kv8_attention_shared", q.data_ptr(), q.stride(0), q.stride(1), k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(),
                     v_scale.data_ptr(), n, block_table.data_ptr(), width, seq_lens.data_ptr(), None if cu_tokens is None else cu_tokens.data_ptr(),
-                    batch, tokens, most, max_len, shared, heads, kv_heads, dim, _KV_TYPES[q.dtype], scale, int(bool(causal)), out.data_ptr(),
+                    batch, tokens, most, max_len if known else 1 << 62, shared, heads, kv_heads, dim, _KV_TYPES[q.dtype], scale, int(bool(causal)), out.data_ptr(),
                     out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr() if needed else None, needed, _stream(q))
     return (out, lse) if return_lse else out
 

@@ -128,6 +128,26 @@ def test_first_rows_that_are_none(hip_lib):
         assert (out[:5] == 7).all() and (out[95:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("own", [(1, 2), (64, 3000), (255, 256), (257, 1), (700, 0, 1400), (4000, 4001, 5, 130, 1025)])
+def test_own_keys_by_many_workgroups(hip_lib, own, dim, dtype):
+    """Few sequences, whose own keys are shared among workgroups, four tiles each in turn; bounds of the lengths that are right, too small, too large, and none."""
+    from latentq_llm_amd import ops
+    shared, heads, kv_heads = 14, 4, 2
+    lens = [64 * shared + n for n in own]
+    pool = shared + sum(-(-n // 64) for n in own) + 2
+    cache = ref.Cache(pool, kv_heads, dim, seed=dim)
+    table, q = table_of(lens, shared, pool, dim, width=shared + 70), rows((len(own), heads, dim), dtype, 3)
+    want, _, bound = ref.attention(cache, q, table, lens, [1] * len(own))
+    bound = bound + (max(lens) / 32 + 4) * 2.0 ** -24 * 255 * cache.scale[1].max()
+    tensors, tab, length, x = cache.tensors(), i32(table), i32(lens), q.cuda()
+    for max_len in (max(lens), 64 * shared + 1, tab.shape[1] * 64, 1 << 40, None):
+        plan = ops.kv8_attention_shared_plan(len(own), len(own), 1, 1 << 31 if max_len is None else max_len, heads, kv_heads, dim, shared)
+        assert plan[0] > 0 and (max_len is not None or plan[1] > 4)
+        holds(ops.kv8_attention_shared(x, *tensors, tab, length, shared, max_len=max_len), want, bound)
+
+
 def test_sequences_on_the_device_share_by_default(hip_lib):
     """A pass described with no bound but its rows is cut as one with the bound that its sequences keep, and gives the same bits."""
     from latentq_llm_amd import ops
@@ -141,7 +161,7 @@ def test_sequences_on_the_device_share_by_default(hip_lib):
     x = torch.randn((2 * batch, heads, dim), generator=gen).to(BF16).cuda()
     for bounds in ({}, {"max_tokens": 2}, {"max_tokens": 2 * batch}):
         step = seqs.extend(torch.full((batch,), 2, dtype=torch.int32, device="cuda"), 2 * batch, **bounds)
-        assert ops.kv8_attention_shared_plan(batch, 2 * batch, step.max_tokens, step.max_len, heads, kv_heads, dim, shared)[0] > 0
+        assert ops.kv8_attention_shared_plan(batch, 2 * batch, step.max_tokens, 1 << 31, heads, kv_heads, dim, shared)[0] > 0
         cache.append(x[:, :kv_heads], x[:, kv_heads:2 * kv_heads], step)
         results.append(cache.attend(x, step))
         seqs.give_back(torch.full((batch,), 2, dtype=torch.int32, device="cuda"))

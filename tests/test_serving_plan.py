@@ -35,3 +35,15 @@ def test_a_plan_made_again_with_the_bytes_that_it_took(hip_lib):
     for batch, total, bound in ((64, 64, 64), (17, 60, 40), (40, 300, 200), (5, 5, 5)):
         first = plan(batch, total, bound, 9000, 32, 8, 128, 128)
         assert first[0] > 0 and plan(batch, total, bound, 9000, 32, 8, 128, 128, workspace_bytes=first[2]) == first
+
+
+@pytest.mark.parametrize("batch, tokens, shared, own, heads, kv_heads, dim", [(64, 1, 128, 512, 32, 8, 128), (16, 1, 2048, 257, 32, 8, 128), (8, 5, 64, 640, 32, 32, 64), (4, 1, 128, 100, 32, 8, 128),
+                                                                             (8, 4, 16, 300, 32, 32, 128)])
+def test_lengths_that_are_not_known(hip_lib, batch, tokens, shared, own, heads, kv_heads, dim):
+    """Without a bound of the lengths the shared keys are cut as for sequences that have few of their own, not by all that the table has room for."""
+    args = (heads, kv_heads, dim, shared)
+    exact = plan(batch, batch * tokens, tokens, 64 * shared + own, *args)
+    unknown = plan(batch, batch * tokens, tokens, 1 << 31, *args)
+    assert unknown[0] >= exact[0] > 0 and unknown[0] <= 2 * exact[0]
+    assert plan(batch, batch * tokens, tokens, (1 << 63) - 1, *args) == unknown
+    assert plan(batch, batch * tokens, tokens, 1 << 31, *args, workspace_bytes=unknown[2]) == unknown
