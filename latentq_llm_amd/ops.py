@@ -1162,8 +1162,10 @@ def _kv8_attention_checked(q, k_codes, v_codes, k_scale, v_scale, block_table, s
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale <= 3.4e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
+    max_len = None if max_len is None else int(max_len)
     known = max_len is not None and max_len <= width * KV_BLOCK
-    max_len = int(max_len) if known else width * KV_BLOCK
+    if not known:
+        max_len = width * KV_BLOCK
     if max_len < 0:
         raise ValueError(f"max_len must not be negative, got {max_len}")
     if out is None:

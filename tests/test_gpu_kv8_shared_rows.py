@@ -193,3 +193,22 @@ def test_a_captured_call_with_a_bound_above(hip_lib):
         want = call()
         torch.cuda.synchronize()
         assert torch.equal(out, want), n
+
+
+def test_bounds_that_are_no_numbers(hip_lib):
+    """What the binding cannot convert is the wrapper's to refuse, or to take where it is a whole number."""
+    from latentq_llm_amd import ops
+    shared, lens = 14, [14 * 64 + 3, 14 * 64 + 70]
+    cache = ref.Cache(20, 2, 64, seed=1)
+    t, table, length, q = cache.tensors(), i32(table_of(lens, shared, 20, 1)), i32(lens), rows((2, 4, 64), BF16, 2).cuda()
+    for name in ("max_len", "scale"):
+        with pytest.raises(ValueError):
+            ops.kv8_attention_shared(q, *t, table, length, shared, **{name: "x"})
+    with pytest.raises(ValueError, match="max_len must not be negative"):
+        ops.kv8_attention_shared(q, *t, table, length, shared, max_len=-1)
+    want = ops.kv8_attention_shared(q, *t, table, length, shared, max_len=966)
+    for max_len in (966.0, np.float32(966)):
+        assert torch.equal(ops.kv8_attention_shared(q, *t, table, length, shared, max_len=max_len), want)
+    want = ops.kv8_attention_shared(q, *t, table, length, shared)
+    for max_len in (1e9, 1 << 40):  # as one that is not known
+        assert torch.equal(ops.kv8_attention_shared(q, *t, table, length, shared, max_len=max_len), want)
