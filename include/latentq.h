@@ -582,8 +582,8 @@ int lq_kv8_attention_plan(int64_t batch, int64_t tokens, int64_t max_tokens, int
  * block_table are the same in every row, which is the caller's promise (which row's entries are read is not said). Those keys are
  * read once for all rows, where that is faster, and the result is that of lq_kv8_attention but for roundings: codes enter the products as 1 .. 255, and 128 times the sum of the queries, or of
  * the weights, is taken off, so that the fp32 sums are of numbers up to 255 where they are up to 127 there. A sequence may be shorter than the shared blocks: its rows
- * see what is theirs. What is faster goes by the rows that the pass has for a sequence on average (up to 64, query heads of a kv head counted), so that max_tokens may be a bound far above what the sequences
- * have. workspace as there, and without one, or with too little, every sequence is read by itself. */
+ * see what is theirs. What is faster goes by the rows of a sequence (up to 64, query heads of a kv head counted): by max_tokens, or by the pass's average where that is half of it or less, so that max_tokens
+ * may be a bound far above what the sequences have. workspace as there, and without one, or with too little, every sequence is read by itself. */
 int lq_kv8_attention_shared(const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k_codes, const void *v_codes, const float *k_scale,
                             const float *v_scale, int64_t num_blocks, const int32_t *block_table, int64_t table_width, const int32_t *seq_lens,
                             const int32_t *cu_tokens, int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int64_t shared, int heads, int kv_heads,

@@ -526,10 +526,11 @@ bool pays(int64_t batch, int64_t own_rows, int kv_heads, int dim, int64_t common
 // The rows that a sequence is taken to have: as many as it may have, but where that is far from what the pass has for each (it may be a bound that nobody looked for, or that of one
 // sequence alone) the latter; those beyond are found in place_beyond(). us with the bound exact / all rows of the pass / each sequence by itself, 32 heads on 8 of 128: 64 x 1 behind 8192 29.1 / 29.4 /
 // 94, 17 x 1 behind 131072 83 / 86 / 660, 300 x 1 behind 4096 62 / 63 / 200; 8 x 5 behind 4096, 32 heads of 64, 13.5 / 13.5 / 21. With one sequence of more rows, taken to have as many as
-// it / as the others: 15 x 1 and one of 12 behind 4096 17.9 / 15.0, 63 x 1 and one of 512 behind 8192 631 / 155 (each by itself 690).
+// it / as the others: 15 x 1 and one of 12 behind 4096 17.9 / 15.0, 63 x 1 and one of 512 behind 8192 631 / 155 (each by itself 690). With 1 to 33 tokens each, 64 behind 4096 145, by itself 274;
+// with 12 to 20, where the bound says what they have, 89 and 59 behind 1024, 228 and 302 behind 8192.
 int64_t rows_of_a_sequence(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t group) {
     const int64_t most = max_tokens * group, average = (tokens + batch - 1) / batch * group;
-    return most > kFewRows || (most + 15) / 16 >= 3 * ((average + 15) / 16) ? std::min(average, most) : most;
+    return most > kFewRows ? (most >= 2 * average ? average : most) : (most + 15) / 16 >= 3 * ((average + 15) / 16) ? average : most;
 }
 
 Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len, int heads, int kv_heads, int dim, int64_t common, int64_t workspace, int cus) {
@@ -545,8 +546,9 @@ Plan plan_of(int64_t batch, int64_t tokens, int64_t max_tokens, int64_t max_len,
     const int64_t own_tiles = std::max(blocks_of(max_len) - common, (int64_t)0), slot = tokens * heads * ((int64_t)dim + 1) * 4;
     // Slices of the prefix, by an estimate in us: a compute unit gives a tile of an item `a_tile` (its arithmetic, or its bytes where no other row tile
     // brings them; a tenth less of several row tiles with two items at a time), ways in and out are 4 us, and partial results go there and back. Items shorter than what all the work takes gain nothing. (Own keys count half: max_len is the
-    // longest sequence's.) us by slices, 128 dimensions: 12 sequences behind 2048 with up to 1019 of their own 2: 20.0, 4: 20.0, 8: 21.5; 64 behind 8192, 32 heads on 8,
-    // 3: 30.0, 4: 26.9, 8: 31.5; 16 behind 131072 16: 58, 32: 59, 48: 63; 64 behind 32768 4: 56, 8: 55, 16: 57; 8 x 5 behind 4096, 32 heads of 64, 2: 16.4, 4: 12.6, 8: 13.5.
+    // longest sequence's.) us by slices, the same inputs again in a graph, 128 dimensions: 12 sequences behind 2048 with up to 1019 of their own 2: 20.1, 4: 20.1, 8: 21.4; 64 behind 8192, 32 heads on 8,
+    // 3: 28.4, 4: 25.8, 8: 31.5; 16 behind 131072 8: 88, 16: 59, 32: 59, 48: 62; 64 behind 32768 3: 66, 4: 56, 8: 58, 16: 65; 8 x 5 behind 4096, 32 heads of 64, 2: 16.4, 4: 12.8, 8: 15.2; 64 behind 8192,
+    // 8 heads on 1 of 256, 4: 34.1, 8: 27.1, 16: 33.7, 24 on 8 1: 81, 2: 57, 4: 61.
     const int64_t units = kv_heads * p.row_tiles;
     // Where max_len is not known the number is that for no own keys, which costs little where there are many: 64 behind 8192 with 512 of their own
     // 30.9, by what the table has room for, 4096 or more, 54; 16 behind 131072 with room for 65536 60, 162; with 1500 of their own 58, of a known length 49.

@@ -1065,7 +1065,7 @@ def kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, 
     layout and rounding: include/latentq.h). seq_lens counts the new tokens. cos, sin (float32 [positions, rotated dims / 2]):
     keys are rotated by their position, and so is q [tokens, heads, dim], which is returned (q_out may be q itself). With
     several tokens a sequence, cu_tokens (int32 [batch + 1]) has each sequence's first row; max_tokens, the largest number of new tokens
-    of a sequence, sizes the launch (default: what the number of rows allows). Returns the rotated q, or None."""
+    of a sequence, sizes the launch (default: what the number of rows allows). Returns the rotated q, or None; rows of it that no sequence has are not written."""
     done = (_native or _fast()).kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, q, cos, sin, cu_tokens, max_tokens, q_out)
     if done is not None:
         return None if q is None else done
@@ -1225,8 +1225,8 @@ def kv8_attention_shared_plan(batch: int, tokens: int, max_tokens: int, max_len:
 def kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, *, cu_tokens=None, max_tokens=None, max_len=None, scale=None,
                          causal=True, out=None, return_lse=False):
     """kv8_attention of a batch whose sequences all begin with the same `shared` blocks (lq_kv8_attention_shared): the first `shared` columns of
-    block_table are the same in every row. Their keys and values are read once for all rows, where that is faster (the pass has up to 64 rows for a sequence and kv head on average, ...:
-    kv8_attention_shared_plan says). Arguments and results otherwise as kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
+    block_table are the same in every row. Their keys and values are read once for all rows, where that is faster (up to 64 rows of a sequence and kv head, on average
+    where max_tokens is far above it; kv8_attention_shared_plan says). Arguments and results otherwise as kv8_attention's, without a window; the sequences may have any lengths, shorter than the shared blocks too."""
     r = (_native or _fast()).kv8_attention_shared(q, k_codes, v_codes, k_scale, v_scale, block_table, seq_lens, shared, cu_tokens, max_tokens, max_len, scale, causal, return_lse,
                                                   out)
     if r is not None:

@@ -31,6 +31,12 @@ def test_sequences_that_have_many_rows_themselves(hip_lib, tokens, group, shares
         assert (plan(8, 8 * tokens, bound, 9000, 8 * group, 8, 128, 128)[0] > 0) == shares
 
 
+def test_a_bound_close_to_what_the_sequences_have(hip_lib):
+    """More than 64 rows at the most, and not half of that on average: as many rows as the bound says."""
+    for total, shares in ((64 * 10, True), (64 * 13, False), (64 * 15, False)):  # of up to 20 tokens each, four heads to a kv head
+        assert (plan(64, total, 20, 9000, 32, 8, 128, 128)[0] > 0) == shares
+
+
 def test_a_plan_made_again_with_the_bytes_that_it_took(hip_lib):
     for batch, total, bound in ((64, 64, 64), (17, 60, 40), (40, 300, 200), (5, 5, 5)):
         first = plan(batch, total, bound, 9000, 32, 8, 128, 128)
