@@ -10,7 +10,7 @@
 // many rows are a second launch.
 //
 // Bound: latency, of loads that wait for each other (lengths and changes, the list, the table's blocks, the rows) and the launch: 1 sequence 1.9 us, 64
-// with up to 8 tokens each 3.6, 128 with up to 512 3.4 and another 3.4 for the rows.
+// with up to 8 tokens each 3.9, 128 with up to 512 3.3 and another 3.4 for the rows.
 #include "lq_kv8.h"
 
 namespace {

@@ -13,8 +13,9 @@
 // instructions and were slower or level at all sizes: 64 rows of 128 dimensions 71 / 64 us, 64 x 8192 of 64 dimensions 31.6 / 24.2, of 96 37 / 33, 1024 rows of 128 48.8 / 50.2. 64 rows to a
 // wave do not fit (80 bytes spilled; 93 us).
 //
-// Bound: 64 rows of 128 dimensions on 131072 keys 59 us, 4.7 TB/s, with the vector units 52 % and the matrix units 30 % busy; 12 sequences behind 2048 keys with up to
-// 1019 of their own, 32 heads of 128, 18.4 us, 4.6 TB/s; 64 behind 8192, 32 heads on 8, 23.8 us, the vector units 56 % and the matrix units 22 %. The join is 4 to 5.
+// Bound: 64 rows of 128 dimensions on 131072 keys 60 us, 4.6 TB/s, with the vector units 52 % and the matrix units 30 % busy; 12 sequences behind 2048 keys with up to
+// 1019 of their own, 32 heads of 128, 19.0 us, 4.4 TB/s; 64 behind 8192, 32 heads on 8, 24.0 us, the vector units 56 % and the matrix units 22 %; the same of 256 dimensions, 24 heads on 8, 57 us,
+// 38 % and 14 %: one wave a SIMD, and every 16 rows convert all codes again. The join is 4 to 5.
 #include "lq_kv8.h"
 
 #include <algorithm>

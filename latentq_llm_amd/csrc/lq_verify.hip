@@ -14,8 +14,9 @@
 // sequence, makes the rows' tests, finds the slice in which the sum passes the number by the slices' sums, and the entry in it. With them what is left of a
 // row needs both rows' sums first: one launch more takes the sums of max(p - q, 0) in blocks of the one row of each sequence.
 //
-// Bound: latency of the launches and of the loads in them that wait for each other while rows are few (1 row of 32000: 3.9 + 4.6 us; 8 x 5 with the
-// drafter's logits 5.8 + 5.1 + 4.9), the exponentials and the memory in turn when they are many (320 rows of 32000 fp32 logits: 13.8 us, 3.1 TB/s).
+// Bound: latency of the launches and of the loads in them that wait for each other while rows are few (1 row of 32000: 3.8 + 4.6 us; 8 x 5 with the
+// drafter's logits 5.8 + 4.9 + 4.7), the exponentials and the memory in turn when they are many (the rows of 64 sequences of up to 6, 32000 fp32 logits, and the drafter's: 14.2 us, 3.0 TB/s). The largest logit:
+// 1 row 3.4 + 2.4, 8 x 5 3.6 + 3.3, 64 x 6 of fp32 11.5 + 3.9 (4.3 TB/s).
 #include "lq_common.h"
 
 #include <algorithm>
